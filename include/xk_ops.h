@@ -494,6 +494,138 @@ int xk_chunk_fwd_o(const void* q, const void* k, const void* v, const void* h,
                    xk_dtype cu_dtype, int64_t N, void* workspace,
                    size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Gated linear recurrence over the channels of a token (no reference
+ * counterpart; the elementwise relative of the gated delta rule):
+ *     r = sigmoid(a_t), i = sigmoid(b_t), l = -c softplus(lam) r,
+ *     h_t = exp(l) h_{t-1} + sqrt(1 - exp(2 l)) i x_t,    y_t = h_t
+ * per channel, in fp32 whatever the inputs' type.
+ *   x, a, b, y : [total_tokens, D] rows with token pitches (at least D) in
+ *     `dtype` (f32/bf16/f16), any alignment; lam fp32 [D]; c >= 0.  y may be
+ *     x, a or b itself (the same start and pitch).
+ *   Sequences are cu_seqlens[n]..cu_seqlens[n+1] (int32/int64, device,
+ *     ascending; values are clamped to [0, total_tokens]), or N runs of
+ *     total_tokens / N tokens when cu_seqlens is NULL; a sequence may be empty.
+ *     Rows of y outside every sequence are left as they were.
+ *   initial_state, final_state : fp32 [N, D] (NULL = zero / not written); they
+ *     may be the same buffer.  An empty sequence's final state is its initial
+ *     state.
+ *   states : NULL, or fp32 [ceil(total_tokens / XK_GLR_WINDOW), D], what the
+ *     backward pass starts from: row w is the state before token
+ *     w * XK_GLR_WINDOW where that token is inside a sequence and not its
+ *     first; other rows are unspecified.
+ *   Cuts of the work fall on multiples of a tile of tokens counted from row 0
+ *     of the batch: a sequence's bits depend on where in the batch it stands,
+ *     but not on the other sequences, and not on the run.
+ *   workspace >= xk_gated_linear_recurrence_workspace_bytes(...) bytes,
+ *     256-byte aligned; 0 bytes (NULL) for few tokens.  Calls that overlap in
+ *     time need a workspace each.
+ */
+#define XK_GLR_WINDOW 16
+int64_t xk_gated_linear_recurrence_workspace_bytes(int64_t total_tokens, int64_t D);
+int xk_gated_linear_recurrence(
+    const void* x, int64_t stride_x_tok, const void* a, int64_t stride_a_tok, const void* b,
+    int64_t stride_b_tok, xk_dtype dtype, const float* lam, float c, void* y,
+    int64_t stride_y_tok, const float* initial_state, float* final_state, float* states,
+    const void* cu_seqlens, xk_dtype cu_dtype, int64_t N, int64_t total_tokens, int64_t D,
+    void* workspace, size_t workspace_bytes, void* stream);
+
+/* The recurrence's decode step on a pool of states: one token, or a few
+ * drafted ones, of every sequence (the slot rules of xk_gdn_recurrent).
+ *   x, a, b, y as above ([tokens, D], y dense or with a pitch); sequence n is
+ *     rows cu_seqlens[n]..cu_seqlens[n+1], or T rows from n * T when
+ *     cu_seqlens is NULL (T then positive).
+ *   state : fp32 [num_slots, D] (slot pitch at least D), updated in place.
+ *     state_indices int32 NULL (slot = n), [N] (num_cols = 0) or [N, num_cols]
+ *     (row pitch num_cols).  A sequence starts from the slot in column 0 (or
+ *     num_accepted_tokens[n] - 1, clamped to the columns) and writes its last
+ *     state to that slot; with num_cols > 0 it writes the state after token t
+ *     to the slot in column t instead (tokens beyond the columns are not
+ *     written).  A slot outside [0, num_slots) starts from zero and is not
+ *     written.  A slot must not be one that another sequence of the call
+ *     writes.
+ */
+int xk_gated_linear_recurrence_update(
+    const void* x, int64_t stride_x_tok, const void* a, int64_t stride_a_tok, const void* b,
+    int64_t stride_b_tok, xk_dtype dtype, const float* lam, float c, void* y,
+    int64_t stride_y_tok, float* state, int64_t stride_state_slot, int64_t num_slots,
+    const int32_t* state_indices, int64_t num_cols, const int32_t* num_accepted_tokens,
+    const void* cu_seqlens, xk_dtype cu_dtype, int64_t N, int64_t T, int64_t total_tokens,
+    int64_t D, void* stream);
+
+/* Backward pass of xk_gated_linear_recurrence.  With G_t = dy_t +
+ * exp(l_{t+1}) G_{t+1} (beyond the last token: d_final_state, NULL = zero):
+ *     dx = G s i, db = G s x i (1 - i), s = sqrt(1 - exp(2 l)),
+ *     dl = G (exp(l) h_{t-1} - i x exp(2 l) / s), da = dl l (1 - r),
+ *     dlam = -c sigmoid(lam) sum_t dl r, d_initial_state = exp(l_1) G_1
+ * (where a closed gate makes s zero, the limits).
+ *   dy, dx, da, db : [total_tokens, D] in `dtype` with token pitches; rows
+ *     outside every sequence are left as they were.  states is what the
+ *     forward call wrote for the same arguments.  h_t is computed again from
+ *     it in fp32; the rounded outputs of the forward pass are not used.
+ *   dlam : fp32 [D], written (not accumulated), or NULL.  d_initial_state :
+ *     fp32 [N, D] or NULL; an empty sequence's is its d_final_state.
+ *   The sums over tokens have a fixed order: the same call gives the same bits.
+ *   workspace >= xk_gated_linear_recurrence_bwd_workspace_bytes(...) bytes,
+ *     256-byte aligned.
+ */
+int64_t xk_gated_linear_recurrence_bwd_workspace_bytes(int64_t total_tokens, int64_t N,
+                                                       int64_t D);
+int xk_gated_linear_recurrence_bwd(
+    const void* dy, int64_t stride_dy_tok, const void* x, int64_t stride_x_tok, const void* a,
+    int64_t stride_a_tok, const void* b, int64_t stride_b_tok, xk_dtype dtype, const float* lam,
+    float c, const float* states, const float* initial_state, const float* d_final_state,
+    void* dx, int64_t stride_dx_tok, void* da, int64_t stride_da_tok, void* db,
+    int64_t stride_db_tok, float* dlam, float* d_initial_state, const void* cu_seqlens,
+    xk_dtype cu_dtype, int64_t N, int64_t total_tokens, int64_t D, void* workspace,
+    size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
+ * The step from one block to the next in one pass (no reference counterpart;
+ * a sandwich of the RMSNorms above with the residual sum):
+ *     n = x / sqrt(mean(x^2) + eps) * post_weight     (NULL: n = x)
+ *     v = n * gate * sigmoid(gate)                    (NULL: v = n)
+ *     h = residual + scale * v                        (NULL: scale = 1)
+ *     y = h / sqrt(mean(h^2) + eps) * pre_weight      (NULL: no y)
+ * in fp32; y is formed from h before its rounding.  With unit_offset != 0
+ * both norms multiply by (1 + weight), as xk_gemma_rms_norm does.
+ *   x, gate, y : [M, N] rows (pitch at least N) in `dtype`; residual, h in
+ *     rdtype (`dtype` or f32); post_weight, pre_weight, scale : [N], wdtype
+ *     (`dtype` or f32).  Any alignment.  h may be residual, y may be x or
+ *     gate (the same start and pitch).
+ *   rstd_post, rstd_pre : fp32 [M] or NULL: 1 / sqrt(mean + eps) of the norms
+ *     that run, for the backward pass.
+ */
+int xk_gated_residual_rms_norm(
+    const void* x, int64_t stride_x_row, const void* residual, int64_t stride_res_row,
+    const void* gate, int64_t stride_gate_row, const void* post_weight, const void* scale,
+    const void* pre_weight, void* h, int64_t stride_h_row, void* y, int64_t stride_y_row,
+    float* rstd_post, float* rstd_pre, int64_t M, int64_t N, float eps, int unit_offset,
+    xk_dtype dtype, xk_dtype rdtype, xk_dtype wdtype, void* stream);
+
+/* Backward pass of xk_gated_residual_rms_norm: gradients of everything that
+ * the forward call was given.  The forward inputs come again (h is formed
+ * again in fp32), with the rstd that it wrote (needed where its norm runs).
+ *   dh : gradient of h (rdtype) or NULL (zero); dy : of y (dtype), or NULL
+ *     (zero; then pre_weight takes no part).  One of them at least.
+ *   dx, dgate (dtype), dresidual (rdtype) : [M, N] rows.  dgate is written
+ *     where gate is given.  dx, dgate and dresidual may each be NULL.
+ *   dpost_weight, dscale, dpre_weight : [N] in wdtype, or NULL: sums over the
+ *     rows in fp32 in a fixed order (M = 0: zeros).
+ *   workspace >= xk_gated_residual_rms_norm_bwd_workspace_bytes(M, N) bytes,
+ *     256-byte aligned, where one of the three sums is asked for.
+ */
+int64_t xk_gated_residual_rms_norm_bwd_workspace_bytes(int64_t M, int64_t N);
+int xk_gated_residual_rms_norm_bwd(
+    const void* dh, int64_t stride_dh_row, const void* dy, int64_t stride_dy_row, const void* x,
+    int64_t stride_x_row, const void* residual, int64_t stride_res_row, const void* gate,
+    int64_t stride_gate_row, const void* post_weight, const void* scale, const void* pre_weight,
+    const float* rstd_post, const float* rstd_pre, void* dx, int64_t stride_dx_row,
+    void* dresidual, int64_t stride_dres_row, void* dgate, int64_t stride_dgate_row,
+    void* dpost_weight, void* dscale, void* dpre_weight, int64_t M, int64_t N, int unit_offset,
+    xk_dtype dtype, xk_dtype rdtype, xk_dtype wdtype, void* workspace, size_t workspace_bytes,
+    void* stream);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif

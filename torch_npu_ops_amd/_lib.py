@@ -30,6 +30,8 @@ SZ = ctypes.c_size_t
 XK_F32, XK_BF16, XK_F16, XK_I32, XK_I64 = 0, 1, 2, 3, 4
 XK_OK, XK_ERR_INVALID, XK_ERR_UNSUPPORTED, XK_ERR_WORKSPACE, XK_ERR_SCRATCH = 0, -1, -2, -3, -4
 
+XK_GLR_WINDOW = 16  # tokens per saved state of the gated linear recurrence
+
 # Argument lists, in declaration order of include/xk_ops.h.
 SIGNATURES: dict[str, tuple[list, object]] = {
     "xk_version": ([], ctypes.c_char_p),
@@ -95,6 +97,24 @@ SIGNATURES: dict[str, tuple[list, object]] = {
     "xk_chunk_fwd_o": (
         [P, P, P, P, I64, INT, P, P, F32, I64, I64, I64, I64, I64, P, INT, I64,
          P, SZ, P], INT),
+    "xk_gated_linear_recurrence_workspace_bytes": ([I64, I64], I64),
+    "xk_gated_linear_recurrence": (
+        [P, I64, P, I64, P, I64, INT, P, F32, P, I64, P, P, P, P, INT, I64, I64, I64, P, SZ, P],
+        INT),
+    "xk_gated_linear_recurrence_update": (
+        [P, I64, P, I64, P, I64, INT, P, F32, P, I64, P, I64, I64, P, I64, P, P, INT, I64, I64,
+         I64, I64, P], INT),
+    "xk_gated_linear_recurrence_bwd_workspace_bytes": ([I64, I64, I64], I64),
+    "xk_gated_linear_recurrence_bwd": (
+        [P, I64, P, I64, P, I64, P, I64, INT, P, F32, P, P, P, P, I64, P, I64, P, I64, P, P, P,
+         INT, I64, I64, I64, P, SZ, P], INT),
+    "xk_gated_residual_rms_norm": (
+        [P, I64, P, I64, P, I64, P, P, P, P, I64, P, I64, P, P, I64, I64, F32, INT, INT, INT,
+         INT, P], INT),
+    "xk_gated_residual_rms_norm_bwd_workspace_bytes": ([I64, I64], I64),
+    "xk_gated_residual_rms_norm_bwd": (
+        [P, I64, P, I64, P, I64, P, I64, P, I64, P, P, P, P, P, P, I64, P, I64, P, I64, P, P, P,
+         I64, I64, INT, INT, INT, INT, P, SZ, P], INT),
 }
 
 _LIB = None

@@ -80,6 +80,14 @@ class OperationFactory {
              "fused_qkvzba_split_reshape_cat_gqa_r4_kernel")
   XK_FACTORY(chunk_gated_delta_rule_fused, ChunkGatedDeltaRuleFusedOp, "xk_gdn_chunk_fwd")
   XK_FACTORY(gdn_conv_decode, GdnConvDecodeOp, "xk_gdn_conv_decode")
+  XK_FACTORY(gated_linear_recurrence, GatedLinearRecurrenceOp, "xk_gated_linear_recurrence")
+  XK_FACTORY(gated_linear_recurrence_update, GatedLinearRecurrenceUpdateOp,
+             "xk_gated_linear_recurrence_update")
+  XK_FACTORY(gated_linear_recurrence_bwd, GatedLinearRecurrenceBwdOp,
+             "xk_gated_linear_recurrence_bwd")
+  XK_FACTORY(gated_residual_rms_norm, GatedResidualRmsNormOp, "xk_gated_residual_rms_norm")
+  XK_FACTORY(gated_residual_rms_norm_bwd, GatedResidualRmsNormBwdOp,
+             "xk_gated_residual_rms_norm_bwd")
 
 #undef XK_FACTORY
 

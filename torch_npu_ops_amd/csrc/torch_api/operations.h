@@ -82,9 +82,15 @@ XK_OPERATION(FusedQkvzbaSplitReshapeGqaR1Op, xk_fused_qkvzba_split_reshape_cat);
 XK_OPERATION(FusedQkvzbaSplitReshapeGqaR2Op, xk_fused_qkvzba_split_reshape_cat);
 XK_OPERATION(FusedQkvzbaSplitReshapeGqaR3Op, xk_fused_qkvzba_split_reshape_cat);
 XK_OPERATION(FusedQkvzbaSplitReshapeGqaR4Op, xk_fused_qkvzba_split_reshape_cat);
-// No reference counterpart: the whole chunked pipeline and the fused decode step.
+// No reference counterpart: the whole chunked pipeline, the fused decode step,
+// the gated linear recurrence and the block-to-block norm.
 XK_OPERATION(ChunkGatedDeltaRuleFusedOp, xk_gdn_chunk_fwd);
 XK_OPERATION(GdnConvDecodeOp, xk_gdn_conv_decode);
+XK_OPERATION(GatedLinearRecurrenceOp, xk_gated_linear_recurrence);
+XK_OPERATION(GatedLinearRecurrenceUpdateOp, xk_gated_linear_recurrence_update);
+XK_OPERATION(GatedLinearRecurrenceBwdOp, xk_gated_linear_recurrence_bwd);
+XK_OPERATION(GatedResidualRmsNormOp, xk_gated_residual_rms_norm);
+XK_OPERATION(GatedResidualRmsNormBwdOp, xk_gated_residual_rms_norm_bwd);
 
 #undef XK_OPERATION
 

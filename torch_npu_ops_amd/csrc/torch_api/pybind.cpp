@@ -79,6 +79,22 @@ PYBIND11_MODULE(_xk_torch, m) {
         "scale"_a = std::optional<float>(), "conv_bias"_a = OptT(),
         "conv_state_indices"_a = OptT(), "ssm_state_indices"_a = OptT(), "pad_slot_id"_a = -1,
         "softplus_beta"_a = 1.0f, "softplus_threshold"_a = 20.0f, "use_qk_l2norm"_a = true);
+  m.def("npu_gated_linear_recurrence", &npu::npu_gated_linear_recurrence, "x"_a, "a"_a, "b"_a,
+        "lam"_a, "c"_a = 8.0, "initial_state"_a = OptT(), "output_final_state"_a = false,
+        "cu_seqlens"_a = OptT(), "output_states"_a = false);
+  m.def("npu_gated_linear_recurrence_update", &npu::npu_gated_linear_recurrence_update, "x"_a,
+        "a"_a, "b"_a, "lam"_a, "state"_a, "c"_a = 8.0, "state_indices"_a = OptT(),
+        "num_accepted_tokens"_a = OptT(), "cu_seqlens"_a = OptT());
+  m.def("npu_gated_linear_recurrence_bwd", &npu::npu_gated_linear_recurrence_bwd, "dy"_a, "x"_a,
+        "a"_a, "b"_a, "lam"_a, "states"_a, "c"_a = 8.0, "initial_state"_a = OptT(),
+        "d_final_state"_a = OptT(), "cu_seqlens"_a = OptT());
+  m.def("npu_gated_residual_rms_norm", &npu::npu_gated_residual_rms_norm, "x"_a, "residual"_a,
+        "post_weight"_a = OptT(), "gate"_a = OptT(), "scale"_a = OptT(),
+        "pre_weight"_a = OptT(), "eps"_a = 1e-6, "unit_offset"_a = false);
+  m.def("npu_gated_residual_rms_norm_bwd", &npu::npu_gated_residual_rms_norm_bwd, "dh"_a,
+        "dy"_a, "x"_a, "residual"_a, "rstd_post"_a, "rstd_pre"_a, "post_weight"_a = OptT(),
+        "gate"_a = OptT(), "scale"_a = OptT(), "pre_weight"_a = OptT(),
+        "unit_offset"_a = false);
   // npu_ops (AscendC API): gemma returns (rstd, y) for its two out-params.
   m.def("npu_ops_gemma_rms_norm", [](const torch::Tensor& x, const torch::Tensor& gamma,
                                      double eps) {

@@ -6,6 +6,7 @@
 #include "ascendc_ops_api.h"
 #include "triton_ops_api.h"
 
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
 #include <cmath>
@@ -829,6 +830,374 @@ torch::Tensor npu_gdn_conv_sigmoid_gating_decode(
             stream_of(x)),
         "xk_gdn_conv_gating_decode");
   return o;
+}
+
+// ---------------------------------------------------------------------------
+// Gated linear recurrence and the block-to-block norm (no reference
+// counterpart).  Each call runs with its tensors' device current.
+// ---------------------------------------------------------------------------
+namespace {
+
+void same_device(const torch::Tensor& t, const torch::Tensor& x, const char* name) {
+  TORCH_CHECK(t.device() == x.device(), name, " must be on ", x.device(), ", is on ", t.device());
+}
+
+// [B, T, D] (or [rows, N]) as rows of D with one pitch between them, unit
+// column stride: a view if it has that form, else a contiguous copy.
+// `pitch` receives the elements from row to row.
+torch::Tensor pitched_rows(const torch::Tensor& x, int64_t& pitch) {
+  const int64_t D = x.size(-1);
+  int64_t p = D, count = 1;
+  bool ok = D == 1 || x.stride(-1) == 1;
+  for (int64_t d = x.dim() - 2; d >= 0 && ok; --d) {
+    if (x.size(d) == 1) continue;
+    if (count == 1) {
+      p = x.stride(d);
+      ok = p >= D;
+    } else {
+      ok = x.stride(d) == p * count;
+    }
+    count *= x.size(d);
+  }
+  pitch = ok ? p : D;
+  return ok ? x : x.contiguous();
+}
+
+void glr_check(const torch::Tensor& x, const torch::Tensor& a, const torch::Tensor& b,
+               const torch::Tensor& lam, double c) {
+  for (const auto& [t, name] : {std::make_pair(&a, "a"), std::make_pair(&b, "b")}) {
+    TORCH_CHECK(t->sizes() == x.sizes() && t->scalar_type() == x.scalar_type(), name,
+                " must have x's shape and dtype");
+    same_device(*t, x, name);
+  }
+  TORCH_CHECK(x.scalar_type() == torch::kFloat32 || x.scalar_type() == torch::kBFloat16 ||
+                  x.scalar_type() == torch::kFloat16,
+              "x must be float32, bfloat16 or float16");
+  TORCH_CHECK(x.size(-1) > 0, "x must have channels");
+  TORCH_CHECK(lam.scalar_type() == torch::kFloat32 && lam.dim() == 1 &&
+                  lam.size(0) == x.size(-1),
+              "lam must be float32 [D]");
+  same_device(lam, x, "lam");
+  TORCH_CHECK(c >= 0 && std::isfinite(c), "c must be finite and not negative");
+}
+
+// cu_seqlens as the kernels read it (undefined: x's batch rows), and the
+// number of sequences.
+std::pair<torch::Tensor, int64_t> glr_seqs(const torch::Tensor& x,
+                                           const std::optional<torch::Tensor>& cu_seqlens) {
+  if (!has(cu_seqlens)) return {torch::Tensor(), x.size(0)};
+  const auto& cu = *cu_seqlens;
+  TORCH_CHECK((cu.scalar_type() == torch::kInt32 || cu.scalar_type() == torch::kInt64) &&
+                  cu.dim() == 1 && cu.size(0) >= 1,
+              "cu_seqlens must be int32 or int64 [N + 1]");
+  same_device(cu, x, "cu_seqlens");
+  return {cu.contiguous(), cu.size(0) - 1};
+}
+
+torch::Tensor glr_state(const std::optional<torch::Tensor>& s, const torch::Tensor& x, int64_t N,
+                        const char* name) {
+  if (!has(s)) return {};
+  TORCH_CHECK(s->scalar_type() == torch::kFloat32 && s->dim() == 2 && s->size(0) == N &&
+                  s->size(1) == x.size(-1),
+              name, " must be float32 [N, D]");
+  same_device(*s, x, name);
+  return s->contiguous();
+}
+
+float* fptr(const torch::Tensor& t) {
+  return t.defined() ? static_cast<float*>(t.data_ptr()) : nullptr;
+}
+
+std::optional<torch::Tensor> given(const torch::Tensor& t) {
+  return t.defined() ? std::optional<torch::Tensor>(t) : std::nullopt;
+}
+
+}  // namespace
+
+std::tuple<torch::Tensor, std::optional<torch::Tensor>, std::optional<torch::Tensor>>
+npu_gated_linear_recurrence(const torch::Tensor& x, const torch::Tensor& a,
+                            const torch::Tensor& b, const torch::Tensor& lam, double c,
+                            const std::optional<torch::Tensor>& initial_state,
+                            bool output_final_state,
+                            const std::optional<torch::Tensor>& cu_seqlens, bool output_states) {
+  TORCH_CHECK(x.dim() == 3, "gated_linear_recurrence expects x [B, T, D]");
+  glr_check(x, a, b, lam, c);
+  void* stream = stream_of(x);
+  c10::DeviceGuard guard(x.device());
+  auto [cu, N] = glr_seqs(x, cu_seqlens);
+  const int64_t D = x.size(2), total = x.size(0) * x.size(1);
+  auto h0 = glr_state(initial_state, x, N, "initial_state");
+  int64_t px, pa, pb;
+  auto xr = pitched_rows(x, px), ar = pitched_rows(a, pa), br = pitched_rows(b, pb);
+  auto l = lam.contiguous();
+  const auto f32 = x.options().dtype(torch::kFloat32);
+  auto y = torch::empty(x.sizes(), x.options());
+  torch::Tensor fin, states;
+  if (output_final_state) fin = torch::empty({N, D}, f32);
+  if (output_states) states = torch::empty({(total + XK_GLR_WINDOW - 1) / XK_GLR_WINDOW, D}, f32);
+  const int64_t bytes = xk_gated_linear_recurrence_workspace_bytes(total, D);
+  torch::Tensor ws;
+  if (bytes > 0) ws = workspace(bytes, x.device());
+  check(xk_gated_linear_recurrence(xr.data_ptr(), px, ar.data_ptr(), pa, br.data_ptr(), pb,
+                                   xdt(x), fptr(l), static_cast<float>(c), y.data_ptr(), D,
+                                   fptr(h0), fptr(fin), fptr(states), ptr(cu), cu.defined() ? xdt(cu) : XK_I32, N,
+                                   total, D, mptr(ws), static_cast<size_t>(bytes), stream),
+        "xk_gated_linear_recurrence");
+  return {y, given(fin), given(states)};
+}
+
+torch::Tensor npu_gated_linear_recurrence_update(
+    const torch::Tensor& x, const torch::Tensor& a, const torch::Tensor& b,
+    const torch::Tensor& lam, torch::Tensor& state, double c,
+    const std::optional<torch::Tensor>& state_indices,
+    const std::optional<torch::Tensor>& num_accepted_tokens,
+    const std::optional<torch::Tensor>& cu_seqlens) {
+  TORCH_CHECK(x.dim() == 2 || x.dim() == 3,
+              "gated_linear_recurrence_update expects x [B, D] or [B, T, D]");
+  glr_check(x, a, b, lam, c);
+  const int64_t D = x.size(-1), T = x.dim() == 3 ? x.size(1) : 1, total = x.size(0) * T;
+  TORCH_CHECK(state.scalar_type() == torch::kFloat32 && state.dim() == 2 && state.size(1) == D,
+              "state must be float32 [slots, D]");
+  TORCH_CHECK((D == 1 || state.stride(1) == 1) && (state.size(0) <= 1 || state.stride(0) >= D),
+              "state must have rows of contiguous channels");
+  same_device(state, x, "state");
+  int64_t N = x.size(0);
+  torch::Tensor cu, idx, acc;
+  if (has(cu_seqlens)) std::tie(cu, N) = glr_seqs(x, cu_seqlens);
+  int64_t cols = 0;
+  if (has(state_indices)) {
+    TORCH_CHECK(state_indices->scalar_type() == torch::kInt32 &&
+                    (state_indices->dim() == 1 || state_indices->dim() == 2) &&
+                    state_indices->size(0) == N,
+                "state_indices must be int32 [N] or [N, columns]");
+    same_device(*state_indices, x, "state_indices");
+    idx = state_indices->contiguous();
+    if (idx.dim() == 2) {
+      cols = idx.size(1);
+      TORCH_CHECK(cols > 0, "state_indices must have a column");
+    }
+  } else {
+    TORCH_CHECK(state.size(0) >= N, "state must have a slot for every sequence");
+  }
+  if (has(num_accepted_tokens)) {
+    TORCH_CHECK(num_accepted_tokens->scalar_type() == torch::kInt32 &&
+                    num_accepted_tokens->dim() == 1 && num_accepted_tokens->size(0) == N,
+                "num_accepted_tokens must be int32 [N]");
+    TORCH_CHECK(cols > 0, "num_accepted_tokens needs state_indices [N, columns]");
+    same_device(*num_accepted_tokens, x, "num_accepted_tokens");
+    acc = num_accepted_tokens->contiguous();
+  }
+  void* stream = stream_of(x);
+  c10::DeviceGuard guard(x.device());
+  int64_t px, pa, pb;
+  auto xr = pitched_rows(x, px), ar = pitched_rows(a, pa), br = pitched_rows(b, pb);
+  auto l = lam.contiguous();
+  auto y = torch::empty(x.sizes(), x.options());
+  if (total == 0) return y;
+  check(xk_gated_linear_recurrence_update(
+            xr.data_ptr(), px, ar.data_ptr(), pa, br.data_ptr(), pb, xdt(x), fptr(l),
+            static_cast<float>(c), y.data_ptr(), D, fptr(state),
+            state.size(0) > 1 ? state.stride(0) : D, state.size(0),
+            static_cast<const int32_t*>(ptr(idx)), cols,
+            static_cast<const int32_t*>(ptr(acc)), ptr(cu), cu.defined() ? xdt(cu) : XK_I32, N,
+            T, total, D, stream),
+        "xk_gated_linear_recurrence_update");
+  return y;
+}
+
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor>
+npu_gated_linear_recurrence_bwd(const torch::Tensor& dy, const torch::Tensor& x,
+                                const torch::Tensor& a, const torch::Tensor& b,
+                                const torch::Tensor& lam, const torch::Tensor& states, double c,
+                                const std::optional<torch::Tensor>& initial_state,
+                                const std::optional<torch::Tensor>& d_final_state,
+                                const std::optional<torch::Tensor>& cu_seqlens) {
+  TORCH_CHECK(x.dim() == 3, "gated_linear_recurrence_bwd expects x [B, T, D]");
+  glr_check(x, a, b, lam, c);
+  TORCH_CHECK(dy.sizes() == x.sizes() && dy.scalar_type() == x.scalar_type(),
+              "dy must have x's shape and dtype");
+  same_device(dy, x, "dy");
+  const int64_t D = x.size(2), total = x.size(0) * x.size(1);
+  TORCH_CHECK(states.scalar_type() == torch::kFloat32 && states.dim() == 2 &&
+                  states.size(0) == (total + XK_GLR_WINDOW - 1) / XK_GLR_WINDOW &&
+                  states.size(1) == D,
+              "states must be the forward call's (float32 [ceil(tokens / ", XK_GLR_WINDOW,
+              "), D])");
+  same_device(states, x, "states");
+  void* stream = stream_of(x);
+  c10::DeviceGuard guard(x.device());
+  auto [cu, N] = glr_seqs(x, cu_seqlens);
+  auto h0 = glr_state(initial_state, x, N, "initial_state");
+  auto df = glr_state(d_final_state, x, N, "d_final_state");
+  int64_t pd, px, pa, pb;
+  auto dr = pitched_rows(dy, pd), xr = pitched_rows(x, px), ar = pitched_rows(a, pa),
+       br = pitched_rows(b, pb);
+  auto l = lam.contiguous(), st = states.contiguous();
+  const auto f32 = x.options().dtype(torch::kFloat32);
+  auto dx = torch::empty(x.sizes(), x.options()), da = torch::empty(x.sizes(), x.options()),
+       db = torch::empty(x.sizes(), x.options());
+  auto dlam = torch::empty({D}, f32), dh0 = torch::empty({N, D}, f32);
+  const int64_t bytes = xk_gated_linear_recurrence_bwd_workspace_bytes(total, N, D);
+  auto ws = workspace(bytes, x.device());
+  check(xk_gated_linear_recurrence_bwd(
+            dr.data_ptr(), pd, xr.data_ptr(), px, ar.data_ptr(), pa, br.data_ptr(), pb, xdt(x),
+            fptr(l), static_cast<float>(c), fptr(st), fptr(h0), fptr(df), dx.data_ptr(), D,
+            da.data_ptr(), D, db.data_ptr(), D, fptr(dlam), fptr(dh0), ptr(cu),
+            cu.defined() ? xdt(cu) : XK_I32, N, total, D, ws.data_ptr(), static_cast<size_t>(bytes), stream),
+        "xk_gated_linear_recurrence_bwd");
+  return {dx, da, db, dlam, dh0};
+}
+
+namespace {
+
+// What both directions of the block-to-block norm check: x [..., N] and its
+// companions.  The weights' dtype (x's where there is no weight).
+torch::ScalarType grn_check(const torch::Tensor& x, const torch::Tensor& residual,
+                            const std::optional<torch::Tensor>& post_weight,
+                            const std::optional<torch::Tensor>& gate,
+                            const std::optional<torch::Tensor>& scale,
+                            const std::optional<torch::Tensor>& pre_weight) {
+  TORCH_CHECK(x.dim() >= 1 && x.size(-1) > 0, "gated_residual_rms_norm expects x [..., N]");
+  TORCH_CHECK(x.scalar_type() == torch::kFloat32 || x.scalar_type() == torch::kBFloat16 ||
+                  x.scalar_type() == torch::kFloat16,
+              "x must be float32, bfloat16 or float16");
+  TORCH_CHECK(residual.sizes() == x.sizes() &&
+                  (residual.scalar_type() == x.scalar_type() ||
+                   residual.scalar_type() == torch::kFloat32),
+              "residual must have x's shape, and x's dtype or float32");
+  same_device(residual, x, "residual");
+  if (has(gate)) {
+    TORCH_CHECK(gate->sizes() == x.sizes() && gate->scalar_type() == x.scalar_type(),
+                "gate must have x's shape and dtype");
+    same_device(*gate, x, "gate");
+  }
+  std::optional<torch::ScalarType> wt;
+  for (const auto& [w, name] : {std::make_pair(&post_weight, "post_weight"),
+                                std::make_pair(&scale, "scale"),
+                                std::make_pair(&pre_weight, "pre_weight")}) {
+    if (!has(*w)) continue;
+    const auto& t = **w;
+    TORCH_CHECK(t.dim() == 1 && t.size(0) == x.size(-1), name, " must be [N]");
+    TORCH_CHECK(t.scalar_type() == x.scalar_type() || t.scalar_type() == torch::kFloat32, name,
+                " must have x's dtype or float32");
+    TORCH_CHECK(!wt || *wt == t.scalar_type(), "the weights must have one dtype");
+    wt = t.scalar_type();
+    same_device(t, x, name);
+  }
+  return wt.value_or(x.scalar_type());
+}
+
+xk_dtype xdt_of(torch::ScalarType t) {
+  return t == torch::kFloat32 ? XK_F32 : (t == torch::kBFloat16 ? XK_BF16 : XK_F16);
+}
+
+torch::Tensor weight_of(const std::optional<torch::Tensor>& w) {
+  return has(w) ? w->contiguous() : torch::Tensor();
+}
+
+}  // namespace
+
+std::tuple<torch::Tensor, std::optional<torch::Tensor>, std::optional<torch::Tensor>,
+           std::optional<torch::Tensor>>
+npu_gated_residual_rms_norm(const torch::Tensor& x, const torch::Tensor& residual,
+                            const std::optional<torch::Tensor>& post_weight,
+                            const std::optional<torch::Tensor>& gate,
+                            const std::optional<torch::Tensor>& scale,
+                            const std::optional<torch::Tensor>& pre_weight, double eps,
+                            bool unit_offset) {
+  const auto wt = grn_check(x, residual, post_weight, gate, scale, pre_weight);
+  TORCH_CHECK(eps >= 0, "eps must not be negative");
+  void* stream = stream_of(x);
+  c10::DeviceGuard guard(x.device());
+  const int64_t N = x.size(-1), M = x.numel() / N;
+  int64_t px, pr, pz = N;
+  auto xr = pitched_rows(x, px), rr = pitched_rows(residual, pr);
+  torch::Tensor zr;
+  if (has(gate)) zr = pitched_rows(*gate, pz);
+  auto post = weight_of(post_weight), sc = weight_of(scale), pre = weight_of(pre_weight);
+  const auto f32 = x.options().dtype(torch::kFloat32);
+  auto h = torch::empty(x.sizes(), residual.options());
+  torch::Tensor y, r1, r2;
+  const auto lead = x.sizes().slice(0, x.dim() - 1);
+  if (post.defined()) r1 = torch::empty(lead, f32);
+  if (pre.defined()) {
+    y = torch::empty(x.sizes(), x.options());
+    r2 = torch::empty(lead, f32);
+  }
+  check(xk_gated_residual_rms_norm(xr.data_ptr(), px, rr.data_ptr(), pr, ptr(zr), pz, ptr(post),
+                                   ptr(sc), ptr(pre), h.data_ptr(), N, mptr(y), N, fptr(r1),
+                                   fptr(r2), M, N, static_cast<float>(eps), unit_offset, xdt(x),
+                                   xdt(residual), xdt_of(wt), stream),
+        "xk_gated_residual_rms_norm");
+  return {h, given(y), given(r1), given(r2)};
+}
+
+std::tuple<torch::Tensor, torch::Tensor, std::optional<torch::Tensor>,
+           std::optional<torch::Tensor>, std::optional<torch::Tensor>,
+           std::optional<torch::Tensor>>
+npu_gated_residual_rms_norm_bwd(const std::optional<torch::Tensor>& dh,
+                                const std::optional<torch::Tensor>& dy, const torch::Tensor& x,
+                                const torch::Tensor& residual,
+                                const std::optional<torch::Tensor>& rstd_post,
+                                const std::optional<torch::Tensor>& rstd_pre,
+                                const std::optional<torch::Tensor>& post_weight,
+                                const std::optional<torch::Tensor>& gate,
+                                const std::optional<torch::Tensor>& scale,
+                                const std::optional<torch::Tensor>& pre_weight,
+                                bool unit_offset) {
+  const auto wt = grn_check(x, residual, post_weight, gate, scale, pre_weight);
+  TORCH_CHECK(has(dh) || has(dy), "gated_residual_rms_norm_bwd needs dh or dy");
+  TORCH_CHECK(!has(dy) || has(pre_weight), "dy needs pre_weight");
+  if (has(dh)) {
+    TORCH_CHECK(dh->sizes() == x.sizes() && dh->scalar_type() == residual.scalar_type(),
+                "dh must have x's shape and residual's dtype");
+    same_device(*dh, x, "dh");
+  }
+  if (has(dy)) {
+    TORCH_CHECK(dy->sizes() == x.sizes() && dy->scalar_type() == x.scalar_type(),
+                "dy must have x's shape and dtype");
+    same_device(*dy, x, "dy");
+  }
+  const int64_t N = x.size(-1), M = x.numel() / N;
+  torch::Tensor r1, r2;
+  for (const auto& [need, r, to, name] :
+       {std::make_tuple(has(post_weight), &rstd_post, &r1, "rstd_post"),
+        std::make_tuple(has(dy), &rstd_pre, &r2, "rstd_pre")}) {
+    if (!need) continue;
+    TORCH_CHECK(has(*r) && (*r)->scalar_type() == torch::kFloat32 && (*r)->numel() == M, name,
+                " must be the forward call's");
+    same_device(**r, x, name);
+    *to = (*r)->contiguous();
+  }
+  void* stream = stream_of(x);
+  c10::DeviceGuard guard(x.device());
+  int64_t px, pr, pz = N, pdh = N, pdy = N;
+  auto xr = pitched_rows(x, px), rr = pitched_rows(residual, pr);
+  torch::Tensor zr, dhr, dyr, dgate, dpost, dscale, dpre, ws;
+  if (has(gate)) {
+    zr = pitched_rows(*gate, pz);
+    dgate = torch::empty(x.sizes(), x.options());
+  }
+  if (has(dh)) dhr = pitched_rows(*dh, pdh);
+  if (has(dy)) dyr = pitched_rows(*dy, pdy);
+  auto post = weight_of(post_weight), sc = weight_of(scale), pre = weight_of(pre_weight);
+  if (post.defined()) dpost = torch::empty_like(post);
+  if (sc.defined()) dscale = torch::empty_like(sc);
+  if (pre.defined()) dpre = torch::empty_like(pre);
+  auto dx = torch::empty(x.sizes(), x.options());
+  auto dres = torch::empty(x.sizes(), residual.options());
+  int64_t bytes = 0;
+  if (post.defined() || sc.defined() || pre.defined()) {
+    bytes = xk_gated_residual_rms_norm_bwd_workspace_bytes(M, N);
+    ws = workspace(bytes, x.device());
+  }
+  check(xk_gated_residual_rms_norm_bwd(
+            ptr(dhr), pdh, ptr(dyr), pdy, xr.data_ptr(), px, rr.data_ptr(), pr, ptr(zr), pz,
+            ptr(post), ptr(sc), ptr(pre), fptr(r1), fptr(r2), dx.data_ptr(), N, dres.data_ptr(),
+            N, mptr(dgate), N, mptr(dpost), mptr(dscale), mptr(dpre), M, N, unit_offset, xdt(x),
+            xdt(residual), xdt_of(wt), mptr(ws), static_cast<size_t>(bytes), stream),
+        "xk_gated_residual_rms_norm_bwd");
+  return {dx, dres, given(dgate), given(dpost), given(dscale), given(dpre)};
 }
 
 }  // namespace xllm::kernel::npu

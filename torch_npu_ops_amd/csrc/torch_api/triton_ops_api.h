@@ -159,4 +159,74 @@ torch::Tensor npu_gdn_conv_sigmoid_gating_decode(
     int32_t pad_slot_id = -1, float softplus_beta = 1.0f, float softplus_threshold = 20.0f,
     bool use_qk_l2norm = true);
 
+// Gated linear recurrence (xk_gated_linear_recurrence, whose comment in
+// xk_ops.h has the formulas): x, a, b [B, T, D] of one dtype (fp32, bf16 or
+// fp16), lam fp32 [D].  Sequences are the B rows, or cu_seqlens
+// (int32/int64 on x's device) over the B * T tokens.  initial_state and the
+// final state are fp32 [N, D].  Views whose tokens have one pitch (a and b as
+// halves of one product's rows) are read in place.  Returns (y, final state
+// if asked for, states if asked for: what the backward pass needs).
+std::tuple<torch::Tensor, std::optional<torch::Tensor>, std::optional<torch::Tensor>>
+npu_gated_linear_recurrence(const torch::Tensor& x, const torch::Tensor& a,
+                            const torch::Tensor& b, const torch::Tensor& lam, double c = 8.0,
+                            const std::optional<torch::Tensor>& initial_state = std::nullopt,
+                            bool output_final_state = false,
+                            const std::optional<torch::Tensor>& cu_seqlens = std::nullopt,
+                            bool output_states = false);
+
+// One token, or a few drafted ones, of every sequence on a pool of states
+// (fp32 [slots, D], updated in place): x, a, b [B, D] or [B, T, D], or, with
+// cu_seqlens, [1, tokens, D].  state_indices int32 [N] or [N, columns], a
+// column for the state after each token; num_accepted_tokens int32 [N].
+// Returns y, shaped like x.
+torch::Tensor npu_gated_linear_recurrence_update(
+    const torch::Tensor& x, const torch::Tensor& a, const torch::Tensor& b,
+    const torch::Tensor& lam, torch::Tensor& state, double c = 8.0,
+    const std::optional<torch::Tensor>& state_indices = std::nullopt,
+    const std::optional<torch::Tensor>& num_accepted_tokens = std::nullopt,
+    const std::optional<torch::Tensor>& cu_seqlens = std::nullopt);
+
+// Gradients of npu_gated_linear_recurrence for its arguments and the states
+// it returned: (dx, da, db, dlam fp32 [D], d_initial_state fp32 [N, D]).
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor>
+npu_gated_linear_recurrence_bwd(const torch::Tensor& dy, const torch::Tensor& x,
+                                const torch::Tensor& a, const torch::Tensor& b,
+                                const torch::Tensor& lam, const torch::Tensor& states,
+                                double c = 8.0,
+                                const std::optional<torch::Tensor>& initial_state = std::nullopt,
+                                const std::optional<torch::Tensor>& d_final_state = std::nullopt,
+                                const std::optional<torch::Tensor>& cu_seqlens = std::nullopt);
+
+// From one block to the next (xk_gated_residual_rms_norm): RMSNorm of the
+// block's output x by post_weight, its SiLU gate, its scale per channel, the
+// residual sum h, and the RMSNorm y of h by pre_weight; a part that is not
+// given is left out.  x and gate of one dtype, residual that dtype or fp32,
+// the weights of one dtype (x's or fp32).  Returns (h, y, rstd_post,
+// rstd_pre), the last three where their norm runs.
+std::tuple<torch::Tensor, std::optional<torch::Tensor>, std::optional<torch::Tensor>,
+           std::optional<torch::Tensor>>
+npu_gated_residual_rms_norm(const torch::Tensor& x, const torch::Tensor& residual,
+                            const std::optional<torch::Tensor>& post_weight = std::nullopt,
+                            const std::optional<torch::Tensor>& gate = std::nullopt,
+                            const std::optional<torch::Tensor>& scale = std::nullopt,
+                            const std::optional<torch::Tensor>& pre_weight = std::nullopt,
+                            double eps = 1e-6, bool unit_offset = false);
+
+// Its gradients (dx, dresidual, dgate, dpost_weight, dscale, dpre_weight),
+// those of parts that were given.  dh and dy are the gradients of h and y;
+// either may be left out.
+std::tuple<torch::Tensor, torch::Tensor, std::optional<torch::Tensor>,
+           std::optional<torch::Tensor>, std::optional<torch::Tensor>,
+           std::optional<torch::Tensor>>
+npu_gated_residual_rms_norm_bwd(const std::optional<torch::Tensor>& dh,
+                                const std::optional<torch::Tensor>& dy, const torch::Tensor& x,
+                                const torch::Tensor& residual,
+                                const std::optional<torch::Tensor>& rstd_post,
+                                const std::optional<torch::Tensor>& rstd_pre,
+                                const std::optional<torch::Tensor>& post_weight = std::nullopt,
+                                const std::optional<torch::Tensor>& gate = std::nullopt,
+                                const std::optional<torch::Tensor>& scale = std::nullopt,
+                                const std::optional<torch::Tensor>& pre_weight = std::nullopt,
+                                bool unit_offset = false);
+
 }  // namespace xllm::kernel::npu

@@ -932,3 +932,331 @@ def npu_l2norm_last_dim(x: torch.Tensor, eps: float = 1e-6,
                                   xk_dtype(y), _stream(x))
     check(st, "xk_l2norm_last_dim")
     return y
+
+
+# ---------------------------------------------------------------------------
+# Gated linear recurrence and the block-to-block norm (no reference
+# counterpart; the same calls as npu_gated_* of csrc/torch_api)
+# ---------------------------------------------------------------------------
+_FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def _same_device(x, **others):
+    for name, t in others.items():
+        if t is not None and t.device != x.device:
+            raise ValueError(f"{name} must be on {x.device}, is on {t.device}")
+
+
+def _pitched_rows(x: torch.Tensor):
+    """(x as rows of its last dim with one pitch between them, a copy only if
+    it has no such form; the pitch in elements)."""
+    D = x.size(-1)
+    pitch, count, ok = D, 1, D == 1 or x.stride(-1) == 1
+    for d in range(x.dim() - 2, -1, -1):
+        if not ok or x.size(d) == 1:
+            continue
+        if count == 1:
+            pitch = x.stride(d)
+            ok = pitch >= D
+        else:
+            ok = x.stride(d) == pitch * count
+        count *= x.size(d)
+    return (x, pitch) if ok else (x.contiguous(), D)
+
+
+def _glr_check(x, a, b, lam, c):
+    for t, name in ((a, "a"), (b, "b")):
+        if t.shape != x.shape or t.dtype != x.dtype:
+            raise ValueError(f"{name} must have x's shape and dtype")
+    if x.dtype not in _FLOATS:
+        raise ValueError("x must be float32, bfloat16 or float16")
+    if x.size(-1) == 0:
+        raise ValueError("x must have channels")
+    if lam.dtype != torch.float32 or lam.shape != (x.size(-1),):
+        raise ValueError("lam must be float32 [D]")
+    if not (c >= 0 and math.isfinite(c)):
+        raise ValueError("c must be finite and not negative")
+    _same_device(x, a=a, b=b, lam=lam)
+
+
+def _glr_seqs(x, cu_seqlens):
+    if cu_seqlens is None:
+        return None, x.size(0)
+    if (cu_seqlens.dtype not in (torch.int32, torch.int64) or cu_seqlens.dim() != 1
+            or cu_seqlens.numel() < 1):
+        raise ValueError("cu_seqlens must be int32 or int64 [N + 1]")
+    _same_device(x, cu_seqlens=cu_seqlens)
+    return cu_seqlens.contiguous(), cu_seqlens.numel() - 1
+
+
+def _glr_state(s, x, N, name):
+    if s is None:
+        return None
+    if s.dtype != torch.float32 or s.shape != (N, x.size(-1)):
+        raise ValueError(f"{name} must be float32 [N, D]")
+    _same_device(x, **{name: s})
+    return s.contiguous()
+
+
+def npu_gated_linear_recurrence(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
+                                lam: torch.Tensor, c: float = 8.0,
+                                initial_state: Optional[torch.Tensor] = None,
+                                output_final_state: bool = False,
+                                cu_seqlens: Optional[torch.Tensor] = None,
+                                output_states: bool = False):
+    """h_t = alpha_t h_{t-1} + sqrt(1 - alpha_t^2) sigmoid(b_t) x_t per
+    channel, alpha_t = exp(-c softplus(lam) sigmoid(a_t)); returns (y = h in
+    x's dtype, final state or None, states or None).
+
+    x, a, b [B, T, D] (fp32, bf16 or fp16), lam fp32 [D]; sequences are the B
+    rows, or cu_seqlens (int32/int64) over the B * T tokens; states are fp32
+    [N, D].  ``output_states`` returns what npu_gated_linear_recurrence_bwd
+    starts from.  Views whose tokens have one pitch are read in place.
+    """
+    if x.dim() != 3:
+        raise ValueError("gated_linear_recurrence expects x [B, T, D]")
+    _glr_check(x, a, b, lam, c)
+    stream = _stream(x)
+    cu, N = _glr_seqs(x, cu_seqlens)
+    D, total = x.size(2), x.size(0) * x.size(1)
+    h0 = _glr_state(initial_state, x, N, "initial_state")
+    (xr, px), (ar, pa), (br, pb) = _pitched_rows(x), _pitched_rows(a), _pitched_rows(b)
+    lam = lam.contiguous()
+    with torch.cuda.device(x.device):
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        fin = torch.empty(N, D, device=x.device) if output_final_state else None
+        states = (torch.empty(-(-total // _lib.XK_GLR_WINDOW), D, device=x.device)
+                  if output_states else None)
+        size = lib().xk_gated_linear_recurrence_workspace_bytes(total, D)
+        ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+        st = lib().xk_gated_linear_recurrence(
+            xr.data_ptr(), px, ar.data_ptr(), pa, br.data_ptr(), pb, xk_dtype(x),
+            lam.data_ptr(), float(c), y.data_ptr(), D, _ptr(h0), _ptr(fin), _ptr(states),
+            _ptr(cu), xk_dtype(cu) if cu is not None else _lib.XK_I32, N, total, D, _ptr(ws),
+            size, stream)
+    check(st, "xk_gated_linear_recurrence")
+    return y, fin, states
+
+
+def npu_gated_linear_recurrence_update(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
+                                       lam: torch.Tensor, state: torch.Tensor, c: float = 8.0,
+                                       state_indices: Optional[torch.Tensor] = None,
+                                       num_accepted_tokens: Optional[torch.Tensor] = None,
+                                       cu_seqlens: Optional[torch.Tensor] = None):
+    """The recurrence's decode step on a pool of states (fp32 [slots, D],
+    updated in place); returns y shaped like x.
+
+    x, a, b [B, D] or [B, T, D], or with cu_seqlens [1, tokens, D].
+    state_indices int32 [N] (one slot a sequence) or [N, columns] (a slot for
+    the state after each token; a sequence starts from column
+    num_accepted_tokens - 1, or 0).  A slot outside the pool starts from zero
+    and is not written.
+    """
+    if x.dim() not in (2, 3):
+        raise ValueError("gated_linear_recurrence_update expects x [B, D] or [B, T, D]")
+    _glr_check(x, a, b, lam, c)
+    D, T = x.size(-1), x.size(1) if x.dim() == 3 else 1
+    total = x.size(0) * T
+    if state.dtype != torch.float32 or state.dim() != 2 or state.size(1) != D:
+        raise ValueError("state must be float32 [slots, D]")
+    if (D != 1 and state.stride(1) != 1) or (state.size(0) > 1 and state.stride(0) < D):
+        raise ValueError("state must have rows of contiguous channels")
+    cu, N = _glr_seqs(x, cu_seqlens)
+    idx, cols, acc = None, 0, None
+    if state_indices is not None:
+        if (state_indices.dtype != torch.int32 or state_indices.dim() not in (1, 2)
+                or state_indices.size(0) != N):
+            raise ValueError("state_indices must be int32 [N] or [N, columns]")
+        idx = state_indices.contiguous()
+        if idx.dim() == 2:
+            cols = idx.size(1)
+            if cols == 0:
+                raise ValueError("state_indices must have a column")
+    elif state.size(0) < N:
+        raise ValueError("state must have a slot for every sequence")
+    if num_accepted_tokens is not None:
+        if num_accepted_tokens.dtype != torch.int32 or num_accepted_tokens.shape != (N,):
+            raise ValueError("num_accepted_tokens must be int32 [N]")
+        if cols == 0:
+            raise ValueError("num_accepted_tokens needs state_indices [N, columns]")
+        acc = num_accepted_tokens.contiguous()
+    _same_device(x, state=state, state_indices=idx, num_accepted_tokens=acc)
+    stream = _stream(x)
+    (xr, px), (ar, pa), (br, pb) = _pitched_rows(x), _pitched_rows(a), _pitched_rows(b)
+    lam = lam.contiguous()
+    with torch.cuda.device(x.device):
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        if total == 0:
+            return y
+        st = lib().xk_gated_linear_recurrence_update(
+            xr.data_ptr(), px, ar.data_ptr(), pa, br.data_ptr(), pb, xk_dtype(x),
+            lam.data_ptr(), float(c), y.data_ptr(), D, state.data_ptr(),
+            state.stride(0) if state.size(0) > 1 else D, state.size(0), _ptr(idx), cols,
+            _ptr(acc), _ptr(cu), xk_dtype(cu) if cu is not None else _lib.XK_I32, N, T, total,
+            D, stream)
+    check(st, "xk_gated_linear_recurrence_update")
+    return y
+
+
+def npu_gated_linear_recurrence_bwd(dy: torch.Tensor, x: torch.Tensor, a: torch.Tensor,
+                                    b: torch.Tensor, lam: torch.Tensor, states: torch.Tensor,
+                                    c: float = 8.0,
+                                    initial_state: Optional[torch.Tensor] = None,
+                                    d_final_state: Optional[torch.Tensor] = None,
+                                    cu_seqlens: Optional[torch.Tensor] = None):
+    """Gradients (dx, da, db, dlam fp32 [D], d_initial_state fp32 [N, D]) of
+    npu_gated_linear_recurrence for its arguments and the states it returned."""
+    if x.dim() != 3:
+        raise ValueError("gated_linear_recurrence_bwd expects x [B, T, D]")
+    _glr_check(x, a, b, lam, c)
+    if dy.shape != x.shape or dy.dtype != x.dtype:
+        raise ValueError("dy must have x's shape and dtype")
+    D, total = x.size(2), x.size(0) * x.size(1)
+    if (states.dtype != torch.float32
+            or states.shape != (-(-total // _lib.XK_GLR_WINDOW), D)):
+        raise ValueError("states must be the forward call's")
+    _same_device(x, dy=dy, states=states)
+    stream = _stream(x)
+    cu, N = _glr_seqs(x, cu_seqlens)
+    h0 = _glr_state(initial_state, x, N, "initial_state")
+    df = _glr_state(d_final_state, x, N, "d_final_state")
+    (dr, pd), (xr, px) = _pitched_rows(dy), _pitched_rows(x)
+    (ar, pa), (br, pb) = _pitched_rows(a), _pitched_rows(b)
+    lam, states = lam.contiguous(), states.contiguous()
+    with torch.cuda.device(x.device):
+        dx, da, db = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for _ in range(3))
+        dlam, dh0 = torch.empty(D, device=x.device), torch.empty(N, D, device=x.device)
+        size = lib().xk_gated_linear_recurrence_bwd_workspace_bytes(total, N, D)
+        ws = torch.empty(max(size, 1), dtype=torch.uint8, device=x.device)
+        st = lib().xk_gated_linear_recurrence_bwd(
+            dr.data_ptr(), pd, xr.data_ptr(), px, ar.data_ptr(), pa, br.data_ptr(), pb,
+            xk_dtype(x), lam.data_ptr(), float(c), states.data_ptr(), _ptr(h0), _ptr(df),
+            dx.data_ptr(), D, da.data_ptr(), D, db.data_ptr(), D, dlam.data_ptr(),
+            dh0.data_ptr(), _ptr(cu), xk_dtype(cu) if cu is not None else _lib.XK_I32, N, total,
+            D, ws.data_ptr(), size, stream)
+    check(st, "xk_gated_linear_recurrence_bwd")
+    return dx, da, db, dlam, dh0
+
+
+def _grn_check(x, residual, post_weight, gate, scale, pre_weight):
+    """Checks shared by both directions; returns the weights' dtype."""
+    if x.dim() < 1 or x.size(-1) == 0:
+        raise ValueError("gated_residual_rms_norm expects x [..., N]")
+    if x.dtype not in _FLOATS:
+        raise ValueError("x must be float32, bfloat16 or float16")
+    if residual.shape != x.shape or residual.dtype not in (x.dtype, torch.float32):
+        raise ValueError("residual must have x's shape, and x's dtype or float32")
+    if gate is not None and (gate.shape != x.shape or gate.dtype != x.dtype):
+        raise ValueError("gate must have x's shape and dtype")
+    wt = None
+    for w, name in ((post_weight, "post_weight"), (scale, "scale"), (pre_weight, "pre_weight")):
+        if w is None:
+            continue
+        if w.shape != (x.size(-1),):
+            raise ValueError(f"{name} must be [N]")
+        if w.dtype not in (x.dtype, torch.float32):
+            raise ValueError(f"{name} must have x's dtype or float32")
+        if wt not in (None, w.dtype):
+            raise ValueError("the weights must have one dtype")
+        wt = w.dtype
+    _same_device(x, residual=residual, gate=gate, post_weight=post_weight, scale=scale,
+                 pre_weight=pre_weight)
+    return wt or x.dtype
+
+
+def _contig(t):
+    return None if t is None else t.contiguous()
+
+
+def npu_gated_residual_rms_norm(x: torch.Tensor, residual: torch.Tensor,
+                                post_weight: Optional[torch.Tensor] = None,
+                                gate: Optional[torch.Tensor] = None,
+                                scale: Optional[torch.Tensor] = None,
+                                pre_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                                unit_offset: bool = False):
+    """h = residual + scale * (RMSNorm(x; post_weight) * silu(gate)) and y =
+    RMSNorm(h; pre_weight), parts that are not given left out; returns (h, y,
+    rstd_post, rstd_pre), the last three None where their norm does not run.
+
+    x, gate [..., N] of one dtype, residual (and h) that dtype or fp32, the
+    weights [N] of one dtype (x's or fp32).  ``unit_offset`` multiplies by
+    (1 + weight) in both norms.  y is formed from h before its rounding.
+    """
+    wt = _grn_check(x, residual, post_weight, gate, scale, pre_weight)
+    if not eps >= 0:
+        raise ValueError("eps must not be negative")
+    stream = _stream(x)
+    N = x.size(-1)
+    M = x.numel() // N
+    (xr, px), (rr, pr) = _pitched_rows(x), _pitched_rows(residual)
+    zr, pz = _pitched_rows(gate) if gate is not None else (None, N)
+    post, sc, pre = _contig(post_weight), _contig(scale), _contig(pre_weight)
+    with torch.cuda.device(x.device):
+        h = torch.empty(x.shape, dtype=residual.dtype, device=x.device)
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if pre is not None else None
+        r1 = torch.empty(x.shape[:-1], device=x.device) if post is not None else None
+        r2 = torch.empty(x.shape[:-1], device=x.device) if pre is not None else None
+        st = lib().xk_gated_residual_rms_norm(
+            xr.data_ptr(), px, rr.data_ptr(), pr, _ptr(zr), pz, _ptr(post), _ptr(sc), _ptr(pre),
+            h.data_ptr(), N, _ptr(y), N, _ptr(r1), _ptr(r2), M, N, float(eps),
+            int(unit_offset), xk_dtype(x), xk_dtype(residual), _DT[wt], stream)
+    check(st, "xk_gated_residual_rms_norm")
+    return h, y, r1, r2
+
+
+def npu_gated_residual_rms_norm_bwd(dh: Optional[torch.Tensor], dy: Optional[torch.Tensor],
+                                    x: torch.Tensor, residual: torch.Tensor,
+                                    rstd_post: Optional[torch.Tensor],
+                                    rstd_pre: Optional[torch.Tensor],
+                                    post_weight: Optional[torch.Tensor] = None,
+                                    gate: Optional[torch.Tensor] = None,
+                                    scale: Optional[torch.Tensor] = None,
+                                    pre_weight: Optional[torch.Tensor] = None,
+                                    unit_offset: bool = False):
+    """Gradients (dx, dresidual, dgate, dpost_weight, dscale, dpre_weight) of
+    npu_gated_residual_rms_norm, None for parts that were not given; dh and
+    dy are the gradients of h and y, either may be None."""
+    wt = _grn_check(x, residual, post_weight, gate, scale, pre_weight)
+    if dh is None and dy is None:
+        raise ValueError("gated_residual_rms_norm_bwd needs dh or dy")
+    if dy is not None and pre_weight is None:
+        raise ValueError("dy needs pre_weight")
+    if dh is not None and (dh.shape != x.shape or dh.dtype != residual.dtype):
+        raise ValueError("dh must have x's shape and residual's dtype")
+    if dy is not None and (dy.shape != x.shape or dy.dtype != x.dtype):
+        raise ValueError("dy must have x's shape and dtype")
+    N = x.size(-1)
+    M = x.numel() // N
+    r1 = r2 = None
+    if post_weight is not None:
+        if rstd_post is None or rstd_post.dtype != torch.float32 or rstd_post.numel() != M:
+            raise ValueError("rstd_post must be the forward call's")
+        r1 = rstd_post.contiguous()
+    if dy is not None:
+        if rstd_pre is None or rstd_pre.dtype != torch.float32 or rstd_pre.numel() != M:
+            raise ValueError("rstd_pre must be the forward call's")
+        r2 = rstd_pre.contiguous()
+    _same_device(x, dh=dh, dy=dy, rstd_post=r1, rstd_pre=r2)
+    stream = _stream(x)
+    (xr, px), (rr, pr) = _pitched_rows(x), _pitched_rows(residual)
+    zr, pz = _pitched_rows(gate) if gate is not None else (None, N)
+    dhr, pdh = _pitched_rows(dh) if dh is not None else (None, N)
+    dyr, pdy = _pitched_rows(dy) if dy is not None else (None, N)
+    post, sc, pre = _contig(post_weight), _contig(scale), _contig(pre_weight)
+    with torch.cuda.device(x.device):
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        dres = torch.empty(x.shape, dtype=residual.dtype, device=x.device)
+        dgate = torch.empty_like(dx) if gate is not None else None
+        dpost, dscale, dpre = (None if w is None else torch.empty_like(w)
+                               for w in (post, sc, pre))
+        size, ws = 0, None
+        if post is not None or sc is not None or pre is not None:
+            size = lib().xk_gated_residual_rms_norm_bwd_workspace_bytes(M, N)
+            ws = torch.empty(max(size, 1), dtype=torch.uint8, device=x.device)
+        st = lib().xk_gated_residual_rms_norm_bwd(
+            _ptr(dhr), pdh, _ptr(dyr), pdy, xr.data_ptr(), px, rr.data_ptr(), pr, _ptr(zr), pz,
+            _ptr(post), _ptr(sc), _ptr(pre), _ptr(r1), _ptr(r2), dx.data_ptr(), N,
+            dres.data_ptr(), N, _ptr(dgate), N, _ptr(dpost), _ptr(dscale), _ptr(dpre), M, N,
+            int(unit_offset), xk_dtype(x), xk_dtype(residual), _DT[wt], _ptr(ws), size, stream)
+    check(st, "xk_gated_residual_rms_norm_bwd")
+    return dx, dres, dgate, dpost, dscale, dpre
