@@ -9,6 +9,8 @@
 // keeps nearly all of its state (alpha near 1, the case that matters).
 #include <math.h>
 
+#include <algorithm>
+
 #include "xk_common.h"
 
 namespace xk {
@@ -66,6 +68,9 @@ struct FwdParams {
   const void* cu;
   int cu64;
   int64_t N, T, total, D;
+  unsigned long long* words;  // [tiles][blocks * channels of a block]
+  unsigned int* ticket;
+  int blocks;
 };
 
 // First token of sequence n (N: the end); without cu_seqlens, N equal runs.
@@ -77,25 +82,414 @@ __device__ __forceinline__ int64_t cu_at(const void* cu, int cu64, int64_t n, in
   return v < 0 ? 0 : (v > total ? total : v);
 }
 
-// One lane per (sequence, channel), token by token.
-template <typename T>
-__global__ void __launch_bounds__(64) glr_fwd_kernel(FwdParams p) {
-  const int64_t ch = static_cast<int64_t>(blockIdx.x) * 64 + threadIdx.x;
-  const int64_t n = blockIdx.y;
-  if (ch >= p.D) return;
-  const int64_t t0 = cu_at(p.cu, p.cu64, n, p.T, p.total), t1 = cu_at(p.cu, p.cu64, n + 1, p.T, p.total);
-  const float k = -p.c * softplus_f32(p.lam[ch]);
-  float h = p.h0 ? p.h0[n * p.D + ch] : 0.f;
-  for (int64_t t = t0; t < t1; ++t) {
-    const float x = to_f32(static_cast<const T*>(p.x)[t * p.sx + ch]);
-    const float r = sigmoid(to_f32(static_cast<const T*>(p.a)[t * p.sa + ch]));
-    const float i = sigmoid(to_f32(static_cast<const T*>(p.b)[t * p.sb + ch]));
-    const Gate g = gate_of(k, r);
-    if (p.states && t % kWin == 0 && t != t0) p.states[t / kWin * p.D + ch] = h;
-    h = decayed(g.em1, h) + g.s * (i * x);
-    static_cast<T*>(p.y)[t * p.sy + ch] = from_f32<T>(h);
+// ---------------------------------------------------------------------------
+// Tiles.  The token axis of the whole batch is cut into windows of kTok tokens,
+// one per wave, and tiles of up to kMaxWaves windows, one per block; a lane
+// has VEC channels (4 bytes of a row), so a block covers 64 VEC channels.  A
+// window's tokens are read once and stay in registers as (alpha - 1, input).
+//
+// Any span of tokens maps the state before it to the state after it by
+// h -> A h + B, and a span in which a sequence starts maps every state to the
+// same one (the sequence's own start is part of its B): it is "final", marked
+// by A = -1.  A block joins its waves' spans in LDS.  Between tiles each block
+// publishes its span per channel as one 64-bit word (A, B), waits for the words
+// of the tiles before it, back to a final one, and once it knows the state
+// that enters it, replaces its own word by the final (-1, state).  The state
+// between tiles is always the chain H_k = fma(A_k, H_{k-1}, B_k), whoever
+// computes it and whichever final word it starts from, so the bits do not
+// depend on timing.
+//
+// A block takes its tile from a counter: a tile is waited for only by tiles
+// that were taken after it, so the one taken first of those that still run
+// never waits for a block that has not started, and every wait ends.  Words
+// and counter are cleared by a kernel before.  A word is one atomic access
+// and carries its own validity (kUnset is no pair that is published), so no
+// fences are needed.
+// ---------------------------------------------------------------------------
+constexpr int kTok = kWin;
+constexpr int kMaxWaves = 8;
+constexpr int kBack = 16;  // tiles before its own that a block looks at together
+constexpr unsigned long long kUnset = ~0ull;
+
+struct Span {
+  float A, B;
+};
+
+__device__ __forceinline__ unsigned long long pack(Span s) {
+  // A NaN of all ones must not read as kUnset.
+  const float A = s.A != s.A ? __builtin_nanf("") : s.A;
+  return static_cast<unsigned long long>(__builtin_bit_cast(unsigned int, A)) |
+         static_cast<unsigned long long>(__builtin_bit_cast(unsigned int, s.B)) << 32;
+}
+__device__ __forceinline__ Span unpack(unsigned long long w) {
+  return {__builtin_bit_cast(float, static_cast<unsigned int>(w)),
+          __builtin_bit_cast(float, static_cast<unsigned int>(w >> 32))};
+}
+__device__ __forceinline__ void publish(unsigned long long* p, Span s) {
+  __hip_atomic_store(p, pack(s), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ unsigned long long peek(const unsigned long long* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// The state after span s from the state h before it.
+__device__ __forceinline__ float apply(Span s, float h) {
+  return s.A < 0.f ? s.B : fmaf(s.A, h, s.B);
+}
+// Span p, then span s.
+__device__ __forceinline__ Span join(Span p, Span s) {
+  if (s.A < 0.f) return s;
+  return {p.A < 0.f ? -1.f : p.A * s.A, fmaf(s.A, p.B, s.B)};
+}
+
+__global__ void __launch_bounds__(256)
+    glr_clear_kernel(unsigned long long* words, int64_t n, unsigned int* ticket) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i < n) words[i] = kUnset;
+  if (i == 0) *ticket = 0;
+}
+
+// VEC elements at any address, of which the first `nv` exist.
+template <typename T, int VEC>
+__device__ __forceinline__ Arr<T, VEC> ld_lane(const T* p, int nv) {
+  Arr<T, VEC> out;
+  if constexpr (VEC == 1) {
+    out.v[0] = nv > 0 ? __builtin_nontemporal_load(p) : from_f32<T>(0.f);
+  } else {
+    static_assert(VEC == 2 && sizeof(T) == 2, "4 bytes");
+    typedef unsigned int u32a2 __attribute__((aligned(2)));
+    if (nv == 2) {
+      const unsigned int r = __builtin_nontemporal_load(reinterpret_cast<const u32a2*>(p));
+      __builtin_memcpy(&out, &r, 4);
+    } else {
+      out.v[0] = nv > 0 ? p[0] : from_f32<T>(0.f);
+      out.v[1] = from_f32<T>(0.f);
+    }
   }
-  if (p.fin) p.fin[n * p.D + ch] = h;
+  return out;
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void st_lane(T* p, const float (&v)[VEC], int nv) {
+  if constexpr (VEC == 1) {
+    if (nv > 0) __builtin_nontemporal_store(from_f32<T>(v[0]), p);
+  } else {
+    typedef unsigned int u32a2 __attribute__((aligned(2)));
+    if (nv == 2) {
+      Arr<T, 2> t{{from_f32<T>(v[0]), from_f32<T>(v[1])}};
+      unsigned int r;
+      __builtin_memcpy(&r, &t, 4);
+      __builtin_nontemporal_store(r, reinterpret_cast<u32a2*>(p));
+    } else if (nv > 0) {
+      p[0] = from_f32<T>(v[0]);
+    }
+  }
+}
+// fp32 rows of the same channels.
+template <int VEC>
+__device__ __forceinline__ void ld_f32(const float* p, int nv, float (&v)[VEC]) {
+#pragma unroll
+  for (int u = 0; u < VEC; ++u) v[u] = u < nv ? p[u] : 0.f;
+}
+template <int VEC>
+__device__ __forceinline__ void st_f32(float* p, int nv, const float (&v)[VEC]) {
+#pragma unroll
+  for (int u = 0; u < VEC; ++u)
+    if (u < nv) p[u] = v[u];
+}
+
+// Where sequences start and end in a window: bit j of a mask and entry j of a
+// table (the sequence) for token w0 + j.  `lo`, `hi`: the tokens that belong to
+// sequences.
+struct Marks {
+  unsigned int starts, ends;
+  int64_t lo, hi;
+};
+
+// Called by a whole wave; seqs: 2 * kTok entries of LDS of its own.  empty(n) is
+// called, by the wave together, for every empty sequence that the window
+// answers for: the ones that stand before one of its tokens, and behind the
+// last token those of the last window.
+template <typename Empty>
+__device__ __forceinline__ Marks find_marks(const void* cu, int cu64, int64_t N, int64_t run,
+                                            int64_t total, int64_t w0, bool last, int* seqs,
+                                            Empty empty) {
+  const int lane = threadIdx.x % kWave;
+  auto at = [&](int64_t n) { return cu_at(cu, cu64, n, run, total); };
+  Marks m;
+  m.lo = at(0);
+  m.hi = at(N);
+  if (lane < 2 * kTok) seqs[lane] = -1;
+  // The first sequence that does not end before the window.
+  int64_t base = 0, len = N;
+  while (len > kWave) {
+    const int64_t step = cdiv(len, kWave);
+    const int64_t q = lane * step + step - 1;
+    const uint64_t hit = __ballot(q >= len - 1 || at(base + q + 1) >= w0);
+    const int64_t f = static_cast<int64_t>(__builtin_ctzll(hit)) * step;
+    base += f;
+    len = len - f < step ? len - f : step;
+  }
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  for (; base < N; base += kWave) {
+    const int64_t n = base + lane;
+    int64_t t0 = total, t1 = total;
+    if (n < N) {
+      t0 = at(n);
+      t1 = at(n + 1);
+    }
+    if (t0 < t1) {
+      if (t0 >= w0 && t0 < w0 + kTok) seqs[t0 - w0] = static_cast<int>(n);
+      if (t1 > w0 && t1 <= w0 + kTok) seqs[kTok + t1 - 1 - w0] = static_cast<int>(n);
+    }
+    const bool mine = n < N && t0 >= t1 && t0 >= w0 && (t0 < w0 + kTok || last);
+    for (uint64_t left = __ballot(mine); left; left &= left - 1)
+      empty(base + __builtin_ctzll(left));
+    if (!last && __any(t0 >= w0 + kTok)) break;
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  m.starts = static_cast<unsigned int>(__ballot(lane < kTok && seqs[lane & (kTok - 1)] >= 0));
+  m.ends = static_cast<unsigned int>(
+      __ballot(lane < kTok && seqs[kTok + (lane & (kTok - 1))] >= 0));
+  return m;
+}
+
+// The state that enters a tile: the words of up to kBack tiles before it
+// (`step` from one to the one before), shared through `look`, until there is
+// a final one among them for every channel.  Called by all waves of a block.
+template <int VEC>
+__device__ __forceinline__ void enter(const unsigned long long* words, int64_t step, int64_t before,
+                                      int lane, int wave, int waves, Span (*look)[kWave * VEC],
+                                      float (&H)[VEC]) {
+  const int reach = static_cast<int>(before < kBack ? before : kBack);
+  for (;;) {
+    for (int d = wave; d < reach; d += waves) {
+      unsigned long long w[VEC];
+      for (;;) {
+        bool unset = false;
+#pragma unroll
+        for (int u = 0; u < VEC; ++u) {
+          w[u] = peek(words - (d + 1) * step + lane * VEC + u);
+          unset |= w[u] == kUnset;
+        }
+        if (!__any(unset)) break;
+        __builtin_amdgcn_s_sleep(1);
+      }
+#pragma unroll
+      for (int u = 0; u < VEC; ++u) look[d][lane * VEC + u] = unpack(w[u]);
+    }
+    __syncthreads();
+    bool known[VEC];
+#pragma unroll
+    for (int u = 0; u < VEC; ++u) {
+      known[u] = false;
+      H[u] = 0.f;
+    }
+    for (int d = reach - 1; d >= 0; --d) {
+#pragma unroll
+      for (int u = 0; u < VEC; ++u) {
+        const Span s = look[d][lane * VEC + u];
+        known[u] |= s.A < 0.f;
+        H[u] = apply(s, H[u]);
+      }
+    }
+    bool all = true;
+#pragma unroll
+    for (int u = 0; u < VEC; ++u) all &= known[u];
+    // Every wave read the same words, so all waves leave together.
+    if (__all(all)) return;
+    __syncthreads();
+    __builtin_amdgcn_s_sleep(1);
+  }
+}
+
+template <typename T, bool LOOK>
+__global__ void __launch_bounds__(kMaxWaves * kWave) glr_fwd_kernel(FwdParams p) {
+  constexpr int VEC = 4 / sizeof(T);
+  __shared__ unsigned int taken;
+  __shared__ int seqs[kMaxWaves][2 * kTok];
+  __shared__ Span spans[kMaxWaves][kWave * VEC];
+  __shared__ Span look[LOOK ? kBack : 1][kWave * VEC];
+  __shared__ int open;  // the tile needs the state before it
+
+  const int lane = threadIdx.x % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int waves = blockDim.x / kWave;
+  unsigned int id = blockIdx.x;
+  if constexpr (LOOK) {
+    if (threadIdx.x == 0)
+      taken = __hip_atomic_fetch_add(p.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    id = __builtin_amdgcn_readfirstlane(taken);
+  }
+  const int64_t tile = id / p.blocks;
+  const int blk = id % p.blocks;
+  const int64_t w0 = (tile * waves + wave) * kTok;
+  const int64_t ch = (static_cast<int64_t>(blk) * kWave + lane) * VEC;
+  const int nv = p.D - ch < VEC ? (p.D > ch ? static_cast<int>(p.D - ch) : 0) : VEC;
+
+  // All of the window's loads, before anything else.
+  Arr<T, VEC> x[kTok], a[kTok], b[kTok];
+  const T* xp = static_cast<const T*>(p.x) + w0 * p.sx + ch;
+  const T* ap = static_cast<const T*>(p.a) + w0 * p.sa + ch;
+  const T* bp = static_cast<const T*>(p.b) + w0 * p.sb + ch;
+  if (w0 + kTok <= p.total && (blk + 1) * static_cast<int64_t>(kWave * VEC) <= p.D) {
+#pragma unroll
+    for (int j = 0; j < kTok; ++j) {
+      x[j] = ld_lane<T, VEC>(xp + j * p.sx, VEC);
+      a[j] = ld_lane<T, VEC>(ap + j * p.sa, VEC);
+      b[j] = ld_lane<T, VEC>(bp + j * p.sb, VEC);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < kTok; ++j) {
+      const int have = w0 + j < p.total ? nv : 0;
+      x[j] = ld_lane<T, VEC>(xp + j * p.sx, have);
+      a[j] = ld_lane<T, VEC>(ap + j * p.sa, have);
+      b[j] = ld_lane<T, VEC>(bp + j * p.sb, have);
+    }
+  }
+  float k[VEC];
+  ld_f32<VEC>(p.lam + ch, nv, k);
+#pragma unroll
+  for (int u = 0; u < VEC; ++u) k[u] = -p.c * softplus_f32(k[u]);
+
+  const Marks m = find_marks(p.cu, p.cu64, p.N, p.T, p.total, w0,
+                             w0 < p.total + kTok && w0 + kTok >= p.total, seqs[wave],
+                             [&](int64_t n) {
+                               if (!p.fin) return;
+                               float h[VEC] = {};
+                               if (p.h0) ld_f32<VEC>(p.h0 + n * p.D + ch, nv, h);
+                               st_f32<VEC>(p.fin + n * p.D + ch, nv, h);
+                             });
+
+  // The window's gates, and its span.
+  float em1[kTok][VEC], add[kTok][VEC];
+  Span span[VEC];
+#pragma unroll
+  for (int u = 0; u < VEC; ++u) span[u] = {1.f, 0.f};
+#pragma unroll
+  for (int j = 0; j < kTok; ++j) {
+#pragma unroll
+    for (int u = 0; u < VEC; ++u) {
+      const Gate g = gate_of(k[u], sigmoid(to_f32(a[j].v[u])));
+      em1[j][u] = g.em1;
+      add[j][u] = g.s * (sigmoid(to_f32(b[j].v[u])) * to_f32(x[j].v[u]));
+    }
+    if (m.starts >> j & 1) {
+      float h[VEC] = {};
+      if (p.h0) ld_f32<VEC>(p.h0 + static_cast<int64_t>(seqs[wave][j]) * p.D + ch, nv, h);
+#pragma unroll
+      for (int u = 0; u < VEC; ++u) {
+        add[j][u] += decayed(em1[j][u], h[u]);
+        span[u].B = 0.f;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < VEC; ++u) {
+      span[u].A = decayed(em1[j][u], span[u].A);
+      span[u].B = decayed(em1[j][u], span[u].B) + add[j][u];
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < VEC; ++u) {
+    if (m.starts) span[u].A = -1.f;
+    spans[wave][lane * VEC + u] = span[u];
+  }
+  if (wave == 0 && lane == 0) open = !(m.starts & 1);
+  __syncthreads();
+
+  // From the tile's start to this window's.
+  Span head[VEC];
+#pragma unroll
+  for (int u = 0; u < VEC; ++u) head[u] = {1.f, 0.f};
+  for (int w = 0; w < wave; ++w) {
+#pragma unroll
+    for (int u = 0; u < VEC; ++u) head[u] = join(head[u], spans[w][lane * VEC + u]);
+  }
+  float H[VEC] = {};
+  if constexpr (LOOK) {
+    const int64_t width = static_cast<int64_t>(p.blocks) * kWave * VEC;
+    unsigned long long* words = p.words + tile * width + static_cast<int64_t>(blk) * kWave * VEC;
+    Span whole[VEC];
+    const bool closing = wave == waves - 1;
+    if (closing) {
+#pragma unroll
+      for (int u = 0; u < VEC; ++u) {
+        whole[u] = join(head[u], span[u]);
+        if (tile == 0) whole[u].A = -1.f;
+        publish(words + lane * VEC + u, whole[u]);
+      }
+    }
+    if (tile > 0 && open) {
+      enter<VEC>(words, width, tile, lane, wave, waves, look, H);
+      if (closing) {
+#pragma unroll
+        for (int u = 0; u < VEC; ++u)
+          if (whole[u].A >= 0.f || whole[u].A != whole[u].A)
+            publish(words + lane * VEC + u, {-1.f, apply(whole[u], H[u])});
+      }
+    }
+  }
+
+  float h[VEC];
+#pragma unroll
+  for (int u = 0; u < VEC; ++u) h[u] = apply(head[u], H[u]);
+  if (p.states && w0 < p.total) st_f32<VEC>(p.states + w0 / kWin * p.D + ch, nv, h);
+  T* yp = static_cast<T*>(p.y) + w0 * p.sy + ch;
+  const bool whole_window = w0 >= m.lo && w0 + kTok <= m.hi;
+#pragma unroll
+  for (int j = 0; j < kTok; ++j) {
+    if (m.starts >> j & 1) {
+#pragma unroll
+      for (int u = 0; u < VEC; ++u) h[u] = 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < VEC; ++u) h[u] = decayed(em1[j][u], h[u]) + add[j][u];
+    if (whole_window || (w0 + j >= m.lo && w0 + j < m.hi))
+      st_lane<T, VEC>(yp + j * p.sy, h, nv);
+    if ((m.ends >> j & 1) && p.fin)
+      st_f32<VEC>(p.fin + static_cast<int64_t>(seqs[wave][kTok + j]) * p.D + ch, nv, h);
+  }
+}
+
+// Tiles, channel blocks and waves of a block for a problem.
+struct Cut {
+  int64_t tiles;
+  int blocks, waves;
+  int64_t width;  // words of a tile
+};
+inline Cut cut_of(int64_t total, int64_t D, int vec, int max_waves) {
+  Cut c;
+  const int64_t windows = std::max<int64_t>(cdiv(total, kTok), 1);
+  c.waves = static_cast<int>(std::min<int64_t>(windows, max_waves));
+  c.tiles = cdiv(windows, c.waves);
+  c.blocks = static_cast<int>(cdiv(D, kWave * vec));
+  c.width = static_cast<int64_t>(c.blocks) * kWave * vec;
+  return c;
+}
+// Bytes of a pass's counter (its own cache line) and words; none for one tile.
+inline int64_t words_bytes(const Cut& c) { return c.tiles > 1 ? 256 + c.tiles * c.width * 8 : 0; }
+
+inline void clear_words(const Cut& c, void* workspace, hipStream_t s) {
+  const int64_t n = c.tiles * c.width;
+  hipLaunchKernelGGL(glr_clear_kernel, dim3(cdiv(n, 256)), dim3(256), 0, s,
+                     reinterpret_cast<unsigned long long*>(static_cast<char*>(workspace) + 256), n,
+                     static_cast<unsigned int*>(workspace));
+}
+
+template <typename T>
+int launch_fwd(FwdParams p, void* workspace, hipStream_t s) {
+  const Cut c = cut_of(p.total, p.D, 4 / sizeof(T), kMaxWaves);
+  p.blocks = c.blocks;
+  const dim3 grid(c.tiles * c.blocks), block(c.waves * kWave);
+  if (c.tiles > 1) {
+    p.ticket = static_cast<unsigned int*>(workspace);
+    p.words = reinterpret_cast<unsigned long long*>(static_cast<char*>(workspace) + 256);
+    clear_words(c, workspace, s);
+    hipLaunchKernelGGL((glr_fwd_kernel<T, true>), grid, block, 0, s, p);
+  } else {
+    hipLaunchKernelGGL((glr_fwd_kernel<T, false>), grid, block, 0, s, p);
+  }
+  return launch_status();
 }
 
 struct UpdateParams {
@@ -235,6 +629,13 @@ __global__ void __launch_bounds__(64) glr_dlam_kernel(const float* part, int64_t
   dlam[ch] = s * slope_ratio(lam[ch]);
 }
 
+// Tokens, sequences and tiles are counted in 31 bits, a batch's elements in 62.
+bool bad_sizes(int64_t N, int64_t total, int64_t D) {
+  constexpr int64_t kMost = int64_t{1} << 31;
+  return N < 0 || N >= kMost || total < 0 || total >= kMost || D <= 0 || D >= kMost ||
+         cdiv(std::max<int64_t>(total, 1), kTok) * cdiv(D, kWave) >= kMost;
+}
+
 bool pitch_ok(int64_t pitch, int64_t D) { return pitch >= D; }
 
 // cu_seqlens of a readable type, or none and N equal runs.
@@ -247,7 +648,12 @@ bool seqs_ok(const void* cu, xk_dtype dt, int64_t N, int64_t total) {
 
 using namespace xk;
 
-extern "C" int64_t xk_gated_linear_recurrence_workspace_bytes(int64_t, int64_t) { return 0; }
+extern "C" int64_t xk_gated_linear_recurrence_workspace_bytes(int64_t total_tokens, int64_t D) {
+  if (total_tokens <= 0 || D <= 0) return 0;
+  // 4-byte elements take more, narrower channel blocks.
+  return std::max(words_bytes(cut_of(total_tokens, D, 1, kMaxWaves)),
+                  words_bytes(cut_of(total_tokens, D, 2, kMaxWaves)));
+}
 
 extern "C" int xk_gated_linear_recurrence(
     const void* x, int64_t stride_x_tok, const void* a, int64_t stride_a_tok, const void* b,
@@ -255,7 +661,7 @@ extern "C" int xk_gated_linear_recurrence(
     int64_t stride_y_tok, const float* initial_state, float* final_state, float* states,
     const void* cu_seqlens, xk_dtype cu_dtype, int64_t N, int64_t total_tokens, int64_t D,
     void* workspace, size_t workspace_bytes, void* stream) {
-  if (N < 0 || total_tokens < 0 || D <= 0 || !(c >= 0.f)) return XK_ERR_INVALID;
+  if (bad_sizes(N, total_tokens, D) || !(c >= 0.f)) return XK_ERR_INVALID;
   if (!is_float_dtype(dtype)) return XK_ERR_UNSUPPORTED;
   if (N == 0) return XK_OK;
   if (!seqs_ok(cu_seqlens, cu_dtype, N, total_tokens) || !lam) return XK_ERR_INVALID;
@@ -263,17 +669,19 @@ extern "C" int xk_gated_linear_recurrence(
       (!x || !a || !b || !y || !pitch_ok(stride_x_tok, D) || !pitch_ok(stride_a_tok, D) ||
        !pitch_ok(stride_b_tok, D) || !pitch_ok(stride_y_tok, D)))
     return XK_ERR_INVALID;
-  FwdParams p{x, a, b, y, stride_x_tok, stride_a_tok, stride_b_tok, stride_y_tok, lam, c,
-              initial_state, final_state, states, cu_seqlens, cu_dtype == XK_I64, N,
-              total_tokens / N, total_tokens, D};
-  const dim3 grid(cdiv(D, 64), N);
+  const int64_t need = xk_gated_linear_recurrence_workspace_bytes(total_tokens, D);
+  if (need > 0 && (!workspace || workspace_bytes < static_cast<size_t>(need) ||
+                   !aligned(workspace, 256)))
+    return XK_ERR_WORKSPACE;
+  const FwdParams p{x, a, b, y, stride_x_tok, stride_a_tok, stride_b_tok, stride_y_tok, lam, c,
+                    initial_state, final_state, states, cu_seqlens, cu_dtype == XK_I64, N,
+                    total_tokens / N, total_tokens, D, nullptr, nullptr, 0};
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (dtype) {
-    case XK_F32: hipLaunchKernelGGL(glr_fwd_kernel<float>, grid, dim3(64), 0, s, p); break;
-    case XK_BF16: hipLaunchKernelGGL(glr_fwd_kernel<bf16>, grid, dim3(64), 0, s, p); break;
-    default: hipLaunchKernelGGL(glr_fwd_kernel<f16>, grid, dim3(64), 0, s, p); break;
+    case XK_F32: return launch_fwd<float>(p, workspace, s);
+    case XK_BF16: return launch_fwd<bf16>(p, workspace, s);
+    default: return launch_fwd<f16>(p, workspace, s);
   }
-  return launch_status();
 }
 
 extern "C" int xk_gated_linear_recurrence_update(
@@ -283,7 +691,7 @@ extern "C" int xk_gated_linear_recurrence_update(
     const int32_t* state_indices, int64_t num_cols, const int32_t* num_accepted_tokens,
     const void* cu_seqlens, xk_dtype cu_dtype, int64_t N, int64_t T, int64_t total_tokens,
     int64_t D, void* stream) {
-  if (N < 0 || total_tokens < 0 || D <= 0 || num_slots < 0 || num_cols < 0 || !(c >= 0.f))
+  if (bad_sizes(N, total_tokens, D) || num_slots < 0 || num_cols < 0 || !(c >= 0.f))
     return XK_ERR_INVALID;
   if (!is_float_dtype(dtype)) return XK_ERR_UNSUPPORTED;
   if (N == 0 || total_tokens == 0) return XK_OK;
@@ -319,7 +727,7 @@ extern "C" int xk_gated_linear_recurrence_bwd(
     int64_t stride_db_tok, float* dlam, float* d_initial_state, const void* cu_seqlens,
     xk_dtype cu_dtype, int64_t N, int64_t total_tokens, int64_t D, void* workspace,
     size_t workspace_bytes, void* stream) {
-  if (N < 0 || total_tokens < 0 || D <= 0 || !(c >= 0.f)) return XK_ERR_INVALID;
+  if (bad_sizes(N, total_tokens, D) || !(c >= 0.f)) return XK_ERR_INVALID;
   if (!is_float_dtype(dtype)) return XK_ERR_UNSUPPORTED;
   if (!lam || (N > 0 && !seqs_ok(cu_seqlens, cu_dtype, N, total_tokens))) return XK_ERR_INVALID;
   if (total_tokens > 0 &&
