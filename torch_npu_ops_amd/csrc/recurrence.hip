@@ -148,39 +148,51 @@ __global__ void __launch_bounds__(256)
   if (i == 0) *ticket = 0;
 }
 
-// VEC elements at any address, of which the first `nv` exist.
+template <int ALIGN> struct LaneWord;
+template <> struct LaneWord<2> { typedef unsigned int type __attribute__((aligned(2))); };
+template <> struct LaneWord<4> { typedef unsigned int type; };
+
+// A lane's 4 bytes of a row: VEC elements at any address, of which the first
+// `nv` exist.
 template <typename T, int VEC>
-__device__ __forceinline__ Arr<T, VEC> ld_lane(const T* p, int nv) {
-  Arr<T, VEC> out;
-  if constexpr (VEC == 1) {
-    out.v[0] = nv > 0 ? __builtin_nontemporal_load(p) : from_f32<T>(0.f);
-  } else {
-    static_assert(VEC == 2 && sizeof(T) == 2, "4 bytes");
-    typedef unsigned int u32a2 __attribute__((aligned(2)));
-    if (nv == 2) {
-      const unsigned int r = __builtin_nontemporal_load(reinterpret_cast<const u32a2*>(p));
-      __builtin_memcpy(&out, &r, 4);
-    } else {
-      out.v[0] = nv > 0 ? p[0] : from_f32<T>(0.f);
-      out.v[1] = from_f32<T>(0.f);
-    }
+__device__ __forceinline__ unsigned int ld_lane(const T* p, int nv) {
+  static_assert(VEC * sizeof(T) == 4, "4 bytes");
+  using W = typename LaneWord<sizeof(T)>::type;
+  if (nv == VEC) return __builtin_nontemporal_load(reinterpret_cast<const W*>(p));
+  if constexpr (VEC == 2) {
+    if (nv == 1) return __builtin_bit_cast(unsigned short, p[0]);
   }
-  return out;
+  return 0;
 }
+template <typename T>
+__device__ __forceinline__ float lane_f32(unsigned int r, int u) {
+  if constexpr (sizeof(T) == 4) {
+    return __builtin_bit_cast(float, r);
+  } else if constexpr (std::is_same<T, bf16>::value) {
+    return __builtin_bit_cast(float, u ? r & 0xffff0000u : r << 16);
+  } else {
+    return to_f32(__builtin_bit_cast(T, static_cast<unsigned short>(u ? r >> 16 : r)));
+  }
+}
+// What is computed from v later is computed then: keeps the compiler from
+// holding a second pass's values in registers from the first one on.
+template <typename V>
+__device__ __forceinline__ void later(V& v) {
+  asm volatile("" : "+v"(v));
+}
+
 template <typename T, int VEC>
 __device__ __forceinline__ void st_lane(T* p, const float (&v)[VEC], int nv) {
-  if constexpr (VEC == 1) {
-    if (nv > 0) __builtin_nontemporal_store(from_f32<T>(v[0]), p);
-  } else {
-    typedef unsigned int u32a2 __attribute__((aligned(2)));
-    if (nv == 2) {
-      Arr<T, 2> t{{from_f32<T>(v[0]), from_f32<T>(v[1])}};
-      unsigned int r;
-      __builtin_memcpy(&r, &t, 4);
-      __builtin_nontemporal_store(r, reinterpret_cast<u32a2*>(p));
-    } else if (nv > 0) {
-      p[0] = from_f32<T>(v[0]);
-    }
+  Arr<T, VEC> t;
+#pragma unroll
+  for (int u = 0; u < VEC; ++u) t.v[u] = from_f32<T>(v[u]);
+  using W = typename LaneWord<sizeof(T)>::type;
+  if (nv == VEC) {
+    unsigned int r;
+    __builtin_memcpy(&r, &t, 4);
+    __builtin_nontemporal_store(r, reinterpret_cast<W*>(p));
+  } else if (VEC == 2 && nv == 1) {
+    p[0] = t.v[0];
   }
 }
 // fp32 rows of the same channels.
@@ -327,7 +339,7 @@ __global__ void __launch_bounds__(kMaxWaves * kWave) glr_fwd_kernel(FwdParams p)
   const int nv = p.D - ch < VEC ? (p.D > ch ? static_cast<int>(p.D - ch) : 0) : VEC;
 
   // All of the window's loads, before anything else.
-  Arr<T, VEC> x[kTok], a[kTok], b[kTok];
+  unsigned int x[kTok], a[kTok], b[kTok];
   const T* xp = static_cast<const T*>(p.x) + w0 * p.sx + ch;
   const T* ap = static_cast<const T*>(p.a) + w0 * p.sa + ch;
   const T* bp = static_cast<const T*>(p.b) + w0 * p.sb + ch;
@@ -370,9 +382,9 @@ __global__ void __launch_bounds__(kMaxWaves * kWave) glr_fwd_kernel(FwdParams p)
   for (int j = 0; j < kTok; ++j) {
 #pragma unroll
     for (int u = 0; u < VEC; ++u) {
-      const Gate g = gate_of(k[u], sigmoid(to_f32(a[j].v[u])));
+      const Gate g = gate_of(k[u], sigmoid(lane_f32<T>(a[j], u)));
       em1[j][u] = g.em1;
-      add[j][u] = g.s * (sigmoid(to_f32(b[j].v[u])) * to_f32(x[j].v[u]));
+      add[j][u] = g.s * (sigmoid(lane_f32<T>(b[j], u)) * lane_f32<T>(x[j], u));
     }
     if (m.starts >> j & 1) {
       float h[VEC] = {};
@@ -424,7 +436,7 @@ __global__ void __launch_bounds__(kMaxWaves * kWave) glr_fwd_kernel(FwdParams p)
       if (closing) {
 #pragma unroll
         for (int u = 0; u < VEC; ++u)
-          if (whole[u].A >= 0.f || whole[u].A != whole[u].A)
+          if (!(whole[u].A < 0.f))
             publish(words + lane * VEC + u, {-1.f, apply(whole[u], H[u])});
       }
     }
@@ -555,10 +567,14 @@ struct BwdParams {
   const float* h0;
   const float* dfin;
   float* dh0;
-  float* part;  // dlam's parts, [N, D]
+  float* part;  // dlam's parts, [tiles][D]; NULL: not asked for
   const void* cu;
   int cu64;
   int64_t N, T, total, D;
+  unsigned long long* words;
+  unsigned int* ticket;
+  int64_t tiles;
+  int blocks;
 };
 
 // sigmoid(lam) / softplus(lam), 1 in the limit lam -> -inf.
@@ -567,66 +583,266 @@ __device__ __forceinline__ float slope_ratio(float lam) {
   return 1.f / ((1.f + expf(-lam)) * softplus_f32(lam));
 }
 
-template <typename T>
-__global__ void __launch_bounds__(64) glr_bwd_kernel(BwdParams p) {
-  const int64_t ch = static_cast<int64_t>(blockIdx.x) * 64 + threadIdx.x;
-  const int64_t n = blockIdx.y;
-  if (ch >= p.D) return;
-  const int64_t t0 = cu_at(p.cu, p.cu64, n, p.T, p.total), t1 = cu_at(p.cu, p.cu64, n + 1, p.T, p.total);
-  const float k = -p.c * softplus_f32(p.lam[ch]);
-  float q = p.dfin ? p.dfin[n * p.D + ch] : 0.f;  // gradient of the state after token t
-  float sum = 0.f;
-  for (int64_t hi = t1; hi > t0;) {
-    int64_t lo = (hi - 1) / kWin * kWin;
-    lo = lo < t0 ? t0 : lo;
-    float h = lo == t0 ? (p.h0 ? p.h0[n * p.D + ch] : 0.f) : p.states[lo / kWin * p.D + ch];
-    float before[kWin];
-#pragma unroll
-    for (int j = 0; j < kWin; ++j) {
-      const int64_t t = lo + j;
-      if (t < hi) {
-        before[j] = h;
-        const float x = to_f32(static_cast<const T*>(p.x)[t * p.sx + ch]);
-        const float r = sigmoid(to_f32(static_cast<const T*>(p.a)[t * p.sa + ch]));
-        const float i = sigmoid(to_f32(static_cast<const T*>(p.b)[t * p.sb + ch]));
-        const Gate g = gate_of(k, r);
-        h = decayed(g.em1, h) + g.s * (i * x);
-      }
-    }
-#pragma unroll
-    for (int j = kWin - 1; j >= 0; --j) {
-      const int64_t t = lo + j;
-      if (t < hi) {
-        const float x = to_f32(static_cast<const T*>(p.x)[t * p.sx + ch]);
-        const float av = to_f32(static_cast<const T*>(p.a)[t * p.sa + ch]);
-        const float bv = to_f32(static_cast<const T*>(p.b)[t * p.sb + ch]);
-        const float r = sigmoid(av), i = sigmoid(bv);
-        const Gate g = gate_of(k, r);
-        const float l = k * r;
-        const float G = to_f32(static_cast<const T*>(p.dy)[t * p.sdy + ch]) + q;
-        const float l_s = g.s > 0.f ? l / g.s : 0.f;
-        const float e = G * g.alpha * (before[j] * l - i * x * g.alpha * l_s);
-        static_cast<T*>(p.dx)[t * p.sdx + ch] = from_f32<T>(G * g.s * i);
-        static_cast<T*>(p.da)[t * p.sda + ch] = from_f32<T>(e * sigmoid(-av));
-        static_cast<T*>(p.db)[t * p.sdb + ch] = from_f32<T>(G * g.s * i * x * sigmoid(-bv));
-        sum += e;
-        q = decayed(g.em1, G);
-      }
-    }
-    hi = lo;
-  }
-  if (p.dh0) p.dh0[n * p.D + ch] = q;
-  if (p.part) p.part[n * p.D + ch] = sum;
+// exp(-v) for a sigmoid's value r = 1 / (1 + e) and its complement 1 - r = e r;
+// capped at 2^100, so that e r is 1 and not inf * 0 for a closed gate.
+__device__ __forceinline__ float exp_neg(float v) {
+  return __builtin_amdgcn_exp2f(fminf(v * -1.44269504f, 100.f));
 }
 
-// dlam = sum over parts of (sum dl l) sigmoid(lam) / softplus(lam).
-__global__ void __launch_bounds__(64) glr_dlam_kernel(const float* part, int64_t parts,
-                                                      const float* lam, float* dlam, int64_t D) {
-  const int64_t ch = static_cast<int64_t>(blockIdx.x) * 64 + threadIdx.x;
-  if (ch >= D) return;
+// ---------------------------------------------------------------------------
+// Backward.  The gradient q that enters a token from behind (of its state)
+// leaves it in front as alpha (dy + q): a span of tokens maps q -> A q + B, and
+// a sequence's last token makes a span final, its q being d_final_state.  So
+// the tiles of the forward kernel run here from the end, in the same way, with
+// the sequences' ends in the place of their starts.
+//  * h_{t-1} comes from the window's saved state, in the same pass that forms
+//    the window's span (in token order: A is the running product of alpha and
+//    B the sum of A_t dy_t, so nothing but h_{t-1} is kept for a token).
+//  * The second pass, in reverse order, forms the gates again from exp(-a) and
+//    exp(-b), which stay in registers.
+//  * E = (dL/dl) l = G alpha (h_{t-1} l - i x alpha l / s) gives da = E (1 - r)
+//    and dlam = sum E sigmoid(lam) / softplus(lam), with no division by what
+//    vanishes as a gate closes: l / s -> 0 with s.
+// ---------------------------------------------------------------------------
+constexpr int kBwdWaves = 4;
+
+template <typename T, bool LOOK>
+__global__ void __launch_bounds__(kBwdWaves * kWave) glr_bwd_kernel(BwdParams p) {
+  constexpr int VEC = 4 / sizeof(T);
+  __shared__ unsigned int taken;
+  __shared__ int seqs[kBwdWaves][2 * kTok];
+  __shared__ Span spans[kBwdWaves][kWave * VEC];
+  __shared__ Span look[LOOK ? kBack : 1][kWave * VEC];
+  __shared__ float sums[kBwdWaves][kWave * VEC];
+  __shared__ int open;  // the tile needs the gradient from behind it
+
+  const int lane = threadIdx.x % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int waves = blockDim.x / kWave;
+  unsigned int id = blockIdx.x;
+  if constexpr (LOOK) {
+    if (threadIdx.x == 0)
+      taken = __hip_atomic_fetch_add(p.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    id = __builtin_amdgcn_readfirstlane(taken);
+  }
+  const int64_t after = id / p.blocks;  // tiles behind this one
+  const int64_t tile = p.tiles - 1 - after;
+  const int blk = id % p.blocks;
+  const int64_t w0 = (tile * waves + wave) * kTok;
+  const int64_t ch = (static_cast<int64_t>(blk) * kWave + lane) * VEC;
+  const int nv = p.D - ch < VEC ? (p.D > ch ? static_cast<int>(p.D - ch) : 0) : VEC;
+
+  unsigned int x[kTok], dy[kTok], a[kTok], b[kTok];
+  const T* xp = static_cast<const T*>(p.x) + w0 * p.sx + ch;
+  const T* ap = static_cast<const T*>(p.a) + w0 * p.sa + ch;
+  const T* bp = static_cast<const T*>(p.b) + w0 * p.sb + ch;
+  const T* gp = static_cast<const T*>(p.dy) + w0 * p.sdy + ch;
+  if (w0 + kTok <= p.total && (blk + 1) * static_cast<int64_t>(kWave * VEC) <= p.D) {
+#pragma unroll
+    for (int j = 0; j < kTok; ++j) {
+      a[j] = ld_lane<T, VEC>(ap + j * p.sa, VEC);
+      b[j] = ld_lane<T, VEC>(bp + j * p.sb, VEC);
+      x[j] = ld_lane<T, VEC>(xp + j * p.sx, VEC);
+      dy[j] = ld_lane<T, VEC>(gp + j * p.sdy, VEC);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < kTok; ++j) {
+      const int have = w0 + j < p.total ? nv : 0;
+      a[j] = ld_lane<T, VEC>(ap + j * p.sa, have);
+      b[j] = ld_lane<T, VEC>(bp + j * p.sb, have);
+      x[j] = ld_lane<T, VEC>(xp + j * p.sx, have);
+      dy[j] = ld_lane<T, VEC>(gp + j * p.sdy, have);
+    }
+  }
+  float k[VEC], h[VEC] = {};
+  ld_f32<VEC>(p.lam + ch, nv, k);
+  if (w0 < p.total) ld_f32<VEC>(p.states + w0 / kWin * p.D + ch, nv, h);
+#pragma unroll
+  for (int u = 0; u < VEC; ++u) k[u] = -p.c * softplus_f32(k[u]);
+
+  const Marks m = find_marks(p.cu, p.cu64, p.N, p.T, p.total, w0,
+                             w0 < p.total + kTok && w0 + kTok >= p.total, seqs[wave],
+                             [&](int64_t n) {
+                               if (!p.dh0) return;
+                               float q[VEC] = {};
+                               if (p.dfin) ld_f32<VEC>(p.dfin + n * p.D + ch, nv, q);
+                               st_f32<VEC>(p.dh0 + n * p.D + ch, nv, q);
+                             });
+
+  float before[kTok][VEC], ea[kTok][VEC], eb[kTok][VEC];
+  Span span[VEC];
+#pragma unroll
+  for (int u = 0; u < VEC; ++u) span[u] = {1.f, 0.f};
+#pragma unroll
+  for (int j = 0; j < kTok; ++j) {
+    if (m.starts >> j & 1) {
+#pragma unroll
+      for (int u = 0; u < VEC; ++u) h[u] = 0.f;
+      if (p.h0) ld_f32<VEC>(p.h0 + static_cast<int64_t>(seqs[wave][j]) * p.D + ch, nv, h);
+    }
+#pragma unroll
+    for (int u = 0; u < VEC; ++u) {
+      ea[j][u] = exp_neg(lane_f32<T>(a[j], u));
+      eb[j][u] = exp_neg(lane_f32<T>(b[j], u));
+      const Gate g = gate_of(k[u], fast_rcp(1.f + ea[j][u]));
+      before[j][u] = h[u];
+      h[u] = decayed(g.em1, h[u]) + g.s * (fast_rcp(1.f + eb[j][u]) * lane_f32<T>(x[j], u));
+      if (!(m.ends & ((1u << j) - 1))) {  // no sequence ended before: q comes this far
+        span[u].A = decayed(g.em1, span[u].A);
+        span[u].B = fmaf(span[u].A, lane_f32<T>(dy[j], u), span[u].B);
+      }
+    }
+    if ((m.ends >> j & 1) && !(m.ends & ((1u << j) - 1)) && p.dfin) {
+      float q[VEC];
+      ld_f32<VEC>(p.dfin + static_cast<int64_t>(seqs[wave][kTok + j]) * p.D + ch, nv, q);
+#pragma unroll
+      for (int u = 0; u < VEC; ++u) span[u].B = fmaf(span[u].A, q[u], span[u].B);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < VEC; ++u) {
+    if (m.ends) span[u].A = -1.f;
+    spans[wave][lane * VEC + u] = span[u];
+  }
+  if (wave == waves - 1 && lane == 0) open = !(m.ends >> (kTok - 1) & 1);
+  __syncthreads();
+
+  // From the tile's end to this window's.
+  Span head[VEC];
+#pragma unroll
+  for (int u = 0; u < VEC; ++u) head[u] = {1.f, 0.f};
+  for (int w = waves - 1; w > wave; --w) {
+#pragma unroll
+    for (int u = 0; u < VEC; ++u) head[u] = join(head[u], spans[w][lane * VEC + u]);
+  }
+  float Q[VEC] = {};
+  if constexpr (LOOK) {
+    const int64_t width = static_cast<int64_t>(p.blocks) * kWave * VEC;
+    unsigned long long* words = p.words + after * width + static_cast<int64_t>(blk) * kWave * VEC;
+    Span whole[VEC];
+    if (wave == 0) {
+#pragma unroll
+      for (int u = 0; u < VEC; ++u) {
+        whole[u] = join(head[u], span[u]);
+        if (after == 0) whole[u].A = -1.f;
+        publish(words + lane * VEC + u, whole[u]);
+      }
+    }
+    if (after > 0 && open) {
+      enter<VEC>(words, width, after, lane, wave, waves, look, Q);
+      if (wave == 0) {
+#pragma unroll
+        for (int u = 0; u < VEC; ++u)
+          if (!(whole[u].A < 0.f))
+            publish(words + lane * VEC + u, {-1.f, apply(whole[u], Q[u])});
+      }
+    }
+  }
+
+#pragma unroll
+  for (int j = 0; j < kTok; ++j) {
+    later(x[j]);
+    later(dy[j]);
+#pragma unroll
+    for (int u = 0; u < VEC; ++u) {
+      later(ea[j][u]);
+      later(eb[j][u]);
+    }
+  }
+  float q[VEC], sum[VEC] = {};
+#pragma unroll
+  for (int u = 0; u < VEC; ++u) q[u] = apply(head[u], Q[u]);
+  T* dxp = static_cast<T*>(p.dx) + w0 * p.sdx + ch;
+  T* dap = static_cast<T*>(p.da) + w0 * p.sda + ch;
+  T* dbp = static_cast<T*>(p.db) + w0 * p.sdb + ch;
+  const bool whole_window = w0 >= m.lo && w0 + kTok <= m.hi;
+#pragma unroll
+  for (int j = kTok - 1; j >= 0; --j) {
+    if (m.ends >> j & 1) {
+#pragma unroll
+      for (int u = 0; u < VEC; ++u) q[u] = 0.f;
+      if (p.dfin)
+        ld_f32<VEC>(p.dfin + static_cast<int64_t>(seqs[wave][kTok + j]) * p.D + ch, nv, q);
+    }
+    const bool live = whole_window || (w0 + j >= m.lo && w0 + j < m.hi);
+    float dx[VEC], da[VEC], db[VEC];
+#pragma unroll
+    for (int u = 0; u < VEC; ++u) {
+      const float r = fast_rcp(1.f + ea[j][u]), i = fast_rcp(1.f + eb[j][u]);
+      const float xf = lane_f32<T>(x[j], u), l = k[u] * r;
+      const Decay d = decay_of(l);
+      const float w = -d.em1 * (1.f + d.alpha);  // s^2
+      // The instruction takes a denormal w for 0.
+      const float inv = w >= 1.17549435e-38f ? __builtin_amdgcn_rsqf(w) : 0.f;
+      const float G = lane_f32<T>(dy[j], u) + q[u];
+      dx[u] = G * (w * inv) * i;
+      db[u] = dx[u] * xf * (eb[j][u] * i);
+      const float e = G * d.alpha * (before[j][u] * l - i * xf * d.alpha * (l * inv));
+      da[u] = e * (ea[j][u] * r);
+      if (live) sum[u] += e;
+      q[u] = decayed(d.em1, G);
+    }
+    if (live) {
+      st_lane<T, VEC>(dxp + j * p.sdx, dx, nv);
+      st_lane<T, VEC>(dap + j * p.sda, da, nv);
+      st_lane<T, VEC>(dbp + j * p.sdb, db, nv);
+    }
+    if ((m.starts >> j & 1) && p.dh0)
+      st_f32<VEC>(p.dh0 + static_cast<int64_t>(seqs[wave][j]) * p.D + ch, nv, q);
+  }
+  if (p.part) {
+#pragma unroll
+    for (int u = 0; u < VEC; ++u) sums[wave][lane * VEC + u] = sum[u];
+    __syncthreads();
+    if (wave == 0) {
+      for (int w = 1; w < waves; ++w) {
+#pragma unroll
+        for (int u = 0; u < VEC; ++u) sum[u] += sums[w][lane * VEC + u];
+      }
+      st_f32<VEC>(p.part + tile * p.D + ch, nv, sum);
+    }
+  }
+}
+
+// dlam = sum over tiles of (sum E) sigmoid(lam) / softplus(lam): a block takes
+// 64 channels, each of its 16 waves every 16th tile.
+__global__ void __launch_bounds__(1024) glr_dlam_kernel(const float* part, int64_t tiles,
+                                                        const float* lam, float* dlam, int64_t D) {
+  __shared__ float red[16][kWave];
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int64_t ch = static_cast<int64_t>(blockIdx.x) * kWave + lane;
   float s = 0.f;
-  for (int64_t j = 0; j < parts; ++j) s += part[j * D + ch];
-  dlam[ch] = s * slope_ratio(lam[ch]);
+  if (ch < D)
+    for (int64_t j = wave; j < tiles; j += 16) s += part[j * D + ch];
+  red[wave][lane] = s;
+  __syncthreads();
+  if (wave == 0 && ch < D) {
+    s = 0.f;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) s += red[w][lane];
+    dlam[ch] = s * slope_ratio(lam[ch]);
+  }
+}
+
+template <typename T>
+int launch_bwd(BwdParams p, bool sums, void* workspace, hipStream_t s) {
+  const Cut c = cut_of(p.total, p.D, 4 / sizeof(T), kBwdWaves);
+  p.blocks = c.blocks;
+  p.tiles = c.tiles;
+  // The workspace: counter and words, then dlam's parts.
+  if (sums) p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + words_bytes(c));
+  const dim3 grid(c.tiles * c.blocks), block(c.waves * kWave);
+  if (c.tiles > 1) {
+    p.ticket = static_cast<unsigned int*>(workspace);
+    p.words = reinterpret_cast<unsigned long long*>(static_cast<char*>(workspace) + 256);
+    clear_words(c, workspace, s);
+    hipLaunchKernelGGL((glr_bwd_kernel<T, true>), grid, block, 0, s, p);
+  } else {
+    hipLaunchKernelGGL((glr_bwd_kernel<T, false>), grid, block, 0, s, p);
+  }
+  return launch_status();
 }
 
 // Tokens, sequences and tiles are counted in 31 bits, a batch's elements in 62.
@@ -714,9 +930,11 @@ extern "C" int xk_gated_linear_recurrence_update(
   return launch_status();
 }
 
-extern "C" int64_t xk_gated_linear_recurrence_bwd_workspace_bytes(int64_t, int64_t N,
+extern "C" int64_t xk_gated_linear_recurrence_bwd_workspace_bytes(int64_t total_tokens, int64_t N,
                                                                   int64_t D) {
-  return N * D * 4;
+  if (total_tokens < 0 || N <= 0 || D <= 0) return 0;
+  const Cut c1 = cut_of(total_tokens, D, 1, kBwdWaves), c2 = cut_of(total_tokens, D, 2, kBwdWaves);
+  return std::max(words_bytes(c1), words_bytes(c2)) + c1.tiles * D * 4;
 }
 
 extern "C" int xk_gated_linear_recurrence_bwd(
@@ -739,21 +957,25 @@ extern "C" int xk_gated_linear_recurrence_bwd(
   if (need > 0 && (!workspace || workspace_bytes < static_cast<size_t>(need) ||
                    !aligned(workspace, 256)))
     return XK_ERR_WORKSPACE;
-  BwdParams p{dy, x, a, b, dx, da, db, stride_dy_tok, stride_x_tok, stride_a_tok, stride_b_tok,
-              stride_dx_tok, stride_da_tok, stride_db_tok, lam, c, states, initial_state,
-              d_final_state, d_initial_state, static_cast<float*>(workspace), cu_seqlens,
-              cu_dtype == XK_I64, N, N > 0 ? total_tokens / N : 0, total_tokens, D};
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (N > 0) {
-    const dim3 grid(cdiv(D, 64), N);
-    switch (dtype) {
-      case XK_F32: hipLaunchKernelGGL(glr_bwd_kernel<float>, grid, dim3(64), 0, s, p); break;
-      case XK_BF16: hipLaunchKernelGGL(glr_bwd_kernel<bf16>, grid, dim3(64), 0, s, p); break;
-      default: hipLaunchKernelGGL(glr_bwd_kernel<f16>, grid, dim3(64), 0, s, p); break;
-    }
+    const BwdParams p{dy, x, a, b, dx, da, db, stride_dy_tok, stride_x_tok, stride_a_tok,
+                      stride_b_tok, stride_dx_tok, stride_da_tok, stride_db_tok, lam, c, states,
+                      initial_state, d_final_state, d_initial_state, nullptr, cu_seqlens,
+                      cu_dtype == XK_I64, N, total_tokens / N, total_tokens, D, nullptr, nullptr,
+                      0, 0};
+    const int st = dtype == XK_F32    ? launch_bwd<float>(p, dlam, workspace, s)
+                   : dtype == XK_BF16 ? launch_bwd<bf16>(p, dlam, workspace, s)
+                                      : launch_bwd<f16>(p, dlam, workspace, s);
+    if (st != XK_OK) return st;
   }
-  if (dlam)
-    hipLaunchKernelGGL(glr_dlam_kernel, dim3(cdiv(D, 64)), dim3(64), 0, s,
-                       static_cast<const float*>(workspace), N, lam, dlam, D);
+  if (dlam) {
+    const Cut cut = cut_of(total_tokens, D, dtype == XK_F32 ? 1 : 2, kBwdWaves);
+    const float* part = N > 0 ? reinterpret_cast<const float*>(static_cast<char*>(workspace) +
+                                                               words_bytes(cut))
+                              : nullptr;
+    hipLaunchKernelGGL(glr_dlam_kernel, dim3(cdiv(D, kWave)), dim3(1024), 0, s, part,
+                       N > 0 ? cut.tiles : 0, lam, dlam, D);
+  }
   return launch_status();
 }
