@@ -10,6 +10,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "xk_common.h"
 
@@ -24,19 +25,23 @@ __device__ __forceinline__ float softplus_f32(float v) {
 }
 
 // The decay of a token for l <= 0: alpha = exp(l) and alpha - 1, each to its
-// own last digits.  Above -1/4 the power series to l^6 / 720 (the next term is
-// 5e-8 of the sum) gives alpha - 1, below it the exponential gives alpha.
+// own last digits.  From -1/4 up a polynomial of (exp(l) - 1) / l (least
+// largest relative error, 2.5e-9 before rounding) gives alpha - 1, below it
+// the exponential gives alpha.  NEAR: no channel of the wave goes below (k r,
+// r < 1); the same bits without the exponential.
+constexpr float kNear = -0.25f;
 struct Decay {
   float alpha, em1;
 };
+template <bool NEAR>
 __device__ __forceinline__ Decay decay_of(float l) {
-  float p = fmaf(l, 1.f / 720.f, 1.f / 120.f);
-  p = fmaf(p, l, 1.f / 24.f);
-  p = fmaf(p, l, 1.f / 6.f);
-  p = fmaf(p, l, 0.5f);
+  float p = fmaf(l, 0.007510221f, 0.041488957f);
+  p = fmaf(p, l, 0.16665082f);
+  p = fmaf(p, l, 0.4999995f);
   p = fmaf(p, l, 1.f) * l;
+  if constexpr (NEAR) return {1.f + p, p};
   const float e = __expf(l);
-  const bool near = l > -0.25f;
+  const bool near = l >= kNear;
   return {near ? 1.f + p : e, near ? p : e - 1.f};
 }
 
@@ -44,8 +49,9 @@ struct Gate {
   float alpha, em1;
   float s;  // sqrt(1 - alpha^2)
 };
+template <bool NEAR>
 __device__ __forceinline__ Gate gate_of(float k, float r) {
-  const Decay d = decay_of(k * r);
+  const Decay d = decay_of<NEAR>(k * r);
   return {d.alpha, d.em1, __builtin_amdgcn_sqrtf(-d.em1 * (1.f + d.alpha))};
 }
 
@@ -68,47 +74,57 @@ struct FwdParams {
   const void* cu;
   int cu64;
   int64_t N, T, total, D;
-  unsigned long long* words;  // [tiles][blocks * channels of a block]
+  const float* k;             // [width], where tiles are joined
+  const int* plain;           // [windows]
+  unsigned long long* words;  // [tiles][width], then [groups][width]
   unsigned int* ticket;
+  int64_t tiles, width;  // width: channels of all blocks
   int blocks;
 };
 
-// First token of sequence n (N: the end); without cu_seqlens, N equal runs.
-__device__ __forceinline__ int64_t cu_at(const void* cu, int cu64, int64_t n, int64_t run,
-                                         int64_t total) {
+// First token of sequence n (N: the end), clamped to the batch; without
+// cu_seqlens, N equal runs.  Both types are read as 32-bit words with no
+// branch between them, so that several reads are under way together.
+__device__ __forceinline__ int cu_at(const void* cu, int cu64, int n, int run, int total) {
   if (!cu) return n * run;
-  const int64_t v = cu64 ? static_cast<const int64_t*>(cu)[n]
-                         : static_cast<int64_t>(static_cast<const int32_t*>(cu)[n]);
+  const int* w = static_cast<const int*>(cu) + (static_cast<int64_t>(n) << cu64);
+  const int low = w[0], high = w[cu64];  // int32: the same word
+  const int v = cu64 ? (high == 0 && low >= 0 ? low : (high < 0 ? 0 : total)) : low;
   return v < 0 ? 0 : (v > total ? total : v);
 }
 
 // ---------------------------------------------------------------------------
 // Tiles.  The token axis of the whole batch is cut into windows of kTok tokens,
-// one per wave, and tiles of up to kMaxWaves windows, one per block; a lane
-// has VEC channels (4 bytes of a row), so a block covers 64 VEC channels.  A
+// one per wave, and tiles of up to kFwdWaves (kBwdWaves) windows, one per block; a lane has
+// VEC channels (4 bytes of a row), so a tile covers 64 VEC channels.  A
 // window's tokens are read once and stay in registers as (alpha - 1, input).
 //
 // Any span of tokens maps the state before it to the state after it by
 // h -> A h + B, and a span in which a sequence starts maps every state to the
 // same one (the sequence's own start is part of its B): it is "final", marked
 // by A = -1.  A block joins its waves' spans in LDS.  Between tiles each block
-// publishes its span per channel as one 64-bit word (A, B), waits for the words
-// of the tiles before it, back to a final one, and once it knows the state
-// that enters it, replaces its own word by the final (-1, state).  The state
-// between tiles is always the chain H_k = fma(A_k, H_{k-1}, B_k), whoever
-// computes it and whichever final word it starts from, so the bits do not
-// depend on timing.
+// publishes its span per channel as one 64-bit word (A, B); the last tile of
+// a group of kGroup joins the group's words and publishes the group's span,
+// and once it knows the state that enters the group, replaces it by the final
+// (-1, state behind the group).  A tile needs the words before it in its group
+// and the group's word back to a final one.  The state between groups is
+// always the chain G_k = fma(A_k, G_{k-1}, B_k), whoever computes it and
+// whichever final word it starts from, so the bits do not depend on timing.
+// (With the chain from tile to tile, 2.6 us for every 8 of them, 32,768
+// tokens x 1,024 channels took 97 us.)
 //
 // A block takes its tile from a counter: a tile is waited for only by tiles
 // that were taken after it, so the one taken first of those that still run
-// never waits for a block that has not started, and every wait ends.  Words
-// and counter are cleared by a kernel before.  A word is one atomic access
-// and carries its own validity (kUnset is no pair that is published), so no
-// fences are needed.
+// waits for finished ones only, and every wait ends, whatever blocks are
+// resident.  Words and counter are cleared by a kernel before.  A word is one atomic
+// access and carries its own validity (kUnset is no pair that is published),
+// so no fences are needed.
 // ---------------------------------------------------------------------------
 constexpr int kTok = kWin;
-constexpr int kMaxWaves = 8;
-constexpr int kBack = 16;  // tiles before its own that a block looks at together
+constexpr int kFwdWaves = 8, kBwdWaves = 4;
+constexpr int kFwdOcc = 4, kBwdOcc = 2;  // waves a SIMD holds, by their registers
+constexpr int kGroup = 8;  // tiles of a group
+constexpr int kBack = 4;   // groups before its own that a tile looks at together
 constexpr unsigned long long kUnset = ~0ull;
 
 struct Span {
@@ -141,29 +157,118 @@ __device__ __forceinline__ Span join(Span p, Span s) {
   return {p.A < 0.f ? -1.f : p.A * s.A, fmaf(s.A, p.B, s.B)};
 }
 
-__global__ void __launch_bounds__(256)
-    glr_clear_kernel(unsigned long long* words, int64_t n, unsigned int* ticket) {
+// What the tiles of a pass start from, formed by a kernel before them: no
+// word is set, no tile is taken; the channels' -c softplus(lam), which every
+// window would otherwise form again; and for each window whether all of its
+// tokens are inner ones of one sequence, which most windows' are.
+struct Begin {
+  unsigned long long* words;
+  int64_t num_words;
+  unsigned int* ticket;
+  const float* lam;
+  float c;
+  float* k;
+  int64_t D, width;
+  int* plain;
+  int64_t windows;
+  const void* cu;
+  int cu64, N, run, total;
+};
+__global__ void __launch_bounds__(256) glr_begin_kernel(Begin p) {
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (i < n) words[i] = kUnset;
-  if (i == 0) *ticket = 0;
-}
-
-template <int ALIGN> struct LaneWord;
-template <> struct LaneWord<2> { typedef unsigned int type __attribute__((aligned(2))); };
-template <> struct LaneWord<4> { typedef unsigned int type; };
-
-// A lane's 4 bytes of a row: VEC elements at any address, of which the first
-// `nv` exist.
-template <typename T, int VEC>
-__device__ __forceinline__ unsigned int ld_lane(const T* p, int nv) {
-  static_assert(VEC * sizeof(T) == 4, "4 bytes");
-  using W = typename LaneWord<sizeof(T)>::type;
-  if (nv == VEC) return __builtin_nontemporal_load(reinterpret_cast<const W*>(p));
-  if constexpr (VEC == 2) {
-    if (nv == 1) return __builtin_bit_cast(unsigned short, p[0]);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
+  for (int64_t w = i; w < p.windows; w += step) {
+    const int64_t w0 = w * kTok, w1 = w0 + kTok;
+    int lo = 0, hi = p.N;  // the first sequence that ends behind token w1
+    while (lo < hi) {
+      const int mid = lo + (hi - lo) / 2;
+      if (cu_at(p.cu, p.cu64, mid + 1, p.run, p.total) > w1)
+        hi = mid;
+      else
+        lo = mid + 1;
+    }
+    p.plain[w] = lo < p.N && cu_at(p.cu, p.cu64, lo, p.run, p.total) < w0;
   }
-  return 0;
+  for (int64_t j = i; j < p.width; j += step) p.k[j] = j < p.D ? -p.c * softplus_f32(p.lam[j]) : 0.f;
+  for (int64_t j = i; j < p.num_words; j += step) p.words[j] = kUnset;
+  if (i == 0) *p.ticket = 0;
 }
+
+// The channels of a lane: VEC of them, 4 bytes of a row (2 where a 16-bit row
+// has one channel).  The last lane of an odd D takes the last two channels and
+// answers for the second one only.
+constexpr unsigned int kRange = 1u << 31;  // more than 16 rows span (checked on the host)
+template <int VEC>
+struct Lane {
+  unsigned int off;  // of its first element in the block's rows, kRange: no channels
+  int64_t ch;        // its first channel
+  bool ok[VEC];
+  bool half;  // ok[1] alone
+  bool odd;   // the block has such a lane
+};
+template <typename T, int VEC>
+__device__ __forceinline__ Lane<VEC> lane_of(unsigned int lane, int64_t col, int64_t D) {
+  const int64_t left = D - col - static_cast<int64_t>(lane) * VEC;
+  Lane<VEC> l;
+  l.odd = VEC == 2 && (D & 1) && D - col < kWave * VEC;
+  l.half = VEC == 2 && left == 1;
+  l.ch = col + lane * VEC - l.half;
+  // Rows of an odd block start one element before its channels.
+  l.off = left > 0 ? (lane * VEC + (l.odd && !l.half)) * static_cast<unsigned int>(sizeof(T))
+                   : kRange;
+#pragma unroll
+  for (int u = 0; u < VEC; ++u) l.ok[u] = left > 0 && !(l.half && u == 0);
+  return l;
+}
+
+// A window's rows of one tensor at the block's channels, as a buffer: the row
+// of a token is a scalar offset, a lane's word, at any address, a vector
+// offset that lanes without channels put out of range, where loads give 0 and
+// stores do nothing.
+template <typename T, int VEC>
+struct Rows {
+  __amdgpu_buffer_rsrc_t rsrc;
+  unsigned int pitch;  // bytes
+  __device__ __forceinline__ Rows(const void* p, int64_t row, int64_t pitch_elems, int64_t col,
+                                  bool odd)
+      : rsrc(__builtin_amdgcn_make_buffer_rsrc(
+            const_cast<char*>(static_cast<const char*>(p)) +
+                (row * pitch_elems + col - odd) * static_cast<int64_t>(sizeof(T)),
+            0, kRange, 0x00027000)),
+        pitch(static_cast<unsigned int>(pitch_elems * sizeof(T))) {}
+  __device__ __forceinline__ unsigned int ld(int j, unsigned int off) const {
+    if constexpr (kBytes == 2)
+      return __builtin_amdgcn_raw_buffer_load_b16(rsrc, off, j * pitch, kStream);
+    else
+      return __builtin_amdgcn_raw_buffer_load_b32(rsrc, off, j * pitch, kStream);
+  }
+  // ODD: the block may have a half lane.
+  template <bool ODD>
+  __device__ __forceinline__ void st(int j, const Lane<VEC>& at, const float (&v)[VEC]) const {
+    Arr<T, VEC> t;
+#pragma unroll
+    for (int u = 0; u < VEC; ++u) t.v[u] = from_f32<T>(v[u]);
+    if constexpr (kBytes == 2) {
+      __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, t), rsrc, at.off,
+                                            j * pitch, kStream);
+    } else {
+      const unsigned int w = __builtin_bit_cast(unsigned int, t);
+      if (ODD && VEC == 2 && at.odd) {
+        __builtin_amdgcn_raw_buffer_store_b32(w, rsrc, at.half ? kRange : at.off, j * pitch,
+                                              kStream);
+        __builtin_amdgcn_raw_buffer_store_b16(static_cast<unsigned short>(w >> 16), rsrc,
+                                              at.half ? at.off + 2 : kRange, j * pitch, kStream);
+      } else {
+        __builtin_amdgcn_raw_buffer_store_b32(w, rsrc, at.off, j * pitch, kStream);
+      }
+    }
+  }
+
+ private:
+  static constexpr int kBytes = VEC * sizeof(T);
+  static constexpr int kStream = 2;  // nt: read or written once
+};
+
 template <typename T>
 __device__ __forceinline__ float lane_f32(unsigned int r, int u) {
   if constexpr (sizeof(T) == 4) {
@@ -181,39 +286,57 @@ __device__ __forceinline__ void later(V& v) {
   asm volatile("" : "+v"(v));
 }
 
-template <typename T, int VEC>
-__device__ __forceinline__ void st_lane(T* p, const float (&v)[VEC], int nv) {
-  Arr<T, VEC> t;
+// A lane's -c softplus(lam); `ch`: its place in k, which has one for each word.
+template <int VEC, bool LOOK, typename P>
+__device__ __forceinline__ void ld_k(const P& p, const Lane<VEC>& at, int64_t ch, float (&k)[VEC]) {
 #pragma unroll
-  for (int u = 0; u < VEC; ++u) t.v[u] = from_f32<T>(v[u]);
-  using W = typename LaneWord<sizeof(T)>::type;
-  if (nv == VEC) {
-    unsigned int r;
-    __builtin_memcpy(&r, &t, 4);
-    __builtin_nontemporal_store(r, reinterpret_cast<W*>(p));
-  } else if (VEC == 2 && nv == 1) {
-    p[0] = t.v[0];
+  for (int u = 0; u < VEC; ++u) {
+    if constexpr (LOOK)
+      k[u] = p.k[ch + u - at.half];
+    else
+      k[u] = at.ok[u] ? -p.c * softplus_f32(p.lam[at.ch + u]) : 0.f;
   }
 }
-// fp32 rows of the same channels.
+
+// fp32 rows of the same channels; `p`: at channel 0.
 template <int VEC>
-__device__ __forceinline__ void ld_f32(const float* p, int nv, float (&v)[VEC]) {
+__device__ __forceinline__ void ld_f32(const float* p, const Lane<VEC>& at, float (&v)[VEC]) {
 #pragma unroll
-  for (int u = 0; u < VEC; ++u) v[u] = u < nv ? p[u] : 0.f;
+  for (int u = 0; u < VEC; ++u) v[u] = at.ok[u] ? p[at.ch + u] : 0.f;
 }
 template <int VEC>
-__device__ __forceinline__ void st_f32(float* p, int nv, const float (&v)[VEC]) {
+__device__ __forceinline__ void st_f32(float* p, const Lane<VEC>& at, const float (&v)[VEC]) {
 #pragma unroll
   for (int u = 0; u < VEC; ++u)
-    if (u < nv) p[u] = v[u];
+    if (at.ok[u]) p[at.ch + u] = v[u];
 }
+
+// The sequences' bounds.  The lane's own (of the first 64 sequences) are
+// requested before a window's inputs, so that no wait for them waits for those.
+struct Seqs {
+  const void* cu;
+  int cu64, N, run, total;
+  int t0, t1, lo, hi;
+  __device__ __forceinline__ int operator()(int n) const {
+    return cu_at(cu, cu64, n, run, total);
+  }
+  __device__ __forceinline__ Seqs(const void* c, int c64, int64_t n, int64_t r, int64_t tokens)
+      : cu(c), cu64(c64), N(static_cast<int>(n)), run(static_cast<int>(r)),
+        total(static_cast<int>(tokens)) {
+    const int lane = threadIdx.x % kWave;
+    t0 = (*this)(lane < N ? lane : N);
+    t1 = (*this)(lane < N ? lane + 1 : N);
+    lo = (*this)(0);
+    hi = (*this)(N);
+  }
+};
 
 // Where sequences start and end in a window: bit j of a mask and entry j of a
 // table (the sequence) for token w0 + j.  `lo`, `hi`: the tokens that belong to
 // sequences.
 struct Marks {
   unsigned int starts, ends;
-  int64_t lo, hi;
+  int lo, hi;
 };
 
 // Called by a whole wave; seqs: 2 * kTok entries of LDS of its own.  empty(n) is
@@ -221,192 +344,268 @@ struct Marks {
 // answers for: the ones that stand before one of its tokens, and behind the
 // last token those of the last window.
 template <typename Empty>
-__device__ __forceinline__ Marks find_marks(const void* cu, int cu64, int64_t N, int64_t run,
-                                            int64_t total, int64_t w0, bool last, int* seqs,
-                                            Empty empty) {
-  const int lane = threadIdx.x % kWave;
-  auto at = [&](int64_t n) { return cu_at(cu, cu64, n, run, total); };
+__device__ __forceinline__ Marks find_marks(const Seqs& at, int w0, int* seqs, Empty empty) {
+  const int lane = threadIdx.x % kWave, N = at.N, total = at.total;
+  const bool last = w0 < total + kTok && w0 + kTok >= total;
   Marks m;
-  m.lo = at(0);
-  m.hi = at(N);
-  if (lane < 2 * kTok) seqs[lane] = -1;
+  m.lo = __builtin_amdgcn_readfirstlane(at.lo);
+  m.hi = __builtin_amdgcn_readfirstlane(at.hi);
+  m.starts = m.ends = 0;
+  bool any = false;
   // The first sequence that does not end before the window.
-  int64_t base = 0, len = N;
+  int base = 0, len = N;
   while (len > kWave) {
-    const int64_t step = cdiv(len, kWave);
-    const int64_t q = lane * step + step - 1;
-    const uint64_t hit = __ballot(q >= len - 1 || at(base + q + 1) >= w0);
-    const int64_t f = static_cast<int64_t>(__builtin_ctzll(hit)) * step;
+    const int step = (len - 1) / kWave + 1;
+    const int64_t q = static_cast<int64_t>(lane) * step + step - 1;
+    const uint64_t hit = __ballot(q >= len - 1 || at(base + static_cast<int>(q) + 1) >= w0);
+    const int f = __builtin_ctzll(hit) * step;
     base += f;
     len = len - f < step ? len - f : step;
   }
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  for (; base < N; base += kWave) {
-    const int64_t n = base + lane;
-    int64_t t0 = total, t1 = total;
-    if (n < N) {
-      t0 = at(n);
-      t1 = at(n + 1);
+  for (; base < N; base = base > N - kWave ? N : base + kWave) {
+    const int n = base + lane;  // below 2^31 + 64: compared as unsigned
+    int t0 = at.t0, t1 = at.t1;
+    const bool in = static_cast<unsigned int>(n) < static_cast<unsigned int>(N);
+    if (base > 0) {
+      t0 = at(in ? n : N);
+      t1 = at(in ? n + 1 : N);
     }
-    if (t0 < t1) {
-      if (t0 >= w0 && t0 < w0 + kTok) seqs[t0 - w0] = static_cast<int>(n);
-      if (t1 > w0 && t1 <= w0 + kTok) seqs[kTok + t1 - 1 - w0] = static_cast<int>(n);
+    const unsigned int s = t0 - w0, e = t1 - 1 - w0;
+    const bool starts = t0 < t1 && s < kTok, ends = t0 < t1 && e < kTok;
+    if (__any(starts || ends)) {
+      if (!any && lane < 2 * kTok) seqs[lane] = -1;
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      any = true;
+      if (starts) seqs[s] = n;
+      if (ends) seqs[kTok + e] = n;
     }
-    const bool mine = n < N && t0 >= t1 && t0 >= w0 && (t0 < w0 + kTok || last);
+    const bool mine = in && t0 >= t1 && t0 >= w0 && (t0 < w0 + kTok || last);
     for (uint64_t left = __ballot(mine); left; left &= left - 1)
-      empty(base + __builtin_ctzll(left));
+      empty(static_cast<int64_t>(base) + __builtin_ctzll(left));
     if (!last && __any(t0 >= w0 + kTok)) break;
   }
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  m.starts = static_cast<unsigned int>(__ballot(lane < kTok && seqs[lane & (kTok - 1)] >= 0));
-  m.ends = static_cast<unsigned int>(
-      __ballot(lane < kTok && seqs[kTok + (lane & (kTok - 1))] >= 0));
+  if (any) {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const uint64_t set = __ballot(lane < 2 * kTok && seqs[lane & (2 * kTok - 1)] >= 0);
+    m.starts = static_cast<unsigned int>(set) & ((1u << kTok) - 1);
+    m.ends = static_cast<unsigned int>(set >> kTok) & ((1u << kTok) - 1);
+  }
   return m;
 }
 
-// The state that enters a tile: the words of up to kBack tiles before it
-// (`step` from one to the one before), shared through `look`, until there is
-// a final one among them for every channel.  Called by all waves of a block.
+// The words of a pass: tiles [tiles][width], groups [groups][width].
+struct Words {
+  unsigned long long* tile;
+  unsigned long long* group;
+  int64_t width;
+};
+
+// Publishes the span of tile `at` (counted in the order of the pass, `whole`
+// in the closing wave) and gives the state that enters the tile to all waves
+// of the block; `need`: the tile does not begin with a sequence.
 template <int VEC>
-__device__ __forceinline__ void enter(const unsigned long long* words, int64_t step, int64_t before,
-                                      int lane, int wave, int waves, Span (*look)[kWave * VEC],
-                                      float (&H)[VEC]) {
-  const int reach = static_cast<int>(before < kBack ? before : kBack);
-  for (;;) {
-    for (int d = wave; d < reach; d += waves) {
-      unsigned long long w[VEC];
-      for (;;) {
-        bool unset = false;
+__device__ __forceinline__ void enter(const Words& words, unsigned int at, unsigned int lane,
+                                      int wave, int waves, bool closing, bool need,
+                                      const Span (&whole)[VEC], Span (*look)[kWave * VEC],
+                                      float (*state)[kWave * VEC], float (&H)[VEC]) {
+  const unsigned int group = at / kGroup;
+  const int inside = at % kGroup;
+  const bool leads = inside == kGroup - 1;  // answers for the group's word
+  unsigned long long* mine = words.tile + at * words.width + lane * VEC;
+  if (closing) {
 #pragma unroll
-        for (int u = 0; u < VEC; ++u) {
-          w[u] = peek(words - (d + 1) * step + lane * VEC + u);
-          unset |= w[u] == kUnset;
-        }
-        if (!__any(unset)) break;
-        __builtin_amdgcn_s_sleep(1);
-      }
-#pragma unroll
-      for (int u = 0; u < VEC; ++u) look[d][lane * VEC + u] = unpack(w[u]);
-    }
-    __syncthreads();
-    bool known[VEC];
-#pragma unroll
-    for (int u = 0; u < VEC; ++u) {
-      known[u] = false;
-      H[u] = 0.f;
-    }
-    for (int d = reach - 1; d >= 0; --d) {
+    for (int u = 0; u < VEC; ++u)
+      publish(mine + u, at == 0 ? Span{-1.f, apply(whole[u], 0.f)} : whole[u]);
+  }
+  if (at == 0 || !(need || leads)) return;
+
+  // The words before this tile's in the group: look[d - 1] is d tiles before.
+  for (int d = wave + 1; d <= inside; d += waves) {
+    unsigned long long w[VEC];
+    for (;;) {
+      bool unset = false;
 #pragma unroll
       for (int u = 0; u < VEC; ++u) {
-        const Span s = look[d][lane * VEC + u];
-        known[u] |= s.A < 0.f;
-        H[u] = apply(s, H[u]);
+        w[u] = peek(mine - d * words.width + u);
+        unset |= w[u] == kUnset;
+      }
+      if (!__any(unset)) break;
+      __builtin_amdgcn_s_sleep(1);
+    }
+#pragma unroll
+    for (int u = 0; u < VEC; ++u) look[d - 1][lane * VEC + u] = unpack(w[u]);
+  }
+  __syncthreads();
+  if (closing) {
+    // From the group's start to this tile's, and with this tile.
+    Span head[VEC], all[VEC];
+    bool known = true;
+#pragma unroll
+    for (int u = 0; u < VEC; ++u) head[u] = {1.f, 0.f};
+    for (int d = inside; d > 0; --d) {
+#pragma unroll
+      for (int u = 0; u < VEC; ++u) head[u] = join(head[u], look[d - 1][lane * VEC + u]);
+    }
+    unsigned long long* out = words.group + group * words.width + lane * VEC;
+#pragma unroll
+    for (int u = 0; u < VEC; ++u) {
+      all[u] = join(head[u], whole[u]);
+      if (leads) publish(out + u, all[u]);
+      known &= head[u].A < 0.f;
+    }
+    float G[VEC] = {};  // the state that enters the group
+    if (!__all(known)) {
+      const int back = group < kBack ? static_cast<int>(group) : kBack;
+      for (;;) {
+        unsigned long long w[kBack][VEC];
+#pragma unroll
+        for (int d = 0; d < kBack; ++d)
+#pragma unroll
+          for (int u = 0; u < VEC; ++u)
+            w[d][u] = d < back ? peek(out - (d + 1) * words.width + u) : kUnset;
+        // The nearest word that is final for every channel, if all nearer
+        // ones are set.
+        int last = -1;
+        bool clear = true;
+#pragma unroll
+        for (int d = 0; d < kBack; ++d) {
+          bool unset = false, final = true;
+#pragma unroll
+          for (int u = 0; u < VEC; ++u) {
+            unset |= w[d][u] == kUnset;
+            final &= unpack(w[d][u]).A < 0.f;
+          }
+          if (__any(unset)) clear = false;
+          if (clear && last < 0 && __all(final)) last = d;
+        }
+        if (last >= 0) {
+#pragma unroll
+          for (int d = kBack - 1; d >= 0; --d) {
+            if (d <= last) {
+#pragma unroll
+              for (int u = 0; u < VEC; ++u) G[u] = apply(unpack(w[d][u]), G[u]);
+            }
+          }
+          break;
+        }
+        __builtin_amdgcn_s_sleep(1);
       }
     }
-    bool all = true;
 #pragma unroll
-    for (int u = 0; u < VEC; ++u) all &= known[u];
-    // Every wave read the same words, so all waves leave together.
-    if (__all(all)) return;
-    __syncthreads();
-    __builtin_amdgcn_s_sleep(1);
+    for (int u = 0; u < VEC; ++u) {
+      state[0][lane * VEC + u] = apply(head[u], G[u]);
+      if (leads) publish(out + u, {-1.f, apply(all[u], G[u])});
+    }
   }
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < VEC; ++u) H[u] = state[0][lane * VEC + u];
 }
 
-template <typename T, bool LOOK>
-__global__ void __launch_bounds__(kMaxWaves * kWave) glr_fwd_kernel(FwdParams p) {
-  constexpr int VEC = 4 / sizeof(T);
+template <typename T, int VEC, bool LOOK>
+__global__ void __launch_bounds__(kFwdWaves * kWave, LOOK ? kFwdOcc : 1) glr_fwd_kernel(FwdParams p) {
+  constexpr int kCols = kWave * VEC;
   __shared__ unsigned int taken;
-  __shared__ int seqs[kMaxWaves][2 * kTok];
-  __shared__ Span spans[kMaxWaves][kWave * VEC];
-  __shared__ Span look[LOOK ? kBack : 1][kWave * VEC];
+  __shared__ int seqs[kFwdWaves][2 * kTok];
+  __shared__ Span spans[kFwdWaves][kCols];
+  __shared__ Span look[LOOK ? kGroup - 1 : 1][kCols];
+  __shared__ float state[1][kCols];
   __shared__ int open;  // the tile needs the state before it
 
-  const int lane = threadIdx.x % kWave;
+  const unsigned int lane = threadIdx.x % kWave;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int waves = blockDim.x / kWave;
+  const int total = static_cast<int>(p.total);
   unsigned int id = blockIdx.x;
   if constexpr (LOOK) {
     if (threadIdx.x == 0)
       taken = __hip_atomic_fetch_add(p.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  if constexpr (LOOK) {
     __syncthreads();
     id = __builtin_amdgcn_readfirstlane(taken);
   }
-  const int64_t tile = id / p.blocks;
-  const int blk = id % p.blocks;
-  const int64_t w0 = (tile * waves + wave) * kTok;
-  const int64_t ch = (static_cast<int64_t>(blk) * kWave + lane) * VEC;
-  const int nv = p.D - ch < VEC ? (p.D > ch ? static_cast<int>(p.D - ch) : 0) : VEC;
+  const unsigned int tile = id / static_cast<unsigned int>(p.blocks);
+  const unsigned int blk = id % static_cast<unsigned int>(p.blocks);
+  const int64_t row = (static_cast<int64_t>(tile) * waves + wave) * kTok;
+  const int64_t col = static_cast<int64_t>(blk) * kCols;
+  // Windows behind the last token hold none of them.
+  const int w0 = row < total + kTok ? static_cast<int>(row) : total + kTok;
+  const Lane<VEC> at = lane_of<T, VEC>(lane, col, p.D);
 
+  float k[VEC];
+  const bool plain = LOOK && !at.odd && p.plain[tile * waves + wave];
+  ld_k<VEC, LOOK>(p, at, col + lane * VEC, k);
   // All of the window's loads, before anything else.
   unsigned int x[kTok], a[kTok], b[kTok];
-  const T* xp = static_cast<const T*>(p.x) + w0 * p.sx + ch;
-  const T* ap = static_cast<const T*>(p.a) + w0 * p.sa + ch;
-  const T* bp = static_cast<const T*>(p.b) + w0 * p.sb + ch;
-  if (w0 + kTok <= p.total && (blk + 1) * static_cast<int64_t>(kWave * VEC) <= p.D) {
+  {
+    const Rows<T, VEC> xr(p.x, row, p.sx, col, at.odd), ar(p.a, row, p.sa, col, at.odd),
+        br(p.b, row, p.sb, col, at.odd);
 #pragma unroll
     for (int j = 0; j < kTok; ++j) {
-      x[j] = ld_lane<T, VEC>(xp + j * p.sx, VEC);
-      a[j] = ld_lane<T, VEC>(ap + j * p.sa, VEC);
-      b[j] = ld_lane<T, VEC>(bp + j * p.sb, VEC);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < kTok; ++j) {
-      const int have = w0 + j < p.total ? nv : 0;
-      x[j] = ld_lane<T, VEC>(xp + j * p.sx, have);
-      a[j] = ld_lane<T, VEC>(ap + j * p.sa, have);
-      b[j] = ld_lane<T, VEC>(bp + j * p.sb, have);
+      const unsigned int off = w0 + j < total ? at.off : kRange;
+      a[j] = ar.ld(j, off);
+      b[j] = br.ld(j, off);
+      x[j] = xr.ld(j, off);
     }
   }
-  float k[VEC];
-  ld_f32<VEC>(p.lam + ch, nv, k);
-#pragma unroll
-  for (int u = 0; u < VEC; ++u) k[u] = -p.c * softplus_f32(k[u]);
+  auto seq_row = [&](int n) {
+    return static_cast<int64_t>(__builtin_amdgcn_readfirstlane(n)) * p.D;
+  };
+  Marks m{0, 0, 0, 0};
+  if (!plain) {
+    m = find_marks(Seqs(p.cu, p.cu64, p.N, p.T, p.total), w0, seqs[wave], [&](int64_t n) {
+      if (!p.fin) return;
+      float h[VEC] = {};
+      if (p.h0) ld_f32<VEC>(p.h0 + n * p.D, at, h);
+      st_f32<VEC>(p.fin + n * p.D, at, h);
+    });
+  }
 
-  const Marks m = find_marks(p.cu, p.cu64, p.N, p.T, p.total, w0,
-                             w0 < p.total + kTok && w0 + kTok >= p.total, seqs[wave],
-                             [&](int64_t n) {
-                               if (!p.fin) return;
-                               float h[VEC] = {};
-                               if (p.h0) ld_f32<VEC>(p.h0 + n * p.D + ch, nv, h);
-                               st_f32<VEC>(p.fin + n * p.D + ch, nv, h);
-                             });
-
-  // The window's gates, and its span.
+  // The window's gates, and its span; a start folds its state into the input.
   float em1[kTok][VEC], add[kTok][VEC];
   Span span[VEC];
 #pragma unroll
   for (int u = 0; u < VEC; ++u) span[u] = {1.f, 0.f};
+  auto gates = [&](auto near, auto starts) {
 #pragma unroll
-  for (int j = 0; j < kTok; ++j) {
-#pragma unroll
-    for (int u = 0; u < VEC; ++u) {
-      const Gate g = gate_of(k[u], sigmoid(lane_f32<T>(a[j], u)));
-      em1[j][u] = g.em1;
-      add[j][u] = g.s * (sigmoid(lane_f32<T>(b[j], u)) * lane_f32<T>(x[j], u));
-    }
-    if (m.starts >> j & 1) {
-      float h[VEC] = {};
-      if (p.h0) ld_f32<VEC>(p.h0 + static_cast<int64_t>(seqs[wave][j]) * p.D + ch, nv, h);
+    for (int j = 0; j < kTok; ++j) {
 #pragma unroll
       for (int u = 0; u < VEC; ++u) {
-        add[j][u] += decayed(em1[j][u], h[u]);
-        span[u].B = 0.f;
+        const Gate g = gate_of<near>(k[u], sigmoid(lane_f32<T>(a[j], u)));
+        em1[j][u] = g.em1;
+        add[j][u] = g.s * (sigmoid(lane_f32<T>(b[j], u)) * lane_f32<T>(x[j], u));
+      }
+      if (starts && (m.starts >> j & 1)) {
+        float h[VEC] = {};
+        if (p.h0) ld_f32<VEC>(p.h0 + seq_row(seqs[wave][j]), at, h);
+#pragma unroll
+        for (int u = 0; u < VEC; ++u) {
+          add[j][u] += decayed(em1[j][u], h[u]);
+          span[u].B = 0.f;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < VEC; ++u) {
+        span[u].A = decayed(em1[j][u], span[u].A);
+        span[u].B = decayed(em1[j][u], span[u].B) + add[j][u];
       }
     }
+    if (starts && m.starts) {
 #pragma unroll
-    for (int u = 0; u < VEC; ++u) {
-      span[u].A = decayed(em1[j][u], span[u].A);
-      span[u].B = decayed(em1[j][u], span[u].B) + add[j][u];
+      for (int u = 0; u < VEC; ++u) span[u].A = -1.f;
     }
-  }
+  };
+  bool near = true;
 #pragma unroll
-  for (int u = 0; u < VEC; ++u) {
-    if (m.starts) span[u].A = -1.f;
-    spans[wave][lane * VEC + u] = span[u];
-  }
-  if (wave == 0 && lane == 0) open = !(m.starts & 1);
+  for (int u = 0; u < VEC; ++u) near &= k[u] >= kNear;
+  if (plain && __all(near))
+    gates(std::true_type(), std::false_type());
+  else
+    gates(std::false_type(), std::true_type());
+#pragma unroll
+  for (int u = 0; u < VEC; ++u) spans[wave][lane * VEC + u] = span[u];
+  if (threadIdx.x == 0) open = !(m.starts & 1);
   __syncthreads();
 
   // From the tile's start to this window's.
@@ -417,37 +616,27 @@ __global__ void __launch_bounds__(kMaxWaves * kWave) glr_fwd_kernel(FwdParams p)
 #pragma unroll
     for (int u = 0; u < VEC; ++u) head[u] = join(head[u], spans[w][lane * VEC + u]);
   }
-  float H[VEC] = {};
+  float h[VEC] = {};
   if constexpr (LOOK) {
-    const int64_t width = static_cast<int64_t>(p.blocks) * kWave * VEC;
-    unsigned long long* words = p.words + tile * width + static_cast<int64_t>(blk) * kWave * VEC;
+    const Words words{p.words + col, p.words + p.tiles * p.width + col, p.width};
     Span whole[VEC];
-    const bool closing = wave == waves - 1;
-    if (closing) {
 #pragma unroll
-      for (int u = 0; u < VEC; ++u) {
-        whole[u] = join(head[u], span[u]);
-        if (tile == 0) whole[u].A = -1.f;
-        publish(words + lane * VEC + u, whole[u]);
-      }
-    }
-    if (tile > 0 && open) {
-      enter<VEC>(words, width, tile, lane, wave, waves, look, H);
-      if (closing) {
-#pragma unroll
-        for (int u = 0; u < VEC; ++u)
-          if (!(whole[u].A < 0.f))
-            publish(words + lane * VEC + u, {-1.f, apply(whole[u], H[u])});
-      }
-    }
+    for (int u = 0; u < VEC; ++u) whole[u] = join(head[u], span[u]);
+    enter<VEC>(words, tile, lane, wave, waves, wave == waves - 1, open, whole, look, state, h);
   }
-
-  float h[VEC];
 #pragma unroll
-  for (int u = 0; u < VEC; ++u) h[u] = apply(head[u], H[u]);
-  if (p.states && w0 < p.total) st_f32<VEC>(p.states + w0 / kWin * p.D + ch, nv, h);
-  T* yp = static_cast<T*>(p.y) + w0 * p.sy + ch;
-  const bool whole_window = w0 >= m.lo && w0 + kTok <= m.hi;
+  for (int u = 0; u < VEC; ++u) h[u] = apply(head[u], h[u]);
+  if (p.states && w0 < total) st_f32<VEC>(p.states + row / kWin * p.D, at, h);
+  const Rows<T, VEC> yr(p.y, row, p.sy, col, at.odd);
+  if (plain) {
+#pragma unroll
+    for (int j = 0; j < kTok; ++j) {
+#pragma unroll
+      for (int u = 0; u < VEC; ++u) h[u] = decayed(em1[j][u], h[u]) + add[j][u];
+      yr.template st<false>(j, at, h);
+    }
+    return;
+  }
 #pragma unroll
   for (int j = 0; j < kTok; ++j) {
     if (m.starts >> j & 1) {
@@ -456,10 +645,8 @@ __global__ void __launch_bounds__(kMaxWaves * kWave) glr_fwd_kernel(FwdParams p)
     }
 #pragma unroll
     for (int u = 0; u < VEC; ++u) h[u] = decayed(em1[j][u], h[u]) + add[j][u];
-    if (whole_window || (w0 + j >= m.lo && w0 + j < m.hi))
-      st_lane<T, VEC>(yp + j * p.sy, h, nv);
-    if ((m.ends >> j & 1) && p.fin)
-      st_f32<VEC>(p.fin + static_cast<int64_t>(seqs[wave][kTok + j]) * p.D + ch, nv, h);
+    if (w0 + j >= m.lo && w0 + j < m.hi) yr.template st<true>(j, at, h);
+    if ((m.ends >> j & 1) && p.fin) st_f32<VEC>(p.fin + seq_row(seqs[wave][kTok + j]), at, h);
   }
 }
 
@@ -478,30 +665,54 @@ inline Cut cut_of(int64_t total, int64_t D, int vec, int max_waves) {
   c.width = static_cast<int64_t>(c.blocks) * kWave * vec;
   return c;
 }
-// Bytes of a pass's counter (its own cache line) and words; none for one tile.
-inline int64_t words_bytes(const Cut& c) { return c.tiles > 1 ? 256 + c.tiles * c.width * 8 : 0; }
-
-inline void clear_words(const Cut& c, void* workspace, hipStream_t s) {
-  const int64_t n = c.tiles * c.width;
-  hipLaunchKernelGGL(glr_clear_kernel, dim3(cdiv(n, 256)), dim3(256), 0, s,
-                     reinterpret_cast<unsigned long long*>(static_cast<char*>(workspace) + 256), n,
-                     static_cast<unsigned int*>(workspace));
+// The workspace of a pass: its counter (a cache line of its own), its
+// channels' k, its windows' flags and the words of its tiles and groups; none
+// for one tile.
+inline int64_t up256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+inline int64_t words_of(const Cut& c) { return (c.tiles + cdiv(c.tiles, kGroup)) * c.width; }
+inline int64_t words_bytes(const Cut& c) {
+  if (c.tiles == 1) return 0;
+  return 256 + up256(c.width * 4) + up256(c.tiles * c.waves * 4) + words_of(c) * 8;
 }
 
-template <typename T>
-int launch_fwd(FwdParams p, void* workspace, hipStream_t s) {
-  const Cut c = cut_of(p.total, p.D, 4 / sizeof(T), kMaxWaves);
+// Lays a pass out in p and starts the kernel that readies its workspace.
+template <typename P>
+void begin(P& p, const Cut& c, void* workspace, hipStream_t s) {
   p.blocks = c.blocks;
+  p.tiles = c.tiles;
+  p.width = c.width;
+  if (c.tiles == 1) return;
+  char* at = static_cast<char*>(workspace);
+  p.ticket = reinterpret_cast<unsigned int*>(at);
+  float* k = reinterpret_cast<float*>(at += 256);
+  int* plain = reinterpret_cast<int*>(at += up256(c.width * 4));
+  p.words = reinterpret_cast<unsigned long long*>(at += up256(c.tiles * c.waves * 4));
+  p.k = k;
+  p.plain = plain;
+  const Begin b{p.words, words_of(c), p.ticket, p.lam, p.c, k, p.D, c.width, plain,
+                c.tiles * c.waves, p.cu, p.cu64, static_cast<int>(p.N), static_cast<int>(p.T),
+                static_cast<int>(p.total)};
+  const int64_t grid = std::min<int64_t>(cdiv(b.num_words, 4 * 256), 4 * num_cus());
+  hipLaunchKernelGGL(glr_begin_kernel, dim3(grid), dim3(256), 0, s, b);
+}
+
+template <typename T, int VEC>
+int launch_fwd_vec(FwdParams p, void* workspace, hipStream_t s) {
+  const Cut c = cut_of(p.total, p.D, VEC, kFwdWaves);
+  begin(p, c, workspace, s);
   const dim3 grid(c.tiles * c.blocks), block(c.waves * kWave);
-  if (c.tiles > 1) {
-    p.ticket = static_cast<unsigned int*>(workspace);
-    p.words = reinterpret_cast<unsigned long long*>(static_cast<char*>(workspace) + 256);
-    clear_words(c, workspace, s);
-    hipLaunchKernelGGL((glr_fwd_kernel<T, true>), grid, block, 0, s, p);
-  } else {
-    hipLaunchKernelGGL((glr_fwd_kernel<T, false>), grid, block, 0, s, p);
-  }
+  if (c.tiles > 1)
+    hipLaunchKernelGGL((glr_fwd_kernel<T, VEC, true>), grid, block, 0, s, p);
+  else
+    hipLaunchKernelGGL((glr_fwd_kernel<T, VEC, false>), grid, block, 0, s, p);
   return launch_status();
+}
+template <typename T>
+int launch_fwd(const FwdParams& p, void* workspace, hipStream_t s) {
+  if constexpr (sizeof(T) == 2) {
+    if (p.D > 1) return launch_fwd_vec<T, 2>(p, workspace, s);
+  }
+  return launch_fwd_vec<T, 1>(p, workspace, s);
 }
 
 struct UpdateParams {
@@ -541,7 +752,7 @@ __global__ void __launch_bounds__(64) glr_update_kernel(UpdateParams p) {
     const float x = to_f32(static_cast<const T*>(p.x)[t * p.sx + ch]);
     const float r = sigmoid(to_f32(static_cast<const T*>(p.a)[t * p.sa + ch]));
     const float i = sigmoid(to_f32(static_cast<const T*>(p.b)[t * p.sb + ch]));
-    const Gate g = gate_of(k, r);
+    const Gate g = gate_of<false>(k, r);
     h = decayed(g.em1, h) + g.s * (i * x);
     static_cast<T*>(p.y)[t * p.sy + ch] = from_f32<T>(h);
     if (p.cols > 0 && t - t0 < p.cols) {
@@ -571,9 +782,11 @@ struct BwdParams {
   const void* cu;
   int cu64;
   int64_t N, T, total, D;
+  const float* k;
+  const int* plain;
   unsigned long long* words;
   unsigned int* ticket;
-  int64_t tiles;
+  int64_t tiles, width;
   int blocks;
 };
 
@@ -604,103 +817,112 @@ __device__ __forceinline__ float exp_neg(float v) {
 //    and dlam = sum E sigmoid(lam) / softplus(lam), with no division by what
 //    vanishes as a gate closes: l / s -> 0 with s.
 // ---------------------------------------------------------------------------
-constexpr int kBwdWaves = 4;
-
-template <typename T, bool LOOK>
-__global__ void __launch_bounds__(kBwdWaves * kWave) glr_bwd_kernel(BwdParams p) {
-  constexpr int VEC = 4 / sizeof(T);
+template <typename T, int VEC, bool LOOK>
+__global__ void __launch_bounds__(kBwdWaves * kWave, LOOK ? kBwdOcc : 1) glr_bwd_kernel(BwdParams p) {
+  constexpr int kCols = kWave * VEC;
   __shared__ unsigned int taken;
   __shared__ int seqs[kBwdWaves][2 * kTok];
-  __shared__ Span spans[kBwdWaves][kWave * VEC];
-  __shared__ Span look[LOOK ? kBack : 1][kWave * VEC];
-  __shared__ float sums[kBwdWaves][kWave * VEC];
+  __shared__ Span spans[kBwdWaves][kCols];
+  __shared__ Span look[LOOK ? kGroup - 1 : 1][kCols];
+  __shared__ float state[1][kCols];
+  __shared__ float sums[kBwdWaves][kCols];
   __shared__ int open;  // the tile needs the gradient from behind it
 
-  const int lane = threadIdx.x % kWave;
+  const unsigned int lane = threadIdx.x % kWave;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int waves = blockDim.x / kWave;
+  const int total = static_cast<int>(p.total);
   unsigned int id = blockIdx.x;
   if constexpr (LOOK) {
     if (threadIdx.x == 0)
       taken = __hip_atomic_fetch_add(p.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  if constexpr (LOOK) {
     __syncthreads();
     id = __builtin_amdgcn_readfirstlane(taken);
   }
-  const int64_t after = id / p.blocks;  // tiles behind this one
-  const int64_t tile = p.tiles - 1 - after;
-  const int blk = id % p.blocks;
-  const int64_t w0 = (tile * waves + wave) * kTok;
-  const int64_t ch = (static_cast<int64_t>(blk) * kWave + lane) * VEC;
-  const int nv = p.D - ch < VEC ? (p.D > ch ? static_cast<int>(p.D - ch) : 0) : VEC;
+  // Tiles are counted from the end here.
+  const unsigned int behind = id / static_cast<unsigned int>(p.blocks);
+  const unsigned int blk = id % static_cast<unsigned int>(p.blocks);
+  const int64_t tile = p.tiles - 1 - behind;
+  const int64_t row = (tile * waves + wave) * kTok;
+  const int64_t col = static_cast<int64_t>(blk) * kCols;
+  const int w0 = row < total + kTok ? static_cast<int>(row) : total + kTok;
+  const Lane<VEC> at = lane_of<T, VEC>(lane, col, p.D);
 
+  float k[VEC], h[VEC] = {};
+  const bool plain = LOOK && !at.odd && p.plain[tile * waves + wave];
+  ld_k<VEC, LOOK>(p, at, col + lane * VEC, k);
+  if (w0 < total) ld_f32<VEC>(p.states + row / kWin * p.D, at, h);
   unsigned int x[kTok], dy[kTok], a[kTok], b[kTok];
-  const T* xp = static_cast<const T*>(p.x) + w0 * p.sx + ch;
-  const T* ap = static_cast<const T*>(p.a) + w0 * p.sa + ch;
-  const T* bp = static_cast<const T*>(p.b) + w0 * p.sb + ch;
-  const T* gp = static_cast<const T*>(p.dy) + w0 * p.sdy + ch;
-  if (w0 + kTok <= p.total && (blk + 1) * static_cast<int64_t>(kWave * VEC) <= p.D) {
+  {
+    const Rows<T, VEC> xr(p.x, row, p.sx, col, at.odd), ar(p.a, row, p.sa, col, at.odd),
+        br(p.b, row, p.sb, col, at.odd), gr(p.dy, row, p.sdy, col, at.odd);
 #pragma unroll
     for (int j = 0; j < kTok; ++j) {
-      a[j] = ld_lane<T, VEC>(ap + j * p.sa, VEC);
-      b[j] = ld_lane<T, VEC>(bp + j * p.sb, VEC);
-      x[j] = ld_lane<T, VEC>(xp + j * p.sx, VEC);
-      dy[j] = ld_lane<T, VEC>(gp + j * p.sdy, VEC);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < kTok; ++j) {
-      const int have = w0 + j < p.total ? nv : 0;
-      a[j] = ld_lane<T, VEC>(ap + j * p.sa, have);
-      b[j] = ld_lane<T, VEC>(bp + j * p.sb, have);
-      x[j] = ld_lane<T, VEC>(xp + j * p.sx, have);
-      dy[j] = ld_lane<T, VEC>(gp + j * p.sdy, have);
+      const unsigned int off = w0 + j < total ? at.off : kRange;
+      a[j] = ar.ld(j, off);
+      b[j] = br.ld(j, off);
+      x[j] = xr.ld(j, off);
+      dy[j] = gr.ld(j, off);
     }
   }
-  float k[VEC], h[VEC] = {};
-  ld_f32<VEC>(p.lam + ch, nv, k);
-  if (w0 < p.total) ld_f32<VEC>(p.states + w0 / kWin * p.D + ch, nv, h);
-#pragma unroll
-  for (int u = 0; u < VEC; ++u) k[u] = -p.c * softplus_f32(k[u]);
-
-  const Marks m = find_marks(p.cu, p.cu64, p.N, p.T, p.total, w0,
-                             w0 < p.total + kTok && w0 + kTok >= p.total, seqs[wave],
-                             [&](int64_t n) {
-                               if (!p.dh0) return;
-                               float q[VEC] = {};
-                               if (p.dfin) ld_f32<VEC>(p.dfin + n * p.D + ch, nv, q);
-                               st_f32<VEC>(p.dh0 + n * p.D + ch, nv, q);
-                             });
+  auto seq_row = [&](int n) {
+    return static_cast<int64_t>(__builtin_amdgcn_readfirstlane(n)) * p.D;
+  };
+  Marks m{0, 0, 0, 0};
+  if (!plain) {
+    m = find_marks(Seqs(p.cu, p.cu64, p.N, p.T, p.total), w0, seqs[wave], [&](int64_t n) {
+      if (!p.dh0) return;
+      float q[VEC] = {};
+      if (p.dfin) ld_f32<VEC>(p.dfin + n * p.D, at, q);
+      st_f32<VEC>(p.dh0 + n * p.D, at, q);
+    });
+  }
 
   float before[kTok][VEC], ea[kTok][VEC], eb[kTok][VEC];
   Span span[VEC];
 #pragma unroll
   for (int u = 0; u < VEC; ++u) span[u] = {1.f, 0.f};
+  auto first = [&](auto near, auto marks) {
 #pragma unroll
-  for (int j = 0; j < kTok; ++j) {
-    if (m.starts >> j & 1) {
+    for (int j = 0; j < kTok; ++j) {
+      if (marks && (m.starts >> j & 1)) {
 #pragma unroll
-      for (int u = 0; u < VEC; ++u) h[u] = 0.f;
-      if (p.h0) ld_f32<VEC>(p.h0 + static_cast<int64_t>(seqs[wave][j]) * p.D + ch, nv, h);
-    }
+        for (int u = 0; u < VEC; ++u) h[u] = 0.f;
+        if (p.h0) ld_f32<VEC>(p.h0 + seq_row(seqs[wave][j]), at, h);
+      }
+      // No sequence ended before this token: the gradient comes this far.
+      const bool reached = !marks || !(m.ends & ((1u << j) - 1));
 #pragma unroll
-    for (int u = 0; u < VEC; ++u) {
-      ea[j][u] = exp_neg(lane_f32<T>(a[j], u));
-      eb[j][u] = exp_neg(lane_f32<T>(b[j], u));
-      const Gate g = gate_of(k[u], fast_rcp(1.f + ea[j][u]));
-      before[j][u] = h[u];
-      h[u] = decayed(g.em1, h[u]) + g.s * (fast_rcp(1.f + eb[j][u]) * lane_f32<T>(x[j], u));
-      if (!(m.ends & ((1u << j) - 1))) {  // no sequence ended before: q comes this far
-        span[u].A = decayed(g.em1, span[u].A);
-        span[u].B = fmaf(span[u].A, lane_f32<T>(dy[j], u), span[u].B);
+      for (int u = 0; u < VEC; ++u) {
+        ea[j][u] = exp_neg(lane_f32<T>(a[j], u));
+        eb[j][u] = exp_neg(lane_f32<T>(b[j], u));
+        const Gate g = gate_of<near>(k[u], fast_rcp(1.f + ea[j][u]));
+        before[j][u] = h[u];
+        h[u] = decayed(g.em1, h[u]) +
+               g.s * (fast_rcp(1.f + eb[j][u]) * lane_f32<T>(x[j], u));
+        if (reached) {
+          span[u].A = decayed(g.em1, span[u].A);
+          span[u].B = fmaf(span[u].A, lane_f32<T>(dy[j], u), span[u].B);
+        }
+      }
+      if (marks && reached && (m.ends >> j & 1) && p.dfin) {
+        float q[VEC];
+        ld_f32<VEC>(p.dfin + seq_row(seqs[wave][kTok + j]), at, q);
+#pragma unroll
+        for (int u = 0; u < VEC; ++u) span[u].B = fmaf(span[u].A, q[u], span[u].B);
       }
     }
-    if ((m.ends >> j & 1) && !(m.ends & ((1u << j) - 1)) && p.dfin) {
-      float q[VEC];
-      ld_f32<VEC>(p.dfin + static_cast<int64_t>(seqs[wave][kTok + j]) * p.D + ch, nv, q);
+  };
+  bool near = true;
 #pragma unroll
-      for (int u = 0; u < VEC; ++u) span[u].B = fmaf(span[u].A, q[u], span[u].B);
-    }
-  }
+  for (int u = 0; u < VEC; ++u) near &= k[u] >= kNear;
+  const bool fast = plain && __all(near);
+  if (fast)
+    first(std::true_type(), std::false_type());
+  else
+    first(std::false_type(), std::true_type());
 #pragma unroll
   for (int u = 0; u < VEC; ++u) {
     if (m.ends) span[u].A = -1.f;
@@ -717,30 +939,16 @@ __global__ void __launch_bounds__(kBwdWaves * kWave) glr_bwd_kernel(BwdParams p)
 #pragma unroll
     for (int u = 0; u < VEC; ++u) head[u] = join(head[u], spans[w][lane * VEC + u]);
   }
-  float Q[VEC] = {};
+  float q[VEC] = {};
   if constexpr (LOOK) {
-    const int64_t width = static_cast<int64_t>(p.blocks) * kWave * VEC;
-    unsigned long long* words = p.words + after * width + static_cast<int64_t>(blk) * kWave * VEC;
+    const Words words{p.words + col, p.words + p.tiles * p.width + col, p.width};
     Span whole[VEC];
-    if (wave == 0) {
 #pragma unroll
-      for (int u = 0; u < VEC; ++u) {
-        whole[u] = join(head[u], span[u]);
-        if (after == 0) whole[u].A = -1.f;
-        publish(words + lane * VEC + u, whole[u]);
-      }
-    }
-    if (after > 0 && open) {
-      enter<VEC>(words, width, after, lane, wave, waves, look, Q);
-      if (wave == 0) {
-#pragma unroll
-        for (int u = 0; u < VEC; ++u)
-          if (!(whole[u].A < 0.f))
-            publish(words + lane * VEC + u, {-1.f, apply(whole[u], Q[u])});
-      }
-    }
+    for (int u = 0; u < VEC; ++u) whole[u] = join(head[u], span[u]);
+    enter<VEC>(words, behind, lane, wave, waves, wave == 0, open, whole, look, state, q);
   }
-
+#pragma unroll
+  for (int u = 0; u < VEC; ++u) q[u] = apply(head[u], q[u]);
 #pragma unroll
   for (int j = 0; j < kTok; ++j) {
     later(x[j]);
@@ -751,47 +959,48 @@ __global__ void __launch_bounds__(kBwdWaves * kWave) glr_bwd_kernel(BwdParams p)
       later(eb[j][u]);
     }
   }
-  float q[VEC], sum[VEC] = {};
+  float sum[VEC] = {};
+  const Rows<T, VEC> dxr(p.dx, row, p.sdx, col, at.odd), dar(p.da, row, p.sda, col, at.odd),
+      dbr(p.db, row, p.sdb, col, at.odd);
+  auto second = [&](auto near, auto marks) {
 #pragma unroll
-  for (int u = 0; u < VEC; ++u) q[u] = apply(head[u], Q[u]);
-  T* dxp = static_cast<T*>(p.dx) + w0 * p.sdx + ch;
-  T* dap = static_cast<T*>(p.da) + w0 * p.sda + ch;
-  T* dbp = static_cast<T*>(p.db) + w0 * p.sdb + ch;
-  const bool whole_window = w0 >= m.lo && w0 + kTok <= m.hi;
+    for (int j = kTok - 1; j >= 0; --j) {
+      if (marks && (m.ends >> j & 1)) {
 #pragma unroll
-  for (int j = kTok - 1; j >= 0; --j) {
-    if (m.ends >> j & 1) {
+        for (int u = 0; u < VEC; ++u) q[u] = 0.f;
+        if (p.dfin) ld_f32<VEC>(p.dfin + seq_row(seqs[wave][kTok + j]), at, q);
+      }
+      const bool live = !marks || plain || (w0 + j >= m.lo && w0 + j < m.hi);
+      float dx[VEC], da[VEC], db[VEC];
 #pragma unroll
-      for (int u = 0; u < VEC; ++u) q[u] = 0.f;
-      if (p.dfin)
-        ld_f32<VEC>(p.dfin + static_cast<int64_t>(seqs[wave][kTok + j]) * p.D + ch, nv, q);
+      for (int u = 0; u < VEC; ++u) {
+        const float r = fast_rcp(1.f + ea[j][u]), i = fast_rcp(1.f + eb[j][u]);
+        const float xf = lane_f32<T>(x[j], u), l = k[u] * r;
+        const Decay d = decay_of<near>(l);
+        const float w = -d.em1 * (1.f + d.alpha);  // s^2
+        // The instruction takes a denormal w for 0.
+        const float inv = w >= 1.17549435e-38f ? __builtin_amdgcn_rsqf(w) : 0.f;
+        const float G = lane_f32<T>(dy[j], u) + q[u];
+        dx[u] = G * (w * inv) * i;
+        db[u] = dx[u] * xf * (eb[j][u] * i);
+        const float e = G * d.alpha * (before[j][u] * l - i * xf * d.alpha * (l * inv));
+        da[u] = e * (ea[j][u] * r);
+        if (live) sum[u] += e;
+        q[u] = decayed(d.em1, G);
+      }
+      if (live) {
+        dxr.template st<marks>(j, at, dx);
+        dar.template st<marks>(j, at, da);
+        dbr.template st<marks>(j, at, db);
+      }
+      if (marks && (m.starts >> j & 1) && p.dh0)
+        st_f32<VEC>(p.dh0 + seq_row(seqs[wave][j]), at, q);
     }
-    const bool live = whole_window || (w0 + j >= m.lo && w0 + j < m.hi);
-    float dx[VEC], da[VEC], db[VEC];
-#pragma unroll
-    for (int u = 0; u < VEC; ++u) {
-      const float r = fast_rcp(1.f + ea[j][u]), i = fast_rcp(1.f + eb[j][u]);
-      const float xf = lane_f32<T>(x[j], u), l = k[u] * r;
-      const Decay d = decay_of(l);
-      const float w = -d.em1 * (1.f + d.alpha);  // s^2
-      // The instruction takes a denormal w for 0.
-      const float inv = w >= 1.17549435e-38f ? __builtin_amdgcn_rsqf(w) : 0.f;
-      const float G = lane_f32<T>(dy[j], u) + q[u];
-      dx[u] = G * (w * inv) * i;
-      db[u] = dx[u] * xf * (eb[j][u] * i);
-      const float e = G * d.alpha * (before[j][u] * l - i * xf * d.alpha * (l * inv));
-      da[u] = e * (ea[j][u] * r);
-      if (live) sum[u] += e;
-      q[u] = decayed(d.em1, G);
-    }
-    if (live) {
-      st_lane<T, VEC>(dxp + j * p.sdx, dx, nv);
-      st_lane<T, VEC>(dap + j * p.sda, da, nv);
-      st_lane<T, VEC>(dbp + j * p.sdb, db, nv);
-    }
-    if ((m.starts >> j & 1) && p.dh0)
-      st_f32<VEC>(p.dh0 + static_cast<int64_t>(seqs[wave][j]) * p.D + ch, nv, q);
-  }
+  };
+  if (fast)
+    second(std::true_type(), std::false_type());
+  else
+    second(std::false_type(), std::true_type());
   if (p.part) {
 #pragma unroll
     for (int u = 0; u < VEC; ++u) sums[wave][lane * VEC + u] = sum[u];
@@ -801,7 +1010,7 @@ __global__ void __launch_bounds__(kBwdWaves * kWave) glr_bwd_kernel(BwdParams p)
 #pragma unroll
         for (int u = 0; u < VEC; ++u) sum[u] += sums[w][lane * VEC + u];
       }
-      st_f32<VEC>(p.part + tile * p.D + ch, nv, sum);
+      st_f32<VEC>(p.part + tile * p.D, at, sum);
     }
   }
 }
@@ -826,23 +1035,25 @@ __global__ void __launch_bounds__(1024) glr_dlam_kernel(const float* part, int64
   }
 }
 
-template <typename T>
-int launch_bwd(BwdParams p, bool sums, void* workspace, hipStream_t s) {
-  const Cut c = cut_of(p.total, p.D, 4 / sizeof(T), kBwdWaves);
-  p.blocks = c.blocks;
-  p.tiles = c.tiles;
-  // The workspace: counter and words, then dlam's parts.
+template <typename T, int VEC>
+int launch_bwd_vec(BwdParams p, bool sums, void* workspace, hipStream_t s) {
+  const Cut c = cut_of(p.total, p.D, VEC, kBwdWaves);
+  // The workspace: counter, k and words, then dlam's parts.
   if (sums) p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + words_bytes(c));
+  begin(p, c, workspace, s);
   const dim3 grid(c.tiles * c.blocks), block(c.waves * kWave);
-  if (c.tiles > 1) {
-    p.ticket = static_cast<unsigned int*>(workspace);
-    p.words = reinterpret_cast<unsigned long long*>(static_cast<char*>(workspace) + 256);
-    clear_words(c, workspace, s);
-    hipLaunchKernelGGL((glr_bwd_kernel<T, true>), grid, block, 0, s, p);
-  } else {
-    hipLaunchKernelGGL((glr_bwd_kernel<T, false>), grid, block, 0, s, p);
-  }
+  if (c.tiles > 1)
+    hipLaunchKernelGGL((glr_bwd_kernel<T, VEC, true>), grid, block, 0, s, p);
+  else
+    hipLaunchKernelGGL((glr_bwd_kernel<T, VEC, false>), grid, block, 0, s, p);
   return launch_status();
+}
+template <typename T>
+int launch_bwd(const BwdParams& p, bool sums, void* workspace, hipStream_t s) {
+  if constexpr (sizeof(T) == 2) {
+    if (p.D > 1) return launch_bwd_vec<T, 2>(p, sums, workspace, s);
+  }
+  return launch_bwd_vec<T, 1>(p, sums, workspace, s);
 }
 
 // Tokens, sequences and tiles are counted in 31 bits, a batch's elements in 62.
@@ -852,7 +1063,10 @@ bool bad_sizes(int64_t N, int64_t total, int64_t D) {
          cdiv(std::max<int64_t>(total, 1), kTok) * cdiv(D, kWave) >= kMost;
 }
 
-bool pitch_ok(int64_t pitch, int64_t D) { return pitch >= D; }
+// A window's rows have to lie within kRange bytes.
+bool pitch_ok(int64_t pitch, int64_t D) {
+  return pitch >= D && pitch < static_cast<int64_t>(kRange / (4 * kTok));
+}
 
 // cu_seqlens of a readable type, or none and N equal runs.
 bool seqs_ok(const void* cu, xk_dtype dt, int64_t N, int64_t total) {
@@ -867,8 +1081,8 @@ using namespace xk;
 extern "C" int64_t xk_gated_linear_recurrence_workspace_bytes(int64_t total_tokens, int64_t D) {
   if (total_tokens <= 0 || D <= 0) return 0;
   // 4-byte elements take more, narrower channel blocks.
-  return std::max(words_bytes(cut_of(total_tokens, D, 1, kMaxWaves)),
-                  words_bytes(cut_of(total_tokens, D, 2, kMaxWaves)));
+  return std::max(words_bytes(cut_of(total_tokens, D, 1, kFwdWaves)),
+                  words_bytes(cut_of(total_tokens, D, 2, kFwdWaves)));
 }
 
 extern "C" int xk_gated_linear_recurrence(
@@ -891,7 +1105,7 @@ extern "C" int xk_gated_linear_recurrence(
     return XK_ERR_WORKSPACE;
   const FwdParams p{x, a, b, y, stride_x_tok, stride_a_tok, stride_b_tok, stride_y_tok, lam, c,
                     initial_state, final_state, states, cu_seqlens, cu_dtype == XK_I64, N,
-                    total_tokens / N, total_tokens, D, nullptr, nullptr, 0};
+                    total_tokens / N, total_tokens, D, nullptr, nullptr, nullptr, nullptr, 0, 0, 0};
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (dtype) {
     case XK_F32: return launch_fwd<float>(p, workspace, s);
@@ -963,14 +1177,14 @@ extern "C" int xk_gated_linear_recurrence_bwd(
                       stride_b_tok, stride_dx_tok, stride_da_tok, stride_db_tok, lam, c, states,
                       initial_state, d_final_state, d_initial_state, nullptr, cu_seqlens,
                       cu_dtype == XK_I64, N, total_tokens / N, total_tokens, D, nullptr, nullptr,
-                      0, 0};
+                      nullptr, nullptr, 0, 0, 0};
     const int st = dtype == XK_F32    ? launch_bwd<float>(p, dlam, workspace, s)
                    : dtype == XK_BF16 ? launch_bwd<bf16>(p, dlam, workspace, s)
                                       : launch_bwd<f16>(p, dlam, workspace, s);
     if (st != XK_OK) return st;
   }
   if (dlam) {
-    const Cut cut = cut_of(total_tokens, D, dtype == XK_F32 ? 1 : 2, kBwdWaves);
+    const Cut cut = cut_of(total_tokens, D, dtype == XK_F32 || D == 1 ? 1 : 2, kBwdWaves);
     const float* part = N > 0 ? reinterpret_cast<const float*>(static_cast<char*>(workspace) +
                                                                words_bytes(cut))
                               : nullptr;
