@@ -123,7 +123,7 @@ __device__ __forceinline__ int cu_at(const void* cu, int cu64, int n, int run, i
 constexpr int kTok = kWin;
 constexpr int kFwdWaves = 8, kBwdWaves = 4;
 constexpr int kFwdOcc = 4, kBwdOcc = 2;  // waves a SIMD holds, by their registers
-constexpr int kGroup = 8;  // tiles of a group
+constexpr int kGroup = 4;  // tiles of a group
 constexpr int kBack = 4;   // groups before its own that a tile looks at together
 constexpr unsigned long long kUnset = ~0ull;
 
@@ -401,13 +401,14 @@ struct Words {
 };
 
 // Publishes the span of tile `at` (counted in the order of the pass, `whole`
-// in the closing wave) and gives the state that enters the tile to all waves
+// in the wave `closer`) and gives the state that enters the tile to all waves
 // of the block; `need`: the tile does not begin with a sequence.
 template <int VEC>
 __device__ __forceinline__ void enter(const Words& words, unsigned int at, unsigned int lane,
-                                      int wave, int waves, bool closing, bool need,
+                                      int wave, int waves, int closer, bool need,
                                       const Span (&whole)[VEC], Span (*look)[kWave * VEC],
                                       float (*state)[kWave * VEC], float (&H)[VEC]) {
+  const bool closing = wave == closer;
   const unsigned int group = at / kGroup;
   const int inside = at % kGroup;
   const bool leads = inside == kGroup - 1;  // answers for the group's word
@@ -419,21 +420,39 @@ __device__ __forceinline__ void enter(const Words& words, unsigned int at, unsig
   }
   if (at == 0 || !(need || leads)) return;
 
-  // The words before this tile's in the group: look[d - 1] is d tiles before.
-  for (int d = wave + 1; d <= inside; d += waves) {
-    unsigned long long w[VEC];
-    for (;;) {
-      bool unset = false;
+  // The closing wave asks for the groups' words, the others for those before
+  // this tile's in the group: look[d - 1] is d tiles before.
+  const int back = group < kBack ? static_cast<int>(group) : kBack;
+  unsigned long long* out = words.group + group * words.width + lane * VEC;
+  unsigned long long g[kBack][VEC];
+  auto ask = [&]() {
 #pragma unroll
-      for (int u = 0; u < VEC; ++u) {
-        w[u] = peek(mine - d * words.width + u);
-        unset |= w[u] == kUnset;
-      }
-      if (!__any(unset)) break;
-      __builtin_amdgcn_s_sleep(1);
+    for (int d = 0; d < kBack; ++d) {
+      // Beyond the first group: the nearest one again.
+      const int64_t at_d = d < back ? d + 1 : (back > 0 ? 1 : 0);
+#pragma unroll
+      for (int u = 0; u < VEC; ++u) g[d][u] = peek(out - at_d * words.width + u);
     }
+  };
+  const int askers = waves > 1 ? waves - 1 : 1;
+  if (closing) ask();
+  if (!closing || waves == 1) {
+    const int first = waves == 1 || wave < closer ? wave : wave - 1;
+    for (int d = first + 1; d <= inside; d += askers) {
+      unsigned long long w[VEC];
+      for (;;) {
+        bool unset = false;
 #pragma unroll
-    for (int u = 0; u < VEC; ++u) look[d - 1][lane * VEC + u] = unpack(w[u]);
+        for (int u = 0; u < VEC; ++u) {
+          w[u] = peek(mine - d * words.width + u);
+          unset |= w[u] == kUnset;
+        }
+        if (!__any(unset)) break;
+        __builtin_amdgcn_s_sleep(1);
+      }
+#pragma unroll
+      for (int u = 0; u < VEC; ++u) look[d - 1][lane * VEC + u] = unpack(w[u]);
+    }
   }
   __syncthreads();
   if (closing) {
@@ -446,7 +465,6 @@ __device__ __forceinline__ void enter(const Words& words, unsigned int at, unsig
 #pragma unroll
       for (int u = 0; u < VEC; ++u) head[u] = join(head[u], look[d - 1][lane * VEC + u]);
     }
-    unsigned long long* out = words.group + group * words.width + lane * VEC;
 #pragma unroll
     for (int u = 0; u < VEC; ++u) {
       all[u] = join(head[u], whole[u]);
@@ -455,25 +473,18 @@ __device__ __forceinline__ void enter(const Words& words, unsigned int at, unsig
     }
     float G[VEC] = {};  // the state that enters the group
     if (!__all(known)) {
-      const int back = group < kBack ? static_cast<int>(group) : kBack;
       for (;;) {
-        unsigned long long w[kBack][VEC];
-#pragma unroll
-        for (int d = 0; d < kBack; ++d)
-#pragma unroll
-          for (int u = 0; u < VEC; ++u)
-            w[d][u] = d < back ? peek(out - (d + 1) * words.width + u) : kUnset;
         // The nearest word that is final for every channel, if all nearer
         // ones are set.
         int last = -1;
         bool clear = true;
 #pragma unroll
         for (int d = 0; d < kBack; ++d) {
-          bool unset = false, final = true;
+          bool unset = d >= back, final = true;
 #pragma unroll
           for (int u = 0; u < VEC; ++u) {
-            unset |= w[d][u] == kUnset;
-            final &= unpack(w[d][u]).A < 0.f;
+            unset |= g[d][u] == kUnset;
+            final &= unpack(g[d][u]).A < 0.f;
           }
           if (__any(unset)) clear = false;
           if (clear && last < 0 && __all(final)) last = d;
@@ -483,12 +494,13 @@ __device__ __forceinline__ void enter(const Words& words, unsigned int at, unsig
           for (int d = kBack - 1; d >= 0; --d) {
             if (d <= last) {
 #pragma unroll
-              for (int u = 0; u < VEC; ++u) G[u] = apply(unpack(w[d][u]), G[u]);
+              for (int u = 0; u < VEC; ++u) G[u] = apply(unpack(g[d][u]), G[u]);
             }
           }
           break;
         }
         __builtin_amdgcn_s_sleep(1);
+        ask();
       }
     }
 #pragma unroll
@@ -622,7 +634,7 @@ __global__ void __launch_bounds__(kFwdWaves * kWave, LOOK ? kFwdOcc : 1) glr_fwd
     Span whole[VEC];
 #pragma unroll
     for (int u = 0; u < VEC; ++u) whole[u] = join(head[u], span[u]);
-    enter<VEC>(words, tile, lane, wave, waves, wave == waves - 1, open, whole, look, state, h);
+    enter<VEC>(words, tile, lane, wave, waves, waves - 1, open, whole, look, state, h);
   }
 #pragma unroll
   for (int u = 0; u < VEC; ++u) h[u] = apply(head[u], h[u]);
@@ -945,7 +957,7 @@ __global__ void __launch_bounds__(kBwdWaves * kWave, LOOK ? kBwdOcc : 1) glr_bwd
     Span whole[VEC];
 #pragma unroll
     for (int u = 0; u < VEC; ++u) whole[u] = join(head[u], span[u]);
-    enter<VEC>(words, behind, lane, wave, waves, wave == 0, open, whole, look, state, q);
+    enter<VEC>(words, behind, lane, wave, waves, 0, open, whole, look, state, q);
   }
 #pragma unroll
   for (int u = 0; u < VEC; ++u) q[u] = apply(head[u], q[u]);
