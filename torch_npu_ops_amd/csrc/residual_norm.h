@@ -53,7 +53,7 @@ struct BwdParams {
   void* dx;
   void* dres;
   void* dgate;
-  float* part;  // [parts][3][N]: sums for post, scale, pre
+  float* part;  // [parts][3][part_pitch(N)]: sums for post, scale, pre
   int64_t parts;
   int sums;  // bit 0: post, 1: scale, 2: pre
   int64_t sdh, sdy, sx, sres, sgate, sdx, sdres, sdgate;
@@ -62,84 +62,110 @@ struct BwdParams {
   xk_dtype dt, rdt, wdt;
 };
 
+// Lanes that hold a row in the backward pass, 16 bytes of x each (0: the row
+// is too long for a block).
+inline int bwd_lanes(int64_t N, int vec) {
+  const int64_t nvec = cdiv(N, vec);
+  return nvec <= 64 ? 64 : nvec <= 128 ? 128 : nvec <= 256 ? 256 : nvec <= 512 ? 512
+                                                              : nvec <= 1024 ? 1024 : 0;
+}
 // Parts that the backward pass's column sums are split into: a row at least
-// for each; a team works on one part.
-inline int64_t sum_parts(int64_t M, int64_t N) {
-  const int64_t cap = N > 8192 ? 256 : (N > 1024 ? 512 : 2048);
+// for each, and one for every team that the chip holds (1024 lanes a compute
+// unit).
+inline int64_t sum_parts(int64_t M, int64_t N, int vec) {
+  const int lanes = bwd_lanes(N, vec);
+  const int64_t cap = 256 * (lanes ? 1024 / lanes : 1);
   return M < cap ? M : cap;
 }
+// Floats from one row of parts to the next: whole lanes of 16-bit rows.
+__host__ __device__ inline int64_t part_pitch(int64_t N) { return (N + 7) / 8 * 8; }
 
-// VEC elements from any address.
+// VEC elements of a row as the words they were loaded in: unpacked where they
+// are used, which costs less than holding them in fp32.
 template <typename T, int VEC>
 struct Row {
-  T v[VEC];
+  static constexpr int kWords = VEC * sizeof(T) / 4, kPer = 4 / sizeof(T);
+  unsigned int w[kWords];
+  __device__ __forceinline__ float operator[](int u) const {
+    const unsigned int r = w[u / kPer];
+    if constexpr (sizeof(T) == 4) {
+      return __builtin_bit_cast(float, r);
+    } else if constexpr (std::is_same<T, bf16>::value) {
+      return __builtin_bit_cast(float, u & 1 ? r & 0xffff0000u : r << 16);
+    } else {
+      return to_f32(__builtin_bit_cast(T, static_cast<unsigned short>(u & 1 ? r >> 16 : r)));
+    }
+  }
+  // From here on the elements are unpacked again: keeps the compiler from
+  // holding an earlier use's fp32 values in registers.
+  __device__ __forceinline__ void again() {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) asm volatile("" : "+v"(w[i]));
+  }
 };
-typedef unsigned int u32;
-template <int BYTES, int ALIGN> struct RawAt { using type = void; };
-template <> struct RawAt<32, 4> { typedef u32x4 type __attribute__((aligned(4))); };
-template <> struct RawAt<16, 4> { typedef u32x4 type __attribute__((aligned(4))); };
-template <> struct RawAt<16, 2> { typedef u32x4 type __attribute__((aligned(2))); };
+template <typename T, int VEC>
+__device__ __forceinline__ Row<T, VEC> pack(const float (&v)[VEC]) {
+  Arr<T, VEC> t;
+#pragma unroll
+  for (int u = 0; u < VEC; ++u) t.v[u] = from_f32<T>(v[u]);
+  return __builtin_bit_cast(Row<T, VEC>, t);
+}
 
-template <typename T, int VEC>
-__device__ __forceinline__ Row<T, VEC> ld_at(const T* p) {
-  Row<T, VEC> out;
-  constexpr int kBytes = VEC * sizeof(T), kChunk = 16, kPer = kChunk / sizeof(T);
-  using U = typename RawAt<kChunk, sizeof(T)>::type;
-#pragma unroll
-  for (int c = 0; c < kBytes / kChunk; ++c) {
-    const u32x4 r = __builtin_nontemporal_load(reinterpret_cast<const U*>(p + c * kPer));
-    __builtin_memcpy(&out.v[c * kPer], &r, kChunk);
-  }
-  return out;
-}
-template <typename T, int VEC>
-__device__ __forceinline__ void st_at(T* p, const Row<T, VEC>& in) {
-  constexpr int kBytes = VEC * sizeof(T), kChunk = 16, kPer = kChunk / sizeof(T);
-  using U = typename RawAt<kChunk, sizeof(T)>::type;
-#pragma unroll
-  for (int c = 0; c < kBytes / kChunk; ++c) {
-    u32x4 r;
-    __builtin_memcpy(&r, &in.v[c * kPer], kChunk);
-    __builtin_nontemporal_store(r, reinterpret_cast<U*>(p + c * kPer));
-  }
-}
-// The same with `left` elements of the row left (may be <= 0): zeros beyond.
-template <typename T, int VEC>
+// Moves of a lane's elements, 16 bytes at a time and at any address; `left`
+// elements of the row are left at p.  TAIL: rows may end inside a lane, whose
+// elements then go one by one (without it a row's lanes are full or empty).
+// Loads give zeros beyond the row.  STREAM: read or written once.
+typedef u32x4 Word4At2 __attribute__((aligned(2)));
+typedef u32x4 Word4At4 __attribute__((aligned(4)));
+template <typename T>
+using Word4 = typename std::conditional<sizeof(T) == 2, const Word4At2*, const Word4At4*>::type;
+template <typename T>
+using Word4Out = typename std::conditional<sizeof(T) == 2, Word4At2*, Word4At4*>::type;
+
+template <typename T, int VEC, bool TAIL, bool STREAM = true>
 __device__ __forceinline__ Row<T, VEC> ld_row(const T* p, int left) {
-  if (left >= VEC) return ld_at<T, VEC>(p);
-  Row<T, VEC> out;
+  Row<T, VEC> out{};
+  if (left >= VEC) {
 #pragma unroll
-  for (int u = 0; u < VEC; ++u) out.v[u] = u < left ? p[u] : from_f32<T>(0.f);
+    for (int c = 0; c < out.kWords / 4; ++c) {
+      const Word4<T> q = reinterpret_cast<Word4<T>>(p + c * (16 / sizeof(T)));
+      u32x4 r;
+      if constexpr (STREAM)
+        r = __builtin_nontemporal_load(q);
+      else
+        r = *q;
+      out.w[4 * c] = r.x;
+      out.w[4 * c + 1] = r.y;
+      out.w[4 * c + 2] = r.z;
+      out.w[4 * c + 3] = r.w;
+    }
+  } else if constexpr (TAIL) {
+    Arr<T, VEC> t;
+#pragma unroll
+    for (int u = 0; u < VEC; ++u) t.v[u] = u < left ? p[u] : from_f32<T>(0.f);
+    out = __builtin_bit_cast(Row<T, VEC>, t);
+  }
   return out;
 }
-template <typename T, int VEC>
+template <typename T, int VEC, bool TAIL>
 __device__ __forceinline__ void st_row(T* p, const Row<T, VEC>& in, int left) {
   if (left >= VEC) {
-    st_at<T, VEC>(p, in);
-  } else {
+#pragma unroll
+    for (int c = 0; c < in.kWords / 4; ++c) {
+      const u32x4 r = {in.w[4 * c], in.w[4 * c + 1], in.w[4 * c + 2], in.w[4 * c + 3]};
+      __builtin_nontemporal_store(r, reinterpret_cast<Word4Out<T>>(p + c * (16 / sizeof(T))));
+    }
+  } else if constexpr (TAIL) {
+    const Arr<T, VEC> t = __builtin_bit_cast(Arr<T, VEC>, in);
 #pragma unroll
     for (int u = 0; u < VEC; ++u)
-      if (u < left) p[u] = in.v[u];
+      if (u < left) p[u] = t.v[u];
   }
 }
 // Weights are read again by every row and stay in the caches.
-template <typename W, int VEC>
+template <typename W, int VEC, bool TAIL>
 __device__ __forceinline__ Row<W, VEC> ld_weight(const void* base, int at, int left) {
-  const W* p = static_cast<const W*>(base) + at;
-  Row<W, VEC> out;
-  if (left >= VEC) {
-    constexpr int kPer = 16 / sizeof(W);
-    using U = typename RawAt<16, sizeof(W)>::type;
-#pragma unroll
-    for (int c = 0; c < VEC / kPer; ++c) {
-      const u32x4 r = *reinterpret_cast<const U*>(p + c * kPer);
-      __builtin_memcpy(&out.v[c * kPer], &r, 16);
-    }
-  } else {
-#pragma unroll
-    for (int u = 0; u < VEC; ++u) out.v[u] = u < left ? p[u] : from_f32<W>(0.f);
-  }
-  return out;
+  return ld_row<W, VEC, TAIL, false>(static_cast<const W*>(base) + at, left);
 }
 
 // Sum over the TPR lanes of a team.  Teams wider than a wave are the whole
@@ -160,13 +186,17 @@ __device__ __forceinline__ float team_sum(float v, float* red, int turn) {
   return v;
 }
 
+// Teams of a wave share blocks of four; wider ones are a block.
 template <int TPR>
-constexpr int block_of() { return TPR > 256 ? TPR : 256; }
+constexpr int block_of() { return TPR > kWave ? TPR : 256; }
 
-template <typename T, typename RT, typename WT, int TPR, int NV>
+// FULL: every part is there, with no branches on them.
+template <typename T, typename RT, typename WT, int TPR, int NV, bool FULL, bool TAIL>
 __global__ void __launch_bounds__(block_of<TPR>()) fwd_kernel(FwdParams p) {
   constexpr int VEC = 16 / sizeof(T), kTeams = block_of<TPR>() / TPR;
   __shared__ float red[2 * (TPR > kWave ? TPR / kWave : 1)];
+  const bool post = FULL || p.post, gate = FULL || p.gate, scale = FULL || p.scale,
+             pre = FULL || p.pre;
   const int lane = threadIdx.x % TPR, N = static_cast<int>(p.N);
   const float inv_n = 1.f / static_cast<float>(p.N);
   const int64_t step = static_cast<int64_t>(gridDim.x) * kTeams;
@@ -179,21 +209,29 @@ __global__ void __launch_bounds__(block_of<TPR>()) fwd_kernel(FwdParams p) {
     const T* zr = static_cast<const T*>(p.gate) + row * p.sgate;
     Row<T, VEC> x[NV], z[NV];
     Row<RT, VEC> res[NV];
+    Row<WT, VEC> w1[NV], w2[NV], sc[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int at = (j * TPR + lane) * VEC;
-      x[j] = ld_row<T, VEC>(xr + at, N - at);
-      res[j] = ld_row<RT, VEC>(rr + at, N - at);
-      if (p.gate) z[j] = ld_row<T, VEC>(zr + at, N - at);
+      x[j] = ld_row<T, VEC, TAIL>(xr + at, N - at);
+      if (gate) z[j] = ld_row<T, VEC, TAIL>(zr + at, N - at);
+      res[j] = ld_row<RT, VEC, TAIL>(rr + at, N - at);
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int at = (j * TPR + lane) * VEC;
+      if (post) w1[j] = ld_weight<WT, VEC, TAIL>(p.post, at, N - at);
+      if (scale) sc[j] = ld_weight<WT, VEC, TAIL>(p.scale, at, N - at);
+      if (pre) w2[j] = ld_weight<WT, VEC, TAIL>(p.pre, at, N - at);
     }
     float r1 = 1.f;
-    if (p.post) {
+    if (post) {
       float ss = 0.f;
 #pragma unroll
       for (int j = 0; j < NV; ++j)
 #pragma unroll
         for (int u = 0; u < VEC; ++u) {
-          const float f = to_f32(x[j].v[u]);
+          const float f = x[j][u];
           ss = fmaf(f, f, ss);
         }
       r1 = 1.f / sqrtf(team_sum<TPR>(ss, red, 0) * inv_n + p.eps);
@@ -203,170 +241,150 @@ __global__ void __launch_bounds__(block_of<TPR>()) fwd_kernel(FwdParams p) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int at = (j * TPR + lane) * VEC;
-#pragma unroll
-      for (int u = 0; u < VEC; ++u) h[j][u] = to_f32(x[j].v[u]);
-      if (p.post) {
-        const Row<WT, VEC> w = ld_weight<WT, VEC>(p.post, at, N - at);
-#pragma unroll
-        for (int u = 0; u < VEC; ++u) h[j][u] *= r1 * (to_f32(w.v[u]) + p.off);
-      }
-      if (p.gate) {
-#pragma unroll
-        for (int u = 0; u < VEC; ++u) h[j][u] *= silu(to_f32(z[j].v[u]));
-      }
-      if (p.scale) {
-        const Row<WT, VEC> w = ld_weight<WT, VEC>(p.scale, at, N - at);
-#pragma unroll
-        for (int u = 0; u < VEC; ++u) h[j][u] *= to_f32(w.v[u]);
-      }
-      Row<RT, VEC> out;
+      float out[VEC];
 #pragma unroll
       for (int u = 0; u < VEC; ++u) {
-        h[j][u] += to_f32(res[j].v[u]);
-        ss = fmaf(h[j][u], h[j][u], ss);
-        out.v[u] = from_f32<RT>(h[j][u]);
+        float v = x[j][u];
+        if (post) v *= r1 * (w1[j][u] + p.off);
+        if (gate) v *= silu(z[j][u]);
+        v = scale ? fmaf(v, sc[j][u], res[j][u]) : v + res[j][u];
+        ss = fmaf(v, v, ss);
+        h[j][u] = out[u] = v;
       }
-      st_row<RT, VEC>(static_cast<RT*>(p.h) + row * p.sh + at, out, N - at);
+      st_row<RT, VEC, TAIL>(static_cast<RT*>(p.h) + row * p.sh + at, pack<RT, VEC>(out), N - at);
     }
-    if (p.pre) {
+    if (pre) {
       const float r2 = 1.f / sqrtf(team_sum<TPR>(ss, red, 1) * inv_n + p.eps);
       if (p.r2 && lane == 0) p.r2[row] = r2;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         const int at = (j * TPR + lane) * VEC;
-        const Row<WT, VEC> w = ld_weight<WT, VEC>(p.pre, at, N - at);
-        Row<T, VEC> out;
+        float out[VEC];
 #pragma unroll
-        for (int u = 0; u < VEC; ++u)
-          out.v[u] = from_f32<T>(h[j][u] * r2 * (to_f32(w.v[u]) + p.off));
-        st_row<T, VEC>(static_cast<T*>(p.y) + row * p.sy + at, out, N - at);
+        for (int u = 0; u < VEC; ++u) out[u] = h[j][u] * r2 * (w2[j][u] + p.off);
+        st_row<T, VEC, TAIL>(static_cast<T*>(p.y) + row * p.sy + at, pack<T, VEC>(out), N - at);
       }
     }
     // One barrier more where only one of the two sums runs: its half of `red`
     // is the next row's too.
     if constexpr (TPR > kWave) {
-      if (!p.post || !p.pre) __syncthreads();
+      if (!post || !pre) __syncthreads();
     }
   }
 }
 
-template <typename T, typename RT, typename WT, int TPR, int NV>
-__global__ void __launch_bounds__(block_of<TPR>()) bwd_kernel(BwdParams p) {
+// Backward: a team walks every parts-th row and keeps the column sums of its
+// elements in registers.  Per row: h and rstd2's sum from x, gate, residual;
+// then dh's total, the gate's and the branch's gradients and rstd1's sum; then
+// dx.  The sigmoid is kept between the passes, the cheap products are formed
+// again.
+template <typename T, typename RT, typename WT, int TPR, bool TAIL>
+__global__ void __launch_bounds__(block_of<TPR>(), 4) bwd_kernel(BwdParams p) {
   constexpr int VEC = 16 / sizeof(T), kTeams = block_of<TPR>() / TPR;
   __shared__ float red[2 * (TPR > kWave ? TPR / kWave : 1)];
+  const bool post = p.post, gate = p.gate, scale = p.scale, has_dy = p.dy, has_dh = p.dh;
   const int lane = threadIdx.x % TPR, N = static_cast<int>(p.N);
+  const int at = lane * VEC, left = N - at;
   const float inv_n = 1.f / static_cast<float>(p.N);
   const int64_t team = static_cast<int64_t>(blockIdx.x) * kTeams + threadIdx.x / TPR;
-  float a_post[NV][VEC] = {}, a_scale[NV][VEC] = {}, a_pre[NV][VEC] = {};
+  float a_post[VEC] = {}, a_scale[VEC] = {}, a_pre[VEC] = {};
+  Row<WT, VEC> w1{}, w2{}, sc{};
+  if (post) w1 = ld_weight<WT, VEC, TAIL>(p.post, at, left);
+  if (has_dy) w2 = ld_weight<WT, VEC, TAIL>(p.pre, at, left);
+  if (scale) sc = ld_weight<WT, VEC, TAIL>(p.scale, at, left);
   for (int64_t row = team; team < p.parts && row < p.M; row += p.parts) {
-    Row<T, VEC> x[NV], z[NV], dy[NV];
-    Row<RT, VEC> res[NV], dh[NV];
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int at = (j * TPR + lane) * VEC;
-      x[j] = ld_row<T, VEC>(static_cast<const T*>(p.x) + row * p.sx + at, N - at);
-      res[j] = ld_row<RT, VEC>(static_cast<const RT*>(p.res) + row * p.sres + at, N - at);
-      if (p.gate) z[j] = ld_row<T, VEC>(static_cast<const T*>(p.gate) + row * p.sgate + at, N - at);
-      if (p.dy) dy[j] = ld_row<T, VEC>(static_cast<const T*>(p.dy) + row * p.sdy + at, N - at);
-      if (p.dh) dh[j] = ld_row<RT, VEC>(static_cast<const RT*>(p.dh) + row * p.sdh + at, N - at);
+    Row<T, VEC> x, z{}, dy{};
+    Row<RT, VEC> res{}, dh{};
+    w1.again();
+    w2.again();
+    sc.again();
+    x = ld_row<T, VEC, TAIL>(static_cast<const T*>(p.x) + row * p.sx + at, left);
+    if (gate) z = ld_row<T, VEC, TAIL>(static_cast<const T*>(p.gate) + row * p.sgate + at, left);
+    if (has_dy) {
+      dy = ld_row<T, VEC, TAIL>(static_cast<const T*>(p.dy) + row * p.sdy + at, left);
+      res = ld_row<RT, VEC, TAIL>(static_cast<const RT*>(p.res) + row * p.sres + at, left);
     }
-    const float r1 = p.post ? p.r1[row] : 1.f;
-    const float r2 = p.dy ? p.r2[row] : 0.f;
-    // h rstd2, and the mean of it with w2' dy.
-    float d[NV][VEC], ss = 0.f;  // d: w2' dy, then dH, then w1' dn
-    auto branch = [&](int j, int u, const Row<WT, VEC>& w1, float& xh, float& n, float& sg) {
-      xh = to_f32(x[j].v[u]) * r1;
-      n = p.post ? xh * (to_f32(w1.v[u]) + p.off) : xh;
-      sg = p.gate ? sigmoid(to_f32(z[j].v[u])) : 1.f;
-      return p.gate ? n * to_f32(z[j].v[u]) * sg : n;
+    if (has_dh) dh = ld_row<RT, VEC, TAIL>(static_cast<const RT*>(p.dh) + row * p.sdh + at, left);
+    const float r1 = post ? p.r1[row] : 1.f;
+    const float r2 = has_dy ? p.r2[row] : 0.f;
+    float sg[VEC], hh[VEC], ss = 0.f;  // hh: h rstd2, then w1' dn
+    // n = x rstd1 w1' and v = n z sigmoid(z) of an element.
+    auto norm_of = [&](int u) {
+      const float f = x[u] * r1;
+      return post ? f * (w1[u] + p.off) : f;
     };
-    if (p.dy) {
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const int at = (j * TPR + lane) * VEC;
-        Row<WT, VEC> w1, sc;
-        if (p.post) w1 = ld_weight<WT, VEC>(p.post, at, N - at);
-        if (p.scale) sc = ld_weight<WT, VEC>(p.scale, at, N - at);
-        const Row<WT, VEC> w2 = ld_weight<WT, VEC>(p.pre, at, N - at);
-#pragma unroll
-        for (int u = 0; u < VEC; ++u) {
-          float xh, n, sg;
-          const float v = branch(j, u, w1, xh, n, sg);
-          const float hh = fmaf(p.scale ? to_f32(sc.v[u]) : 1.f, v, to_f32(res[j].v[u])) * r2;
-          const float g = to_f32(dy[j].v[u]);
-          a_pre[j][u] = fmaf(g, hh, a_pre[j][u]);
-          d[j][u] = g * (to_f32(w2.v[u]) + p.off);
-          ss = fmaf(d[j][u], hh, ss);
-        }
+    for (int u = 0; u < VEC; ++u) {
+      if (gate) sg[u] = sigmoid(z[u]);
+      if (has_dy) {
+        float v = norm_of(u);
+        if (gate) v *= z[u] * sg[u];
+        hh[u] = (scale ? fmaf(v, sc[u], res[u]) : v + res[u]) * r2;
+        const float g = dy[u];
+        a_pre[u] = fmaf(g, hh[u], a_pre[u]);
+        ss = fmaf(g * (w2[u] + p.off), hh[u], ss);
       }
-      ss = team_sum<TPR>(ss, red, 0) * inv_n;
     }
+    if (has_dy) ss = team_sum<TPR>(ss, red, 0) * inv_n;
     float dot = 0.f;
+    x.again();
+    z.again();
+    dy.again();
+    w1.again();
+    w2.again();
+    sc.again();
+    float o_res[VEC], o_gate[VEC];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int at = (j * TPR + lane) * VEC;
-      Row<WT, VEC> w1, sc;
-      if (p.post) w1 = ld_weight<WT, VEC>(p.post, at, N - at);
-      if (p.scale) sc = ld_weight<WT, VEC>(p.scale, at, N - at);
-      Row<RT, VEC> o_res;
-      Row<T, VEC> o_gate;
-#pragma unroll
-      for (int u = 0; u < VEC; ++u) {
-        float xh, n, sg;
-        const float v = branch(j, u, w1, xh, n, sg);
-        const float s = p.scale ? to_f32(sc.v[u]) : 1.f;
-        float g = 0.f;
-        if (p.dy) g = r2 * (d[j][u] - fmaf(s, v, to_f32(res[j].v[u])) * r2 * ss);
-        if (p.dh) g += to_f32(dh[j].v[u]);
-        o_res.v[u] = from_f32<RT>(g);
-        a_scale[j][u] = fmaf(g, v, a_scale[j][u]);
-        g *= s;
-        if (p.gate) {
-          const float zf = to_f32(z[j].v[u]);
-          o_gate.v[u] = from_f32<T>(g * n * sg * fmaf(zf, 1.f - sg, 1.f));
-          g *= zf * sg;
-        }
-        if (p.post) {
-          a_post[j][u] = fmaf(g, xh, a_post[j][u]);
-          g *= to_f32(w1.v[u]) + p.off;
-          dot = fmaf(g, xh, dot);
-        }
-        d[j][u] = g;
+    for (int u = 0; u < VEC; ++u) {
+      const float xh = x[u] * r1, n = norm_of(u);
+      float g = has_dh ? dh[u] : 0.f;
+      if (has_dy)
+        g = fmaf(r2, fmaf(dy[u], w2[u] + p.off, -hh[u] * ss), g);
+      o_res[u] = g;
+      const float silu_z = gate ? z[u] * sg[u] : 1.f;
+      a_scale[u] = fmaf(g, n * silu_z, a_scale[u]);
+      if (scale) g *= sc[u];
+      if (gate) {
+        o_gate[u] = g * n * fmaf(silu_z, 1.f - sg[u], sg[u]);
+        g *= silu_z;
       }
-      if (p.dres) st_row<RT, VEC>(static_cast<RT*>(p.dres) + row * p.sdres + at, o_res, N - at);
-      if (p.gate && p.dgate)
-        st_row<T, VEC>(static_cast<T*>(p.dgate) + row * p.sdgate + at, o_gate, N - at);
+      if (post) {
+        a_post[u] = fmaf(g, xh, a_post[u]);
+        g *= w1[u] + p.off;
+        dot = fmaf(g, xh, dot);
+      }
+      hh[u] = g;
     }
-    if (p.post) dot = team_sum<TPR>(dot, red, 1) * inv_n;
+    if (p.dres)
+      st_row<RT, VEC, TAIL>(static_cast<RT*>(p.dres) + row * p.sdres + at, pack<RT, VEC>(o_res), left);
+    if (gate && p.dgate)
+      st_row<T, VEC, TAIL>(static_cast<T*>(p.dgate) + row * p.sdgate + at, pack<T, VEC>(o_gate),
+                     left);
+    if (post) dot = team_sum<TPR>(dot, red, 1) * inv_n;
     if (p.dx) {
+      x.again();
+      float out[VEC];
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const int at = (j * TPR + lane) * VEC;
-        Row<T, VEC> out;
-#pragma unroll
-        for (int u = 0; u < VEC; ++u)
-          out.v[u] = from_f32<T>(
-              p.post ? r1 * (d[j][u] - to_f32(x[j].v[u]) * r1 * dot) : d[j][u]);
-        st_row<T, VEC>(static_cast<T*>(p.dx) + row * p.sdx + at, out, N - at);
-      }
+      for (int u = 0; u < VEC; ++u) out[u] = post ? r1 * fmaf(x[u] * -r1, dot, hh[u]) : hh[u];
+      st_row<T, VEC, TAIL>(static_cast<T*>(p.dx) + row * p.sdx + at, pack<T, VEC>(out), left);
     }
     if constexpr (TPR > kWave) {
-      if (!p.post || !p.dy) __syncthreads();
+      if (!post || !has_dy) __syncthreads();
     }
   }
-  if (p.sums && team < p.parts) {
-    float* out = p.part + team * 3 * p.N;
+  if (p.sums && team < p.parts && left > 0) {
+    // Rows of parts are padded to whole lanes.
+    const int64_t pitch = part_pitch(p.N);
+    float* out = p.part + team * 3 * pitch + at;
+    auto put = [&](const float (&v)[VEC]) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-      for (int u = 0; u < VEC; ++u) {
-        const int at = (j * TPR + lane) * VEC + u;
-        if (at < N) {
-          if (p.sums & 1) out[at] = a_post[j][u];
-          if (p.sums & 2) out[p.N + at] = a_scale[j][u];
-          if (p.sums & 4) out[2 * p.N + at] = a_pre[j][u];
-        }
-      }
+      for (int u = 0; u < VEC; u += 4)
+        *reinterpret_cast<Vec<float, 4>*>(out + u) = {{v[u], v[u + 1], v[u + 2], v[u + 3]}};
+      out += pitch;
+    };
+    put(a_post);
+    put(a_scale);
+    put(a_pre);
   }
 }
 
@@ -374,17 +392,24 @@ template <typename T, typename RT, typename WT, int TPR, int NV>
 int launch_fwd(const FwdParams& p, hipStream_t s) {
   constexpr int kTeams = block_of<TPR>() / TPR;
   const int64_t most = static_cast<int64_t>(num_cus()) * (2048 / block_of<TPR>());
-  const int64_t grid = std::min(cdiv(p.M, kTeams), most);
-  hipLaunchKernelGGL((fwd_kernel<T, RT, WT, TPR, NV>), dim3(grid), dim3(block_of<TPR>()), 0, s,
-                     p);
+  const dim3 grid(std::min(cdiv(p.M, kTeams), most)), block(block_of<TPR>());
+  if (p.N % (16 / static_cast<int>(sizeof(T))))
+    hipLaunchKernelGGL((fwd_kernel<T, RT, WT, TPR, NV, false, true>), grid, block, 0, s, p);
+  else if (p.post && p.gate && p.scale && p.pre)
+    hipLaunchKernelGGL((fwd_kernel<T, RT, WT, TPR, NV, true, false>), grid, block, 0, s, p);
+  else
+    hipLaunchKernelGGL((fwd_kernel<T, RT, WT, TPR, NV, false, false>), grid, block, 0, s, p);
   return launch_status();
 }
 
-template <typename T, typename RT, typename WT, int TPR, int NV>
+template <typename T, typename RT, typename WT, int TPR>
 int launch_bwd(const BwdParams& p, hipStream_t s) {
   constexpr int kTeams = block_of<TPR>() / TPR;
-  hipLaunchKernelGGL((bwd_kernel<T, RT, WT, TPR, NV>), dim3(cdiv(p.parts, kTeams)),
-                     dim3(block_of<TPR>()), 0, s, p);
+  const dim3 grid(cdiv(p.parts, kTeams)), block(block_of<TPR>());
+  if (p.N % (16 / static_cast<int>(sizeof(T))))
+    hipLaunchKernelGGL((bwd_kernel<T, RT, WT, TPR, true>), grid, block, 0, s, p);
+  else
+    hipLaunchKernelGGL((bwd_kernel<T, RT, WT, TPR, false>), grid, block, 0, s, p);
   return launch_status();
 }
 
@@ -400,7 +425,10 @@ int run_fwd_w(const FwdParams& p, hipStream_t s) {
   if (nvec <= 64) return launch_fwd<T, RT, WT, 64, 1>(p, s);
   if (nvec <= 128) return launch_fwd<T, RT, WT, 64, 2>(p, s);
   if (nvec <= 256) return launch_fwd<T, RT, WT, 256, 1>(p, s);
-  if (nvec <= 512) return launch_fwd<T, RT, WT, 256, 2>(p, s);
+  // A wider residual has the registers of a second vector.
+  if (nvec <= 512)
+    return sizeof(RT) > sizeof(T) ? launch_fwd<T, RT, WT, 512, 1>(p, s)
+                                  : launch_fwd<T, RT, WT, 256, 2>(p, s);
   if (nvec <= 1024) return launch_fwd<T, RT, WT, 1024, 1>(p, s);
   if (nvec <= 2048) return launch_fwd<T, RT, WT, 1024, 2>(p, s);
   if (nvec <= 4096) return launch_fwd<T, RT, WT, 1024, 4>(p, s);
@@ -409,14 +437,14 @@ int run_fwd_w(const FwdParams& p, hipStream_t s) {
 
 template <typename T, typename RT, typename WT>
 int run_bwd_w(const BwdParams& p, hipStream_t s) {
-  constexpr int VEC = 16 / sizeof(T);
-  const int64_t nvec = cdiv(p.N, VEC);
-  if (nvec <= 64) return launch_bwd<T, RT, WT, 64, 1>(p, s);
-  if (nvec <= 128) return launch_bwd<T, RT, WT, 64, 2>(p, s);
-  if (nvec <= 256) return launch_bwd<T, RT, WT, 256, 1>(p, s);
-  if (nvec <= 512) return launch_bwd<T, RT, WT, 256, 2>(p, s);
-  if (nvec <= 1024) return launch_bwd<T, RT, WT, 1024, 1>(p, s);
-  return stream_bwd(p, s);
+  switch (bwd_lanes(p.N, 16 / sizeof(T))) {
+    case 64: return launch_bwd<T, RT, WT, 64>(p, s);
+    case 128: return launch_bwd<T, RT, WT, 128>(p, s);
+    case 256: return launch_bwd<T, RT, WT, 256>(p, s);
+    case 512: return launch_bwd<T, RT, WT, 512>(p, s);
+    case 1024: return launch_bwd<T, RT, WT, 1024>(p, s);
+    default: return stream_bwd(p, s);
+  }
 }
 
 template <typename T>

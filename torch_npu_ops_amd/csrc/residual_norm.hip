@@ -64,7 +64,8 @@ __global__ void __launch_bounds__(1024) stream_fwd_kernel(FwdParams p) {
 __global__ void __launch_bounds__(1024) stream_bwd_kernel(BwdParams p) {
   __shared__ float red[16];
   const float inv_n = 1.f / static_cast<float>(p.N);
-  float* part = p.part + static_cast<int64_t>(blockIdx.x) * 3 * p.N;
+  const int64_t pitch = part_pitch(p.N);
+  float* part = p.part + static_cast<int64_t>(blockIdx.x) * 3 * pitch;
   for (int64_t row = blockIdx.x; row < p.M; row += p.parts) {
     const bool first = row == blockIdx.x;  // this part's sums start here
     const float r1 = p.post ? p.r1[row] : 1.f, r2 = p.dy ? p.r2[row] : 0.f;
@@ -109,7 +110,7 @@ __global__ void __launch_bounds__(1024) stream_bwd_kernel(BwdParams p) {
       dot = block_sum(dot, red) * inv_n;
     }
     auto add = [&](int k, int64_t e, float v) {
-      float* q = part + k * p.N + e;
+      float* q = part + k * pitch + e;
       *q = first ? v : *q + v;
     };
     for (int64_t e = threadIdx.x; e < p.N; e += 1024) {
@@ -135,22 +136,26 @@ __global__ void __launch_bounds__(1024) stream_bwd_kernel(BwdParams p) {
   }
 }
 
-// Column sums of the parts in their order: a block takes 64 columns, each of
-// its 16 waves every 16th part.
-__global__ void __launch_bounds__(1024)
+// Column sums of the parts in their order: a block takes 16 columns, each of
+// its 16 rows of lanes every 16th part.
+constexpr int kSumCols = 16;
+__global__ void __launch_bounds__(256)
     sums_kernel(const float* part, int64_t parts, int64_t N, void* dpost, void* dscale,
                 void* dpre, xk_dtype wdt) {
-  __shared__ float red[16][kWave];
-  const int k = blockIdx.y, lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  __shared__ float red[16][kSumCols + 1];
+  const int k = blockIdx.y, lane = threadIdx.x % kSumCols, first = threadIdx.x / kSumCols;
   void* out = k == 0 ? dpost : (k == 1 ? dscale : dpre);
   if (!out) return;
-  const int64_t col = static_cast<int64_t>(blockIdx.x) * kWave + lane;
+  const int64_t col = static_cast<int64_t>(blockIdx.x) * kSumCols + lane;
+  const int64_t pitch = part_pitch(N);
   float s = 0.f;
-  if (col < N)
-    for (int64_t q = wave; q < parts; q += 16) s += part[(q * 3 + k) * N + col];
-  red[wave][lane] = s;
+  if (col < N) {
+#pragma unroll 8
+    for (int64_t q = first; q < parts; q += 16) s += part[(q * 3 + k) * pitch + col];
+  }
+  red[first][lane] = s;
   __syncthreads();
-  if (wave == 0 && col < N) {
+  if (first == 0 && col < N) {
     s = 0.f;
 #pragma unroll
     for (int w = 0; w < 16; ++w) s += red[w][lane];
@@ -207,7 +212,9 @@ extern "C" int xk_gated_residual_rms_norm(
 
 extern "C" int64_t xk_gated_residual_rms_norm_bwd_workspace_bytes(int64_t M, int64_t N) {
   if (M <= 0 || N <= 0) return 0;
-  return resnorm::sum_parts(M, N) * 3 * N * 4;
+  // The parts of the types with 4 and 8 elements a lane.
+  return std::max(resnorm::sum_parts(M, N, 4), resnorm::sum_parts(M, N, 8)) * 3 *
+         resnorm::part_pitch(N) * 4;
 }
 
 extern "C" int xk_gated_residual_rms_norm_bwd(
@@ -229,7 +236,7 @@ extern "C" int xk_gated_residual_rms_norm_bwd(
     return XK_ERR_INVALID;
   const int sums = (dpost_weight ? 1 : 0) | (dscale ? 2 : 0) | (dpre_weight ? 4 : 0);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const int64_t parts = sum_parts(M, N);
+  const int64_t parts = sum_parts(M, N, 16 / elem_bytes(dtype));
   if (M > 0) {
     if (!x || !residual || (!dh && !dy) || (post_weight && !rstd_post) || (dy && !rstd_pre))
       return XK_ERR_INVALID;
@@ -253,7 +260,7 @@ extern "C" int xk_gated_residual_rms_norm_bwd(
     if (st != XK_OK) return st;
   }
   if (sums) {
-    hipLaunchKernelGGL(sums_kernel, dim3(cdiv(N, kWave), 3), dim3(1024), 0, s,
+    hipLaunchKernelGGL(sums_kernel, dim3(cdiv(N, kSumCols), 3), dim3(256), 0, s,
                        static_cast<const float*>(workspace), parts, N, dpost_weight, dscale,
                        dpre_weight, wdtype);
     return launch_status();
