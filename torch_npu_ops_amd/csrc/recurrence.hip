@@ -940,8 +940,10 @@ __device__ __forceinline__ float exp_neg(float v) {
 //  * h_{t-1} comes from the window's saved state, in the same pass that forms
 //    the window's span (in token order: A is the running product of alpha and
 //    B the sum of A_t dy_t, so nothing but h_{t-1} is kept for a token).
-//  * The second pass, in reverse order, forms the gates again from exp(-a) and
-//    exp(-b), which stay in registers.
+//  * Of the gates exp(-a), exp(-b), r and alpha - 1 stay in registers for the
+//    second pass, in reverse order; the rest is cheaper formed again.  (With
+//    the two exponentials alone 142 us instead of 134 for 8,192 x 4,096 bf16:
+//    the arithmetic is as long as the traffic.)
 //  * E = (dL/dl) l = G alpha (h_{t-1} l - i x alpha l / s) gives da = E (1 - r)
 //    and dlam = sum E sigmoid(lam) / softplus(lam), with no division by what
 //    vanishes as a gate closes: l / s -> 0 with s.
@@ -1009,7 +1011,7 @@ __global__ void __launch_bounds__(kBwdWaves * kWave, LOOK ? kBwdOcc : 1) glr_bwd
     });
   }
 
-  float before[kTok][VEC], ea[kTok][VEC], eb[kTok][VEC];
+  float before[kTok][VEC], ea[kTok][VEC], eb[kTok][VEC], em1[kTok][VEC], rs[kTok][VEC];
   Span span[VEC];
 #pragma unroll
   for (int u = 0; u < VEC; ++u) span[u] = {1.f, 0.f};
@@ -1027,8 +1029,10 @@ __global__ void __launch_bounds__(kBwdWaves * kWave, LOOK ? kBwdOcc : 1) glr_bwd
       for (int u = 0; u < VEC; ++u) {
         ea[j][u] = exp_neg(lane_f32<T>(a[j], u));
         eb[j][u] = exp_neg(lane_f32<T>(b[j], u));
-        const Gate g = gate_of<near>(k[u], fast_rcp(1.f + ea[j][u]));
+        rs[j][u] = fast_rcp(1.f + ea[j][u]);
+        const Gate g = gate_of<near>(k[u], rs[j][u]);
         before[j][u] = h[u];
+        em1[j][u] = g.em1;
         h[u] = decayed(g.em1, h[u]) +
                g.s * (fast_rcp(1.f + eb[j][u]) * lane_f32<T>(x[j], u));
         if (reached) {
@@ -1103,12 +1107,13 @@ __global__ void __launch_bounds__(kBwdWaves * kWave, LOOK ? kBwdOcc : 1) glr_bwd
       float dx[VEC], da[VEC], db[VEC];
 #pragma unroll
       for (int u = 0; u < VEC; ++u) {
-        const float r = fast_rcp(1.f + ea[j][u]), i = fast_rcp(1.f + eb[j][u]);
+        const float r = rs[j][u], i = fast_rcp(1.f + eb[j][u]);
         const float xf = lane_f32<T>(x[j], u), l = k[u] * r;
-        const Decay d = decay_of<near>(l);
+        const Decay d = near ? Decay{1.f + em1[j][u], em1[j][u]} : decay_of<false>(l);
         const float w = -d.em1 * (1.f + d.alpha);  // s^2
-        // The instruction takes a denormal w for 0.
-        const float inv = w >= 1.17549435e-38f ? __builtin_amdgcn_rsqf(w) : 0.f;
+        // The instruction takes a denormal w for 0; l and w, both tiny there,
+        // keep the products with inv at 0 or below 2^-60.
+        const float inv = __builtin_amdgcn_rsqf(fmaxf(w, 1.17549435e-38f));
         const float G = lane_f32<T>(dy[j], u) + q[u];
         dx[u] = G * (w * inv) * i;
         db[u] = dx[u] * xf * (eb[j][u] * i);
