@@ -500,9 +500,11 @@ int xk_chunk_fwd_o(const void* q, const void* k, const void* v, const void* h,
  *     r = sigmoid(a_t), i = sigmoid(b_t), l = -c softplus(lam) r,
  *     h_t = exp(l) h_{t-1} + sqrt(1 - exp(2 l)) i x_t,    y_t = h_t
  * per channel, in fp32 whatever the inputs' type.
- *   x, a, b, y : [total_tokens, D] rows with token pitches (at least D) in
- *     `dtype` (f32/bf16/f16), any alignment; lam fp32 [D]; c >= 0.  y may be
- *     x, a or b itself (the same start and pitch).
+ *   x, a, b, y : [total_tokens, D] rows with token pitches (at least D, below
+ *     2^25 elements) in `dtype` (f32/bf16/f16), any alignment; lam fp32 [D];
+ *     c >= 0.  y may be x, a or b itself (the same start and pitch).
+ *     (ceil(total_tokens / 16) + 8) * ceil(D / 64) must be below 2^26 (64
+ *     billion elements or more), else XK_ERR_INVALID.
  *   Sequences are cu_seqlens[n]..cu_seqlens[n+1] (int32/int64, device,
  *     ascending; values are clamped to [0, total_tokens]), or N runs of
  *     total_tokens / N tokens when cu_seqlens is NULL; a sequence may be empty.
@@ -532,7 +534,8 @@ int xk_gated_linear_recurrence(
 
 /* The recurrence's decode step on a pool of states: one token, or a few
  * drafted ones, of every sequence (the slot rules of xk_gdn_recurrent).
- *   x, a, b, y as above ([tokens, D], y dense or with a pitch); sequence n is
+ *   x, a, b, y as above ([tokens, D], y dense or with a pitch; N *
+ *     ceil(D / 64) below 2^26 as well); sequence n is
  *     rows cu_seqlens[n]..cu_seqlens[n+1], or T rows from n * T when
  *     cu_seqlens is NULL (T then positive).
  *   state : fp32 [num_slots, D] (slot pitch at least D), updated in place.

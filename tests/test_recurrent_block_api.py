@@ -237,3 +237,23 @@ def test_entry_points_are_operations_too():
                  "xk_gated_linear_recurrence_bwd", "xk_gated_residual_rms_norm",
                  "xk_gated_residual_rms_norm_bwd"):
         assert ctypes.cast(getattr(lib, name), ctypes.c_void_p).value
+
+
+def test_sizes_that_no_launch_holds_are_refused():
+    # A launch has fewer than 2^32 threads, a pitch fewer than 2^25 elements.
+    wide = dict(sx=1 << 26, sa=1 << 26, sb=1 << 26)
+    for call, more in ((_glr, dict(sy=1 << 26)), (_bwd, dict(sdy=1 << 26, sdx=1 << 26,
+                                                              sda=1 << 26, sdb=1 << 26))):
+        assert call(total=1 << 30, size=1 << 62, ws=PTR) == _lib.XK_ERR_INVALID
+        assert call(total=1 << 20, D=64 << 10, size=1 << 62, ws=PTR, **wide,
+                    **more) == _lib.XK_ERR_INVALID
+        assert call(total=0, D=1 << 25, size=1 << 62, ws=PTR) == _lib.XK_ERR_INVALID
+        assert call(sx=1 << 25) == _lib.XK_ERR_INVALID
+    assert _update(sy=1 << 25) == _lib.XK_ERR_INVALID
+    assert _update(N=1 << 26, total=1 << 26) == _lib.XK_ERR_INVALID
+    lib = _lib.lib()
+    for total, D in ((1 << 30, 64), (1 << 20, 64 << 10), (16, 1 << 25), (-1, 64), (16, 0)):
+        assert lib.xk_gated_linear_recurrence_workspace_bytes(total, D) == 0
+        assert lib.xk_gated_linear_recurrence_bwd_workspace_bytes(total, 1, D) == 0
+    # The largest that are taken: the workspace of 2^35 elements.
+    assert lib.xk_gated_linear_recurrence_workspace_bytes(1 << 23, 1 << 12) > 0

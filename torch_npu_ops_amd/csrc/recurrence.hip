@@ -878,7 +878,7 @@ __global__ void __launch_bounds__(kWave) glr_update_kernel(UpdateParams p) {
 template <typename T, int VEC>
 int launch_update(UpdateParams p, hipStream_t s) {
   const int64_t blocks = cdiv(p.D, kWave * VEC);
-  if (p.N * blocks >= int64_t{1} << 31) return XK_ERR_INVALID;
+  if (p.N * blocks >= int64_t{1} << 26) return XK_ERR_INVALID;  // 2^32 threads
   p.blocks = static_cast<unsigned int>(blocks);
   hipLaunchKernelGGL((glr_update_kernel<T, VEC>), dim3(p.N * blocks), dim3(kWave), 0, s, p);
   return launch_status();
@@ -1190,16 +1190,15 @@ int launch_bwd(const BwdParams& p, bool sums, void* workspace, hipStream_t s) {
   return launch_bwd_vec<T, 1>(p, sums, workspace, s);
 }
 
-// Tokens, sequences and tiles are counted in 31 bits, a batch's elements in 62.
-bool bad_sizes(int64_t N, int64_t total, int64_t D) {
-  constexpr int64_t kMost = int64_t{1} << 31;
-  return N < 0 || N >= kMost || total < 0 || total >= kMost || D <= 0 || D >= kMost ||
-         cdiv(std::max<int64_t>(total, 1), kTok) * cdiv(D, kWave) >= kMost;
-}
+// A window's rows have to lie within kRange bytes: the most elements of a pitch.
+constexpr int64_t kMostPitch = kRange / (4 * kTok);
+bool pitch_ok(int64_t pitch, int64_t D) { return pitch >= D && pitch < kMostPitch; }
 
-// A window's rows have to lie within kRange bytes.
-bool pitch_ok(int64_t pitch, int64_t D) {
-  return pitch >= D && pitch < static_cast<int64_t>(kRange / (4 * kTok));
+// A launch has fewer than 2^32 threads (of whole tiles), N is counted in 31 bits.
+bool bad_sizes(int64_t N, int64_t total, int64_t D) {
+  constexpr int64_t kMost = int64_t{1} << 26;
+  return N < 0 || N >= int64_t{1} << 31 || total < 0 || total >= kMost * kTok || D <= 0 ||
+         D >= kMostPitch || (cdiv(total, kTok) + kFwdWaves) * cdiv(D, kWave) >= kMost;
 }
 
 // cu_seqlens of a readable type, or none and N equal runs.
@@ -1213,7 +1212,7 @@ bool seqs_ok(const void* cu, xk_dtype dt, int64_t N, int64_t total) {
 using namespace xk;
 
 extern "C" int64_t xk_gated_linear_recurrence_workspace_bytes(int64_t total_tokens, int64_t D) {
-  if (total_tokens <= 0 || D <= 0) return 0;
+  if (bad_sizes(0, total_tokens, D)) return 0;
   // 4-byte elements take more, narrower channel blocks.
   return std::max(words_bytes(cut_of(total_tokens, D, 1, kFwdWaves)),
                   words_bytes(cut_of(total_tokens, D, 2, kFwdWaves)));
@@ -1279,7 +1278,7 @@ extern "C" int xk_gated_linear_recurrence_update(
 
 extern "C" int64_t xk_gated_linear_recurrence_bwd_workspace_bytes(int64_t total_tokens, int64_t N,
                                                                   int64_t D) {
-  if (total_tokens < 0 || N <= 0 || D <= 0) return 0;
+  if (N <= 0 || bad_sizes(N, total_tokens, D)) return 0;
   const Cut c1 = cut_of(total_tokens, D, 1, kBwdWaves), c2 = cut_of(total_tokens, D, 2, kBwdWaves);
   return std::max(words_bytes(c1), words_bytes(c2)) + c1.tiles * D * 4;
 }
