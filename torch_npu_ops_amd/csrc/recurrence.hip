@@ -5,7 +5,7 @@
 //   s = sqrt(1 - alpha^2), h_t = alpha h_{t-1} + s i x_t, y_t = h_t
 //
 // per channel, in fp32.  alpha - 1 is formed as expm1(l) and 1 - alpha^2 as
-// -(alpha - 1)(2 + (alpha - 1)), so neither loses digits where a channel
+// -(alpha - 1)(1 + alpha), so neither loses digits where a channel
 // keeps nearly all of its state (alpha near 1, the case that matters).
 #include <math.h>
 
@@ -137,11 +137,18 @@ __device__ __forceinline__ int cu_at(const void* cu, int cu64, int n, int run, i
 // resident.  Words and counter are cleared by a kernel before.  A word is one atomic
 // access and carries its own validity (kUnset is no pair that is published),
 // so no fences are needed.
+//
+// The forward kernel takes 126 us for 16,384 x 4,096 bf16 (537 MB, 4.3 TB/s):
+// with loads and stores alone 92, without the arithmetic (36 instructions a
+// channel and token) 104, without the chain 115.  The window's 48 loads are
+// issued together, which takes 128 registers: 4 waves a SIMD hide the rest
+// only in part.  Windows of 8 tokens (8 waves) took 150 and more.
 // ---------------------------------------------------------------------------
 constexpr int kTok = kWin;
+// 4 or 16 waves forward, 2 or 8 backward: within 1 to 4% slower.
 constexpr int kFwdWaves = 8, kBwdWaves = 4;
 constexpr int kFwdOcc = 4, kBwdOcc = 2;  // waves a SIMD holds, by their registers
-constexpr int kGroup = 4;  // tiles of a group
+constexpr int kGroup = 4;  // tiles of a group (8, 16: the same times)
 constexpr int kBack = 4;   // groups before its own that a tile looks at together
 constexpr unsigned long long kUnset = ~0ull;
 
