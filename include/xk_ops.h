@@ -517,8 +517,9 @@ int xk_chunk_fwd_o(const void* q, const void* k, const void* v, const void* h,
  *     w * XK_GLR_WINDOW where that token is inside a sequence and not its
  *     first; other rows are unspecified.
  *   Cuts of the work fall on multiples of a tile of tokens counted from row 0
- *     of the batch: a sequence's bits depend on where in the batch it stands,
- *     but not on the other sequences, and not on the run.
+ *     of the batch, a tile's length on total_tokens and D: a sequence's bits
+ *     depend on where in a batch of how many tokens it stands, but not on the
+ *     other sequences, and not on the run.
  *   workspace >= xk_gated_linear_recurrence_workspace_bytes(...) bytes,
  *     256-byte aligned; 0 bytes (NULL) for few tokens.  Calls that overlap in
  *     time need a workspace each.

@@ -499,3 +499,11 @@ def test_prefill_then_decode_equals_one_prefill(dev):
     ref = orc.forward(x[0], a[0], b[0], lam, C, h0, [0, T + more])
     assert_within(torch.cat(ys), ref["h"][T:], ref["h_err"][T:], "y")
     assert_within(state, ref["final"], ref["final_err"], "state")
+
+
+@pytest.mark.parametrize("T, D, dtype", [(2112, 8256, F32), (4112, 4100, BF16), (4099, 640, F32),
+                                         (3000, 2047, F16), (2700, 1, BF16)], ids=str)
+def test_many_tiles_of_either_length(dev, T, D, dtype):
+    # More windows than the rule's limit for long tiles, and fewer.
+    print(f"T={T} D={D} {dtype}", flush=True)
+    _check(dev, _both()["cpp"], [T // 3, 0, 1, T - T // 3 - 1], D, dtype, seed=T)

@@ -113,7 +113,7 @@ __device__ __forceinline__ int cu_at(const void* cu, int cu64, int n, int run, i
 
 // ---------------------------------------------------------------------------
 // Tiles.  The token axis of the whole batch is cut into windows of kTok tokens,
-// one per wave, and tiles of up to kFwdWaves (kBwdWaves) windows, one per block; a lane has
+// one per wave, and tiles of some windows, one per block; a lane has
 // VEC channels (4 bytes of a row), so a tile covers 64 VEC channels.  A
 // window's tokens are read once and stay in registers as (alpha - 1, input).
 //
@@ -145,8 +145,22 @@ __device__ __forceinline__ int cu_at(const void* cu, int cu64, int n, int run, i
 // only in part.  Windows of 8 tokens (8 waves) took 150 and more.
 // ---------------------------------------------------------------------------
 constexpr int kTok = kWin;
-// 4 or 16 waves forward, 2 or 8 backward: within 1 to 4% slower.
-constexpr int kFwdWaves = 8, kBwdWaves = 4;
+// Waves of a block at most: kFew while a pass has no more than kUntil windows
+// over all channel blocks, where the chain between tiles is the longest part
+// and longer tiles shorten it, else kMany.  Forward, one channel a lane, 16
+// against 8 waves: 5,003 x 1,125 29.6 and 32.6 us, 2,048 x 2,048 18.8 and 20.3,
+// 16,384 x 1,000 65.6 and 67.9; 8,192 x 4,096 105 and 96.  Two channels: 8
+// throughout (16: 2,048 x 2,048 20.4 and 17.4; 4: within 1 to 4%).  Backward, two
+// channels, 8 against 4: 2,048 x 2,048 24.7 and 28.4, 16,384 x 1,024 77 and 82;
+// 8,192 x 4,096 143 and 132.  One channel: 4 (4,099 x 640, 8: 27.1 and 25.6).
+template <int VEC>
+struct FwdWaves {
+  static constexpr int kFew = VEC == 1 ? 16 : 8, kMany = 8, kUntil = 16384;
+};
+template <int VEC>
+struct BwdWaves {
+  static constexpr int kFew = VEC == 1 ? 4 : 8, kMany = 4, kUntil = 8192;
+};
 constexpr int kFwdOcc = 4, kBwdOcc = 2;  // waves a SIMD holds, by their registers
 constexpr int kGroup = 4;  // tiles of a group (8, 16: the same times)
 constexpr int kBack = 4;   // groups before its own that a tile looks at together
@@ -542,11 +556,13 @@ __device__ __forceinline__ void enter(const Words& words, unsigned int at, unsig
 }
 
 template <typename T, int VEC, bool LOOK>
-__global__ void __launch_bounds__(kFwdWaves * kWave, LOOK ? kFwdOcc : 1) glr_fwd_kernel(FwdParams p) {
+__global__ void __launch_bounds__(FwdWaves<VEC>::kFew * kWave, LOOK ? kFwdOcc : 1)
+    glr_fwd_kernel(FwdParams p) {
+  constexpr int kWaves = FwdWaves<VEC>::kFew;
   constexpr int kCols = kWave * VEC;
   __shared__ unsigned int taken;
-  __shared__ int seqs[kFwdWaves][2 * kTok];
-  __shared__ Span spans[kFwdWaves][kCols];
+  __shared__ int seqs[kWaves][2 * kTok];
+  __shared__ Span spans[kWaves][kCols];
   __shared__ Span look[LOOK ? kGroup - 1 : 1][kCols];
   __shared__ float state[1][kCols];
   __shared__ int open;  // the tile needs the state before it
@@ -695,13 +711,16 @@ struct Cut {
   int blocks, waves;
   int64_t width;  // words of a tile
 };
-inline Cut cut_of(int64_t total, int64_t D, int vec, int max_waves) {
+template <template <int> class Waves, int VEC>
+Cut cut_of(int64_t total, int64_t D) {
+  using W = Waves<VEC>;
   Cut c;
   const int64_t windows = std::max<int64_t>(cdiv(total, kTok), 1);
-  c.waves = static_cast<int>(std::min<int64_t>(windows, max_waves));
+  c.blocks = static_cast<int>(cdiv(D, kWave * VEC));
+  c.waves = static_cast<int>(
+      std::min<int64_t>(windows, windows * c.blocks <= W::kUntil ? W::kFew : W::kMany));
   c.tiles = cdiv(windows, c.waves);
-  c.blocks = static_cast<int>(cdiv(D, kWave * vec));
-  c.width = static_cast<int64_t>(c.blocks) * kWave * vec;
+  c.width = static_cast<int64_t>(c.blocks) * kWave * VEC;
   return c;
 }
 // The workspace of a pass: its counter (a cache line of its own), its
@@ -737,7 +756,7 @@ void begin(P& p, const Cut& c, void* workspace, hipStream_t s) {
 
 template <typename T, int VEC>
 int launch_fwd_vec(FwdParams p, void* workspace, hipStream_t s) {
-  const Cut c = cut_of(p.total, p.D, VEC, kFwdWaves);
+  const Cut c = cut_of<FwdWaves, VEC>(p.total, p.D);
   begin(p, c, workspace, s);
   const dim3 grid(c.tiles * c.blocks), block(c.waves * kWave);
   if (c.tiles > 1)
@@ -956,14 +975,16 @@ __device__ __forceinline__ float exp_neg(float v) {
 //    vanishes as a gate closes: l / s -> 0 with s.
 // ---------------------------------------------------------------------------
 template <typename T, int VEC, bool LOOK>
-__global__ void __launch_bounds__(kBwdWaves * kWave, LOOK ? kBwdOcc : 1) glr_bwd_kernel(BwdParams p) {
+__global__ void __launch_bounds__(BwdWaves<VEC>::kFew * kWave, LOOK ? kBwdOcc : 1)
+    glr_bwd_kernel(BwdParams p) {
+  constexpr int kWaves = BwdWaves<VEC>::kFew;
   constexpr int kCols = kWave * VEC;
   __shared__ unsigned int taken;
-  __shared__ int seqs[kBwdWaves][2 * kTok];
-  __shared__ Span spans[kBwdWaves][kCols];
+  __shared__ int seqs[kWaves][2 * kTok];
+  __shared__ Span spans[kWaves][kCols];
   __shared__ Span look[LOOK ? kGroup - 1 : 1][kCols];
   __shared__ float state[1][kCols];
-  __shared__ float sums[kBwdWaves][kCols];
+  __shared__ float sums[kWaves][kCols];
   __shared__ int open;  // the tile needs the gradient from behind it
 
   const unsigned int lane = threadIdx.x % kWave;
@@ -1178,7 +1199,7 @@ __global__ void __launch_bounds__(1024) glr_dlam_kernel(const float* part, int64
 
 template <typename T, int VEC>
 int launch_bwd_vec(BwdParams p, bool sums, void* workspace, hipStream_t s) {
-  const Cut c = cut_of(p.total, p.D, VEC, kBwdWaves);
+  const Cut c = cut_of<BwdWaves, VEC>(p.total, p.D);
   // The workspace: counter, k and words, then dlam's parts.
   if (sums) p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + words_bytes(c));
   begin(p, c, workspace, s);
@@ -1203,9 +1224,9 @@ bool pitch_ok(int64_t pitch, int64_t D) { return pitch >= D && pitch < kMostPitc
 
 // A launch has fewer than 2^32 threads (of whole tiles), N is counted in 31 bits.
 bool bad_sizes(int64_t N, int64_t total, int64_t D) {
-  constexpr int64_t kMost = int64_t{1} << 26;
+  constexpr int64_t kMost = int64_t{1} << 26, kMostWaves = 16;
   return N < 0 || N >= int64_t{1} << 31 || total < 0 || total >= kMost * kTok || D <= 0 ||
-         D >= kMostPitch || (cdiv(total, kTok) + kFwdWaves) * cdiv(D, kWave) >= kMost;
+         D >= kMostPitch || (cdiv(total, kTok) + kMostWaves) * cdiv(D, kWave) >= kMost;
 }
 
 // cu_seqlens of a readable type, or none and N equal runs.
@@ -1220,9 +1241,9 @@ using namespace xk;
 
 extern "C" int64_t xk_gated_linear_recurrence_workspace_bytes(int64_t total_tokens, int64_t D) {
   if (bad_sizes(0, total_tokens, D)) return 0;
-  // 4-byte elements take more, narrower channel blocks.
-  return std::max(words_bytes(cut_of(total_tokens, D, 1, kFwdWaves)),
-                  words_bytes(cut_of(total_tokens, D, 2, kFwdWaves)));
+  // Of the types with one and two channels a lane.
+  return std::max(words_bytes(cut_of<FwdWaves, 1>(total_tokens, D)),
+                  words_bytes(cut_of<FwdWaves, 2>(total_tokens, D)));
 }
 
 extern "C" int xk_gated_linear_recurrence(
@@ -1286,8 +1307,8 @@ extern "C" int xk_gated_linear_recurrence_update(
 extern "C" int64_t xk_gated_linear_recurrence_bwd_workspace_bytes(int64_t total_tokens, int64_t N,
                                                                   int64_t D) {
   if (N <= 0 || bad_sizes(N, total_tokens, D)) return 0;
-  const Cut c1 = cut_of(total_tokens, D, 1, kBwdWaves), c2 = cut_of(total_tokens, D, 2, kBwdWaves);
-  return std::max(words_bytes(c1), words_bytes(c2)) + c1.tiles * D * 4;
+  const Cut c1 = cut_of<BwdWaves, 1>(total_tokens, D), c2 = cut_of<BwdWaves, 2>(total_tokens, D);
+  return std::max(words_bytes(c1), words_bytes(c2)) + std::max(c1.tiles, c2.tiles) * D * 4;
 }
 
 extern "C" int xk_gated_linear_recurrence_bwd(
@@ -1323,7 +1344,8 @@ extern "C" int xk_gated_linear_recurrence_bwd(
     if (st != XK_OK) return st;
   }
   if (dlam) {
-    const Cut cut = cut_of(total_tokens, D, dtype == XK_F32 || D == 1 ? 1 : 2, kBwdWaves);
+    const Cut cut = dtype == XK_F32 || D == 1 ? cut_of<BwdWaves, 1>(total_tokens, D)
+                                              : cut_of<BwdWaves, 2>(total_tokens, D);
     const float* part = N > 0 ? reinterpret_cast<const float*>(static_cast<char*>(workspace) +
                                                                words_bytes(cut))
                               : nullptr;
