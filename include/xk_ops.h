@@ -593,7 +593,8 @@ int xk_gated_linear_recurrence_bwd(
  *     y = h / sqrt(mean(h^2) + eps) * pre_weight      (NULL: no y)
  * in fp32; y is formed from h before its rounding.  With unit_offset != 0
  * both norms multiply by (1 + weight), as xk_gemma_rms_norm does.
- *   x, gate, y : [M, N] rows (pitch at least N) in `dtype`; residual, h in
+ *   x, gate, y : [M, N] rows (pitch at least N; N below 2^28, else
+ *     XK_ERR_INVALID) in `dtype`; residual, h in
  *     rdtype (`dtype` or f32); post_weight, pre_weight, scale : [N], wdtype
  *     (`dtype` or f32).  Any alignment.  h may be residual, y may be x or
  *     gate (the same start and pitch).

@@ -257,3 +257,7 @@ def test_sizes_that_no_launch_holds_are_refused():
         assert lib.xk_gated_linear_recurrence_bwd_workspace_bytes(total, 1, D) == 0
     # The largest that are taken: the workspace of 2^35 elements.
     assert lib.xk_gated_linear_recurrence_workspace_bytes(1 << 23, 1 << 12) > 0
+    assert _norm(M=1, N=1 << 28) == _lib.XK_ERR_INVALID
+    assert _norm_bwd(M=1, N=1 << 28, size=1 << 62) == _lib.XK_ERR_INVALID
+    assert lib.xk_gated_residual_rms_norm_bwd_workspace_bytes(1, 1 << 28) == 0
+    assert lib.xk_gated_residual_rms_norm_bwd_workspace_bytes(1, (1 << 28) - 1) > 0

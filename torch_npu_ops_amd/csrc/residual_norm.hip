@@ -163,6 +163,8 @@ __global__ void __launch_bounds__(256)
   }
 }
 
+// 16 elements of a row take 256 lanes of sums_kernel, fewer than 2^32 of them.
+constexpr int64_t kMostRow = int64_t{1} << 28;
 bool pitch_bad(const void* p, int64_t pitch, int64_t N) { return p && pitch < N; }
 
 }  // namespace
@@ -189,7 +191,7 @@ extern "C" int xk_gated_residual_rms_norm(
     float* rstd_post, float* rstd_pre, int64_t M, int64_t N, float eps, int unit_offset,
     xk_dtype dtype, xk_dtype rdtype, xk_dtype wdtype, void* stream) {
   using namespace resnorm;
-  if (M < 0 || N <= 0 || N > (int64_t{1} << 30) || !(eps >= 0.f)) return XK_ERR_INVALID;
+  if (M < 0 || N <= 0 || N >= kMostRow || !(eps >= 0.f)) return XK_ERR_INVALID;
   if (!is_float_dtype(dtype) || (rdtype != dtype && rdtype != XK_F32) ||
       (wdtype != dtype && wdtype != XK_F32))
     return XK_ERR_UNSUPPORTED;
@@ -211,7 +213,7 @@ extern "C" int xk_gated_residual_rms_norm(
 }
 
 extern "C" int64_t xk_gated_residual_rms_norm_bwd_workspace_bytes(int64_t M, int64_t N) {
-  if (M <= 0 || N <= 0) return 0;
+  if (M <= 0 || N <= 0 || N >= resnorm::kMostRow) return 0;
   // The parts of the types with 4 and 8 elements a lane.
   return std::max(resnorm::sum_parts(M, N, 4), resnorm::sum_parts(M, N, 8)) * 3 *
          resnorm::part_pitch(N) * 4;
@@ -227,7 +229,7 @@ extern "C" int xk_gated_residual_rms_norm_bwd(
     xk_dtype dtype, xk_dtype rdtype, xk_dtype wdtype, void* workspace, size_t workspace_bytes,
     void* stream) {
   using namespace resnorm;
-  if (M < 0 || N <= 0 || N > (int64_t{1} << 30)) return XK_ERR_INVALID;
+  if (M < 0 || N <= 0 || N >= kMostRow) return XK_ERR_INVALID;
   if (!is_float_dtype(dtype) || (rdtype != dtype && rdtype != XK_F32) ||
       (wdtype != dtype && wdtype != XK_F32))
     return XK_ERR_UNSUPPORTED;
