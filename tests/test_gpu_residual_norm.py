@@ -301,3 +301,31 @@ def test_same_bits_two_streams_and_graph(dev):
         graph.replay()
         torch.cuda.synchronize()
         assert same(out, eager)
+
+
+@pytest.mark.parametrize("N", [7, 1025, 1027, 1031, 2051, 4101, 8195])
+def test_output_over_residual_where_a_row_ends_inside_a_vector(dev, N):
+    # The last lane reads elements that another wave writes; without the first
+    # norm no barrier stands between.  Around the rows everything stays.
+    from torch_npu_ops_amd import _lib
+    M, pitch = 37, N + 5
+    p = _inputs(N, M, N, BF16, parts=("scale", "pre"))
+    d = _dev(p, dev)
+    h, y, _, _ = _both()["cpp"].npu_gated_residual_rms_norm(*_args(d), EPS)
+    buf = torch.full((M, pitch), 3.0, dtype=BF16, device=dev)
+    out = buf.clone()
+    buf[:, :N] = d["res"]
+    st = _lib.lib().xk_gated_residual_rms_norm(
+        d["x"].data_ptr(), N, buf.data_ptr(), pitch, None, 0, None, d["scale"].data_ptr(),
+        d["pre"].data_ptr(), buf.data_ptr(), pitch, out.data_ptr(), pitch, None, None, M, N, EPS, 0,
+        _lib.XK_BF16, _lib.XK_BF16, _lib.XK_BF16, torch.cuda.current_stream().cuda_stream)
+    assert st == _lib.XK_OK
+    assert torch.equal(buf[:, :N], h) and torch.equal(out[:, :N], y)
+    assert (buf[:, N:] == 3.0).all() and (out[:, N:] == 3.0).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("N", [1, 3, 5, 9, 15, 17, 519, 1023, 1029, 2057])
+def test_every_remainder_of_a_vector(dev, N, dtype):
+    p = _inputs(N, 11, N, dtype, rdtype=F32)
+    _check(_both()["cpp"], p, dev)

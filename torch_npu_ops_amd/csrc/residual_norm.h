@@ -11,7 +11,8 @@
 //  * A team of TPR lanes owns a row and holds it in registers as vectors of
 //    VEC elements, NV per lane, so both norms' sums and the outputs take one
 //    read.  Vectors are read wherever they start (rows of odd length or
-//    offset included): only a row's last, partial vector goes by elements.
+//    offset included); a row's last one overlaps the one before it where the
+//    row ends inside a lane.
 //  * Parts that a call leaves out are uniform branches on their pointers.
 //
 // 16,384 x 4,096 bf16 forward 125 us (671 MB, 5.4 TB/s, 87% of a plain copy);
@@ -116,10 +117,26 @@ __device__ __forceinline__ Row<T, VEC> pack(const float (&v)[VEC]) {
   return __builtin_bit_cast(Row<T, VEC>, t);
 }
 
-// Moves of a lane's elements, 16 bytes at a time and at any address; `left`
-// elements of the row are left at p.  TAIL: rows may end inside a lane, whose
-// elements then go one by one (without it a row's lanes are full or empty).
-// Loads give zeros beyond the row.  STREAM: read or written once.
+// A lane's elements of a row: VEC of them from `at`, or the row's last VEC where
+// it ends inside them (TAIL; N >= VEC): the first `twice` of those are the
+// lane's before it, which count in no sum and are not written (where h lies over
+// the residual they may have changed).  Rows of 3,316 take 28.5 us forward and
+// 71 backward, of 3,312 27 and 57 (3,686 rows); with the last elements loaded
+// one by one 39 and 81.
+// `left`: its own elements if positive and below VEC, nothing if not.
+template <int VEC, bool TAIL>
+struct Place {
+  int at, left, twice;
+  __device__ __forceinline__ Place(int first, int N)
+      : at(TAIL && first > N - VEC ? N - VEC : first), left(N - first), twice(first - at) {}
+  // The sum with element u, or without it.
+  __device__ __forceinline__ float own(int u, float with, float without) const {
+    return TAIL && u < twice ? without : with;
+  }
+};
+
+// Moves of a lane's elements, 16 bytes at a time and at any address.  Loads
+// give zeros to lanes without elements.  STREAM: read or written once.
 typedef u32x4 Word4At2 __attribute__((aligned(2)));
 typedef u32x4 Word4At4 __attribute__((aligned(4)));
 template <typename T>
@@ -128,12 +145,12 @@ template <typename T>
 using Word4Out = typename std::conditional<sizeof(T) == 2, Word4At2*, Word4At4*>::type;
 
 template <typename T, int VEC, bool TAIL, bool STREAM = true>
-__device__ __forceinline__ Row<T, VEC> ld_row(const T* p, int left) {
+__device__ __forceinline__ Row<T, VEC> ld_row(const T* row, const Place<VEC, TAIL>& l) {
   Row<T, VEC> out{};
-  if (left >= VEC) {
+  if (l.left > 0) {
 #pragma unroll
     for (int c = 0; c < out.kWords / 4; ++c) {
-      const Word4<T> q = reinterpret_cast<Word4<T>>(p + c * (16 / sizeof(T)));
+      const Word4<T> q = reinterpret_cast<Word4<T>>(row + l.at + c * (16 / sizeof(T)));
       u32x4 r;
       if constexpr (STREAM)
         r = __builtin_nontemporal_load(q);
@@ -144,33 +161,31 @@ __device__ __forceinline__ Row<T, VEC> ld_row(const T* p, int left) {
       out.w[4 * c + 2] = r.z;
       out.w[4 * c + 3] = r.w;
     }
-  } else if constexpr (TAIL) {
-    Arr<T, VEC> t;
-#pragma unroll
-    for (int u = 0; u < VEC; ++u) t.v[u] = u < left ? p[u] : from_f32<T>(0.f);
-    out = __builtin_bit_cast(Row<T, VEC>, t);
   }
   return out;
 }
 template <typename T, int VEC, bool TAIL>
-__device__ __forceinline__ void st_row(T* p, const Row<T, VEC>& in, int left) {
-  if (left >= VEC) {
+__device__ __forceinline__ void st_row(T* row, const Row<T, VEC>& in, const Place<VEC, TAIL>& l) {
+  T* p = row + l.at;
+  if (l.left >= VEC) {
 #pragma unroll
     for (int c = 0; c < in.kWords / 4; ++c) {
       const u32x4 r = {in.w[4 * c], in.w[4 * c + 1], in.w[4 * c + 2], in.w[4 * c + 3]};
       __builtin_nontemporal_store(r, reinterpret_cast<Word4Out<T>>(p + c * (16 / sizeof(T))));
     }
   } else if constexpr (TAIL) {
-    const Arr<T, VEC> t = __builtin_bit_cast(Arr<T, VEC>, in);
+    if (l.left > 0) {
+      const Arr<T, VEC> t = __builtin_bit_cast(Arr<T, VEC>, in);
 #pragma unroll
-    for (int u = 0; u < VEC; ++u)
-      if (u < left) p[u] = t.v[u];
+      for (int u = 1; u < VEC; ++u)
+        if (u >= l.twice) p[u] = t.v[u];
+    }
   }
 }
 // Weights are read again by every row and stay in the caches.
 template <typename W, int VEC, bool TAIL>
-__device__ __forceinline__ Row<W, VEC> ld_weight(const void* base, int at, int left) {
-  return ld_row<W, VEC, TAIL, false>(static_cast<const W*>(base) + at, left);
+__device__ __forceinline__ Row<W, VEC> ld_weight(const void* base, const Place<VEC, TAIL>& l) {
+  return ld_row<W, VEC, TAIL, false>(static_cast<const W*>(base), l);
 }
 
 // Sum over the TPR lanes of a team.  Teams wider than a wave are the whole
@@ -217,35 +232,37 @@ __global__ void __launch_bounds__(block_of<TPR>()) fwd_kernel(FwdParams p) {
     Row<WT, VEC> w1[NV], w2[NV], sc[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int at = (j * TPR + lane) * VEC;
-      x[j] = ld_row<T, VEC, TAIL>(xr + at, N - at);
-      if (gate) z[j] = ld_row<T, VEC, TAIL>(zr + at, N - at);
-      res[j] = ld_row<RT, VEC, TAIL>(rr + at, N - at);
+      const Place<VEC, TAIL> l((j * TPR + lane) * VEC, N);
+      x[j] = ld_row<T, VEC, TAIL>(xr, l);
+      if (gate) z[j] = ld_row<T, VEC, TAIL>(zr, l);
+      res[j] = ld_row<RT, VEC, TAIL>(rr, l);
     }
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int at = (j * TPR + lane) * VEC;
-      if (post) w1[j] = ld_weight<WT, VEC, TAIL>(p.post, at, N - at);
-      if (scale) sc[j] = ld_weight<WT, VEC, TAIL>(p.scale, at, N - at);
-      if (pre) w2[j] = ld_weight<WT, VEC, TAIL>(p.pre, at, N - at);
+      const Place<VEC, TAIL> l((j * TPR + lane) * VEC, N);
+      if (post) w1[j] = ld_weight<WT, VEC, TAIL>(p.post, l);
+      if (scale) sc[j] = ld_weight<WT, VEC, TAIL>(p.scale, l);
+      if (pre) w2[j] = ld_weight<WT, VEC, TAIL>(p.pre, l);
     }
     float r1 = 1.f;
     if (post) {
       float ss = 0.f;
 #pragma unroll
-      for (int j = 0; j < NV; ++j)
+      for (int j = 0; j < NV; ++j) {
+        const Place<VEC, TAIL> l((j * TPR + lane) * VEC, N);
 #pragma unroll
         for (int u = 0; u < VEC; ++u) {
           const float f = x[j][u];
-          ss = fmaf(f, f, ss);
+          ss = l.own(u, fmaf(f, f, ss), ss);
         }
+      }
       r1 = 1.f / sqrtf(team_sum<TPR>(ss, red, 0) * inv_n + p.eps);
       if (p.r1 && lane == 0) p.r1[row] = r1;
     }
     float h[NV][VEC], ss = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int at = (j * TPR + lane) * VEC;
+      const Place<VEC, TAIL> l((j * TPR + lane) * VEC, N);
       float out[VEC];
 #pragma unroll
       for (int u = 0; u < VEC; ++u) {
@@ -253,21 +270,21 @@ __global__ void __launch_bounds__(block_of<TPR>()) fwd_kernel(FwdParams p) {
         if (post) v *= r1 * (w1[j][u] + p.off);
         if (gate) v *= silu(z[j][u]);
         v = scale ? fmaf(v, sc[j][u], res[j][u]) : v + res[j][u];
-        ss = fmaf(v, v, ss);
         h[j][u] = out[u] = v;
+        ss = l.own(u, fmaf(v, v, ss), ss);
       }
-      st_row<RT, VEC, TAIL>(static_cast<RT*>(p.h) + row * p.sh + at, pack<RT, VEC>(out), N - at);
+      st_row<RT, VEC, TAIL>(static_cast<RT*>(p.h) + row * p.sh, pack<RT, VEC>(out), l);
     }
     if (pre) {
       const float r2 = 1.f / sqrtf(team_sum<TPR>(ss, red, 1) * inv_n + p.eps);
       if (p.r2 && lane == 0) p.r2[row] = r2;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        const int at = (j * TPR + lane) * VEC;
+        const Place<VEC, TAIL> l((j * TPR + lane) * VEC, N);
         float out[VEC];
 #pragma unroll
         for (int u = 0; u < VEC; ++u) out[u] = h[j][u] * r2 * (w2[j][u] + p.off);
-        st_row<T, VEC, TAIL>(static_cast<T*>(p.y) + row * p.sy + at, pack<T, VEC>(out), N - at);
+        st_row<T, VEC, TAIL>(static_cast<T*>(p.y) + row * p.sy, pack<T, VEC>(out), l);
       }
     }
     // One barrier more where only one of the two sums runs: its half of `red`
@@ -289,27 +306,27 @@ __global__ void __launch_bounds__(block_of<TPR>(), 4) bwd_kernel(BwdParams p) {
   __shared__ float red[2 * (TPR > kWave ? TPR / kWave : 1)];
   const bool post = p.post, gate = p.gate, scale = p.scale, has_dy = p.dy, has_dh = p.dh;
   const int lane = threadIdx.x % TPR, N = static_cast<int>(p.N);
-  const int at = lane * VEC, left = N - at;
+  const Place<VEC, TAIL> l(lane * VEC, N);
   const float inv_n = 1.f / static_cast<float>(p.N);
   const int64_t team = static_cast<int64_t>(blockIdx.x) * kTeams + threadIdx.x / TPR;
   float a_post[VEC] = {}, a_scale[VEC] = {}, a_pre[VEC] = {};
   Row<WT, VEC> w1{}, w2{}, sc{};
-  if (post) w1 = ld_weight<WT, VEC, TAIL>(p.post, at, left);
-  if (has_dy) w2 = ld_weight<WT, VEC, TAIL>(p.pre, at, left);
-  if (scale) sc = ld_weight<WT, VEC, TAIL>(p.scale, at, left);
+  if (post) w1 = ld_weight<WT, VEC, TAIL>(p.post, l);
+  if (has_dy) w2 = ld_weight<WT, VEC, TAIL>(p.pre, l);
+  if (scale) sc = ld_weight<WT, VEC, TAIL>(p.scale, l);
   for (int64_t row = team; team < p.parts && row < p.M; row += p.parts) {
     Row<T, VEC> x, z{}, dy{};
     Row<RT, VEC> res{}, dh{};
     w1.again();
     w2.again();
     sc.again();
-    x = ld_row<T, VEC, TAIL>(static_cast<const T*>(p.x) + row * p.sx + at, left);
-    if (gate) z = ld_row<T, VEC, TAIL>(static_cast<const T*>(p.gate) + row * p.sgate + at, left);
+    x = ld_row<T, VEC, TAIL>(static_cast<const T*>(p.x) + row * p.sx, l);
+    if (gate) z = ld_row<T, VEC, TAIL>(static_cast<const T*>(p.gate) + row * p.sgate, l);
     if (has_dy) {
-      dy = ld_row<T, VEC, TAIL>(static_cast<const T*>(p.dy) + row * p.sdy + at, left);
-      res = ld_row<RT, VEC, TAIL>(static_cast<const RT*>(p.res) + row * p.sres + at, left);
+      dy = ld_row<T, VEC, TAIL>(static_cast<const T*>(p.dy) + row * p.sdy, l);
+      res = ld_row<RT, VEC, TAIL>(static_cast<const RT*>(p.res) + row * p.sres, l);
     }
-    if (has_dh) dh = ld_row<RT, VEC, TAIL>(static_cast<const RT*>(p.dh) + row * p.sdh + at, left);
+    if (has_dh) dh = ld_row<RT, VEC, TAIL>(static_cast<const RT*>(p.dh) + row * p.sdh, l);
     const float r1 = post ? p.r1[row] : 1.f;
     const float r2 = has_dy ? p.r2[row] : 0.f;
     float sg[VEC], hh[VEC], ss = 0.f;  // hh: h rstd2, then w1' dn
@@ -327,7 +344,7 @@ __global__ void __launch_bounds__(block_of<TPR>(), 4) bwd_kernel(BwdParams p) {
         hh[u] = (scale ? fmaf(v, sc[u], res[u]) : v + res[u]) * r2;
         const float g = dy[u];
         a_pre[u] = fmaf(g, hh[u], a_pre[u]);
-        ss = fmaf(g * (w2[u] + p.off), hh[u], ss);
+        ss = l.own(u, fmaf(g * (w2[u] + p.off), hh[u], ss), ss);
       }
     }
     if (has_dy) ss = team_sum<TPR>(ss, red, 0) * inv_n;
@@ -356,32 +373,37 @@ __global__ void __launch_bounds__(block_of<TPR>(), 4) bwd_kernel(BwdParams p) {
       if (post) {
         a_post[u] = fmaf(g, xh, a_post[u]);
         g *= w1[u] + p.off;
-        dot = fmaf(g, xh, dot);
+        dot = l.own(u, fmaf(g, xh, dot), dot);
       }
       hh[u] = g;
     }
     if (p.dres)
-      st_row<RT, VEC, TAIL>(static_cast<RT*>(p.dres) + row * p.sdres + at, pack<RT, VEC>(o_res), left);
+      st_row<RT, VEC, TAIL>(static_cast<RT*>(p.dres) + row * p.sdres, pack<RT, VEC>(o_res), l);
     if (gate && p.dgate)
-      st_row<T, VEC, TAIL>(static_cast<T*>(p.dgate) + row * p.sdgate + at, pack<T, VEC>(o_gate),
-                     left);
+      st_row<T, VEC, TAIL>(static_cast<T*>(p.dgate) + row * p.sdgate, pack<T, VEC>(o_gate), l);
     if (post) dot = team_sum<TPR>(dot, red, 1) * inv_n;
     if (p.dx) {
       x.again();
       float out[VEC];
 #pragma unroll
       for (int u = 0; u < VEC; ++u) out[u] = post ? r1 * fmaf(x[u] * -r1, dot, hh[u]) : hh[u];
-      st_row<T, VEC, TAIL>(static_cast<T*>(p.dx) + row * p.sdx + at, pack<T, VEC>(out), left);
+      st_row<T, VEC, TAIL>(static_cast<T*>(p.dx) + row * p.sdx, pack<T, VEC>(out), l);
     }
     if constexpr (TPR > kWave) {
       if (!post || !has_dy) __syncthreads();
     }
   }
-  if (p.sums && team < p.parts && left > 0) {
-    // Rows of parts are padded to whole lanes.
+  if (p.sums && team < p.parts && l.left > 0) {
     const int64_t pitch = part_pitch(p.N);
-    float* out = p.part + team * 3 * pitch + at;
+    float* out = p.part + team * 3 * pitch + l.at;
     auto put = [&](const float (&v)[VEC]) {
+      if (TAIL && l.twice) {
+#pragma unroll
+        for (int u = 1; u < VEC; ++u)
+          if (u >= l.twice) out[u] = v[u];
+        out += pitch;
+        return;
+      }
 #pragma unroll
       for (int u = 0; u < VEC; u += 4)
         *reinterpret_cast<Vec<float, 4>*>(out + u) = {{v[u], v[u + 1], v[u + 2], v[u + 3]}};
@@ -419,7 +441,8 @@ int launch_bwd(const BwdParams& p, hipStream_t s) {
 }
 
 // Rows of any length, one block each, read as often as needed: only for rows
-// longer than a block holds (above 32K elements at 16 bits).
+// longer than a block holds (above 32K elements at 16 bits) and for those of less
+// than a lane's elements.
 int stream_fwd(const FwdParams& p, hipStream_t s);
 int stream_bwd(const BwdParams& p, hipStream_t s);
 
@@ -427,6 +450,7 @@ template <typename T, typename RT, typename WT>
 int run_fwd_w(const FwdParams& p, hipStream_t s) {
   constexpr int VEC = 16 / sizeof(T);
   const int64_t nvec = cdiv(p.N, VEC);
+  if (p.N < VEC) return stream_fwd(p, s);
   if (nvec <= 64) return launch_fwd<T, RT, WT, 64, 1>(p, s);
   if (nvec <= 128) return launch_fwd<T, RT, WT, 64, 2>(p, s);
   if (nvec <= 256) return launch_fwd<T, RT, WT, 256, 1>(p, s);
@@ -442,6 +466,7 @@ int run_fwd_w(const FwdParams& p, hipStream_t s) {
 
 template <typename T, typename RT, typename WT>
 int run_bwd_w(const BwdParams& p, hipStream_t s) {
+  if (p.N < 16 / static_cast<int>(sizeof(T))) return stream_bwd(p, s);
   switch (bwd_lanes(p.N, 16 / sizeof(T))) {
     case 64: return launch_bwd<T, RT, WT, 64>(p, s);
     case 128: return launch_bwd<T, RT, WT, 128>(p, s);
