@@ -329,3 +329,11 @@ def test_output_over_residual_where_a_row_ends_inside_a_vector(dev, N):
 def test_every_remainder_of_a_vector(dev, N, dtype):
     p = _inputs(N, 11, N, dtype, rdtype=F32)
     _check(_both()["cpp"], p, dev)
+
+
+@pytest.mark.parametrize("dtype, rdtype", [(BF16, BF16), (BF16, F32), (F32, F32)], ids=str)
+@pytest.mark.parametrize("vectors", [257, 384, 385, 513, 700, 768, 769, 1000, 1025, 1500, 1537])
+def test_teams_of_every_size(dev, vectors, dtype, rdtype):
+    N = vectors * (16 // dtype.itemsize)
+    for n in (N, N - 3):
+        _check(_both()["cpp"], _inputs(vectors, 5, n, dtype, rdtype=rdtype), dev)
