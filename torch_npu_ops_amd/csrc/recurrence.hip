@@ -147,7 +147,8 @@ __device__ __forceinline__ int cu_at(const void* cu, int cu64, int n, int run, i
 constexpr int kTok = kWin;
 // Waves of a block at most: kFew while a pass has no more than kUntil windows
 // over all channel blocks, where the chain between tiles is the longest part
-// and longer tiles shorten it, else kMany.  Forward, one channel a lane, 16
+// and longer tiles shorten it, else kMany, and where one tile holds the batch
+// (no chain, and registers as a tile's waves need them).  Forward, one channel a lane, 16
 // against 8 waves: 5,003 x 1,125 29.6 and 32.6 us, 2,048 x 2,048 18.8 and 20.3,
 // 16,384 x 1,000 65.6 and 67.9; 8,192 x 4,096 105 and 96.  Two channels: 8
 // throughout (16: 2,048 x 2,048 20.4 and 17.4; 4: within 1 to 4%).  Backward, two
@@ -156,10 +157,12 @@ constexpr int kTok = kWin;
 template <int VEC>
 struct FwdWaves {
   static constexpr int kFew = VEC == 1 ? 16 : 8, kMany = 8, kUntil = 16384;
+  static constexpr int most(bool look) { return look ? kFew : kMany; }
 };
 template <int VEC>
 struct BwdWaves {
   static constexpr int kFew = VEC == 1 ? 4 : 8, kMany = 4, kUntil = 8192;
+  static constexpr int most(bool look) { return look ? kFew : kMany; }
 };
 constexpr int kFwdOcc = 4, kBwdOcc = 2;  // waves a SIMD holds, by their registers
 constexpr int kGroup = 4;  // tiles of a group (8, 16: the same times)
@@ -557,9 +560,9 @@ __device__ __forceinline__ void enter(const Words& words, unsigned int at, unsig
 }
 
 template <typename T, int VEC, bool LOOK>
-__global__ void __launch_bounds__(FwdWaves<VEC>::kFew * kWave, LOOK ? kFwdOcc : 1)
+__global__ void __launch_bounds__(FwdWaves<VEC>::most(LOOK) * kWave, LOOK ? kFwdOcc : 1)
     glr_fwd_kernel(FwdParams p) {
-  constexpr int kWaves = FwdWaves<VEC>::kFew;
+  constexpr int kWaves = FwdWaves<VEC>::most(LOOK);
   constexpr int kCols = kWave * VEC;
   __shared__ unsigned int taken;
   __shared__ int seqs[kWaves][2 * kTok];
@@ -718,8 +721,9 @@ Cut cut_of(int64_t total, int64_t D) {
   Cut c;
   const int64_t windows = std::max<int64_t>(cdiv(total, kTok), 1);
   c.blocks = static_cast<int>(cdiv(D, kWave * VEC));
-  c.waves = static_cast<int>(
-      std::min<int64_t>(windows, windows * c.blocks <= W::kUntil ? W::kFew : W::kMany));
+  const bool few = windows > W::kMany && windows * c.blocks <= W::kUntil;
+  c.waves = static_cast<int>(std::min<int64_t>(windows, few ? W::kFew : W::kMany));
+  if (few && windows <= W::kFew) c.waves = W::kMany;  // two tiles
   c.tiles = cdiv(windows, c.waves);
   c.width = static_cast<int64_t>(c.blocks) * kWave * VEC;
   return c;
@@ -934,7 +938,7 @@ struct BwdParams {
   const float* h0;
   const float* dfin;
   float* dh0;
-  float* part;  // dlam's parts, [tiles][D]; NULL: not asked for
+  float* part;  // dlam's parts, [tiles][D] (one tile: dlam); NULL: not asked for
   const void* cu;
   int cu64;
   int64_t N, T, total, D;
@@ -977,9 +981,9 @@ __device__ __forceinline__ float exp_neg(float v) {
 //    vanishes as a gate closes: l / s -> 0 with s.
 // ---------------------------------------------------------------------------
 template <typename T, int VEC, bool LOOK>
-__global__ void __launch_bounds__(BwdWaves<VEC>::kFew * kWave, LOOK ? kBwdOcc : 1)
+__global__ void __launch_bounds__(BwdWaves<VEC>::most(LOOK) * kWave, LOOK ? kBwdOcc : 1)
     glr_bwd_kernel(BwdParams p) {
-  constexpr int kWaves = BwdWaves<VEC>::kFew;
+  constexpr int kWaves = BwdWaves<VEC>::most(LOOK);
   constexpr int kCols = kWave * VEC;
   __shared__ unsigned int taken;
   __shared__ int seqs[kWaves][2 * kTok];
@@ -1174,6 +1178,11 @@ __global__ void __launch_bounds__(BwdWaves<VEC>::kFew * kWave, LOOK ? kBwdOcc : 
 #pragma unroll
         for (int u = 0; u < VEC; ++u) sum[u] += sums[w][lane * VEC + u];
       }
+      if constexpr (!LOOK) {  // the only tile: dlam itself
+#pragma unroll
+        for (int u = 0; u < VEC; ++u)
+          if (at.ok[u]) sum[u] *= slope_ratio(p.lam[at.ch + u]);
+      }
       st_f32<VEC>(p.part + tile * p.D, at, sum);
     }
   }
@@ -1200,24 +1209,30 @@ __global__ void __launch_bounds__(1024) glr_dlam_kernel(const float* part, int64
 }
 
 template <typename T, int VEC>
-int launch_bwd_vec(BwdParams p, bool sums, void* workspace, hipStream_t s) {
+int launch_bwd_vec(BwdParams p, float* dlam, void* workspace, hipStream_t s) {
   const Cut c = cut_of<BwdWaves, VEC>(p.total, p.D);
   // The workspace: counter, k and words, then dlam's parts.
-  if (sums) p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + words_bytes(c));
+  if (dlam)
+    p.part = c.tiles == 1
+                 ? dlam
+                 : reinterpret_cast<float*>(static_cast<char*>(workspace) + words_bytes(c));
   begin(p, c, workspace, s);
   const dim3 grid(c.tiles * c.blocks), block(c.waves * kWave);
   if (c.tiles > 1)
     hipLaunchKernelGGL((glr_bwd_kernel<T, VEC, true>), grid, block, 0, s, p);
   else
     hipLaunchKernelGGL((glr_bwd_kernel<T, VEC, false>), grid, block, 0, s, p);
+  if (dlam && c.tiles > 1)
+    hipLaunchKernelGGL(glr_dlam_kernel, dim3(cdiv(p.D, kWave)), dim3(1024), 0, s, p.part, c.tiles,
+                       p.lam, dlam, p.D);
   return launch_status();
 }
 template <typename T>
-int launch_bwd(const BwdParams& p, bool sums, void* workspace, hipStream_t s) {
+int launch_bwd(const BwdParams& p, float* dlam, void* workspace, hipStream_t s) {
   if constexpr (sizeof(T) == 2) {
-    if (p.D > 1) return launch_bwd_vec<T, 2>(p, sums, workspace, s);
+    if (p.D > 1) return launch_bwd_vec<T, 2>(p, dlam, workspace, s);
   }
-  return launch_bwd_vec<T, 1>(p, sums, workspace, s);
+  return launch_bwd_vec<T, 1>(p, dlam, workspace, s);
 }
 
 // A window's rows have to lie within kRange bytes: the most elements of a pitch.
@@ -1340,19 +1355,14 @@ extern "C" int xk_gated_linear_recurrence_bwd(
                       initial_state, d_final_state, d_initial_state, nullptr, cu_seqlens,
                       cu_dtype == XK_I64, N, total_tokens / N, total_tokens, D, nullptr, nullptr,
                       nullptr, nullptr, 0, 0, 0};
-    const int st = dtype == XK_F32    ? launch_bwd<float>(p, dlam, workspace, s)
-                   : dtype == XK_BF16 ? launch_bwd<bf16>(p, dlam, workspace, s)
-                                      : launch_bwd<f16>(p, dlam, workspace, s);
-    if (st != XK_OK) return st;
+    switch (dtype) {
+      case XK_F32: return launch_bwd<float>(p, dlam, workspace, s);
+      case XK_BF16: return launch_bwd<bf16>(p, dlam, workspace, s);
+      default: return launch_bwd<f16>(p, dlam, workspace, s);
+    }
   }
-  if (dlam) {
-    const Cut cut = dtype == XK_F32 || D == 1 ? cut_of<BwdWaves, 1>(total_tokens, D)
-                                              : cut_of<BwdWaves, 2>(total_tokens, D);
-    const float* part = N > 0 ? reinterpret_cast<const float*>(static_cast<char*>(workspace) +
-                                                               words_bytes(cut))
-                              : nullptr;
-    hipLaunchKernelGGL(glr_dlam_kernel, dim3(cdiv(D, kWave)), dim3(1024), 0, s, part,
-                       N > 0 ? cut.tiles : 0, lam, dlam, D);
-  }
+  if (dlam)  // no sequences: zeros
+    hipLaunchKernelGGL(glr_dlam_kernel, dim3(cdiv(D, kWave)), dim3(1024), 0, s, nullptr, 0, lam,
+                       dlam, D);
   return launch_status();
 }
