@@ -139,7 +139,7 @@ __device__ __forceinline__ int cu_at(const void* cu, int cu64, int n, int run, i
 // so no fences are needed.
 //
 // The forward kernel takes 126 us for 16,384 x 4,096 bf16 (537 MB, 4.3 TB/s):
-// with loads and stores alone 92, without the arithmetic (36 instructions a
+// with loads and stores alone 92, without the arithmetic (34 instructions a
 // channel and token) 104, without the chain 115.  The window's 48 loads are
 // issued together, which takes 128 registers: 4 waves a SIMD hide the rest
 // only in part.  Windows of 8 tokens (8 waves) took 150 and more.
