@@ -500,6 +500,8 @@ int xk_chunk_fwd_o(const void* q, const void* k, const void* v, const void* h,
  *     r = sigmoid(a_t), i = sigmoid(b_t), l = -c softplus(lam) r,
  *     h_t = exp(l) h_{t-1} + sqrt(1 - exp(2 l)) i x_t,    y_t = h_t
  * per channel, in fp32 whatever the inputs' type.
+ * An infinite input or state makes its channel NaN from a later token on (the
+ * decay is applied as h + (exp(l) - 1) h); other channels are not touched.
  *   x, a, b, y : [total_tokens, D] rows with token pitches (at least D, below
  *     2^25 elements) in `dtype` (f32/bf16/f16), any alignment; lam fp32 [D];
  *     c >= 0.  y may be x, a or b itself (the same start and pitch).

@@ -507,3 +507,29 @@ def test_many_tiles_of_either_length(dev, T, D, dtype):
     # More windows than the rule's limit for long tiles, and fewer.
     print(f"T={T} D={D} {dtype}", flush=True)
     _check(dev, _both()["cpp"], [T // 3, 0, 1, T - T // 3 - 1], D, dtype, seed=T)
+
+
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("where", ["x", "a", "b", "h0"])
+def test_a_value_that_is_not_finite_stays_in_its_channel_and_sequence(dev, where, value):
+    from torch_npu_ops_amd import _xk_torch as xt
+    T, D = 700, 131
+    x, a, b, dy, lam, h0, df = _inputs(23, T, D, 2, BF16)
+    cu = torch.tensor([0, 400, 700], dtype=torch.int32, device=dev)
+    t = {"x": x, "a": a, "b": b, "h0": h0}
+
+    def run():
+        d = {k: v.to(dev) for k, v in t.items()}
+        out = xt.npu_gated_linear_recurrence(d["x"], d["a"], d["b"], lam.to(dev), C, d["h0"], True, cu)
+        return out[0][0].float().cpu()
+    clean = run()
+    if where == "h0":
+        t["h0"][0, 64] = value
+    else:
+        t[where][0, 17, 64] = value
+    got = run()
+    kept = torch.ones_like(clean, dtype=torch.bool)
+    kept[17 if where != "h0" else 0:400, 64] = False
+    assert torch.equal(got[kept], clean[kept])
+    if value != value:  # NaN reaches every later token of the sequence
+        assert got[17:400, 64].isnan().all() and got[400:].isfinite().all()
