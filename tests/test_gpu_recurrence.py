@@ -533,3 +533,22 @@ def test_a_value_that_is_not_finite_stays_in_its_channel_and_sequence(dev, where
     assert torch.equal(got[kept], clean[kept])
     if value != value:  # NaN reaches every later token of the sequence
         assert got[17:400, 64].isnan().all() and got[400:].isfinite().all()
+
+
+@pytest.mark.parametrize("default", [BF16, torch.float64], ids=str)
+def test_another_default_dtype(dev, default):
+    print(f"default dtype {default}", flush=True)
+    torch.set_default_dtype(default)
+    try:
+        x, a, b, dy, lam, h0, df = _inputs(90, 200, 72, 2, BF16)
+        both = {}
+        for name, api in _both().items():
+            d = [t.to(dev) for t in (x, a, b, lam.float())]
+            cu = torch.tensor([0, 70, 200], dtype=torch.int32, device=dev)
+            y, fin, st = api.npu_gated_linear_recurrence(*d, C, None, True, cu, True)
+            both[name] = [y, fin, st[1:4], *api.npu_gated_linear_recurrence_bwd(
+                dy.to(dev), *d, st, C, None, None, cu)]
+        assert all(torch.equal(p, q) and p.dtype == q.dtype
+                   for p, q in zip(both["cpp"], both["py"]))
+    finally:
+        torch.set_default_dtype(torch.float32)

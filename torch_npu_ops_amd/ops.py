@@ -947,6 +947,11 @@ def _same_device(x, **others):
             raise ValueError(f"{name} must be on {x.device}, is on {t.device}")
 
 
+def _f32(x, *sizes):
+    """A new fp32 tensor on x's device, whatever torch's default dtype is."""
+    return torch.empty(sizes, dtype=torch.float32, device=x.device)
+
+
 def _pitched_rows(x: torch.Tensor):
     """(x as rows of its last dim with one pitch between them, a copy only if
     it has no such form; the pitch in elements)."""
@@ -1024,9 +1029,8 @@ def npu_gated_linear_recurrence(x: torch.Tensor, a: torch.Tensor, b: torch.Tenso
     lam = lam.contiguous()
     with torch.cuda.device(x.device):
         y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        fin = torch.empty(N, D, device=x.device) if output_final_state else None
-        states = (torch.empty(-(-total // _lib.XK_GLR_WINDOW), D, device=x.device)
-                  if output_states else None)
+        fin = _f32(x, N, D) if output_final_state else None
+        states = _f32(x, -(-total // _lib.XK_GLR_WINDOW), D) if output_states else None
         size = lib().xk_gated_linear_recurrence_workspace_bytes(total, D)
         ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
         st = lib().xk_gated_linear_recurrence(
@@ -1125,7 +1129,7 @@ def npu_gated_linear_recurrence_bwd(dy: torch.Tensor, x: torch.Tensor, a: torch.
     lam, states = lam.contiguous(), states.contiguous()
     with torch.cuda.device(x.device):
         dx, da, db = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for _ in range(3))
-        dlam, dh0 = torch.empty(D, device=x.device), torch.empty(N, D, device=x.device)
+        dlam, dh0 = _f32(x, D), _f32(x, N, D)
         size = lib().xk_gated_linear_recurrence_bwd_workspace_bytes(total, N, D)
         ws = torch.empty(max(size, 1), dtype=torch.uint8, device=x.device)
         st = lib().xk_gated_linear_recurrence_bwd(
@@ -1194,8 +1198,8 @@ def npu_gated_residual_rms_norm(x: torch.Tensor, residual: torch.Tensor,
     with torch.cuda.device(x.device):
         h = torch.empty(x.shape, dtype=residual.dtype, device=x.device)
         y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if pre is not None else None
-        r1 = torch.empty(x.shape[:-1], device=x.device) if post is not None else None
-        r2 = torch.empty(x.shape[:-1], device=x.device) if pre is not None else None
+        r1 = _f32(x, *x.shape[:-1]) if post is not None else None
+        r2 = _f32(x, *x.shape[:-1]) if pre is not None else None
         st = lib().xk_gated_residual_rms_norm(
             xr.data_ptr(), px, rr.data_ptr(), pr, _ptr(zr), pz, _ptr(post), _ptr(sc), _ptr(pre),
             h.data_ptr(), N, _ptr(y), N, _ptr(r1), _ptr(r2), M, N, float(eps),
