@@ -552,3 +552,58 @@ def test_another_default_dtype(dev, default):
                    for p, q in zip(both["cpp"], both["py"]))
     finally:
         torch.set_default_dtype(torch.float32)
+
+
+# ---------------------------------------------------------------------------
+# values that are not finite
+# ---------------------------------------------------------------------------
+def _spoiled(dev, where, value, at, lens, lam=None):
+    """The forward and backward call on clean inputs and on inputs with one
+    value changed (channel 64; token `at`, for states the first sequence), and
+    the oracle's results for the changed ones, by name."""
+    from torch_npu_ops_amd import _xk_torch as xt
+    cu, D = _cu(lens), 131
+    x, a, b, dy, usual, h0, df = _inputs(23, cu[-1], D, len(lens), BF16)
+    lam = usual if lam is None else torch.full((D,), lam)
+    t = {"x": x, "a": a, "b": b, "dy": dy, "h0": h0, "df": df}
+    cud = torch.tensor(cu, dtype=torch.int32, device=dev)
+
+    def run():
+        d = {k: v.to(dev) for k, v in t.items()}
+        args = d["x"], d["a"], d["b"], lam.to(dev)
+        y, fin, st = xt.npu_gated_linear_recurrence(*args, C, d["h0"], True, cud, True)
+        out = xt.npu_gated_linear_recurrence_bwd(d["dy"], *args, st, C, d["h0"], d["df"], cud)
+        names = ("y", "final", "dx", "da", "db", "dlam", "dh0")
+        return {k: (v[0] if v.dim() == 3 else v).cpu() for k, v in zip(names, (y, fin, *out))}
+    clean = run()
+    if where in ("h0", "df"):
+        t[where][0, 64] = value
+    else:
+        t[where][0, at, 64] = value
+    fwd = orc.forward(x[0], a[0], b[0], lam, C, h0, cu)
+    want = {"y": fwd["h"], "final": fwd["final"]}
+    want.update(orc.backward(dy[0], x[0], a[0], b[0], lam, C, h0, df, cu))
+    return clean, run(), want
+
+
+def _same_but_for_what_is_not_finite(clean, got, want):
+    """Elements that the formulas make NaN or infinite are that, all others
+    have the clean call's bits."""
+    for name, t in got.items():
+        w = want[name]
+        assert torch.equal(t.isnan(), w.isnan()), name
+        inf = w.isinf()
+        assert torch.equal(t[inf].double(), w[inf]), name
+        kept = w.isfinite()
+        assert torch.equal(t[kept], clean[name][kept]), name
+
+
+@pytest.mark.parametrize("at", [0, 17, 31, 395, 399])
+@pytest.mark.parametrize("where", ["x", "a", "b", "dy", "h0", "df"])
+def test_a_nan_reaches_all_that_depends_on_it(dev, where, at):
+    # Inside a window and at its ends, in the sequence's first and last window.
+    clean, got, want = _spoiled(dev, where, float("nan"), at, [400, 300])
+    if where == "b":  # dlam and da alone depend on what comes before a token
+        assert want["dx"][at, 64].isnan() and want["dx"][at + 1:, 64].isfinite().all()
+    assert want["dlam"][64].isnan()
+    _same_but_for_what_is_not_finite(clean, got, want)

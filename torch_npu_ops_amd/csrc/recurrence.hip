@@ -957,9 +957,10 @@ __device__ __forceinline__ float slope_ratio(float lam) {
 }
 
 // exp(-v) for a sigmoid's value r = 1 / (1 + e) and its complement 1 - r = e r;
-// capped at 2^100, so that e r is 1 and not inf * 0 for a closed gate.
+// capped at 2^100, so that e r is 1 and not inf * 0 for a closed gate.  The
+// minimum is the one that keeps a NaN (fminf gives the cap for it).
 __device__ __forceinline__ float exp_neg(float v) {
-  return __builtin_amdgcn_exp2f(fminf(v * -1.44269504f, 100.f));
+  return __builtin_amdgcn_exp2f(__builtin_elementwise_minimum(v * -1.44269504f, 100.f));
 }
 
 // ---------------------------------------------------------------------------
