@@ -607,3 +607,37 @@ def test_a_nan_reaches_all_that_depends_on_it(dev, where, at):
         assert want["dx"][at, 64].isnan() and want["dx"][at + 1:, 64].isfinite().all()
     assert want["dlam"][64].isnan()
     _same_but_for_what_is_not_finite(clean, got, want)
+
+
+@pytest.mark.parametrize("a_value,b_value", [(-75.0, 0.5), (-85.0, 0.5), (0.5, -75.0), (0.5, -85.0),
+                                             (-70.0, -10.0)])
+def test_gradients_of_nearly_closed_gates(dev, a_value, b_value):
+    # A sigmoid at v carries |v| + 2 u from its argument, 0.22 |v| u from the
+    # constant log2 e and 4 u from the exponential, the sum and the reciprocal:
+    # 1.3 |v| + 8 of them.  A gradient holds either gate at most twice.
+    # Where l is no normal number, s^2 = 2 |l| is below 2^-125 and formed from
+    # what is left of l's digits: s, at most 2^-62.5, is off by 2^-62 at most, and
+    # so is l / s, which is s / 2 there.  dx = G i s, db = G i s x (1 - i) and
+    # da = G (h l - i x l / s) (with alpha and 1 - r both 1) are off by that much
+    # times what stands beside s; h l is below 2^-120.
+    from torch_npu_ops_amd import _xk_torch as xt
+    T, D = 40, 70
+    x, _, _, dy, lam, h0, df = _inputs(94, T, D, 1, F32)
+    a, b = torch.full((1, T, D), a_value), torch.full((1, T, D), b_value)
+    d = [t.to(dev) for t in (x, a, b, lam)]
+    st = xt.npu_gated_linear_recurrence(*d, C, h0.to(dev), False, None, True)[2]
+    got = xt.npu_gated_linear_recurrence_bwd(dy.to(dev), *d, st, C, h0.to(dev), df.to(dev))
+    want = orc.backward(dy[0], x[0], a[0], b[0], lam, C, h0, df, [0, T])
+    more = 2 * (1.3 * (abs(a_value) + abs(b_value)) + 16) * orc.U
+    _, i, ell, _, s = orc.gates(a[0], b[0], lam, C)
+    tiny = (ell.abs() < 2.0 ** -126) * 2.0 ** -62 * (want["dx"] / s).abs()  # 2^-62 |G| i
+    beside = {"dx": 1.0, "db": x[0].double().abs(), "da": x[0].double().abs() + 1.0}
+    for name, t in zip(("dx", "da", "db", "dlam", "dh0"), got):
+        t = t[0] if t.dim() == 3 else t
+        room = want[name + "_err"] + more * want[name].abs()
+        if name in beside:
+            room = room + tiny * beside[name]
+        if name == "dlam":
+            room = room + (2 * more * want["da"].abs() + 2 * tiny * beside["da"]).sum(0)
+        assert (want[name] != 0).all() and want[name].isfinite().all()
+        assert_within(t, want[name], room, name)

@@ -957,10 +957,12 @@ __device__ __forceinline__ float slope_ratio(float lam) {
 }
 
 // exp(-v) for a sigmoid's value r = 1 / (1 + e) and its complement 1 - r = e r;
-// capped at 2^100, so that e r is 1 and not inf * 0 for a closed gate.  The
+// capped at 2^126, so that e r is 1 and not inf * 0 for a closed gate: the
+// largest power whose reciprocal is no denormal, which the instruction gives as
+// 0 (at v = -80 a cap of 2^100 left r 4e4 times too large).  The
 // minimum is the one that keeps a NaN (fminf gives the cap for it).
 __device__ __forceinline__ float exp_neg(float v) {
-  return __builtin_amdgcn_exp2f(__builtin_elementwise_minimum(v * -1.44269504f, 100.f));
+  return __builtin_amdgcn_exp2f(__builtin_elementwise_minimum(v * -1.44269504f, 126.f));
 }
 
 // ---------------------------------------------------------------------------
