@@ -12,6 +12,13 @@ hardware's exponential, the reciprocal, the product with -c softplus(lam)
 (itself 4 u), the series of expm1 (5e-8 = 0.8 u truncation, 3 u rounding) and
 the square root add 12 u at most, so 24 u cover a gate.
 
+A decay alpha = exp(l) carries keep(l) = |l| EPS + 6 u of itself, however small
+it is: l's own relative error (18 u of EPS) and that of the exponential's
+argument (1.3 u) are multiplied by |l|; near 1 alpha - 1 = l + l^2 / 2 + ...
+carries EPS, and |alpha - 1| <= 1.14 alpha |l| down to l = -1/4, where the
+exponential takes over (2 u); the product with the state and the joins of tiles
+and waves round a few more times.
+
 Pins (tests/test_oracle_recurrence.py): the closed form for constant gates,
 cumulative sums and products for open ones, float64 autograd and central
 differences for the gradients.
@@ -23,6 +30,11 @@ import torch.nn.functional as F
 
 U = 2.0 ** -24
 EPS = 24 * U
+
+
+def keep(ell):
+    """Relative error of a decay, with its product."""
+    return ell.abs() * EPS + 6 * U
 
 
 def gates(a, b, lam, c):
@@ -55,9 +67,7 @@ def forward(x, a, b, lam, c, h0, cu):
         h, e = start[q].clone(), torch.zeros(D, dtype=torch.float64)
         for t in range(t0, t1):
             out["before"][t], out["before_err"][t] = h, e
-            # alpha = 1 + em1 with em1 to EPS, two roundings of the sum; the
-            # joins of tiles and waves add a few more of the same size.
-            e = alpha[t] * e + h.abs() * ((1 - alpha[t]) * EPS + 6 * U) + add[t].abs() * EPS
+            e = alpha[t] * (e + h.abs() * keep(ell[t])) + add[t].abs() * EPS
             h = alpha[t] * h + add[t]
             e = e + 2 * U * h.abs()
             out["h"][t], out["h_err"][t] = h, e
@@ -84,13 +94,14 @@ def backward(dy, x, a, b, lam, c, h0, dfinal, cu):
             G[t] = dy[t] + q[k]
             Ge[t] = qe[k] + 2 * U * G[t].abs() + 2 * U * q[k].abs()
             q[k] = alpha[t] * G[t]
-            qe[k] = alpha[t] * Ge[t] + G[t].abs() * ((1 - alpha[t]) * EPS + 6 * U)
+            qe[k] = alpha[t] * (Ge[t] + G[t].abs() * keep(ell[t]))
     l_s = torch.where(s > 0, ell / s, torch.zeros_like(s))  # tends to 0 with the gate
     part_h, part_u = alpha * fwd["before"] * ell, i * x * alpha * alpha * l_s
-    # E = (dL/dl) l
+    # E = (dL/dl) l; part_h holds a decay once, part_u twice (s has less than
+    # half of a decay's error: alpha^2 |l| <= s^2 / 2).
     E = G * (part_h - part_u)
     Ee = ((part_h - part_u).abs() * Ge + G.abs() * (alpha * ell).abs() * fwd["before_err"]
-          + G.abs() * (part_h.abs() + part_u.abs()) * 2 * EPS)
+          + G.abs() * (part_h.abs() * (ell.abs() + 2) + part_u.abs() * (2 * ell.abs() + 2)) * EPS)
     out = {"dx": G * s * i, "db": G * s * x * i * (1 - i), "da": E * (1 - r), "dh0": q,
            "dh0_err": qe}
     out["dx_err"] = s * i * Ge + out["dx"].abs() * 2 * EPS
@@ -127,7 +138,7 @@ def update(x, a, b, lam, c, pool, slots, accepted, cu):
         h = start[first].clone() if ok else torch.zeros_like(lam, dtype=torch.float64)
         e = torch.zeros_like(h)
         for t in range(t0, t1):
-            e = alpha[t] * e + h.abs() * ((1 - alpha[t]) * EPS + 3 * U) + add[t].abs() * EPS
+            e = alpha[t] * (e + h.abs() * keep(ell[t])) + add[t].abs() * EPS
             h = alpha[t] * h + add[t]
             e = e + 2 * U * h.abs()
             y[t], y_err[t] = h, e

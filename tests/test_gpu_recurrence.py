@@ -641,3 +641,56 @@ def test_gradients_of_nearly_closed_gates(dev, a_value, b_value):
             room = room + (2 * more * want["da"].abs() + 2 * tiny * beside["da"]).sum(0)
         assert (want[name] != 0).all() and want[name].isfinite().all()
         assert_within(t, want[name], room, name)
+
+
+def _strong(D):
+    # With a = 0 a token keeps 10^-3 to 10^-9 of the state (and 0.8 to 0.9 for
+    # every fourth channel, on the other side of the series).
+    keep = 10.0 ** -torch.linspace(3, 9, D, dtype=torch.float64)
+    keep[::4] = torch.linspace(0.8, 0.9, len(keep[::4]), dtype=torch.float64)
+    return torch.log(torch.expm1(-torch.log(keep) / (C * 0.5))).float()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=str)
+@pytest.mark.parametrize("first", [0, 13, 125, 1021])
+def test_a_strong_decay_keeps_its_digits(dev, first, dtype):
+    # Small inputs beside states of order 1: what is left of the state is seen.
+    # Sequences start 3 tokens before a window's, a tile's or a group's end.
+    lens, D = [3, 1, 2, 5, 40, 300], 70
+    cu = _cu(lens, first)
+    total = cu[-1] + 9
+    x, a, b, dy, _, h0, df = _inputs(91, total, D, len(lens), F32)
+    x, a, b, dy = ((t * f).to(dtype) for t, f in ((x, 1e-12), (a, 0), (b, 1), (dy, 1e-12)))
+    lam = _strong(D)
+    d = [t.to(dev) for t in (x, a, b, lam)]
+    cud, m = torch.tensor(cu, dtype=torch.int32, device=dev), _live(cu, total)
+    want = orc.forward(x[0], a[0], b[0], lam, C, h0, cu)
+    grads = orc.backward(dy[0], x[0], a[0], b[0], lam, C, h0, df, cu)
+    for api in _both().values():
+        y, fin, st = api.npu_gated_linear_recurrence(*d, C, h0.to(dev), True, cud, True)
+        assert_within(y[0].cpu()[m], want["h"][m], want["h_err"][m], "y")
+        assert_within(fin, want["final"], want["final_err"], "final state")
+        got = api.npu_gated_linear_recurrence_bwd(dy.to(dev), *d, st, C, h0.to(dev), df.to(dev),
+                                                  cud)
+        for name, t in zip(("dx", "da", "db"), got):
+            assert_within(t[0].cpu()[m], grads[name][m], grads[name + "_err"][m], name)
+        assert_within(got[3], grads["dlam"], grads["dlam_err"], "dlam")
+        assert_within(got[4], grads["dh0"], grads["dh0_err"], "dh0")
+
+
+@pytest.mark.parametrize("n", [3, 9000])
+def test_update_under_a_strong_decay(dev, n):
+    # Both numbers of channels a lane.
+    from torch_npu_ops_amd import _xk_torch as xt
+    D = 70
+    x, a, b, _, _, pool, _ = _inputs(92, n, D, n, F32)
+    x, a, lam = x * 1e-12, a * 0, _strong(D)
+    r, i, ell, alpha, s = orc.gates(a[0], b[0], lam, C)
+    add = s * i * x[0].double()
+    want = alpha * pool.double() + add
+    err = alpha * pool.abs() * orc.keep(ell) + add.abs() * orc.EPS + 2 * orc.U * want.abs()
+    state = pool.to(dev)
+    y = xt.npu_gated_linear_recurrence_update(x[0].to(dev), a[0].to(dev), b[0].to(dev),
+                                              lam.to(dev), state)
+    assert_within(y, want, err, "y")
+    assert_within(state, want, err, "pool")

@@ -6,7 +6,8 @@
 //
 // per channel, in fp32.  alpha - 1 is formed as expm1(l) and 1 - alpha^2 as
 // -(alpha - 1)(1 + alpha), so neither loses digits where a channel
-// keeps nearly all of its state (alpha near 1, the case that matters).
+// keeps nearly all of its state (alpha near 1, the case that matters); where it
+// keeps little, alpha itself is what is multiplied by.
 #include <math.h>
 
 #include <algorithm>
@@ -47,36 +48,49 @@ __device__ __forceinline__ float softplus_f32(float v) {
 // largest relative error, 2.5e-9 before rounding) gives alpha - 1, below it
 // the exponential gives alpha.  NEAR: no channel of the wave goes below (k r,
 // r < 1); the same bits without the exponential.
+//
+// From -1/4 up alpha v is v + (alpha - 1) v: one rounding, of the sum, where
+// thousands of tokens may lie between a state and its use.  Below it is
+// alpha times v: alpha - 1, rounded near -1, has lost alpha's digits (1% of it
+// at alpha = 1e-6).  `word` holds either, told apart by the sign bit: alpha - 1
+// has it (-0 for a closed gate), alpha has not.  Where channels go below, the
+// choice costs 2 to 4% (16,384 x 4,096 bf16 133 us, with alpha - 1 throughout 128.5).
 constexpr float kNear = -0.25f;
 struct Decay {
-  float alpha, em1;
+  float alpha, em1, word;
 };
 template <bool NEAR>
 __device__ __forceinline__ Decay decay_of(float l) {
   float p = fmaf(l, 0.007510221f, 0.041488957f);
   p = fmaf(p, l, 0.16665082f);
   p = fmaf(p, l, 0.4999995f);
-  p = fmaf(p, l, 1.f) * l;
-  if constexpr (NEAR) return {1.f + p, p};
-  const float e = __expf(l);
-  const bool near = l >= kNear;
-  return {near ? 1.f + p : e, near ? p : e - 1.f};
+  const float q = fmaf(p, l, 1.f), series = fmaf(q, l, 1.f);
+  p = q * l;
+  if constexpr (NEAR) return {series, p, p};
+  // The compiler is kept from carrying the comparison along in scalar
+  // registers, which it spills: the word's sign says the same.
+  float word = l >= kNear ? p : __expf(l);
+  asm("" : "+v"(word));
+  const bool near = __builtin_bit_cast(int, word) < 0;
+  return {near ? series : word, near ? word : word - 1.f, word};
+}
+// alpha v.
+template <bool NEAR>
+__device__ __forceinline__ float decayed(float word, float v) {
+  if constexpr (NEAR) return fmaf(word, v, v);
+  const int near = __builtin_bit_cast(int, word) >> 31;  // all bits, or none
+  return fmaf(word, v, __builtin_bit_cast(float, __builtin_bit_cast(int, v) & near));
 }
 
 struct Gate {
-  float alpha, em1;
+  float alpha, word;
   float s;  // sqrt(1 - alpha^2)
 };
 template <bool NEAR>
 __device__ __forceinline__ Gate gate_of(float k, float r) {
   const Decay d = decay_of<NEAR>(k * r);
-  return {d.alpha, d.em1, __builtin_amdgcn_sqrtf(-d.em1 * (1.f + d.alpha))};
+  return {d.alpha, d.word, __builtin_amdgcn_sqrtf(-d.em1 * (1.f + d.alpha))};
 }
-
-// alpha v from alpha - 1: one rounding, of the product, where alpha is near 1
-// (thousands of tokens may lie between a state and its use); 2^-24 |v| at most
-// where it is not.
-__device__ __forceinline__ float decayed(float em1, float v) { return fmaf(em1, v, v); }
 
 struct FwdParams {
   const void* x;
@@ -115,7 +129,7 @@ __device__ __forceinline__ int cu_at(const void* cu, int cu64, int n, int run, i
 // Tiles.  The token axis of the whole batch is cut into windows of kTok tokens,
 // one per wave, and tiles of some windows, one per block; a lane has
 // VEC channels (4 bytes of a row), so a tile covers 64 VEC channels.  A
-// window's tokens are read once and stay in registers as (alpha - 1, input).
+// window's tokens are read once and stay in registers as (decay, input).
 //
 // Any span of tokens maps the state before it to the state after it by
 // h -> A h + B, and a span in which a sequence starts maps every state to the
@@ -245,7 +259,10 @@ constexpr unsigned int kRange = 1u << 31;  // more than 16 rows span (checked on
 template <int VEC>
 struct Lane {
   unsigned int off;  // of its first element in the block's rows, kRange: no channels
-  int64_t ch;        // its first channel
+  // Its first channel: 32 bits where two channels leave few registers
+  // (16,384 x 4,096 bf16 126.6 us, with 64 bits 128.4; fp32 4,099 x 640 forward
+  // and backward 47.7 and 47.0).
+  typename std::conditional<VEC == 2, unsigned int, int64_t>::type ch;
   bool ok[VEC];
   bool half;  // ok[1] alone
   bool odd;   // the block has such a lane
@@ -256,7 +273,7 @@ __device__ __forceinline__ Lane<VEC> lane_of(unsigned int lane, int64_t col, int
   Lane<VEC> l;
   l.odd = VEC == 2 && (D & 1) && D - col < kWave * VEC;
   l.half = VEC == 2 && left == 1;
-  l.ch = col + lane * VEC - l.half;
+  l.ch = static_cast<decltype(l.ch)>(col) + lane * VEC - l.half;
   // Rows of an odd block start one element before its channels.
   l.off = left > 0 ? (lane * VEC + (l.odd && !l.half)) * static_cast<unsigned int>(sizeof(T))
                    : kRange;
@@ -622,7 +639,7 @@ __global__ void __launch_bounds__(FwdWaves<VEC>::most(LOOK) * kWave, LOOK ? kFwd
   }
 
   // The window's gates, and its span; a start folds its state into the input.
-  float em1[kTok][VEC], add[kTok][VEC];
+  float keep[kTok][VEC], add[kTok][VEC];
   Span span[VEC];
 #pragma unroll
   for (int u = 0; u < VEC; ++u) span[u] = {1.f, 0.f};
@@ -632,7 +649,7 @@ __global__ void __launch_bounds__(FwdWaves<VEC>::most(LOOK) * kWave, LOOK ? kFwd
 #pragma unroll
       for (int u = 0; u < VEC; ++u) {
         const Gate g = gate_of<near>(k[u], sigmoid(lane_f32<T>(a[j], u)));
-        em1[j][u] = g.em1;
+        keep[j][u] = g.word;
         add[j][u] = g.s * (sigmoid(lane_f32<T>(b[j], u)) * lane_f32<T>(x[j], u));
       }
       if (starts && (m.starts >> j & 1)) {
@@ -640,15 +657,18 @@ __global__ void __launch_bounds__(FwdWaves<VEC>::most(LOOK) * kWave, LOOK ? kFwd
         if (p.h0) ld_f32<VEC>(p.h0 + seq_row(seqs[wave][j]), at, h);
 #pragma unroll
         for (int u = 0; u < VEC; ++u) {
-          add[j][u] += decayed(em1[j][u], h[u]);
+          add[j][u] += decayed<near>(keep[j][u], h[u]);
           span[u].B = 0.f;
         }
       }
 #pragma unroll
       for (int u = 0; u < VEC; ++u) {
-        span[u].A = decayed(em1[j][u], span[u].A);
-        span[u].B = decayed(em1[j][u], span[u].B) + add[j][u];
+        span[u].A = decayed<near>(keep[j][u], span[u].A);
+        // Not left for the tokens' end, which would hold every token's choice.
+        if (!near && j % 2) later(span[u].A);
+        span[u].B = decayed<near>(keep[j][u], span[u].B) + add[j][u];
       }
+      if (!near) __builtin_amdgcn_sched_barrier(0);
     }
     if (starts && m.starts) {
 #pragma unroll
@@ -658,7 +678,8 @@ __global__ void __launch_bounds__(FwdWaves<VEC>::most(LOOK) * kWave, LOOK ? kFwd
   bool near = true;
 #pragma unroll
   for (int u = 0; u < VEC; ++u) near &= k[u] >= kNear;
-  if (plain && __all(near))
+  const bool fast = plain && __all(near);
+  if (fast)
     gates(std::true_type(), std::false_type());
   else
     gates(std::false_type(), std::true_type());
@@ -687,26 +708,29 @@ __global__ void __launch_bounds__(FwdWaves<VEC>::most(LOOK) * kWave, LOOK ? kFwd
   for (int u = 0; u < VEC; ++u) h[u] = apply(head[u], h[u]);
   if (p.states && w0 < total) st_f32<VEC>(p.states + row / kWin * p.D, at, h);
   const Rows<T, VEC> yr(p.y, row, p.sy, col, at.odd);
-  if (plain) {
+  auto outputs = [&](auto near, auto marks) {
 #pragma unroll
     for (int j = 0; j < kTok; ++j) {
+      if (marks && (m.starts >> j & 1)) {
 #pragma unroll
-      for (int u = 0; u < VEC; ++u) h[u] = decayed(em1[j][u], h[u]) + add[j][u];
-      yr.template st<false>(j, at, h);
+        for (int u = 0; u < VEC; ++u) h[u] = 0.f;
+      }
+#pragma unroll
+      for (int u = 0; u < VEC; ++u) {
+        if (!near) later(keep[j][u]);  // nor the first pass's
+        h[u] = decayed<near>(keep[j][u], h[u]) + add[j][u];
+      }
+      if (!marks || (w0 + j >= m.lo && w0 + j < m.hi)) yr.template st<marks>(j, at, h);
+      if (marks && (m.ends >> j & 1) && p.fin)
+        st_f32<VEC>(p.fin + seq_row(seqs[wave][kTok + j]), at, h);
     }
-    return;
-  }
-#pragma unroll
-  for (int j = 0; j < kTok; ++j) {
-    if (m.starts >> j & 1) {
-#pragma unroll
-      for (int u = 0; u < VEC; ++u) h[u] = 0.f;
-    }
-#pragma unroll
-    for (int u = 0; u < VEC; ++u) h[u] = decayed(em1[j][u], h[u]) + add[j][u];
-    if (w0 + j >= m.lo && w0 + j < m.hi) yr.template st<true>(j, at, h);
-    if ((m.ends >> j & 1) && p.fin) st_f32<VEC>(p.fin + seq_row(seqs[wave][kTok + j]), at, h);
-  }
+  };
+  if (fast)
+    outputs(std::true_type(), std::false_type());
+  else if (plain)
+    outputs(std::false_type(), std::false_type());
+  else
+    outputs(std::false_type(), std::true_type());
 }
 
 // Tiles, channel blocks and waves of a block for a problem.
@@ -883,8 +907,7 @@ __global__ void __launch_bounds__(kWave) glr_update_kernel(UpdateParams p) {
   }
 #pragma unroll
   for (int u = 0; u < VEC; ++u) k[u] = -p.c * softplus_f32(lam.v[u]);
-  for (int64_t from = t0; from < t1; from += kUpdTok) {
-    if (from > t0) load(from);
+  auto tokens = [&](int64_t from) {
 #pragma unroll
     for (int j = 0; j < kUpdTok; ++j) {
       const int64_t t = from + j;
@@ -892,7 +915,8 @@ __global__ void __launch_bounds__(kWave) glr_update_kernel(UpdateParams p) {
 #pragma unroll
         for (int u = 0; u < VEC; ++u) {
           const Gate g = gate_of<false>(k[u], sigmoid(to_f32(a[j].v[u])));
-          h[u] = decayed(g.em1, h[u]) + g.s * (sigmoid(to_f32(b[j].v[u])) * to_f32(x[j].v[u]));
+          h[u] = decayed<false>(g.word, h[u]) +
+                 g.s * (sigmoid(to_f32(b[j].v[u])) * to_f32(x[j].v[u]));
         }
         st_some<VEC>(static_cast<T*>(p.y) + t * p.sy + ch, h, left);
         if (t - t0 < p.cols) {
@@ -901,6 +925,11 @@ __global__ void __launch_bounds__(kWave) glr_update_kernel(UpdateParams p) {
         }
       }
     }
+  };
+  tokens(t0);
+  for (int64_t from = t0 + kUpdTok; from < t1; from += kUpdTok) {
+    load(from);
+    tokens(from);
   }
   if (p.cols == 0 && t1 > t0 && inside(first))
     st_some<VEC>(p.state + first * p.slot_pitch + ch, h, left);
@@ -974,7 +1003,7 @@ __device__ __forceinline__ float exp_neg(float v) {
 //  * h_{t-1} comes from the window's saved state, in the same pass that forms
 //    the window's span (in token order: A is the running product of alpha and
 //    B the sum of A_t dy_t, so nothing but h_{t-1} is kept for a token).
-//  * Of the gates exp(-a), exp(-b), r and alpha - 1 stay in registers for the
+//  * Of the gates exp(-a), exp(-b), r and the decay stay in registers for the
 //    second pass, in reverse order; the rest is cheaper formed again.  (With
 //    the two exponentials alone 142 us instead of 134 for 8,192 x 4,096 bf16:
 //    the arithmetic is as long as the traffic.)  130 us now, 3.7 TB/s, at 2
@@ -1048,7 +1077,7 @@ __global__ void __launch_bounds__(BwdWaves<VEC>::most(LOOK) * kWave, LOOK ? kBwd
     });
   }
 
-  float before[kTok][VEC], ea[kTok][VEC], eb[kTok][VEC], em1[kTok][VEC], rs[kTok][VEC];
+  float before[kTok][VEC], ea[kTok][VEC], eb[kTok][VEC], keep[kTok][VEC], rs[kTok][VEC];
   Span span[VEC];
 #pragma unroll
   for (int u = 0; u < VEC; ++u) span[u] = {1.f, 0.f};
@@ -1069,11 +1098,11 @@ __global__ void __launch_bounds__(BwdWaves<VEC>::most(LOOK) * kWave, LOOK ? kBwd
         rs[j][u] = fast_rcp(1.f + ea[j][u]);
         const Gate g = gate_of<near>(k[u], rs[j][u]);
         before[j][u] = h[u];
-        em1[j][u] = g.em1;
+        keep[j][u] = g.word;
         // alpha's own rounding is let in: h lives for this window only.
         h[u] = fmaf(g.alpha, h[u], g.s * (fast_rcp(1.f + eb[j][u]) * lane_f32<T>(x[j], u)));
         if (reached) {
-          span[u].A = decayed(g.em1, span[u].A);
+          span[u].A = decayed<near>(g.word, span[u].A);
           span[u].B = fmaf(span[u].A, lane_f32<T>(dy[j], u), span[u].B);
         }
       }
@@ -1146,7 +1175,8 @@ __global__ void __launch_bounds__(BwdWaves<VEC>::most(LOOK) * kWave, LOOK ? kBwd
       for (int u = 0; u < VEC; ++u) {
         const float r = rs[j][u], i = fast_rcp(1.f + eb[j][u]);
         const float xf = lane_f32<T>(x[j], u), l = k[u] * r;
-        const Decay d = near ? Decay{1.f + em1[j][u], em1[j][u]} : decay_of<false>(l);
+        const Decay d =
+            near ? Decay{1.f + keep[j][u], keep[j][u], keep[j][u]} : decay_of<false>(l);
         const float w = -d.em1 * (1.f + d.alpha);  // s^2
         // The instruction takes a denormal w for 0; l and w, both tiny there,
         // keep the products with inv at 0 or below 2^-60.
@@ -1157,7 +1187,7 @@ __global__ void __launch_bounds__(BwdWaves<VEC>::most(LOOK) * kWave, LOOK ? kBwd
         const float e = G * d.alpha * (before[j][u] * l - i * xf * d.alpha * (l * inv));
         da[u] = e * (ea[j][u] * r);
         if (live) sum[u] += e;
-        q[u] = decayed(d.em1, G);
+        q[u] = decayed<near>(d.word, G);
       }
       if (live) {
         dxr.template st<marks>(j, at, dx);
