@@ -500,8 +500,10 @@ int xk_chunk_fwd_o(const void* q, const void* k, const void* v, const void* h,
  *     r = sigmoid(a_t), i = sigmoid(b_t), l = -c softplus(lam) r,
  *     h_t = exp(l) h_{t-1} + sqrt(1 - exp(2 l)) i x_t,    y_t = h_t
  * per channel, in fp32 whatever the inputs' type.
- * An infinite input or state makes its channel NaN from a later token on (the
- * decay is applied as h + (exp(l) - 1) h); other channels are not touched.
+ * A NaN makes all NaN that depends on it.  An infinite x or state leaves its
+ * channel infinite or NaN from there to the sequence's end (a decay near 1 is
+ * applied as h + (exp(l) - 1) h); an infinite a or b is a gate that is 0 or 1.
+ * Nothing else is touched.
  *   x, a, b, y : [total_tokens, D] rows with token pitches (at least D, below
  *     2^25 elements) in `dtype` (f32/bf16/f16), any alignment; lam fp32 [D];
  *     c >= 0.  y may be x, a or b itself (the same start and pitch).
@@ -571,6 +573,9 @@ int xk_gated_linear_recurrence_update(
  *     it in fp32; the rounded outputs of the forward pass are not used.
  *   dlam : fp32 [D], written (not accumulated), or NULL.  d_initial_state :
  *     fp32 [N, D] or NULL; an empty sequence's is its d_final_state.
+ *   Values that are not finite: as in the forward pass.  An infinite dy or
+ *   d_final_state leaves the gradients of its channel infinite or NaN from there
+ *   to the sequence's start.
  *   The sums over tokens have a fixed order: the same call gives the same bits.
  *   workspace >= xk_gated_linear_recurrence_bwd_workspace_bytes(...) bytes,
  *     256-byte aligned.

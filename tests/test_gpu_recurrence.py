@@ -609,6 +609,38 @@ def test_a_nan_reaches_all_that_depends_on_it(dev, where, at):
     _same_but_for_what_is_not_finite(clean, got, want)
 
 
+@pytest.mark.parametrize("value", [float("inf"), float("-inf")])
+@pytest.mark.parametrize("where", ["x", "dy", "h0", "df"])
+@pytest.mark.parametrize("lam", [-6.0, -0.5, 3.0])
+@pytest.mark.parametrize("lens", [[9, 3], [400, 300]], ids=str)
+def test_an_infinite_value_leaves_no_finite_one_that_depends_on_it(dev, lens, lam, where, value):
+    # alpha near 1, around 0.15 and around 10^-5 (whose product over a window is 0).
+    clean, got, want = _spoiled(dev, where, value, 5, lens, lam)
+    if where in ("x", "h0"):
+        assert want["y"][5:lens[0], 64].isinf().all()
+    for name, t in got.items():
+        kept = want[name].isfinite()
+        assert torch.equal(t.isfinite(), kept), name
+        assert torch.equal(t[kept], clean[name][kept]), name
+
+
+@pytest.mark.parametrize("lam", [-6.0, -0.5, 3.0])
+def test_update_of_an_infinite_state(dev, lam):
+    from torch_npu_ops_amd import _xk_torch as xt
+    x, a, b, _, _, pool, _ = _inputs(93, 4, 70, 4, BF16)
+    args = [t[0].to(dev) for t in (x, a, b)] + [torch.full((70,), lam, device=dev)]
+    clean = pool.to(dev)
+    xt.npu_gated_linear_recurrence_update(*args, clean)
+    pool[1, 3], pool[2, 5] = float("inf"), float("-inf")
+    args[0][0, 7] = float("-inf")
+    state = pool.to(dev)
+    y = xt.npu_gated_linear_recurrence_update(*args, state)
+    kept = torch.ones(4, 70, dtype=torch.bool, device=dev)
+    kept[1, 3] = kept[2, 5] = kept[0, 7] = False
+    assert torch.equal(state.isfinite(), kept) and torch.equal(y.isfinite(), kept)
+    assert torch.equal(state[kept], clean[kept])
+
+
 @pytest.mark.parametrize("a_value,b_value", [(-75.0, 0.5), (-85.0, 0.5), (0.5, -75.0), (0.5, -85.0),
                                              (-70.0, -10.0)])
 def test_gradients_of_nearly_closed_gates(dev, a_value, b_value):
