@@ -505,7 +505,7 @@ int xk_chunk_fwd_o(const void* q, const void* k, const void* v, const void* h,
  * applied as h + (exp(l) - 1) h); an infinite a or b is a gate that is 0 or 1.
  * Nothing else is touched.
  *   x, a, b, y : [total_tokens, D] rows with token pitches (at least D, below
- *     2^25 elements) in `dtype` (f32/bf16/f16), any alignment; lam fp32 [D];
+ *     XK_GLR_PITCH elements) in `dtype` (f32/bf16/f16), any alignment; lam fp32 [D];
  *     c >= 0.  y may be x, a or b itself (the same start and pitch).
  *     (ceil(total_tokens / 16) + 8) * ceil(D / 64) must be below 2^26 (64
  *     billion elements or more), else XK_ERR_INVALID.
@@ -529,6 +529,7 @@ int xk_chunk_fwd_o(const void* q, const void* k, const void* v, const void* h,
  *     time need a workspace each.
  */
 #define XK_GLR_WINDOW 16
+#define XK_GLR_PITCH (1 << 25)
 int64_t xk_gated_linear_recurrence_workspace_bytes(int64_t total_tokens, int64_t D);
 int xk_gated_linear_recurrence(
     const void* x, int64_t stride_x_tok, const void* a, int64_t stride_a_tok, const void* b,
@@ -539,8 +540,9 @@ int xk_gated_linear_recurrence(
 
 /* The recurrence's decode step on a pool of states: one token, or a few
  * drafted ones, of every sequence (the slot rules of xk_gdn_recurrent).
- *   x, a, b, y as above ([tokens, D], y dense or with a pitch; N *
- *     ceil(D / 64) below 2^26 as well); sequence n is
+ *   x, a, b, y as above ([tokens, D], y dense or with a pitch; the pitches of
+ *     x, a and b have no upper limit here; N * ceil(D / 64) below 2^26 as
+ *     well); sequence n is
  *     rows cu_seqlens[n]..cu_seqlens[n+1], or T rows from n * T when
  *     cu_seqlens is NULL (T then positive).
  *   state : fp32 [num_slots, D] (slot pitch at least D), updated in place.

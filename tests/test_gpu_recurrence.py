@@ -726,3 +726,27 @@ def test_update_under_a_strong_decay(dev, n):
                                               lam.to(dev), state)
     assert_within(y, want, err, "y")
     assert_within(state, want, err, "pool")
+
+
+@pytest.mark.parametrize("which", ["cpp", "py"])
+def test_rows_further_apart_than_a_tiles_offsets_reach(dev, which):
+    # The last token of a batch of long prompts, and rows of 2^25 elements' pitch.
+    api = _both()[which]
+    B, D, pitch = 3, 72, (1 << 25) + 8
+    x, a, b, dy, lam, h0, df = (t.to(dev) for t in _inputs(95, B, D, B, BF16))
+    wide = torch.empty((B - 1) * pitch + D, dtype=BF16, device=dev)
+    far = wide.as_strided((B, 1, D), (pitch, D, 1))
+    far.copy_(x[0][:, None])
+    pools = h0.clone(), h0.clone()
+    cut = [t[0][:, None] for t in (x, a, b)]
+    one = api.npu_gated_linear_recurrence_update(far, *cut[1:], lam, pools[0])
+    two = api.npu_gated_linear_recurrence_update(*cut, lam, pools[1])
+    assert torch.equal(one, two) and torch.equal(*pools)
+    row = wide.as_strided((1, B, D), (D, pitch, 1))  # a sequence of B tokens
+    y, fin, st = api.npu_gated_linear_recurrence(row, a, b, lam, C, h0[:1], True, None, True)
+    same = api.npu_gated_linear_recurrence(x, a, b, lam, C, h0[:1], True, None, True)
+    assert torch.equal(y, same[0]) and torch.equal(fin, same[1])
+    far.copy_(dy[0][:, None])
+    got = api.npu_gated_linear_recurrence_bwd(row, x, a, b, lam, st, C, h0[:1])
+    want = api.npu_gated_linear_recurrence_bwd(dy, x, a, b, lam, st, C, h0[:1])
+    assert all(torch.equal(p, q) for p, q in zip(got, want))

@@ -51,3 +51,19 @@ def test_fp32_outputs_do_not_follow_torchs_default_dtype(library, default_dtype)
     w = torch.ones(8, dtype=bf16)
     h, y, r1, r2 = ops.npu_gated_residual_rms_norm(x, x.to(f32), w, x, w, w)
     assert (h.dtype, y.dtype, r1.dtype, r2.dtype) == (f32, bf16, f32, f32)
+
+
+def test_rows_too_far_apart_for_a_tile_are_copied_in_prefill_and_backward_alone(library):
+    # 2 tokens, 2^25 elements apart or one less.
+    lam, cu = torch.zeros(8), torch.tensor([0, 2])
+    near = torch.zeros(1, 2, 8, dtype=torch.bfloat16)
+    states = torch.zeros(1, 8)
+    for pitch, want in (((1 << 25) - 1, (1 << 25) - 1), (1 << 25, 8)):
+        x = torch.empty(pitch + 8, dtype=torch.bfloat16).as_strided((1, 2, 8), (8, pitch, 1))
+        ops.npu_gated_linear_recurrence(x, near, near, lam, cu_seqlens=cu)
+        assert library.calls["xk_gated_linear_recurrence"][1] == want
+        ops.npu_gated_linear_recurrence_bwd(x, near, x, near, lam, states, cu_seqlens=cu)
+        assert library.calls["xk_gated_linear_recurrence_bwd"][1] == want
+        assert library.calls["xk_gated_linear_recurrence_bwd"][5] == want
+        ops.npu_gated_linear_recurrence_update(x[0], near[0], near[0], lam, torch.zeros(2, 8))
+        assert library.calls["xk_gated_linear_recurrence_update"][1] == pitch

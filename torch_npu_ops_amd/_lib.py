@@ -31,6 +31,7 @@ XK_F32, XK_BF16, XK_F16, XK_I32, XK_I64 = 0, 1, 2, 3, 4
 XK_OK, XK_ERR_INVALID, XK_ERR_UNSUPPORTED, XK_ERR_WORKSPACE, XK_ERR_SCRATCH = 0, -1, -2, -3, -4
 
 XK_GLR_WINDOW = 16  # tokens per saved state of the gated linear recurrence
+XK_GLR_PITCH = 1 << 25  # its prefill and backward calls take pitches below this
 
 # Argument lists, in declaration order of include/xk_ops.h.
 SIGNATURES: dict[str, tuple[list, object]] = {

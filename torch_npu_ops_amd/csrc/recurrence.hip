@@ -1270,6 +1270,7 @@ int launch_bwd(const BwdParams& p, float* dlam, void* workspace, hipStream_t s) 
 
 // A window's rows have to lie within kRange bytes: the most elements of a pitch.
 constexpr int64_t kMostPitch = kRange / (4 * kTok);
+static_assert(kMostPitch == XK_GLR_PITCH);
 bool pitch_ok(int64_t pitch, int64_t D) { return pitch >= D && pitch < kMostPitch; }
 
 // A launch has fewer than 2^32 threads (of whole tiles), N is counted in 31 bits.
@@ -1338,9 +1339,10 @@ extern "C" int xk_gated_linear_recurrence_update(
   if (N == 0 || total_tokens == 0) return XK_OK;
   if (cu_seqlens ? cu_dtype != XK_I32 && cu_dtype != XK_I64 : T <= 0 || T > total_tokens / N)
     return XK_ERR_INVALID;
+  // The inputs' rows may be any way apart: no offset of this kernel is 32 bits.
   if (!x || !a || !b || !y || !lam || (num_slots > 0 && !state) || stride_state_slot < D ||
-      (num_cols > 0 && !state_indices) || !pitch_ok(stride_x_tok, D) ||
-      !pitch_ok(stride_a_tok, D) || !pitch_ok(stride_b_tok, D) || !pitch_ok(stride_y_tok, D))
+      (num_cols > 0 && !state_indices) || stride_x_tok < D || stride_a_tok < D ||
+      stride_b_tok < D || !pitch_ok(stride_y_tok, D))
     return XK_ERR_INVALID;
   const UpdateParams p{x, a, b, y, stride_x_tok, stride_a_tok, stride_b_tok, stride_y_tok, lam, c,
                        state, stride_state_slot, num_slots, state_indices, num_cols,

@@ -11,6 +11,7 @@
 #include <c10/hip/HIPStream.h>
 
 #include <cmath>
+#include <limits>
 
 #include "xk_ops.h"
 
@@ -850,9 +851,10 @@ void same_device(const torch::Tensor& t, const torch::Tensor& x, const char* nam
 }
 
 // [B, T, D] (or [rows, N]) as rows of D with one pitch between them, unit
-// column stride: a view if it has that form, else a contiguous copy.
-// `pitch` receives the elements from row to row.
-torch::Tensor pitched_rows(const torch::Tensor& x, int64_t& pitch) {
+// column stride: a view if it has that form and a pitch below `most`, else a
+// contiguous copy.  `pitch` receives the elements from row to row.
+torch::Tensor pitched_rows(const torch::Tensor& x, int64_t& pitch,
+                           int64_t most = std::numeric_limits<int64_t>::max()) {
   const int64_t D = x.size(-1);
   int64_t p = D, count = 1;
   bool ok = D == 1 || x.stride(-1) == 1;
@@ -866,6 +868,7 @@ torch::Tensor pitched_rows(const torch::Tensor& x, int64_t& pitch) {
     }
     count *= x.size(d);
   }
+  ok = ok && p < most;
   pitch = ok ? p : D;
   return ok ? x : x.contiguous();
 }
@@ -935,7 +938,8 @@ npu_gated_linear_recurrence(const torch::Tensor& x, const torch::Tensor& a,
   const int64_t D = x.size(2), total = x.size(0) * x.size(1);
   auto h0 = glr_state(initial_state, x, N, "initial_state");
   int64_t px, pa, pb;
-  auto xr = pitched_rows(x, px), ar = pitched_rows(a, pa), br = pitched_rows(b, pb);
+  auto xr = pitched_rows(x, px, XK_GLR_PITCH), ar = pitched_rows(a, pa, XK_GLR_PITCH),
+       br = pitched_rows(b, pb, XK_GLR_PITCH);
   auto l = lam.contiguous();
   auto y = fresh(x.sizes(), x.scalar_type(), x);
   torch::Tensor fin, states;
@@ -1037,8 +1041,8 @@ npu_gated_linear_recurrence_bwd(const torch::Tensor& dy, const torch::Tensor& x,
   auto h0 = glr_state(initial_state, x, N, "initial_state");
   auto df = glr_state(d_final_state, x, N, "d_final_state");
   int64_t pd, px, pa, pb;
-  auto dr = pitched_rows(dy, pd), xr = pitched_rows(x, px), ar = pitched_rows(a, pa),
-       br = pitched_rows(b, pb);
+  auto dr = pitched_rows(dy, pd, XK_GLR_PITCH), xr = pitched_rows(x, px, XK_GLR_PITCH),
+       ar = pitched_rows(a, pa, XK_GLR_PITCH), br = pitched_rows(b, pb, XK_GLR_PITCH);
   auto l = lam.contiguous(), st = states.contiguous();
   auto dx = fresh(x.sizes(), x.scalar_type(), x), da = fresh(x.sizes(), x.scalar_type(), x),
        db = fresh(x.sizes(), x.scalar_type(), x);

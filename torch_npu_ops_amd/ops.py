@@ -952,9 +952,10 @@ def _f32(x, *sizes):
     return torch.empty(sizes, dtype=torch.float32, device=x.device)
 
 
-def _pitched_rows(x: torch.Tensor):
+def _pitched_rows(x: torch.Tensor, most: float = math.inf):
     """(x as rows of its last dim with one pitch between them, a copy only if
-    it has no such form; the pitch in elements)."""
+    it has no such form or the pitch is not below ``most``; the pitch in
+    elements)."""
     D = x.size(-1)
     pitch, count, ok = D, 1, D == 1 or x.stride(-1) == 1
     for d in range(x.dim() - 2, -1, -1):
@@ -966,7 +967,7 @@ def _pitched_rows(x: torch.Tensor):
         else:
             ok = x.stride(d) == pitch * count
         count *= x.size(d)
-    return (x, pitch) if ok else (x.contiguous(), D)
+    return (x, pitch) if ok and pitch < most else (x.contiguous(), D)
 
 
 def _glr_check(x, a, b, lam, c):
@@ -1025,7 +1026,7 @@ def npu_gated_linear_recurrence(x: torch.Tensor, a: torch.Tensor, b: torch.Tenso
     cu, N = _glr_seqs(x, cu_seqlens)
     D, total = x.size(2), x.size(0) * x.size(1)
     h0 = _glr_state(initial_state, x, N, "initial_state")
-    (xr, px), (ar, pa), (br, pb) = _pitched_rows(x), _pitched_rows(a), _pitched_rows(b)
+    (xr, px), (ar, pa), (br, pb) = (_pitched_rows(t, _lib.XK_GLR_PITCH) for t in (x, a, b))
     lam = lam.contiguous()
     with torch.cuda.device(x.device):
         y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
@@ -1124,8 +1125,8 @@ def npu_gated_linear_recurrence_bwd(dy: torch.Tensor, x: torch.Tensor, a: torch.
     cu, N = _glr_seqs(x, cu_seqlens)
     h0 = _glr_state(initial_state, x, N, "initial_state")
     df = _glr_state(d_final_state, x, N, "d_final_state")
-    (dr, pd), (xr, px) = _pitched_rows(dy), _pitched_rows(x)
-    (ar, pa), (br, pb) = _pitched_rows(a), _pitched_rows(b)
+    (dr, pd), (xr, px), (ar, pa), (br, pb) = (_pitched_rows(t, _lib.XK_GLR_PITCH)
+                                              for t in (dy, x, a, b))
     lam, states = lam.contiguous(), states.contiguous()
     with torch.cuda.device(x.device):
         dx, da, db = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for _ in range(3))
