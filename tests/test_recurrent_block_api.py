@@ -261,3 +261,33 @@ def test_sizes_that_no_launch_holds_are_refused():
     assert _norm_bwd(M=1, N=1 << 28, size=1 << 62) == _lib.XK_ERR_INVALID
     assert lib.xk_gated_residual_rms_norm_bwd_workspace_bytes(1, 1 << 28) == 0
     assert lib.xk_gated_residual_rms_norm_bwd_workspace_bytes(1, (1 << 28) - 1) > 0
+
+
+def _documented_limits():
+    """(n, p): the header's (ceil(total_tokens / 16) + n) * ceil(D / 64) < 2^p."""
+    import pathlib
+    import re
+    path = pathlib.Path(__file__).parents[1] / "include" / "xk_ops.h"
+    text = re.sub(r"\s*\n \*\s*", " ", path.read_text())
+    at = re.search(r"\(ceil\(total_tokens / 16\) \+ (\d+)\) \* ceil\(D / 64\) must be below 2\^(\d+)",
+                   text)
+    return int(at[1]), int(at[2])
+
+
+@pytest.mark.parametrize("D", [64, 65, 1000, 4096])
+def test_the_documented_sizes_are_the_ones_that_are_taken(D):
+    more, power = _documented_limits()
+    lib = _lib.lib()
+    blocks = -(-D // 64)
+    windows = -(-(1 << power) // blocks) - more  # the first count of windows that is refused
+    size = (lib.xk_gated_linear_recurrence_workspace_bytes,
+            lambda t, d: lib.xk_gated_linear_recurrence_bwd_workspace_bytes(t, 1, d))
+    for f in size:
+        assert f((windows - 1) * 16, D) > 0
+        assert f((windows - 1) * 16 + 1, D) == 0
+    refused = dict(total=(windows - 1) * 16 + 1, D=D, size=1 << 62, ws=PTR)
+    wide = dict.fromkeys(("sx", "sa", "sb", "sy"), D)
+    assert _glr(**refused, **wide) == _lib.XK_ERR_INVALID
+    # Taken as far as the workspace, which is missing.
+    assert _glr(**{**refused, **wide, "total": (windows - 1) * 16, "ws": None}) == \
+        _lib.XK_ERR_WORKSPACE
