@@ -506,7 +506,7 @@ int xk_chunk_fwd_o(const void* q, const void* k, const void* v, const void* h,
  * Nothing else is touched.
  *   x, a, b, y : [total_tokens, D] rows with token pitches (at least D, below
  *     XK_GLR_PITCH elements) in `dtype` (f32/bf16/f16), any alignment; lam fp32 [D];
- *     c >= 0.  y may be x, a or b itself (the same start and pitch).
+ *     c >= 0 and finite.  y may be x, a or b itself (the same start and pitch).
  *     (ceil(total_tokens / 16) + 16) * ceil(D / 64) must be below 2^26 (64
  *     billion elements or more), else XK_ERR_INVALID.
  *   Sequences are cu_seqlens[n]..cu_seqlens[n+1] (int32/int64, device,

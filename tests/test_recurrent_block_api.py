@@ -291,3 +291,19 @@ def test_the_documented_sizes_are_the_ones_that_are_taken(D):
     # Taken as far as the workspace, which is missing.
     assert _glr(**{**refused, **wide, "total": (windows - 1) * 16, "ws": None}) == \
         _lib.XK_ERR_WORKSPACE
+
+
+@pytest.mark.parametrize("call", [_glr, _update, _bwd])
+def test_an_infinite_c_is_refused(call):
+    assert call(c=float("inf")) == _lib.XK_ERR_INVALID
+
+
+def test_a_c_that_is_infinite_in_fp32_is_refused(api):
+    x, lam, pool = _x(1, 6, 8), torch.zeros(8), torch.zeros(6, 8)
+    for c in (1e39, float("inf")):
+        with pytest.raises(REFUSED, match="c must be"):
+            api.npu_gated_linear_recurrence(x, x, x, lam, c)
+        with pytest.raises(REFUSED, match="c must be"):
+            api.npu_gated_linear_recurrence_update(x[0], x[0], x[0], lam, pool, c)
+        with pytest.raises(REFUSED, match="c must be"):
+            api.npu_gated_linear_recurrence_bwd(x, x, x, x, lam, torch.zeros(1, 8), c)

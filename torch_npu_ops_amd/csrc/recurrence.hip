@@ -11,6 +11,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <limits>
 #include <type_traits>
 
 #include "xk_common.h"
@@ -1280,6 +1281,8 @@ bool bad_sizes(int64_t N, int64_t total, int64_t D) {
          D >= kMostPitch || (cdiv(total, kTok) + kMostWaves) * cdiv(D, kWave) >= kMost;
 }
 
+bool c_ok(float c) { return c >= 0.f && c <= std::numeric_limits<float>::max(); }
+
 // cu_seqlens of a readable type, or none and N equal runs.
 bool seqs_ok(const void* cu, xk_dtype dt, int64_t N, int64_t total) {
   return cu ? dt == XK_I32 || dt == XK_I64 : total % N == 0;
@@ -1303,7 +1306,7 @@ extern "C" int xk_gated_linear_recurrence(
     int64_t stride_y_tok, const float* initial_state, float* final_state, float* states,
     const void* cu_seqlens, xk_dtype cu_dtype, int64_t N, int64_t total_tokens, int64_t D,
     void* workspace, size_t workspace_bytes, void* stream) {
-  if (bad_sizes(N, total_tokens, D) || !(c >= 0.f)) return XK_ERR_INVALID;
+  if (bad_sizes(N, total_tokens, D) || !c_ok(c)) return XK_ERR_INVALID;
   if (!is_float_dtype(dtype)) return XK_ERR_UNSUPPORTED;
   if (N == 0) return XK_OK;
   if (!seqs_ok(cu_seqlens, cu_dtype, N, total_tokens) || !lam) return XK_ERR_INVALID;
@@ -1333,7 +1336,7 @@ extern "C" int xk_gated_linear_recurrence_update(
     const int32_t* state_indices, int64_t num_cols, const int32_t* num_accepted_tokens,
     const void* cu_seqlens, xk_dtype cu_dtype, int64_t N, int64_t T, int64_t total_tokens,
     int64_t D, void* stream) {
-  if (bad_sizes(N, total_tokens, D) || num_slots < 0 || num_cols < 0 || !(c >= 0.f))
+  if (bad_sizes(N, total_tokens, D) || num_slots < 0 || num_cols < 0 || !c_ok(c))
     return XK_ERR_INVALID;
   if (!is_float_dtype(dtype)) return XK_ERR_UNSUPPORTED;
   if (N == 0 || total_tokens == 0) return XK_OK;
@@ -1371,7 +1374,7 @@ extern "C" int xk_gated_linear_recurrence_bwd(
     int64_t stride_db_tok, float* dlam, float* d_initial_state, const void* cu_seqlens,
     xk_dtype cu_dtype, int64_t N, int64_t total_tokens, int64_t D, void* workspace,
     size_t workspace_bytes, void* stream) {
-  if (bad_sizes(N, total_tokens, D) || !(c >= 0.f)) return XK_ERR_INVALID;
+  if (bad_sizes(N, total_tokens, D) || !c_ok(c)) return XK_ERR_INVALID;
   if (!is_float_dtype(dtype)) return XK_ERR_UNSUPPORTED;
   if (!lam || (N > 0 && !seqs_ok(cu_seqlens, cu_dtype, N, total_tokens))) return XK_ERR_INVALID;
   if (total_tokens > 0 &&

@@ -888,7 +888,8 @@ void glr_check(const torch::Tensor& x, const torch::Tensor& a, const torch::Tens
                   lam.size(0) == x.size(-1),
               "lam must be float32 [D]");
   same_device(lam, x, "lam");
-  TORCH_CHECK(c >= 0 && std::isfinite(c), "c must be finite and not negative");
+  TORCH_CHECK(c >= 0 && std::isfinite(static_cast<float>(c)),
+              "c must be finite (in float32) and not negative");
 }
 
 // cu_seqlens as the kernels read it (undefined: x's batch rows), and the

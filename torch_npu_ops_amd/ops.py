@@ -980,8 +980,8 @@ def _glr_check(x, a, b, lam, c):
         raise ValueError("x must have channels")
     if lam.dtype != torch.float32 or lam.shape != (x.size(-1),):
         raise ValueError("lam must be float32 [D]")
-    if not (c >= 0 and math.isfinite(c)):
-        raise ValueError("c must be finite and not negative")
+    if not 0 <= c <= torch.finfo(torch.float32).max:
+        raise ValueError("c must be finite (in float32) and not negative")
     _same_device(x, a=a, b=b, lam=lam)
 
 
