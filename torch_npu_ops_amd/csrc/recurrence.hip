@@ -156,8 +156,8 @@ __device__ __forceinline__ int cu_at(const void* cu, int cu64, int n, int run, i
 // The forward kernel takes 126 us for 16,384 x 4,096 bf16 (537 MB, 4.3 TB/s):
 // with loads and stores alone 92, without the arithmetic (34 instructions a
 // channel and token) 104, without the chain 115.  The window's 48 loads are
-// issued together, which takes 128 registers: 4 waves a SIMD hide the rest
-// only in part.  Windows of 8 tokens (8 waves) took 150 and more.
+// issued together, which takes 128 registers (and 4 spilled in bf16, 2 in fp16;
+// 93 in fp32): 4 waves a SIMD hide the rest only in part.  Windows of 8 tokens (8 waves) took 150 and more.
 // ---------------------------------------------------------------------------
 constexpr int kTok = kWin;
 // Waves of a block at most: kFew while a pass has no more than kUntil windows
@@ -374,8 +374,8 @@ __device__ __forceinline__ void st_f32(float* p, const Lane<VEC>& at, const floa
     if (at.ok[u]) p[at.ch + u] = v[u];
 }
 
-// The sequences' bounds.  The lane's own (of the first 64 sequences) are
-// requested before a window's inputs, so that no wait for them waits for those.
+// The sequences' bounds, with the lane's own (of the first 64 sequences)
+// requested together.  Windows that are known to be plain need none of them.
 struct Seqs {
   const void* cu;
   int cu64, N, run, total;
@@ -1007,7 +1007,7 @@ __device__ __forceinline__ float exp_neg(float v) {
 //  * Of the gates exp(-a), exp(-b), r and the decay stay in registers for the
 //    second pass, in reverse order; the rest is cheaper formed again.  (With
 //    the two exponentials alone 142 us instead of 134 for 8,192 x 4,096 bf16:
-//    the arithmetic is as long as the traffic.)  130 us now, 3.7 TB/s, at 2
+//    the arithmetic is as long as the traffic.)  132 us now, 3.6 TB/s, at 2
 //    waves a SIMD.
 //  * E = (dL/dl) l = G alpha (h_{t-1} l - i x alpha l / s) gives da = E (1 - r)
 //    and dlam = sum E sigmoid(lam) / softplus(lam), with no division by what
