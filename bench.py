@@ -1348,16 +1348,33 @@ def cpu_line(case: Case, gpu_us: float):
     return line
 
 
+CSRC = os.path.join(REPO, "torch_npu_ops_amd", "csrc")
+
+
+def source_files(fname):
+    """A kernel source file and the headers beside it that it includes,
+    directly or through others, by name."""
+    import re
+    files, left = set(), [fname]
+    while left:
+        name = left.pop()
+        if name in files or not os.path.exists(os.path.join(CSRC, name)):
+            continue
+        files.add(name)
+        with open(os.path.join(CSRC, name)) as f:
+            left += re.findall(r'^#include "([^"]+)"', f.read(), re.M)
+    return [fname] + sorted(files - {fname})
+
+
 def source_sha(fname):
-    """Hash of a kernel source file and the headers every kernel includes:
-    recorded with each traffic measurement, so a measurement taken before a
-    kernel changed is not reported as the current kernel's."""
+    """Hash of a kernel source file and of the headers it includes: recorded
+    with each traffic measurement, so a measurement taken before a kernel
+    changed is not reported as the current kernel's.  What other kernels alone
+    include does not count."""
     import hashlib
-    import glob
-    csrc = os.path.join(REPO, "torch_npu_ops_amd", "csrc")
     h = hashlib.sha256()
-    for path in [os.path.join(csrc, fname)] + sorted(glob.glob(os.path.join(csrc, "*.h"))):
-        with open(path, "rb") as f:
+    for name in source_files(fname):
+        with open(os.path.join(CSRC, name), "rb") as f:
             h.update(f.read())
     return h.hexdigest()[:16]
 
@@ -1547,9 +1564,8 @@ def summarize_profile(out_dir):
                 kernel_ops[k].append(op)
     traffic = {k: fetch[k] * 1024 * ff + write[k] * 1024 * wf
                for k in fetch if k in write}
-    csrc = os.path.join(REPO, "torch_npu_ops_amd", "csrc")
     sources = {os.path.basename(f): source_sha(os.path.basename(f))
-               for f in sorted(glob.glob(os.path.join(csrc, "*.hip")))}
+               for f in sorted(glob.glob(os.path.join(CSRC, "*.hip")))}
     with open(TRAFFIC_JSON, "w") as f:
         json.dump({"fetch_factor": ff, "write_factor": wf, "sources": sources,
                    "traffic_bytes": traffic}, f, indent=1)

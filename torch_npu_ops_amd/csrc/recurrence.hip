@@ -283,6 +283,15 @@ __device__ __forceinline__ Lane<VEC> lane_of(unsigned int lane, int64_t col, int
   return l;
 }
 
+// Two 16-bit elements in one word, by one conversion of both (element by
+// element the compiler converts twice and joins the halves).
+template <typename T>
+__device__ __forceinline__ unsigned int pack2(float lo, float hi) {
+  typedef T T2 __attribute__((ext_vector_type(2)));
+  typedef float F2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(unsigned int, __builtin_convertvector((F2{lo, hi}), T2));
+}
+
 // A window's rows of one tensor at the block's channels, as a buffer: the row
 // of a token is a scalar offset, a lane's word, at any address, a vector
 // offset that lanes without channels put out of range, where loads give 0 and

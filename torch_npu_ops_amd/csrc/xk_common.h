@@ -28,14 +28,6 @@ template <typename T>
 __device__ __forceinline__ T from_f32(float v) {
   return static_cast<T>(v);
 }
-// Two 16-bit elements in one word, by one conversion of both (element by
-// element the compiler converts twice and joins the halves).
-template <typename T>
-__device__ __forceinline__ unsigned int pack2(float lo, float hi) {
-  typedef T T2 __attribute__((ext_vector_type(2)));
-  typedef float F2 __attribute__((ext_vector_type(2)));
-  return __builtin_bit_cast(unsigned int, __builtin_convertvector((F2{lo, hi}), T2));
-}
 
 // Load one element whose dtype is only known at run time (used for small
 // parameter vectors such as weights and gates, never in a bandwidth loop).
