@@ -54,8 +54,10 @@ __device__ __forceinline__ float softplus_f32(float v) {
 // thousands of tokens may lie between a state and its use.  Below it is
 // alpha times v: alpha - 1, rounded near -1, has lost alpha's digits (1% of it
 // at alpha = 1e-6).  `word` holds either, told apart by the sign bit: alpha - 1
-// has it (-0 for a closed gate), alpha has not.  Where channels go below, the
-// choice costs 2 to 4% (16,384 x 4,096 bf16 133 us, with alpha - 1 throughout 128.5).
+// has it (-0 for a closed gate), alpha has not.  The choice
+// costs 2 to 4% where channels go below (16,384 x 4,096 bf16 133 us, with alpha - 1
+// throughout 128.5) and up to 7% in windows that are not plain (one tile of
+// 100 x 4,096: 10.9 and 10.2).
 constexpr float kNear = -0.25f;
 struct Decay {
   float alpha, em1, word;
