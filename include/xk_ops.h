@@ -35,7 +35,8 @@ typedef enum xk_dtype {
   XK_BF16 = 1,
   XK_F16 = 2,
   XK_I32 = 3,
-  XK_I64 = 4
+  XK_I64 = 4,
+  XK_F8E4M3 = 5 /* key-value caches only */
 } xk_dtype;
 
 /* Status codes (negative); positive values are hipError_t. */
@@ -638,6 +639,100 @@ int xk_gated_residual_rms_norm_bwd(
     void* dresidual, int64_t stride_dres_row, void* dgate, int64_t stride_dgate_row,
     void* dpost_weight, void* dscale, void* dpre_weight, int64_t M, int64_t N, int unit_offset,
     xk_dtype dtype, xk_dtype rdtype, xk_dtype wdtype, void* workspace, size_t workspace_bytes,
+    void* stream);
+
+/* ------------------------------------------------------------------------
+ * Rotary positions (no reference counterpart in this form; the relatives are
+ * xk_split_rmsnorm_rope and xk_rope_inplace): at position t, pair (u, v) i of
+ * a head becomes
+ *     scale * (u cos(t f_i) - v sin(t f_i)),  scale * (v cos(t f_i) + u sin(t f_i))
+ * with f = inv_freq, fp32 [rotary_dim / 2].  Pairs are elements (i, i +
+ * rotary_dim / 2), or (2i, 2i + 1) with interleaved != 0, of the first
+ * rotary_dim; the others are copied.  A longer context than trained is the
+ * caller's inv_freq and scale.  The angle is formed in 64 bits: positions up
+ * to 2^29 lose nothing.  One rounding, at the end.  inverse != 0 turns by -t f
+ * (and multiplies by scale as well): the backward pass, for gradients.
+ *   q, k : [num_tokens, heads, head_dim] in `dtype` with token and head
+ *     strides (any, zero for broadcast inputs); outputs may be their inputs
+ *     (the same start and strides) and must not overlap otherwise.  Hq or Hk
+ *     may be 0 (its pointers then are not read).  At most 4096 heads each,
+ *     head_dim at most 512, rotary_dim even.  Any alignment; 16-byte vectors
+ *     are used where all of it allows them.
+ *   positions : int32/int64 [num_tokens], any sign.
+ */
+int xk_rotary_embedding(
+    const void* q, int64_t stride_q_tok, int64_t stride_q_head, void* q_out,
+    int64_t stride_qo_tok, int64_t stride_qo_head, int64_t Hq, const void* k,
+    int64_t stride_k_tok, int64_t stride_k_head, void* k_out, int64_t stride_ko_tok,
+    int64_t stride_ko_head, int64_t Hk, const void* positions, xk_dtype pos_dtype,
+    const float* inv_freq, int64_t rotary_dim, int interleaved, float scale, int inverse,
+    int64_t num_tokens, int64_t head_dim, xk_dtype dtype, void* stream);
+
+/* The same turn of q and k, with k and v stored in a paged cache in the same
+ * launch (what reshape_and_cache does in engines, with the rotation on the way).
+ *   positions NULL: nothing is turned (q is copied).  Hq = 0: no q.
+ *   k_cache, v_cache : num_pages pages of page_size places with Hkv rows of
+ *     head_dim each, element strides for page, place and head (both the
+ *     [page, place, head] and the [page, head, place] order are strides), in
+ *     `dtype`, or XK_F8E4M3 for 16-bit tokens: x / k_scale[head] (fp32 [Hkv],
+ *     NULL = 1; positive) to the nearest e4m3 value, at most 448.
+ *   slots : int32/int64 [num_tokens]: page * page_size + place of a token.  A
+ *     slot outside the cache (-1 for padding) stores nothing; q is turned all
+ *     the same.  Two tokens of a call must not have the same slot.
+ */
+int xk_rotary_cache_append(
+    const void* q, int64_t stride_q_tok, int64_t stride_q_head, void* q_out,
+    int64_t stride_qo_tok, int64_t stride_qo_head, int64_t Hq, const void* k,
+    int64_t stride_k_tok, int64_t stride_k_head, const void* v, int64_t stride_v_tok,
+    int64_t stride_v_head, int64_t Hkv, void* k_cache, int64_t stride_kc_page,
+    int64_t stride_kc_slot, int64_t stride_kc_head, void* v_cache, int64_t stride_vc_page,
+    int64_t stride_vc_slot, int64_t stride_vc_head, xk_dtype cache_dtype, int64_t num_pages,
+    int64_t page_size, const void* slots, xk_dtype slot_dtype, const void* positions,
+    xk_dtype pos_dtype, const float* inv_freq, int64_t rotary_dim, int interleaved, float scale,
+    const float* k_scale, const float* v_scale, int64_t num_tokens, int64_t head_dim,
+    xk_dtype dtype, void* stream);
+
+/* Attention of the last T tokens of every sequence (1 in decode, more where
+ * drafts are verified) over the sequence's pages of the cache:
+ *     o = softmax(scale * q k^T) v
+ * over the positions up to the token's own, seq_len - T + t for token t, and
+ * with window > 0 only the last `window` of them.  Scores, softmax and sums in
+ * fp32; one rounding, at the end.  Hq / Hkv query heads share a key-value head.
+ *   q, out : [B, T, Hq, head_dim] with strides in `dtype`; head_dim a multiple
+ *     of 8, at most 256.  lse : fp32 [B, T, Hq] dense or NULL: the natural
+ *     logarithm of the sum of exp(scores), for joining with other parts.
+ *   k_cache, v_cache : as in xk_rotary_cache_append; the new tokens' keys and
+ *     values are in it already.  A value stands for itself times k_scale[head]
+ *     or v_scale[head].
+ *   block_table : int32 [B, max_pages] (row pitch in elements): position j of
+ *     a sequence is in page block_table[j / page_size].  Entries past the last
+ *     position are not read; positions of a page outside [0, num_pages) count
+ *     as masked.  Sequences may share pages.  max_pages * page_size at most 2^28.
+ *   seq_lens : int32 [B], clamped to [0, max_pages * page_size].
+ *   A row that sees nothing (a length below T, an empty sequence) is 0, its lse
+ *   -inf.  What the cache holds at positions that a row does not see (NaN, inf)
+ *   has no part in that row.
+ *   q, k_cache and v_cache 16-byte aligned (8 for an 8-bit cache), their
+ *   strides whole vectors of that size, out's of 4 elements (else
+ *   XK_ERR_UNSUPPORTED); a place's pitch below 2^27 bytes.
+ *   The split of the positions follows from all lengths of the batch: a
+ *   sequence's last bits depend on the batch, but not on the run.
+ *   workspace >= xk_paged_attention_workspace_bytes(...) bytes for the same
+ *   sizes on the current device, 256-byte aligned (NULL for 0); calls that
+ *   overlap in time need one each.  It needs no clearing and keeps nothing.
+ */
+int64_t xk_paged_attention_workspace_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hkv,
+                                           int64_t head_dim, int64_t max_pages,
+                                           int64_t page_size, xk_dtype dtype);
+int xk_paged_attention(
+    const void* q, int64_t stride_q_seq, int64_t stride_q_tok, int64_t stride_q_head,
+    const void* k_cache, int64_t stride_kc_page, int64_t stride_kc_slot, int64_t stride_kc_head,
+    const void* v_cache, int64_t stride_vc_page, int64_t stride_vc_slot, int64_t stride_vc_head,
+    xk_dtype cache_dtype, int64_t num_pages, int64_t page_size, const int32_t* block_table,
+    int64_t stride_table_row, int64_t max_pages, const int32_t* seq_lens, float scale,
+    int64_t window, const float* k_scale, const float* v_scale, void* out, int64_t stride_o_seq,
+    int64_t stride_o_tok, int64_t stride_o_head, float* lse, int64_t B, int64_t T, int64_t Hq,
+    int64_t Hkv, int64_t head_dim, xk_dtype dtype, void* workspace, size_t workspace_bytes,
     void* stream);
 
 #ifdef __cplusplus

@@ -27,7 +27,7 @@ F32 = ctypes.c_float
 SZ = ctypes.c_size_t
 
 # xk_dtype values (include/xk_ops.h)
-XK_F32, XK_BF16, XK_F16, XK_I32, XK_I64 = 0, 1, 2, 3, 4
+XK_F32, XK_BF16, XK_F16, XK_I32, XK_I64, XK_F8E4M3 = 0, 1, 2, 3, 4, 5
 XK_OK, XK_ERR_INVALID, XK_ERR_UNSUPPORTED, XK_ERR_WORKSPACE, XK_ERR_SCRATCH = 0, -1, -2, -3, -4
 
 XK_GLR_WINDOW = 16  # tokens per saved state of the gated linear recurrence
@@ -116,6 +116,16 @@ SIGNATURES: dict[str, tuple[list, object]] = {
     "xk_gated_residual_rms_norm_bwd": (
         [P, I64, P, I64, P, I64, P, I64, P, I64, P, P, P, P, P, P, I64, P, I64, P, I64, P, P, P,
          I64, I64, INT, INT, INT, INT, P, SZ, P], INT),
+    "xk_rotary_embedding": (
+        [P, I64, I64, P, I64, I64, I64, P, I64, I64, P, I64, I64, I64, P, INT, P, I64, INT, F32,
+         INT, I64, I64, INT, P], INT),
+    "xk_rotary_cache_append": (
+        [P, I64, I64, P, I64, I64, I64, P, I64, I64, P, I64, I64, I64, P, I64, I64, I64, P, I64,
+         I64, I64, INT, I64, I64, P, INT, P, INT, P, I64, INT, F32, P, P, I64, I64, INT, P], INT),
+    "xk_paged_attention_workspace_bytes": ([I64, I64, I64, I64, I64, I64, I64, INT], I64),
+    "xk_paged_attention": (
+        [P, I64, I64, I64, P, I64, I64, I64, P, I64, I64, I64, INT, I64, I64, P, I64, I64, P, F32,
+         I64, P, P, P, I64, I64, I64, P, I64, I64, I64, I64, I64, INT, P, SZ, P], INT),
 }
 
 _LIB = None

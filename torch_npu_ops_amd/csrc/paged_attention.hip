@@ -1,0 +1,165 @@
+// xk_paged_attention: checks, the plan's host part and the choice of instance
+// (the kernels are in paged_attention.h).
+#include "paged_attention.h"
+
+namespace xk {
+namespace paged {
+namespace {
+
+constexpr int64_t kMostPositions = int64_t{1} << 28;  // a sequence's, by its table row
+constexpr int64_t kMostPitch = int64_t{1} << 27;      // bytes from one position to the next
+
+struct Plan {
+  int tiles;  // row tiles of a wave
+  int64_t groups, want, slots, bytes;
+  bool alone;
+};
+
+// False where the sizes are beyond what a launch holds.
+bool plan_of(int64_t B, int64_t T, int64_t G, int64_t Hkv, int64_t D, int64_t positions,
+             xk_dtype dtype, Plan& x) {
+  const int64_t M = T * G, tile = dtype == XK_F32 ? 16 : 32;
+  x.tiles = M > 16 && D <= 128 ? 2 : 1;
+  x.groups = cdiv(M, 16 * x.tiles);
+  // Blocks in all: with one sequence the parts are equal, and one round of two
+  // blocks a compute unit is full; ragged batches get four rounds to even out.
+  const int64_t blocks = static_cast<int64_t>(num_cus()) * (B == 1 ? 2 : 8);
+  x.want = std::max<int64_t>(1, blocks / (Hkv * x.groups));
+  const int64_t most = std::max<int64_t>(1, cdiv(cdiv(positions, tile), kMinChunk));
+  x.alone = most == 1;
+  x.slots = std::min(x.want + B, B * most);
+  const int64_t rows = x.slots * Hkv * M;
+  if (x.slots * x.groups * Hkv >= INT32_MAX || rows >= (int64_t{1} << 40)) return false;
+  auto up = [](int64_t n) { return cdiv(n, 256) * 256; };
+  x.bytes = x.alone ? 0 : up(B * 8) + up(rows * 8) + up(rows * D * 4);
+  return true;
+}
+
+int check_sizes(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_pages,
+                int64_t page_size) {
+  if (B < 0 || T <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || D <= 0 || D > 256 || D % 8 ||
+      max_pages < 0 || page_size <= 0)
+    return XK_ERR_INVALID;
+  if (B > (1 << 24) || T > (1 << 20) || Hq > (1 << 16) ||
+      (max_pages > 0 && page_size > kMostPositions / max_pages))
+    return XK_ERR_INVALID;
+  return XK_OK;
+}
+
+}  // namespace
+}  // namespace paged
+}  // namespace xk
+
+using namespace xk;
+
+extern "C" int64_t xk_paged_attention_workspace_bytes(int64_t B, int64_t T, int64_t Hq,
+                                                      int64_t Hkv, int64_t head_dim,
+                                                      int64_t max_pages, int64_t page_size,
+                                                      xk_dtype dtype) {
+  paged::Plan x;
+  if (paged::check_sizes(B, T, Hq, Hkv, head_dim, max_pages, page_size) != XK_OK || B == 0 ||
+      !paged::plan_of(B, T, Hq / Hkv, Hkv, head_dim, max_pages * page_size, dtype, x))
+    return 0;
+  return x.bytes;
+}
+
+extern "C" int xk_paged_attention(
+    const void* q, int64_t stride_q_seq, int64_t stride_q_tok, int64_t stride_q_head,
+    const void* k_cache, int64_t stride_kc_page, int64_t stride_kc_slot, int64_t stride_kc_head,
+    const void* v_cache, int64_t stride_vc_page, int64_t stride_vc_slot, int64_t stride_vc_head,
+    xk_dtype cache_dtype, int64_t num_pages, int64_t page_size, const int32_t* block_table,
+    int64_t stride_table_row, int64_t max_pages, const int32_t* seq_lens, float scale,
+    int64_t window, const float* k_scale, const float* v_scale, void* out, int64_t stride_o_seq,
+    int64_t stride_o_tok, int64_t stride_o_head, float* lse, int64_t B, int64_t T, int64_t Hq,
+    int64_t Hkv, int64_t head_dim, xk_dtype dtype, void* workspace, size_t workspace_bytes,
+    void* stream) {
+  using namespace paged;
+  const int st = check_sizes(B, T, Hq, Hkv, head_dim, max_pages, page_size);
+  if (st != XK_OK) return st;
+  if (num_pages < 0 || num_pages > INT32_MAX || window < 0 || !std::isfinite(scale))
+    return XK_ERR_INVALID;
+  const bool eight = cache_dtype == XK_F8E4M3;
+  if (!is_float_dtype(dtype) || (eight ? dtype == XK_F32 : cache_dtype != dtype))
+    return XK_ERR_UNSUPPORTED;
+  if (!eight && (k_scale || v_scale)) return XK_ERR_INVALID;
+  if (B == 0) return XK_OK;
+  if (!q || !out || !seq_lens || (max_pages && !block_table) ||
+      (num_pages && (!k_cache || !v_cache)))
+    return XK_ERR_INVALID;
+  // Vectors of 16 bytes (8 of an 8-bit cache) have to be aligned.
+  const int eb = elem_bytes(dtype), cb = elem_bytes(cache_dtype), n = 16 / eb;
+  const int cv = n * cb;
+  if (!aligned(q, 16) || stride_q_seq % n || stride_q_tok % n || stride_q_head % n ||
+      !aligned(k_cache, cv) || !aligned(v_cache, cv) || stride_kc_page % n ||
+      stride_kc_slot % n || stride_kc_head % n || stride_vc_page % n || stride_vc_slot % n ||
+      stride_vc_head % n || !aligned(out, 4 * eb) || stride_o_seq % 4 || stride_o_tok % 4 ||
+      stride_o_head % 4)
+    return XK_ERR_UNSUPPORTED;
+  if (stride_kc_slot < 0 || stride_vc_slot < 0 || stride_kc_slot * cb >= kMostPitch ||
+      stride_vc_slot * cb >= kMostPitch)
+    return XK_ERR_INVALID;
+  const int64_t positions = num_pages ? max_pages * page_size : 0;
+  Plan x;
+  if (!plan_of(B, T, Hq / Hkv, Hkv, head_dim, max_pages * page_size, dtype, x))
+    return XK_ERR_INVALID;
+  if (x.bytes && (!workspace || workspace_bytes < static_cast<size_t>(x.bytes) ||
+                  !aligned(workspace, 256)))
+    return XK_ERR_WORKSPACE;
+  Params p{};
+  p.q = q;
+  p.q_seq = stride_q_seq;
+  p.q_tok = stride_q_tok;
+  p.q_head = stride_q_head;
+  p.kc = static_cast<const char*>(k_cache);
+  p.k_page = stride_kc_page * cb;
+  p.k_slot = stride_kc_slot * cb;
+  p.k_head = stride_kc_head * cb;
+  p.vc = static_cast<const char*>(v_cache);
+  p.v_page = stride_vc_page * cb;
+  p.v_slot = stride_vc_slot * cb;
+  p.v_head = stride_vc_head * cb;
+  p.num_pages = static_cast<int>(num_pages);
+  p.page_size = static_cast<int>(page_size);
+  p.page_shift = -1;
+  if ((page_size & (page_size - 1)) == 0)
+    for (p.page_shift = 0; (int64_t{1} << p.page_shift) < page_size;) ++p.page_shift;
+  p.table = block_table;
+  p.table_row = stride_table_row;
+  p.max_pages = static_cast<int>(max_pages);
+  p.lens = seq_lens;
+  p.most_len = static_cast<int>(positions);
+  p.scale2 = scale * 1.44269504088896f;
+  p.window = static_cast<int>(std::min<int64_t>(window, kMostPositions + (1 << 20)));
+  p.k_scale = k_scale;
+  p.v_scale = v_scale;
+  p.out = out;
+  p.o_seq = stride_o_seq;
+  p.o_tok = stride_o_tok;
+  p.o_head = stride_o_head;
+  p.lse = lse;
+  p.B = static_cast<int>(B);
+  p.T = static_cast<int>(T);
+  p.G = static_cast<int>(Hq / Hkv);
+  p.Hkv = static_cast<int>(Hkv);
+  p.D = static_cast<int>(head_dim);
+  p.M = static_cast<int>(T * (Hq / Hkv));
+  p.groups = static_cast<int>(x.groups);
+  p.want = static_cast<int>(x.want);
+  p.slots = static_cast<int>(x.slots);
+  p.alone = x.alone;
+  if (!x.alone) {
+    char* ws = static_cast<char*>(workspace);
+    const int64_t rows = x.slots * Hkv * p.M;
+    p.meta = reinterpret_cast<int2*>(ws);
+    ws += cdiv(B * 8, 256) * 256;
+    p.ml = reinterpret_cast<float2*>(ws);
+    ws += cdiv(rows * 8, 256) * 256;
+    p.acc = reinterpret_cast<float*>(ws);
+  }
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  switch (dtype) {
+    case XK_F32: return run_f32(p, x.tiles, s);
+    case XK_BF16: return eight ? run_bf16_f8(p, x.tiles, s) : run_bf16(p, x.tiles, s);
+    default: return eight ? run_f16_f8(p, x.tiles, s) : run_f16(p, x.tiles, s);
+  }
+}

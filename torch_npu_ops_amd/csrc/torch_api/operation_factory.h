@@ -88,6 +88,9 @@ class OperationFactory {
   XK_FACTORY(gated_residual_rms_norm, GatedResidualRmsNormOp, "xk_gated_residual_rms_norm")
   XK_FACTORY(gated_residual_rms_norm_bwd, GatedResidualRmsNormBwdOp,
              "xk_gated_residual_rms_norm_bwd")
+  XK_FACTORY(rotary_embedding, RotaryEmbeddingOp, "xk_rotary_embedding")
+  XK_FACTORY(rotary_cache_append, RotaryCacheAppendOp, "xk_rotary_cache_append")
+  XK_FACTORY(paged_attention, PagedAttentionOp, "xk_paged_attention")
 
 #undef XK_FACTORY
 

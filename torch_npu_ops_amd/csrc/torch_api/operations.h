@@ -83,7 +83,8 @@ XK_OPERATION(FusedQkvzbaSplitReshapeGqaR2Op, xk_fused_qkvzba_split_reshape_cat);
 XK_OPERATION(FusedQkvzbaSplitReshapeGqaR3Op, xk_fused_qkvzba_split_reshape_cat);
 XK_OPERATION(FusedQkvzbaSplitReshapeGqaR4Op, xk_fused_qkvzba_split_reshape_cat);
 // No reference counterpart: the whole chunked pipeline, the fused decode step,
-// the gated linear recurrence and the block-to-block norm.
+// the gated linear recurrence, the block-to-block norm, rotary positions, the
+// paged cache and attention over it.
 XK_OPERATION(ChunkGatedDeltaRuleFusedOp, xk_gdn_chunk_fwd);
 XK_OPERATION(GdnConvDecodeOp, xk_gdn_conv_decode);
 XK_OPERATION(GatedLinearRecurrenceOp, xk_gated_linear_recurrence);
@@ -91,6 +92,9 @@ XK_OPERATION(GatedLinearRecurrenceUpdateOp, xk_gated_linear_recurrence_update);
 XK_OPERATION(GatedLinearRecurrenceBwdOp, xk_gated_linear_recurrence_bwd);
 XK_OPERATION(GatedResidualRmsNormOp, xk_gated_residual_rms_norm);
 XK_OPERATION(GatedResidualRmsNormBwdOp, xk_gated_residual_rms_norm_bwd);
+XK_OPERATION(RotaryEmbeddingOp, xk_rotary_embedding);
+XK_OPERATION(RotaryCacheAppendOp, xk_rotary_cache_append);
+XK_OPERATION(PagedAttentionOp, xk_paged_attention);
 
 #undef XK_OPERATION
 

@@ -95,6 +95,16 @@ PYBIND11_MODULE(_xk_torch, m) {
         "dy"_a, "x"_a, "residual"_a, "rstd_post"_a, "rstd_pre"_a, "post_weight"_a = OptT(),
         "gate"_a = OptT(), "scale"_a = OptT(), "pre_weight"_a = OptT(),
         "unit_offset"_a = false);
+  m.def("npu_rotary_embedding", &npu::npu_rotary_embedding, "q"_a, "k"_a, "positions"_a,
+        "inv_freq"_a, "interleaved"_a = false, "scale"_a = 1.0);
+  m.def("npu_rotary_embedding_bwd", &npu::npu_rotary_embedding_bwd, "dq"_a, "dk"_a,
+        "positions"_a, "inv_freq"_a, "interleaved"_a = false, "scale"_a = 1.0);
+  m.def("npu_rotary_cache_append", &npu::npu_rotary_cache_append, "q"_a, "k"_a, "v"_a,
+        "k_cache"_a, "v_cache"_a, "slots"_a, "positions"_a = OptT(), "inv_freq"_a = OptT(),
+        "interleaved"_a = false, "scale"_a = 1.0, "k_scale"_a = OptT(), "v_scale"_a = OptT());
+  m.def("npu_paged_attention", &npu::npu_paged_attention, "q"_a, "k_cache"_a, "v_cache"_a,
+        "block_table"_a, "seq_lens"_a, "scale"_a = std::optional<double>(), "window"_a = 0,
+        "k_scale"_a = OptT(), "v_scale"_a = OptT(), "output_lse"_a = false);
   // npu_ops (AscendC API): gemma returns (rstd, y) for its two out-params.
   m.def("npu_ops_gemma_rms_norm", [](const torch::Tensor& x, const torch::Tensor& gamma,
                                      double eps) {

@@ -10,6 +10,7 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
+#include <array>
 #include <cmath>
 #include <limits>
 
@@ -1208,6 +1209,251 @@ npu_gated_residual_rms_norm_bwd(const std::optional<torch::Tensor>& dh,
             xdt(residual), xdt_of(wt), mptr(ws), static_cast<size_t>(bytes), stream),
         "xk_gated_residual_rms_norm_bwd");
   return {dx, dres, given(dgate), given(dpost), given(dscale), given(dpre)};
+}
+
+namespace {
+
+// x [..., heads, D] with its tokens' and heads' strides: itself where its
+// tokens have one pitch, else a contiguous copy.
+torch::Tensor token_heads(const torch::Tensor& x, int64_t& pitch, int64_t& head) {
+  const int64_t heads = x.size(-2), D = x.size(-1);
+  bool ok = D == 1 || x.stride(-1) == 1;
+  int64_t count = 1;
+  pitch = 0;
+  for (int64_t d = x.dim() - 3; d >= 0 && ok; --d) {
+    if (x.size(d) == 1) continue;
+    if (count == 1) pitch = x.stride(d);
+    else ok = x.stride(d) == pitch * count;
+    count *= x.size(d);
+  }
+  auto y = ok ? x : x.contiguous();
+  if (!ok) pitch = heads * D;
+  head = heads > 1 ? y.stride(-2) : 0;
+  return y;
+}
+
+bool is_index(const torch::Tensor& t) {
+  return t.scalar_type() == torch::kInt32 || t.scalar_type() == torch::kInt64;
+}
+
+// Checks of the turn; the number of turned elements of a head.
+int64_t rotary_positions(const torch::Tensor& x, const torch::Tensor& positions,
+                         const torch::Tensor& inv_freq, double scale) {
+  TORCH_CHECK(is_index(positions) && positions.sizes() == x.sizes().slice(0, x.dim() - 2),
+              "positions must be int32 or int64, one for each token");
+  TORCH_CHECK(inv_freq.scalar_type() == torch::kFloat32 && inv_freq.dim() == 1 &&
+                  inv_freq.size(0) > 0 && 2 * inv_freq.size(0) <= x.size(-1),
+              "inv_freq must be float32 [rotary_dim / 2], rotary_dim at most head_dim");
+  TORCH_CHECK(scale > 0 && scale <= std::numeric_limits<float>::max(),
+              "scale must be positive and finite (in float32)");
+  same_device(positions, x, "positions");
+  same_device(inv_freq, x, "inv_freq");
+  return 2 * inv_freq.size(0);
+}
+
+void rotary_check(const torch::Tensor& x, const torch::Tensor& like, const char* name) {
+  TORCH_CHECK(x.dim() >= 3 && (x.scalar_type() == torch::kFloat32 ||
+                               x.scalar_type() == torch::kBFloat16 ||
+                               x.scalar_type() == torch::kFloat16),
+              name, " must be [..., heads, head_dim] of float32, bfloat16 or float16");
+  TORCH_CHECK(x.dim() == like.dim() &&
+                  x.sizes().slice(0, x.dim() - 2) == like.sizes().slice(0, x.dim() - 2) &&
+                  x.size(-1) == like.size(-1) && x.scalar_type() == like.scalar_type(),
+              name, " must have the tokens, head_dim and dtype of the others");
+  TORCH_CHECK(x.size(-1) > 0 && x.size(-1) <= 512, "head_dim must be 1 to 512");
+  TORCH_CHECK(x.size(-2) <= 4096, "at most 4096 heads");
+  same_device(x, like, name);
+}
+
+std::tuple<torch::Tensor, std::optional<torch::Tensor>> turned(
+    const torch::Tensor& q, const std::optional<torch::Tensor>& k,
+    const torch::Tensor& positions, const torch::Tensor& inv_freq, bool interleaved,
+    double scale, bool inverse) {
+  rotary_check(q, q, "q");
+  if (has(k)) rotary_check(*k, q, "k");
+  const int64_t rot = rotary_positions(q, positions, inv_freq, scale);
+  void* stream = stream_of(q);
+  c10::DeviceGuard guard(q.device());
+  const int64_t D = q.size(-1), Hq = q.size(-2), Hk = has(k) ? k->size(-2) : 0;
+  int64_t qt = 0, qh = 0, kt = 0, kh = 0;
+  auto qr = token_heads(q, qt, qh);
+  torch::Tensor kr, ko;
+  if (has(k)) {
+    kr = token_heads(*k, kt, kh);
+    ko = fresh(k->sizes(), k->scalar_type(), q);
+  }
+  auto pos = positions.contiguous(), freq = inv_freq.contiguous();
+  auto qo = fresh(q.sizes(), q.scalar_type(), q);
+  check(xk_rotary_embedding(qr.data_ptr(), qt, qh, qo.data_ptr(), Hq * D, D, Hq, ptr(kr), kt, kh,
+                            mptr(ko), Hk * D, D, Hk, pos.data_ptr(), xdt(pos), fptr(freq), rot,
+                            interleaved, static_cast<float>(scale), inverse, pos.numel(), D,
+                            xdt(q), stream),
+        "xk_rotary_embedding");
+  return {qo, given(ko)};
+}
+
+int64_t pitch_of(const torch::Tensor& x, int64_t d) { return x.size(d) > 1 ? x.stride(d) : 0; }
+
+// The two caches [pages, page, Hkv, D] beside tokens x; their xk dtype.
+xk_dtype cache_check(const torch::Tensor& k_cache, const torch::Tensor& v_cache,
+                     const torch::Tensor& x, int64_t Hkv, bool written) {
+  for (const auto& [c, name] :
+       {std::make_pair(&k_cache, "k_cache"), std::make_pair(&v_cache, "v_cache")}) {
+    TORCH_CHECK(c->dim() == 4 && c->size(3) == x.size(-1) && c->size(1) > 0, name,
+                " must be [pages, page, kv heads, head_dim]");
+    TORCH_CHECK(Hkv < 0 || c->size(2) == Hkv, name, " must have the kv heads of k and v");
+    TORCH_CHECK(c->size(3) == 1 || c->stride(3) == 1, name, " must have contiguous rows");
+    for (int64_t d = 0; d < 3 && written; ++d)
+      TORCH_CHECK(c->size(d) <= 1 || c->stride(d) >= c->size(3), name,
+                  "'s rows must not overlap");
+    same_device(*c, x, name);
+  }
+  TORCH_CHECK(v_cache.sizes() == k_cache.sizes() &&
+                  v_cache.scalar_type() == k_cache.scalar_type(),
+              "v_cache must have k_cache's shape and dtype");
+  if (k_cache.scalar_type() == x.scalar_type()) return xdt(x);
+  TORCH_CHECK(k_cache.scalar_type() == torch::kFloat8_e4m3fn &&
+                  x.scalar_type() != torch::kFloat32,
+              "the cache must have the tokens' dtype, or float8_e4m3fn beside 16 bits");
+  return XK_F8E4M3;
+}
+
+torch::Tensor kv_scale(const std::optional<torch::Tensor>& s, const torch::Tensor& x,
+                       int64_t Hkv, xk_dtype cache, const char* name) {
+  if (!has(s)) return {};
+  TORCH_CHECK(cache == XK_F8E4M3, name, " needs a float8_e4m3fn cache");
+  TORCH_CHECK(s->scalar_type() == torch::kFloat32 && s->dim() == 1 && s->size(0) == Hkv, name,
+              " must be float32 [kv heads]");
+  same_device(*s, x, name);
+  return s->contiguous();
+}
+
+}  // namespace
+
+std::tuple<torch::Tensor, std::optional<torch::Tensor>> npu_rotary_embedding(
+    const torch::Tensor& q, const std::optional<torch::Tensor>& k,
+    const torch::Tensor& positions, const torch::Tensor& inv_freq, bool interleaved,
+    double scale) {
+  return turned(q, k, positions, inv_freq, interleaved, scale, false);
+}
+
+std::tuple<torch::Tensor, std::optional<torch::Tensor>> npu_rotary_embedding_bwd(
+    const torch::Tensor& dq, const std::optional<torch::Tensor>& dk,
+    const torch::Tensor& positions, const torch::Tensor& inv_freq, bool interleaved,
+    double scale) {
+  return turned(dq, dk, positions, inv_freq, interleaved, scale, true);
+}
+
+std::optional<torch::Tensor> npu_rotary_cache_append(
+    const std::optional<torch::Tensor>& q, const torch::Tensor& k, const torch::Tensor& v,
+    torch::Tensor& k_cache, torch::Tensor& v_cache, const torch::Tensor& slots,
+    const std::optional<torch::Tensor>& positions, const std::optional<torch::Tensor>& inv_freq,
+    bool interleaved, double scale, const std::optional<torch::Tensor>& k_scale,
+    const std::optional<torch::Tensor>& v_scale) {
+  rotary_check(k, k, "k");
+  rotary_check(v, k, "v");
+  const int64_t Hkv = k.size(-2), D = k.size(-1), Hq = has(q) ? q->size(-2) : 0;
+  TORCH_CHECK(v.size(-2) == Hkv, "v must have k's heads");
+  TORCH_CHECK(Hkv > 0, "k must have heads");
+  if (has(q)) rotary_check(*q, k, "q");
+  TORCH_CHECK(is_index(slots) && slots.sizes() == k.sizes().slice(0, k.dim() - 2),
+              "slots must be int32 or int64, one for each token");
+  same_device(slots, k, "slots");
+  TORCH_CHECK(has(positions) == has(inv_freq), "positions and inv_freq go together");
+  const int64_t rot = has(positions) ? rotary_positions(k, *positions, *inv_freq, scale) : 0;
+  const xk_dtype cache = cache_check(k_cache, v_cache, k, Hkv, true);
+  auto ks = kv_scale(k_scale, k, Hkv, cache, "k_scale"),
+       vs = kv_scale(v_scale, k, Hkv, cache, "v_scale");
+  void* stream = stream_of(k);
+  c10::DeviceGuard guard(k.device());
+  int64_t qt = 0, qh = 0, kt, kh, vt, vh;
+  torch::Tensor qr, qo, pos, freq;
+  if (has(q)) {
+    qr = token_heads(*q, qt, qh);
+    qo = fresh(q->sizes(), q->scalar_type(), k);
+  }
+  auto kr = token_heads(k, kt, kh), vr = token_heads(v, vt, vh);
+  auto sl = slots.contiguous();
+  if (has(positions)) {
+    pos = positions->contiguous();
+    freq = inv_freq->contiguous();
+  }
+  check(xk_rotary_cache_append(
+            ptr(qr), qt, qh, mptr(qo), Hq * D, D, Hq, kr.data_ptr(), kt, kh, vr.data_ptr(), vt,
+            vh, Hkv, k_cache.data_ptr(), pitch_of(k_cache, 0), pitch_of(k_cache, 1),
+            pitch_of(k_cache, 2), v_cache.data_ptr(), pitch_of(v_cache, 0), pitch_of(v_cache, 1),
+            pitch_of(v_cache, 2), cache, k_cache.size(0), k_cache.size(1), sl.data_ptr(), xdt(sl),
+            ptr(pos), pos.defined() ? xdt(pos) : XK_I32, fptr(freq), rot, interleaved,
+            static_cast<float>(scale), fptr(ks), fptr(vs), sl.numel(), D, xdt(k), stream),
+        "xk_rotary_cache_append");
+  return given(qo);
+}
+
+std::tuple<torch::Tensor, std::optional<torch::Tensor>> npu_paged_attention(
+    const torch::Tensor& q, const torch::Tensor& k_cache, const torch::Tensor& v_cache,
+    const torch::Tensor& block_table, const torch::Tensor& seq_lens,
+    const std::optional<double>& scale, int64_t window,
+    const std::optional<torch::Tensor>& k_scale, const std::optional<torch::Tensor>& v_scale,
+    bool output_lse) {
+  TORCH_CHECK((q.dim() == 3 || q.dim() == 4) && (q.scalar_type() == torch::kFloat32 ||
+                                                 q.scalar_type() == torch::kBFloat16 ||
+                                                 q.scalar_type() == torch::kFloat16),
+              "q must be [B, Hq, D] or [B, T, Hq, D] of float32, bfloat16 or float16");
+  const int64_t B = q.size(0), T = q.dim() == 4 ? q.size(1) : 1, Hq = q.size(-2), D = q.size(-1);
+  TORCH_CHECK(D > 0 && D <= 256 && D % 8 == 0, "head_dim must be a multiple of 8, at most 256");
+  const xk_dtype cache = cache_check(k_cache, v_cache, q, -1, false);
+  const int64_t Hkv = k_cache.size(2);
+  TORCH_CHECK(Hkv > 0 && Hq > 0 && Hq % Hkv == 0,
+              "q's heads must be a multiple of the cache's");
+  TORCH_CHECK(block_table.scalar_type() == torch::kInt32 && block_table.dim() == 2 &&
+                  block_table.size(0) == B,
+              "block_table must be int32 [B, pages]");
+  TORCH_CHECK(seq_lens.scalar_type() == torch::kInt32 && seq_lens.dim() == 1 &&
+                  seq_lens.size(0) == B,
+              "seq_lens must be int32 [B]");
+  TORCH_CHECK(window >= 0, "window must not be negative");
+  const double sc = scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(D));
+  TORCH_CHECK(std::abs(sc) <= std::numeric_limits<float>::max(),
+              "scale must be finite (in float32)");
+  same_device(block_table, q, "block_table");
+  same_device(seq_lens, q, "seq_lens");
+  auto ks = kv_scale(k_scale, q, Hkv, cache, "k_scale"),
+       vs = kv_scale(v_scale, q, Hkv, cache, "v_scale");
+  void* stream = stream_of(q);
+  c10::DeviceGuard guard(q.device());
+  auto o = fresh(q.sizes(), q.scalar_type(), q);
+  torch::Tensor lse, ws;
+  if (output_lse) lse = fresh(q.sizes().slice(0, q.dim() - 1), torch::kFloat32, q);
+  if (T == 0) return {o, given(lse)};
+  // Strides of [B, T, Hq, D] without a dimension of one token.
+  auto strides = [&](const torch::Tensor& x) {
+    return std::array<int64_t, 3>{pitch_of(x, 0), x.dim() == 4 ? pitch_of(x, 1) : 0,
+                                  pitch_of(x, x.dim() - 2)};
+  };
+  auto qr = q;
+  auto s = strides(qr);
+  const int64_t n = 16 / q.element_size();
+  if (q.stride(-1) != 1 || s[0] % n || s[1] % n || s[2] % n ||
+      reinterpret_cast<uintptr_t>(q.data_ptr()) % 16) {
+    qr = q.clone(at::MemoryFormat::Contiguous);
+    s = strides(qr);
+  }
+  auto table = block_table.size(1) <= 1 || block_table.stride(1) == 1 ? block_table
+                                                                      : block_table.contiguous();
+  auto lens = seq_lens.contiguous();
+  const int64_t bytes = xk_paged_attention_workspace_bytes(B, T, Hq, Hkv, D, table.size(1),
+                                                           k_cache.size(1), xdt(q));
+  if (bytes > 0) ws = workspace(bytes, q.device());
+  check(xk_paged_attention(
+            qr.data_ptr(), s[0], s[1], s[2], k_cache.data_ptr(), pitch_of(k_cache, 0),
+            pitch_of(k_cache, 1), pitch_of(k_cache, 2), v_cache.data_ptr(), pitch_of(v_cache, 0),
+            pitch_of(v_cache, 1), pitch_of(v_cache, 2), cache, k_cache.size(0), k_cache.size(1),
+            static_cast<const int32_t*>(table.data_ptr()), pitch_of(table, 0), table.size(1),
+            static_cast<const int32_t*>(lens.data_ptr()), static_cast<float>(sc), window,
+            fptr(ks), fptr(vs), o.data_ptr(), T * Hq * D, Hq * D, D, fptr(lse), B, T, Hq, Hkv, D,
+            xdt(q), mptr(ws), static_cast<size_t>(bytes), stream),
+        "xk_paged_attention");
+  return {o, given(lse)};
 }
 
 }  // namespace xllm::kernel::npu

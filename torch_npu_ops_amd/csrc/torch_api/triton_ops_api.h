@@ -229,4 +229,47 @@ npu_gated_residual_rms_norm_bwd(const std::optional<torch::Tensor>& dh,
                                 const std::optional<torch::Tensor>& pre_weight = std::nullopt,
                                 bool unit_offset = false);
 
+// Rotary positions (xk_rotary_embedding): q and k [..., heads, D] of one dtype
+// (fp32, bf16 or fp16; k may be left out) turned by the angles positions *
+// inv_freq and multiplied by scale in the first 2 * numel(inv_freq) elements
+// of a head, pairs (i, i + half) or (2i, 2i + 1); the others are copied.
+// positions int32/int64 in the tokens' shape, inv_freq fp32.  Views whose
+// tokens have one pitch (parts of one product's rows) are read in place.
+std::tuple<torch::Tensor, std::optional<torch::Tensor>> npu_rotary_embedding(
+    const torch::Tensor& q, const std::optional<torch::Tensor>& k,
+    const torch::Tensor& positions, const torch::Tensor& inv_freq, bool interleaved = false,
+    double scale = 1.0);
+
+// The gradients of q and k from those of the outputs: the same turn backwards.
+std::tuple<torch::Tensor, std::optional<torch::Tensor>> npu_rotary_embedding_bwd(
+    const torch::Tensor& dq, const std::optional<torch::Tensor>& dk,
+    const torch::Tensor& positions, const torch::Tensor& inv_freq, bool interleaved = false,
+    double scale = 1.0);
+
+// The same turn of q and k, with k and v written to their slots (int32/int64,
+// page * page_size + place; outside the cache: not written) of the paged
+// caches [pages, page, kv heads, D], in the tokens' dtype or float8_e4m3fn
+// (x / scale of the kv head; k_scale, v_scale fp32 [kv heads]).  Without
+// positions nothing is turned.  Returns the turned q, if there is a q.  No two
+// tokens may have the same slot.
+std::optional<torch::Tensor> npu_rotary_cache_append(
+    const std::optional<torch::Tensor>& q, const torch::Tensor& k, const torch::Tensor& v,
+    torch::Tensor& k_cache, torch::Tensor& v_cache, const torch::Tensor& slots,
+    const std::optional<torch::Tensor>& positions = std::nullopt,
+    const std::optional<torch::Tensor>& inv_freq = std::nullopt, bool interleaved = false,
+    double scale = 1.0, const std::optional<torch::Tensor>& k_scale = std::nullopt,
+    const std::optional<torch::Tensor>& v_scale = std::nullopt);
+
+// Attention of the last T tokens of every sequence over its pages of the cache
+// (xk_paged_attention): q [B, Hq, D] or [B, T, Hq, D], token t at position
+// seq_lens - T + t, block_table int32 [B, pages], seq_lens int32 [B]; scale
+// nullopt: 1 / sqrt(D); window 0: all positions.  Returns (o shaped like q,
+// lse fp32 [B, T, Hq] if asked for).
+std::tuple<torch::Tensor, std::optional<torch::Tensor>> npu_paged_attention(
+    const torch::Tensor& q, const torch::Tensor& k_cache, const torch::Tensor& v_cache,
+    const torch::Tensor& block_table, const torch::Tensor& seq_lens,
+    const std::optional<double>& scale = std::nullopt, int64_t window = 0,
+    const std::optional<torch::Tensor>& k_scale = std::nullopt,
+    const std::optional<torch::Tensor>& v_scale = std::nullopt, bool output_lse = false);
+
 }  // namespace xllm::kernel::npu

@@ -1265,3 +1265,246 @@ def npu_gated_residual_rms_norm_bwd(dh: Optional[torch.Tensor], dy: Optional[tor
             int(unit_offset), xk_dtype(x), xk_dtype(residual), _DT[wt], _ptr(ws), size, stream)
     check(st, "xk_gated_residual_rms_norm_bwd")
     return dx, dres, dgate, dpost, dscale, dpre
+
+
+# ---------------------------------------------------------------------------
+# Rotary positions, the paged key-value cache and attention over it
+# ---------------------------------------------------------------------------
+def _token_heads(x: torch.Tensor, name: str):
+    """x [..., heads, D] as (tensor, token stride, head stride): itself where
+    its tokens have one pitch, else a contiguous copy."""
+    heads, D = x.size(-2), x.size(-1)
+    ok, pitch, count = D == 1 or x.stride(-1) == 1, 0, 1
+    for d in range(x.dim() - 3, -1, -1):
+        if not ok or x.size(d) == 1:
+            continue
+        if count == 1:
+            pitch = x.stride(d)
+        else:
+            ok = x.stride(d) == pitch * count
+        count *= x.size(d)
+    if not ok:
+        x, pitch = x.contiguous(), heads * D
+    return x, pitch, x.stride(-2) if heads > 1 else 0
+
+
+def _positions(x, positions, inv_freq, scale):
+    """Checks of the turn; the number of turned elements of a head."""
+    if positions.dtype not in (torch.int32, torch.int64) or positions.shape != x.shape[:-2]:
+        raise ValueError("positions must be int32 or int64, one for each token")
+    if (inv_freq.dtype != torch.float32 or inv_freq.dim() != 1
+            or not 0 < 2 * inv_freq.numel() <= x.size(-1)):
+        raise ValueError("inv_freq must be float32 [rotary_dim / 2], rotary_dim at most head_dim")
+    if not 0 < scale <= torch.finfo(torch.float32).max:
+        raise ValueError("scale must be positive and finite (in float32)")
+    _same_device(x, positions=positions, inv_freq=inv_freq)
+    return 2 * inv_freq.numel()
+
+
+def _rotary_check(x, like, name):
+    if x.dim() < 3 or x.dtype not in _FLOATS:
+        raise ValueError(f"{name} must be [..., heads, head_dim] of float32, bfloat16 or float16")
+    if x.shape[:-2] != like.shape[:-2] or x.size(-1) != like.size(-1) or x.dtype != like.dtype:
+        raise ValueError(f"{name} must have the tokens, head_dim and dtype of the others")
+    if x.size(-1) == 0 or x.size(-1) > 512:
+        raise ValueError("head_dim must be 1 to 512")
+    if x.size(-2) > 4096:
+        raise ValueError("at most 4096 heads")
+    _same_device(like, **{name: x})
+
+
+def _turned(q, k, positions, inv_freq, interleaved, scale, inverse):
+    _rotary_check(q, q, "q")
+    if k is not None:
+        _rotary_check(k, q, "k")
+    rot = _positions(q, positions, inv_freq, scale)
+    stream = _stream(q)
+    D, T = q.size(-1), positions.numel()
+    qr, qt, qh = _token_heads(q, "q")
+    kr, kt, kh = _token_heads(k, "k") if k is not None else (None, 0, 0)
+    Hq, Hk = q.size(-2), k.size(-2) if k is not None else 0
+    pos, freq = positions.contiguous(), inv_freq.contiguous()
+    with torch.cuda.device(q.device):
+        qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        ko = torch.empty(k.shape, dtype=k.dtype, device=k.device) if k is not None else None
+        st = lib().xk_rotary_embedding(
+            qr.data_ptr(), qt, qh, qo.data_ptr(), Hq * D, D, Hq, _ptr(kr), kt, kh, _ptr(ko),
+            Hk * D, D, Hk, pos.data_ptr(), xk_dtype(pos), freq.data_ptr(), rot,
+            int(interleaved), float(scale), inverse, T, D, xk_dtype(q), stream)
+    check(st, "xk_rotary_embedding")
+    return qo, ko
+
+
+def npu_rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor,
+                         inv_freq: torch.Tensor, interleaved: bool = False, scale: float = 1.0):
+    """q and k [..., heads, D] (fp32, bf16 or fp16; k may be None) turned by
+    the angles positions * inv_freq and multiplied by scale in the first
+    2 * len(inv_freq) elements of a head, the others copied; returns both.
+
+    Pairs are (i, i + rotary_dim / 2), or (2i, 2i + 1) if ``interleaved``.
+    positions int32/int64 in the tokens' shape, inv_freq fp32.
+    """
+    return _turned(q, k, positions, inv_freq, interleaved, scale, 0)
+
+
+def npu_rotary_embedding_bwd(dq: torch.Tensor, dk: Optional[torch.Tensor],
+                             positions: torch.Tensor, inv_freq: torch.Tensor,
+                             interleaved: bool = False, scale: float = 1.0):
+    """Gradients of npu_rotary_embedding's q and k from those of its outputs
+    (the same turn backwards)."""
+    return _turned(dq, dk, positions, inv_freq, interleaved, scale, 1)
+
+
+def _stride(x, d):
+    return x.stride(d) if x.size(d) > 1 else 0
+
+
+def _cache_check(k_cache, v_cache, x, Hkv, written):
+    """The two caches [pages, page, Hkv, D] and their xk dtype."""
+    for c, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+        if c.dim() != 4 or c.size(3) != x.size(-1) or c.size(1) == 0:
+            raise ValueError(f"{name} must be [pages, page, kv heads, head_dim]")
+        if Hkv is not None and c.size(2) != Hkv:
+            raise ValueError(f"{name} must have the kv heads of k and v")
+        if c.size(3) > 1 and c.stride(3) != 1:
+            raise ValueError(f"{name} must have contiguous rows")
+        if written and any(c.size(d) > 1 and c.stride(d) < c.size(3) for d in range(3)):
+            raise ValueError(f"{name}'s rows must not overlap")
+    if v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype:
+        raise ValueError("v_cache must have k_cache's shape and dtype")
+    _same_device(x, k_cache=k_cache, v_cache=v_cache)
+    if k_cache.dtype == x.dtype:
+        return xk_dtype(x)
+    if k_cache.dtype != torch.float8_e4m3fn or x.dtype == torch.float32:
+        raise ValueError("the cache must have the tokens' dtype, or float8_e4m3fn beside 16 bits")
+    return _lib.XK_F8E4M3
+
+
+def _kv_scales(k_scale, v_scale, x, Hkv, cache_dtype):
+    out = []
+    for s, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+        if s is not None:
+            if cache_dtype != _lib.XK_F8E4M3:
+                raise ValueError(f"{name} needs a float8_e4m3fn cache")
+            if s.dtype != torch.float32 or s.shape != (Hkv,):
+                raise ValueError(f"{name} must be float32 [kv heads]")
+            _same_device(x, **{name: s})
+            s = s.contiguous()
+        out.append(s)
+    return out
+
+
+def npu_rotary_cache_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
+                            k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor,
+                            positions: Optional[torch.Tensor] = None,
+                            inv_freq: Optional[torch.Tensor] = None, interleaved: bool = False,
+                            scale: float = 1.0, k_scale: Optional[torch.Tensor] = None,
+                            v_scale: Optional[torch.Tensor] = None):
+    """npu_rotary_embedding of q and k, with the turned k and v written to
+    ``slots`` (int32/int64, page * page_size + place; outside the cache: not
+    written) of the paged caches [pages, page, kv heads, D] in the same launch;
+    returns the turned q (None without q).
+
+    The caches have the tokens' dtype, or float8_e4m3fn holding x / scale of
+    the kv head (k_scale, v_scale fp32 [kv heads], None = 1).  Without
+    positions nothing is turned.  No two tokens may have the same slot.
+    """
+    _rotary_check(k, k, "k")
+    _rotary_check(v, k, "v")
+    Hkv, D = k.size(-2), k.size(-1)
+    if v.size(-2) != Hkv:
+        raise ValueError("v must have k's heads")
+    if Hkv == 0:
+        raise ValueError("k must have heads")
+    if q is not None:
+        _rotary_check(q, k, "q")
+    if slots.dtype not in (torch.int32, torch.int64) or slots.shape != k.shape[:-2]:
+        raise ValueError("slots must be int32 or int64, one for each token")
+    _same_device(k, slots=slots)
+    if (positions is None) != (inv_freq is None):
+        raise ValueError("positions and inv_freq go together")
+    rot = _positions(k, positions, inv_freq, scale) if positions is not None else 0
+    cdt = _cache_check(k_cache, v_cache, k, Hkv, True)
+    ks, vs = _kv_scales(k_scale, v_scale, k, Hkv, cdt)
+    stream = _stream(k)
+    Hq, T = q.size(-2) if q is not None else 0, slots.numel()
+    qr, qt, qh = _token_heads(q, "q") if q is not None else (None, 0, 0)
+    kr, kt, kh = _token_heads(k, "k")
+    vr, vt, vh = _token_heads(v, "v")
+    sl = slots.contiguous()
+    pos = positions.contiguous() if positions is not None else None
+    freq = inv_freq.contiguous() if inv_freq is not None else None
+    with torch.cuda.device(k.device):
+        qo = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q is not None else None
+        st = lib().xk_rotary_cache_append(
+            _ptr(qr), qt, qh, _ptr(qo), Hq * D, D, Hq, kr.data_ptr(), kt, kh, vr.data_ptr(), vt,
+            vh, Hkv, k_cache.data_ptr(), *(_stride(k_cache, d) for d in range(3)),
+            v_cache.data_ptr(), *(_stride(v_cache, d) for d in range(3)), cdt, k_cache.size(0),
+            k_cache.size(1), sl.data_ptr(), xk_dtype(sl), _ptr(pos),
+            xk_dtype(pos) if pos is not None else _lib.XK_I32, _ptr(freq), rot,
+            int(interleaved), float(scale), _ptr(ks), _ptr(vs), T, D, xk_dtype(k), stream)
+    check(st, "xk_rotary_cache_append")
+    return qo
+
+
+def npu_paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                        block_table: torch.Tensor, seq_lens: torch.Tensor,
+                        scale: Optional[float] = None, window: int = 0,
+                        k_scale: Optional[torch.Tensor] = None,
+                        v_scale: Optional[torch.Tensor] = None, output_lse: bool = False):
+    """softmax(scale q k^T) v of the last T tokens of every sequence over its
+    pages of the cache; returns (o shaped like q, lse fp32 [B, T, Hq] or None).
+
+    q [B, Hq, D] or [B, T, Hq, D]; token t of a sequence is at position
+    seq_lens - T + t and sees the positions up to its own (with ``window`` the
+    last so many); the new tokens' keys and values are in the cache already.
+    block_table int32 [B, pages of a sequence], seq_lens int32 [B], caches as
+    in npu_rotary_cache_append.  scale None: D ** -0.5.
+    """
+    if q.dim() not in (3, 4) or q.dtype not in _FLOATS:
+        raise ValueError("q must be [B, Hq, D] or [B, T, Hq, D] of float32, bfloat16 or float16")
+    q4 = q.unsqueeze(1) if q.dim() == 3 else q
+    B, T, Hq, D = q4.shape
+    if D == 0 or D > 256 or D % 8:
+        raise ValueError("head_dim must be a multiple of 8, at most 256")
+    cdt = _cache_check(k_cache, v_cache, q, None, False)
+    Hkv = k_cache.size(2)
+    if Hkv == 0 or Hq == 0 or Hq % Hkv:
+        raise ValueError("q's heads must be a multiple of the cache's")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.size(0) != B:
+        raise ValueError("block_table must be int32 [B, pages]")
+    if seq_lens.dtype != torch.int32 or seq_lens.shape != (B,):
+        raise ValueError("seq_lens must be int32 [B]")
+    if window < 0:
+        raise ValueError("window must not be negative")
+    scale = D ** -0.5 if scale is None else scale
+    if not abs(scale) <= torch.finfo(torch.float32).max:
+        raise ValueError("scale must be finite (in float32)")
+    _same_device(q, block_table=block_table, seq_lens=seq_lens)
+    ks, vs = _kv_scales(k_scale, v_scale, q, Hkv, cdt)
+    stream = _stream(q)
+    n = 16 // q.element_size()
+    if ((D > 1 and q4.stride(3) != 1) or any(_stride(q4, d) % n for d in range(3))
+            or q4.data_ptr() % 16):
+        q4 = q4.clone(memory_format=torch.contiguous_format)
+    table = block_table if block_table.size(1) <= 1 or block_table.stride(1) == 1 \
+        else block_table.contiguous()
+    lens = seq_lens.contiguous()
+    with torch.cuda.device(q.device):
+        o = torch.empty((B, T, Hq, D), dtype=q.dtype, device=q.device)
+        lse = _f32(q, B, T, Hq) if output_lse else None
+        if T > 0:
+            size = lib().xk_paged_attention_workspace_bytes(B, T, Hq, Hkv, D, table.size(1),
+                                                            k_cache.size(1), xk_dtype(q))
+            ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+            st = lib().xk_paged_attention(
+                q4.data_ptr(), *(_stride(q4, d) for d in range(3)), k_cache.data_ptr(),
+                *(_stride(k_cache, d) for d in range(3)), v_cache.data_ptr(),
+                *(_stride(v_cache, d) for d in range(3)), cdt, k_cache.size(0), k_cache.size(1),
+                table.data_ptr(), _stride(table, 0), table.size(1), lens.data_ptr(),
+                float(scale), window, _ptr(ks), _ptr(vs), o.data_ptr(), T * Hq * D, Hq * D, D,
+                _ptr(lse), B, T, Hq, Hkv, D, xk_dtype(q), _ptr(ws), size, stream)
+            check(st, "xk_paged_attention")
+    if q.dim() == 3:
+        return o[:, 0], lse[:, 0] if output_lse else None
+    return o, lse
