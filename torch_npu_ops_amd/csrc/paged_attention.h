@@ -11,24 +11,30 @@
 // small part of what the matrix cores do at that rate, so the rows of a
 // 16-row MFMA tile that are not used cost nothing.
 //
-// Work: the tiles of every sequence (32 positions of 16-bit rows, 16 of fp32)
-// are cut into parts of equal length on the device, from the lengths that are
-// there (seq_lens never reaches the host); a block of 4 waves takes one part
-// of one head.  Its waves take tiles in turn, each with statistics and sums of
-// its own, and join at the end; parts of one sequence are joined by a second
-// launch.
+// Work: the positions of all sequences, in tiles of 16 to 64, are one line
+// that the blocks of a head cut in equal shares, on the device, from the
+// lengths that are there (seq_lens never reaches the host); as many blocks as
+// the card runs at once.  A block goes through the sequences that its share
+// touches, its 4 waves taking tiles in turn, each with statistics and sums of
+// its own, and joins them at a sequence's end; the pieces of a sequence that
+// lies in several shares are joined by a second launch.
 //
-// Tile: no LDS and no barrier in the loop.  S^T = K Q^T and O^T = V^T P^T, so
-// that lane l holds query row l % 16 throughout (C layout: column l % 16,
-// rows 4 (l / 16) + i): statistics and rescaling stay in the lane, up to the
-// maximum over the four lane groups.  The order of a product's inner index is
-// free as long as both sides use the same:
-//   - the scores of tokens 4g + i and 16 + 4g + i that lane group g holds are
-//     the slots of group g in P^T, with V's tokens loaded to match;
-//   - V's rows are loaded as they lie (16 lanes read one row of 128 elements)
-//     and the lane's 8 tokens x 8 elements turned in registers (v_perm), one
-//     product for each of the 8 elements: product e has row l % 16 <->
-//     element 8 (l % 16) + e, so the sums come out as 8 neighbours.
+// Tile: S^T = K Q^T and O^T = V^T P^T, so that lane l holds query row l % 16
+// throughout (C layout: column l % 16, rows 4 (l / 16) + i): statistics and
+// rescaling stay in the lane, up to the maximum over the four lane groups.
+//   - Both K and V are loaded as they lie (16 lanes of 16 bytes read a row of
+//     128 elements): with a row for each lane instead, as K's operand needs it,
+//     a copy of the loads alone ran at 5.2 TB/s where whole rows ran at 6.7.
+//     K passes through the wave's own part of LDS into the operand's layout.
+//   - The order of a product's inner index is free as long as both sides use
+//     the same: the scores of tokens 4g + i and 16 + 4g + i that lane group g
+//     holds are the slots of group g in P^T, with V's tokens loaded to match,
+//     and the lane's 8 tokens x 8 elements of V are turned in registers
+//     (v_perm), one product for each of the 8 elements: product e has row
+//     l % 16 <-> element 8 (l % 16) + e, so sums come out as 8 neighbours.
+//   - The next tile's loads are requested as soon as this one's registers are
+//     free, and the loop has no condition on them: with one the compiler waits
+//     for the loads at the loop's end, to move their registers.
 // p is split in two 16-bit parts (hi + lo, 16 bits of mantissa and more) for
 // the product with V; fp16's is scaled by 2^14 so that small weights keep
 // their digits.  Scores, statistics and sums are fp32.
@@ -51,16 +57,19 @@ struct f8 {  // e4m3, as stored
 
 constexpr int kWaves = 4;
 constexpr int kBlock = kWaves * kWave;
-constexpr int kMinChunk = kWaves;  // tiles of a part, at the least
 
 struct Params {
   const void* q;
   int64_t q_seq, q_tok, q_head;  // elements
   const char* kc;
-  int64_t k_page, k_slot, k_head;  // bytes
+  int64_t k_page, k_head;  // bytes
+  uint32_t k_slot;
   const char* vc;
-  int64_t v_page, v_slot, v_head;
-  int num_pages, page_size, page_shift;  // shift: -1 where no power of two
+  int64_t v_page, v_head;
+  uint32_t v_slot;
+  int num_pages, page_size;
+  uint32_t page_magic;  // n / page_size = n * magic >> shift for n < 2^28
+  int page_shift;
   const int32_t* table;
   int64_t table_row;
   int max_pages;
@@ -74,15 +83,14 @@ struct Params {
   int64_t o_seq, o_tok, o_head;
   float* lse;
   int B, T, G, Hkv, D, M, groups;  // M = T * G rows of a head in `groups` groups
-  int want;                        // parts wanted in all, beyond one a sequence
-  int slots;                       // parts that the workspace holds
-  bool alone;                      // no sequence can have two parts
-  int2* meta;                      // [B]: first part, parts
-  float2* ml;                      // [slots][Hkv][M]: base, sum
-  float* acc;                      // [slots][Hkv][M][D]
+  int shares;                      // of a head and group, at the most
+  int2* meta;                      // [B]: first piece, pieces
+  float2* ml;                      // [2 * shares][Hkv][M]: base, sum
+  float* acc;                      // [2 * shares][Hkv][M][D]
 };
 
-// A sequence's tiles: from the first that a row sees to the last.
+// A sequence's tiles: from the first that a row sees to the last; an empty
+// sequence has one, so that its rows are written.
 struct Span {
   int len, t0, n;
 };
@@ -91,48 +99,30 @@ __device__ __forceinline__ Span span_of(const Params& p, int b) {
   const int len = max(0, min(p.lens[b], p.most_len));
   const int lo = p.window ? max(0, len - p.T - p.window + 1) : 0;
   const int t0 = lo / TS, t1 = (len + TS - 1) / TS;
-  return {len, t0, max(0, t1 - t0)};
+  return {len, t0, max(1, t1 - t0)};
 }
 
-struct Part {
-  int b;        // -1: none
-  int index, of;  // the part's number in its sequence, and how many there are
-  Span span;
+// 64 sequences from b0 on, one a lane; `incl`: their tiles up to the lane's.
+struct Batch {
+  int b0;
+  Span own;
+  int incl;
 };
-
-// Part `slot` of the batch, found by every wave from the lengths: the chunk is
-// what gives about p.want parts, never below kMinChunk tiles, in whole rounds
-// of the block's waves.  At most p.want + B parts, since a sequence has at
-// least one (an empty one, whose rows are written as zeros).
 template <int TS>
-__device__ __forceinline__ Part locate(const Params& p, int slot) {
-  const int lane = threadIdx.x % kWave;
-  int64_t total = 0;
-  Span own{0, 0, 0};
-  for (int b0 = 0; b0 < p.B; b0 += kWave) {
-    own = b0 + lane < p.B ? span_of<TS>(p, b0 + lane) : Span{0, 0, 0};
-    total += __builtin_amdgcn_readlane(gdn::wave_incl_scan(own.n), kWave - 1);
-  }
-  int64_t c = (total + p.want - 1) / p.want;
-  c = (c + kWaves - 1) / kWaves * kWaves;
-  const int chunk = static_cast<int>(max<int64_t>(kMinChunk, min<int64_t>(c, 1 << 30)));
-  int first = 0;
-  for (int b0 = 0; b0 < p.B; b0 += kWave) {
-    if (p.B > kWave) own = b0 + lane < p.B ? span_of<TS>(p, b0 + lane) : Span{0, 0, 0};
-    const int parts = b0 + lane < p.B ? max(1, (own.n + chunk - 1) / chunk) : 0;
-    const int incl = gdn::wave_incl_scan(parts);
-    const int all = __builtin_amdgcn_readlane(incl, kWave - 1);
-    if (slot < first + all) {
-      const int k = __popcll(__ballot(first + incl <= slot));
-      const int of = __builtin_amdgcn_readlane(parts, k);
-      const int begin = first + __builtin_amdgcn_readlane(incl, k) - of;
-      return {b0 + k, slot - begin, of,
-              {__builtin_amdgcn_readlane(own.len, k), __builtin_amdgcn_readlane(own.t0, k),
-               __builtin_amdgcn_readlane(own.n, k)}};
-    }
-    first += all;
-  }
-  return {-1, 0, 0, {0, 0, 0}};
+__device__ __forceinline__ Batch batch_at(const Params& p, int b0) {
+  const int b = b0 + static_cast<int>(threadIdx.x % kWave);
+  const Span own = b < p.B ? span_of<TS>(p, b) : Span{0, 0, 0};
+  return {b0, own, gdn::wave_incl_scan(own.n)};
+}
+
+// (64-bit division takes 150 instructions.)
+__device__ __forceinline__ int64_t divide(int64_t a, uint32_t b) {
+  return a <= UINT32_MAX ? static_cast<uint32_t>(a) / b : a / b;
+}
+// Tiles of a share: whole rounds of the block's waves.
+__device__ __forceinline__ uint32_t share_size(int64_t total, int shares) {
+  const int64_t n = divide(total + shares - 1, shares);
+  return static_cast<uint32_t>((n + kWaves - 1) / kWaves * kWaves);
 }
 
 // ---------------------------------------------------------------------------
@@ -172,7 +162,7 @@ __device__ __forceinline__ uint32_t widen(uint32_t w, bool high) {
 
 // N elements of the cache as loaded, and as words of T.
 template <typename T, typename C, int N>
-struct Row {
+struct alignas(N * sizeof(C) < 16 ? N * sizeof(C) : 16) Row {
   static constexpr int kBytes = N * static_cast<int>(sizeof(C));
   static constexpr int kRaw = kBytes / 4, kWords = N * static_cast<int>(sizeof(T)) / 4;
   uint32_t raw[kRaw];
@@ -186,7 +176,7 @@ struct Row {
       for (int i = 0; i < kRaw; ++i) raw[i] = x[i];
     }
   }
-  __device__ __forceinline__ void keep(bool yes) {
+  __device__ __forceinline__ void keep(bool yes) {  // or zeros
 #pragma unroll
     for (int i = 0; i < kRaw; ++i) raw[i] = yes ? raw[i] : 0;
   }
@@ -195,20 +185,32 @@ struct Row {
     else return raw[i];
   }
   __device__ __forceinline__ bool finite() const {
-    bool ok = true;
+    uint32_t bad = 0;
 #pragma unroll
     for (int i = 0; i < kWords; ++i) {
       const uint32_t w = word(i);
       if constexpr (sizeof(T) == 4) {
-        ok = ok && (w & 0x7f800000u) != 0x7f800000u;
+        bad |= (w & 0x7f800000u) == 0x7f800000u;
       } else {
         constexpr uint32_t kExp = std::is_same<T, bf16>::value ? 0x7f80u : 0x7c00u;
-        ok = ok && (w & kExp) != kExp && (w >> 16 & kExp) != kExp;
+        bad |= ((w & kExp) == kExp) | ((w >> 16 & kExp) == kExp);
       }
     }
-    return ok;
+    return bad == 0;
   }
 };
+template <typename C>
+__device__ __forceinline__ bool not_finite(C x) {
+  if constexpr (std::is_same<C, f8>::value) return (x.v & 0x7f) == 0x7f;
+  else return !__builtin_isfinite(to_f32(x));
+}
+
+// The wave's lanes see what its others wrote to LDS before.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
 
 // The larger of the values of lanes that differ in bits 4 and 5, and the sum.
 template <typename F>
@@ -224,6 +226,16 @@ __device__ __forceinline__ float over_groups(float v, F f) {
   return f(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y));
 }
 
+// A wave-uniform pointer in scalar registers, to which loads add a lane's 32-bit
+// offset: left to itself the compiler adds offsets first and keeps 64 bits for
+// each lane and load.
+__device__ __forceinline__ const char* scalar(const char* x) {
+  const uint64_t u = reinterpret_cast<uint64_t>(x);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(u));
+  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(u >> 32));
+  return reinterpret_cast<const char*>(static_cast<uint64_t>(hi) << 32 | lo);
+}
+
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // exp2(a - b) for a <= b, 0 where a is -inf (b then may be -inf too).
@@ -231,436 +243,588 @@ __device__ __forceinline__ float weight(float a, float b) {
   return exp2_hw(a - (b == -INFINITY ? 0.f : b));
 }
 
+// Two values in 16 bits and what that leaves, also in 16 bits.  fp16's are cut,
+// not rounded: the second part holds the rest either way (22 bits of both).
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo, bf16) {
+  gdn::bf2_t h, l;
+  gdn::split2(a, b, h, l);
+  hi = __builtin_bit_cast(uint32_t, h);
+  lo = __builtin_bit_cast(uint32_t, l);
+}
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo, f16) {
+  const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
+  const auto l = __builtin_amdgcn_cvt_pkrtz(a - static_cast<float>(h[0]),
+                                            b - static_cast<float>(h[1]));
+  hi = __builtin_bit_cast(uint32_t, h);
+  lo = __builtin_bit_cast(uint32_t, l);
+}
+
+// Writes 4 elements of a finished row, and its lse.
+template <typename T>
+__device__ __forceinline__ void write_row(const Params& p, int b, int head, int r, int d,
+                                          f4_t x, float base, float l) {
+  const int tok = r / p.G;
+  const int64_t hq = static_cast<int64_t>(head) * p.G + (r - tok * p.G);
+  // A row that sees nothing has no weights: 0.
+  const float inv = l == 0.f ? 0.f : (p.v_scale ? p.v_scale[head] : 1.f) / l;
+  float o[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = l == 0.f ? 0.f : x[i] * inv;
+  store_vec_f32<T, 4>(static_cast<T*>(p.out) + b * p.o_seq + tok * p.o_tok + hq * p.o_head + d,
+                      o);
+  if (p.lse && d == 0)
+    p.lse[(static_cast<int64_t>(b) * p.T + tok) * p.Hkv * p.G + hq] =
+        l == 0.f ? -INFINITY : (base + __log2f(l)) * 0.69314718056f;
+}
+
 // ---------------------------------------------------------------------------
 // The kernel.  DP: the head's length, rounded up to 64, 128 or 256.  R: row
 // tiles of a wave.  P16: pages are whole runs of 16 positions, so that a half
 // tile lies in one page and its address is one scalar.
 // ---------------------------------------------------------------------------
+// Tiles hold 8 KB of keys where rows are short: fewer rounds of statistics.
+template <typename T, typename C, int DP>
+constexpr int subs_of() {  // products with V of a tile
+  return DP * static_cast<int>(sizeof(C)) * (64 / static_cast<int>(sizeof(T))) <= 4096 ? 2 : 1;
+}
+// Waves of a SIMD: two where the sums and a tile's keys and values take at most
+// half of 256 registers (a third of that is needed beside them).
+template <typename T, typename C, int DP, int R>
+constexpr int waves_of() {
+  constexpr int kTile = DP * static_cast<int>(sizeof(C)) * subs_of<T, C, DP>() * 64 /
+                        static_cast<int>(sizeof(T)) / 256;
+  return DP * R / 4 + 2 * kTile > 128 ? 1 : 2;
+}
+
 template <typename T, typename C, int DP, int R, bool P16>
-__global__ void __launch_bounds__(kBlock, 2) attention_kernel(Params p) {
+__global__ void __launch_bounds__(kBlock, (waves_of<T, C, DP, R>())) attention_kernel(Params p) {
   using OpT = typename Op<T>::type;
-  constexpr int KV = 16 / sizeof(T);       // values of an operand in a lane
-  constexpr int TS = 4 * KV, NH = TS / 16;  // positions of a tile, halves
-  constexpr int NK = DP / (4 * KV);        // products over a head
+  constexpr int CB = sizeof(C);
+  constexpr int KV = 16 / sizeof(T);  // values of an operand in a lane
+  constexpr int SUB = 4 * KV;         // positions of one product with V
+  constexpr int NS = subs_of<T, C, DP>(), TS = SUB * NS, NH = TS / 16;
+  constexpr int NK = DP / SUB;  // products over a head
+  constexpr int CH = DP / KV;   // K: chunks of a row, a lane each
+  constexpr int RPI = kWave / CH, NL = TS / RPI;   // rows of a load, loads of a tile
+  constexpr int KO = RPI < 16 ? 16 / RPI : 1;      // loads of a half tile
   constexpr int VB = KV < DP / 16 ? KV : DP / 16;  // V: elements of a load
   constexpr int NB = DP / (16 * VB);               // and loads of a row
-  constexpr int CB = sizeof(C);
+  constexpr int NX = KV * NS;                      // scores of a lane and row tile
+  constexpr uint64_t kAll = TS == 64 ? ~uint64_t{0} : (uint64_t{1} << TS) - 1;
   // log2 of what p is scaled by (see above).
   constexpr float kShift = std::is_same<T, f16>::value ? 14.f : 0.f;
+  using KRow = Row<T, C, KV>;
+  using VRow = Row<T, C, VB>;
+
+  constexpr int kPitch = DP + 4;  // rows of the join 4 banks apart
+  union Shared {
+    KRow k[kWaves][TS * CH];
+    float acc[kWaves][16][kPitch];
+  };
+  __shared__ __align__(16) Shared sh;
+  __shared__ __align__(16) OpT sq[R][NK][kWave];  // Q, as the operands take it
+  __shared__ float2 ml[kWaves][16];
+  __shared__ uint16_t poison[kWaves][R][DP];  // a bit for each row of a tile
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lane = threadIdx.x % kWave, l15 = lane % 16, g = lane / 16;
   uint32_t id = blockIdx.x;
   const int head = id % p.Hkv;
   id /= p.Hkv;
-  const int group = id % p.groups, slot = id / p.groups;
-  const Part part = locate<TS>(p, slot);
-  if (part.b < 0) return;  // whole block
-  if (!p.alone && part.index == 0 && head == 0 && group == 0 && threadIdx.x == 0)
-    p.meta[part.b] = make_int2(slot, part.of);
+  const int group = id % p.groups, share = id / p.groups;
 
-  // Rows: token r / G of the sequence's new ones, at position len - T + token.
-  const int r0 = group * 16 * R, len = part.span.len;
-  const int first_tok = r0 / p.G, last_tok = min(p.M - 1, r0 + 16 * R - 1) / p.G;
-  const int first_pos = len - p.T + first_tok, last_pos = len - p.T + last_tok;
-  const int low_first = p.window ? max(0, first_pos - p.window + 1) : 0;
-  const int low_last = p.window ? max(0, last_pos - p.window + 1) : 0;
-  int hi[R], lo[R];
-  OpT q[R][NK];
-#pragma unroll
-  for (int j = 0; j < R; ++j) {
-    const int r = r0 + 16 * j + l15, tok = r / p.G;
-    hi[j] = r < p.M ? len - p.T + tok : -1;
-    lo[j] = p.window ? hi[j] - p.window + 1 : 0;
-    const T* src = static_cast<const T*>(p.q) + part.b * p.q_seq + tok * p.q_tok +
-                   (static_cast<int64_t>(head) * p.G + (r - tok * p.G)) * p.q_head;
-#pragma unroll
-    for (int s = 0; s < NK; ++s) {
-      const int d = (4 * s + g) * KV;
-      OpT x = {};
-      if (r < p.M && d < p.D) x = *reinterpret_cast<const OpT*>(src + d);
-      q[j][s] = x;
-    }
-  }
+  // The block's share of the line, and the sequence that it begins in.
+  Batch bt = batch_at<TS>(p, 0);
+  int64_t total = __builtin_amdgcn_readlane(bt.incl, kWave - 1);
+  for (int b0 = kWave; b0 < p.B; b0 += kWave)
+    total += __builtin_amdgcn_readlane(batch_at<TS>(p, b0).incl, kWave - 1);
+  const uint32_t size = share_size(total, p.shares);
+  const int64_t g0 = static_cast<int64_t>(share) * size, g1 = min<int64_t>(total, g0 + size);
+  if (g0 >= total) return;  // whole block
+  int64_t at = 0;  // where sequence b begins
+  for (int n; at + (n = __builtin_amdgcn_readlane(bt.incl, kWave - 1)) <= g0; at += n)
+    bt = batch_at<TS>(p, bt.b0 + kWave);
+  int b = __popcll(__ballot(at + bt.incl <= g0));
+  at += __builtin_amdgcn_readlane(bt.incl - bt.own.n, b);
+  b += bt.b0;
 
-  // The part's tiles, without those that no row of the group sees.
-  const int each = (part.span.n + part.of - 1) / part.of;
-  int begin = part.span.t0 + part.index * each;
-  int end = min(part.span.t0 + part.span.n, begin + each);
-  begin = max(begin, low_first / TS);
-  end = min(end, last_pos < 0 ? 0 : last_pos / TS + 1);
-
-  float scale2 = p.scale2;
-  if (p.k_scale) scale2 *= p.k_scale[head];
-  const char* const kc = p.kc + head * p.k_head;
-  const char* const vc = p.vc + head * p.v_head;
-  const int32_t* const table = p.table + part.b * p.table_row;
-  const bool ragged = p.D < DP;
-  // Lane offsets inside a row; beyond the head the row's last vector again.
-  uint32_t kd[NK], vd[NB];
+  // What holds for every sequence: lane offsets from the start of a half tile;
+  // beyond the head the row's last vector again.
+  const int chunk = lane % CH, krow = lane / CH;
+  const bool k_in = chunk * KV < p.D;
+  uint32_t k_off[KO], v_off[4][NB];
 #pragma unroll
-  for (int s = 0; s < NK; ++s) kd[s] = min((4 * s + g) * KV, p.D - KV) * CB;
+  for (int i = 0; i < KO; ++i)
+    k_off[i] = (i * RPI + krow) * p.k_slot + min(chunk * KV, p.D - KV) * CB;
 #pragma unroll
-  for (int n = 0; n < NB; ++n) vd[n] = min((n * 16 + l15) * VB, p.D - VB) * CB;
-  const uint32_t k_lane = l15 * static_cast<uint32_t>(p.k_slot);
-  const uint32_t v_lane = 4 * g * static_cast<uint32_t>(p.v_slot);
-
-  Row<T, C, KV> k[NH][NK];
-  Row<T, C, VB> v[KV][NB];
-  f4_t acc[R][NB][VB] = {};
-  float base[R], sum[R];
-#pragma unroll
-  for (int j = 0; j < R; ++j) {
-    base[j] = -INFINITY;
-    sum[j] = 0.f;
-  }
-
-  auto page_of = [&](int pos) { return p.page_shift >= 0 ? pos >> p.page_shift : pos / p.page_size; };
-  // The table's entries of a tile (P16: one for each half; else the lane's
-  // position's), -1 where there is no position.
-  int entry[P16 ? NH : 1];
-  auto look_up = [&](int tile) {
-    if constexpr (P16) {
-#pragma unroll
-      for (int h = 0; h < NH; ++h) {
-        const int pos = tile * TS + 16 * h;
-        entry[h] = tile < end && pos < len ? table[page_of(pos)] : -1;
-      }
-    } else {
-      const int pos = tile * TS + lane % TS;
-      entry[0] = tile < end && pos < len ? table[page_of(pos)] : -1;
-    }
-  };
-  // Where a tile's rows are, and which of its positions there are (a bit
-  // each).  Rows that are not there are read from the first page.
-  const char *kh[NH], *vh[NH];
-  int64_t ko = 0, vo = 0;
-  auto place = [&](int tile) -> uint32_t {
-    if constexpr (P16) {
-      uint32_t ok = 0;
-#pragma unroll
-      for (int h = 0; h < NH; ++h) {
-        const int pos = tile * TS + 16 * h;
-        const int e = __builtin_amdgcn_readfirstlane(entry[h]);
-        const bool in = static_cast<uint32_t>(e) < static_cast<uint32_t>(p.num_pages);
-        const int at = in ? pos - page_of(pos) * p.page_size : 0;
-        const int64_t page = in ? e : 0;
-        kh[h] = kc + page * p.k_page + at * p.k_slot;
-        vh[h] = vc + page * p.v_page + at * p.v_slot;
-        if (in) ok |= 0xffffu << (16 * h);
-      }
-      return ok;
-    } else {
-      const int pos = tile * TS + lane % TS;
-      const bool in = static_cast<uint32_t>(entry[0]) < static_cast<uint32_t>(p.num_pages);
-      const int at = in ? pos - page_of(pos) * p.page_size : 0;
-      const int64_t page = in ? entry[0] : 0;
-      ko = page * p.k_page + at * p.k_slot;
-      vo = page * p.v_page + at * p.v_slot;
-      return static_cast<uint32_t>(__ballot(in)) & static_cast<uint32_t>((uint64_t{1} << TS) - 1);
-    }
-  };
-  auto load_k = [&]() {
-#pragma unroll
-    for (int h = 0; h < NH; ++h) {
-      int64_t off = 0;
-      if constexpr (!P16) off = __shfl(ko, 16 * h + l15);
-#pragma unroll
-      for (int s = 0; s < NK; ++s) {
-        if constexpr (P16) k[h][s].load(kh[h] + (k_lane + kd[s]));
-        else k[h][s].load(kc + off + kd[s]);
-      }
-    }
-  };
-  auto load_v = [&]() {
-#pragma unroll
-    for (int i = 0; i < KV; ++i) {
-      int64_t off = 0;
-      if constexpr (!P16) off = __shfl(vo, 16 * (i / 4) + 4 * g + i % 4);
-#pragma unroll
-      for (int n = 0; n < NB; ++n) {
-        if constexpr (P16) v[i][n].load(vh[i / 4] + (i % 4) * p.v_slot + (v_lane + vd[n]));
-        else v[i][n].load(vc + off + vd[n]);
-      }
-    }
-  };
-  // acc[j] += V^T P^T[j], for the rows that `take` names, without the values
-  // that `cut` takes out of word i of an operand.
-  auto add_values = [&](const OpT (&ph)[R], const OpT (&pl)[R], auto cut, auto take) {
+  for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int n = 0; n < NB; ++n)
+      v_off[i][n] = (4 * g + i) * p.v_slot + min((n * 16 + l15) * VB, p.D - VB) * CB;
+  const char* const kc = p.kc + head * p.k_head;
+  const char* const vc = p.vc + head * p.v_head;
+  // Scores are scaled by something positive, that leaves a masked one -inf: a
+  // sign goes to Q, and 1.2e-38 for 0 makes every finite score 0 too.
+  float scale2 = p.scale2;
+  if (p.k_scale) scale2 *= p.k_scale[head];
+  const bool negate = scale2 < 0.f;
+  scale2 = fmaxf(fabsf(scale2), 1.17549435e-38f);
+  const int r0 = group * 16 * R;
+  const int first_tok = r0 / p.G, last_tok = min(p.M - 1, r0 + 16 * R - 1) / p.G;
+  int tok[R];  // of the lane's rows; beyond them, one that sees nothing
 #pragma unroll
-      for (int e = 0; e < VB; ++e) {
-        u32x4 w;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if constexpr (sizeof(T) == 4)
-            w[i] = v[i][n].word(e);
-          else
-            w[i] = __builtin_amdgcn_perm(v[2 * i + 1][n].word(e / 2), v[2 * i][n].word(e / 2),
-                                         e & 1 ? 0x07060302u : 0x05040100u);
-          w[i] = cut(i, w[i]);
-        }
-        const OpT a = __builtin_bit_cast(OpT, w);
-#pragma unroll
-        for (int j = 0; j < R; ++j) {
-          f4_t x = mma(a, ph[j], acc[j][n][e]);
-          if constexpr (sizeof(T) == 2) x = mma(a, pl[j], x);
-          acc[j][n][e] = take(j) ? x : acc[j][n][e];
-        }
-      }
-  };
-  const auto nothing = [](int, uint32_t w) { return w; };
-  const auto all_rows = [](int) { return true; };
-
-  int tile = begin + wave;
-  look_up(tile);
-  uint32_t ok = place(tile);
-  if (tile < end) {
-    load_k();
-    load_v();
+  for (int j = 0; j < R; ++j) {
+    const int r = r0 + 16 * j + l15;
+    tok[j] = r < p.M ? r / p.G : -(1 << 30);
   }
-  look_up(tile + kWaves);
-  while (tile < end) {
-    const int pos0 = tile * TS;
-    const bool whole = pos0 >= low_last && pos0 + TS - 1 <= first_pos && ok == ((uint64_t{1} << TS) - 1);
-    if (ragged) {
-#pragma unroll
-      for (int s = 0; s < NK; ++s)
-#pragma unroll
-        for (int h = 0; h < NH; ++h) k[h][s].keep((4 * s + g) * KV < p.D);
-    }
-    f4_t sc[R][NH] = {};
-#pragma unroll
-    for (int h = 0; h < NH; ++h)
-#pragma unroll
-      for (int s = 0; s < NK; ++s) {
-        u32x4 w;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = k[h][s].word(i);
-#pragma unroll
-        for (int j = 0; j < R; ++j) sc[j][h] = mma(__builtin_bit_cast(OpT, w), q[j][s], sc[j][h]);
-      }
-    const int next = tile + kWaves;
-    const uint32_t ok_next = place(next);
-    if (next < end) load_k();
-    look_up(next + kWaves);
+  // K's chunks lie in the wave's part of LDS with a row's chunks permuted, so
+  // that the 16 rows of one operand's read fall on different banks.
+  KRow* const kt = sh.k[wave];
+  auto k_place = [&](int row, int c) {
+    return row * CH + (c ^ (CH == 8 ? row / 2 % 8 : row % 16));
+  };
+  auto page_of = [&](int pos) {
+    return static_cast<int>(static_cast<uint64_t>(pos) * p.page_magic >> p.page_shift);
+  };
 
-    OpT ph[R], pl[R];
+  for (;;) {
+    Span span;
+    span.len = __builtin_amdgcn_readlane(bt.own.len, b - bt.b0);
+    span.t0 = __builtin_amdgcn_readlane(bt.own.t0, b - bt.b0);
+    span.n = __builtin_amdgcn_readlane(bt.own.n, b - bt.b0);
+    const int len = span.len;
+    // The block's piece of the sequence; the first of a share and the last
+    // have places of their own where they are not all of it.
+    const int64_t from_g = max<int64_t>(g0, at), to_g = min<int64_t>(g1, at + span.n);
+    const bool all = to_g - from_g == span.n;
+    const int slot = 2 * share + (from_g > g0);
+    if (from_g == at && head == 0 && group == 0 && threadIdx.x == 0) {
+      const int last = static_cast<int>(divide(at + span.n - 1, size));
+      p.meta[b] = make_int2(slot, last - share + 1);
+    }
+
+    // Rows: token r / G of the sequence's new ones, at position len - T + token.
+    const int pos_0 = len - p.T;
+    const int first_pos = pos_0 + first_tok, last_pos = pos_0 + last_tok;
+    const int low_first = p.window ? max(0, first_pos - p.window + 1) : 0;
+    const int low_last = p.window ? max(0, last_pos - p.window + 1) : 0;
+    for (int u = wave; u < R * NK; u += kWaves) {
+      const int j = u / NK, s = u % NK, r = r0 + 16 * j + l15, t = r / p.G;
+      const int d = (4 * s + g) * KV;
+      u32x4 x = {};
+      if (r < p.M && d < p.D)
+        x = *reinterpret_cast<const u32x4*>(
+            static_cast<const T*>(p.q) + b * p.q_seq + t * p.q_tok +
+            (static_cast<int64_t>(head) * p.G + (r - t * p.G)) * p.q_head + d);
+      if (negate) x ^= sizeof(T) == 4 ? 0x80000000u : 0x80008000u;
+      sq[j][s][lane] = __builtin_bit_cast(OpT, x);
+    }
+
+    // The piece's tiles, without those that no row of the group sees.
+    int begin = span.t0 + static_cast<int>(from_g - at);
+    int end = span.t0 + static_cast<int>(to_g - at);
+    begin = max(begin, low_first / TS);
+    end = min(end, last_pos < 0 ? 0 : last_pos / TS + 1);
+    const int32_t* const table = p.table + b * p.table_row;
+
+    KRow k[NL];
+    VRow v[NX][NB];
+    f4_t acc[R][NB][VB] = {};
+    float base[R], sum[R];
 #pragma unroll
     for (int j = 0; j < R; ++j) {
-      float x[KV], top = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < KV; ++i) {
-        x[i] = sc[j][i / 4][i % 4] * scale2;
-        if (!whole) {
-          const int t = 16 * (i / 4) + 4 * g + i % 4, pos = pos0 + t;
-          x[i] = pos <= hi[j] && pos >= lo[j] && (ok >> t & 1) ? x[i] : -INFINITY;
-        }
-        top = fmaxf(top, x[i]);
-      }
-      top = over_groups(top, [](float a, float b) { return fmaxf(a, b); });
-      const float now = fmaxf(base[j], top - kShift);
-      const float from = now == -INFINITY ? 0.f : now;
-      const float keep = exp2_hw(base[j] - from);
-      base[j] = now;
-      float add = 0.f;
-#pragma unroll
-      for (int i = 0; i < KV; ++i) {
-        x[i] = exp2_hw(x[i] - from);
-        add += x[i];
-      }
-      sum[j] = sum[j] * keep + add;
-#pragma unroll
-      for (int i = 0; i < KV; ++i) {
-        if constexpr (sizeof(T) == 4) {
-          ph[j][i] = x[i];
-        } else {
-          const T h = static_cast<T>(x[i]);
-          ph[j][i] = h;
-          pl[j][i] = static_cast<T>(x[i] - static_cast<float>(h));
-        }
-      }
-#pragma unroll
-      for (int n = 0; n < NB; ++n)
-#pragma unroll
-        for (int e = 0; e < VB; ++e) acc[j][n][e] *= keep;
+      base[j] = -INFINITY;
+      sum[j] = 0.f;
     }
-    if (whole) {
-      add_values(ph, pl, nothing, all_rows);
-    } else {
-      // Values at positions that no row sees are no part of the sums, whatever
-      // they are; those that some new tokens see and others do not are taken
-      // for each token apart where one is not finite (0 * inf is NaN).
-      bool fine = true;
+
+    // The table's entries of a tile (P16: one for each half; else the lane's
+    // position's), -1 where there is no position.
+    int entry[P16 ? NH : 1];
+    auto look_up = [&](int tile) {
 #pragma unroll
-      for (int i = 0; i < KV; ++i) {
-        const int t = 16 * (i / 4) + 4 * g + i % 4, pos = pos0 + t;
-        const bool in = pos <= last_pos && pos >= low_first && (ok >> t & 1);
+      for (int h = 0; h < (P16 ? NH : 1); ++h) {
+        const int pos = tile * TS + (P16 ? 16 * h : lane % TS);
+        const bool in = tile < end && pos < len;
+        const int e = table[in ? page_of(pos) : 0];
+        entry[h] = in ? e : -1;
+      }
+    };
+    // Where a tile's rows are, and which of its positions there are (a bit
+    // each).  Rows that are not there are read from the first page.
+    const char *kh[NH], *vh[NH];
+    int64_t ko = 0, vo = 0;
+    auto place = [&](int tile) -> uint64_t {
+      if constexpr (P16) {
+        uint64_t ok = 0;
+#pragma unroll
+        for (int h = 0; h < NH; ++h) {
+          const int pos = tile * TS + 16 * h;
+          const int e = __builtin_amdgcn_readfirstlane(entry[h]);
+          const bool in = static_cast<uint32_t>(e) < static_cast<uint32_t>(p.num_pages);
+          const uint32_t at_row = in ? pos - page_of(pos) * p.page_size : 0;
+          const int64_t page = in ? e : 0;
+          kh[h] = scalar(kc + (page * p.k_page + static_cast<int64_t>(at_row) * p.k_slot));
+          vh[h] = scalar(vc + (page * p.v_page + static_cast<int64_t>(at_row) * p.v_slot));
+          ok |= in ? uint64_t{0xffff} << (16 * h) : 0;
+        }
+        return ok;
+      } else {
+        const int pos = tile * TS + lane % TS;
+        const bool in = static_cast<uint32_t>(entry[0]) < static_cast<uint32_t>(p.num_pages);
+        const uint32_t at_row = in ? pos - page_of(pos) * p.page_size : 0;
+        const int64_t page = in ? entry[0] : 0;
+        ko = page * p.k_page + static_cast<int64_t>(at_row) * p.k_slot;
+        vo = page * p.v_page + static_cast<int64_t>(at_row) * p.v_slot;
+        return __ballot(in) & kAll;
+      }
+    };
+    auto load_k = [&]() {
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        if constexpr (P16)
+          k[i].load(kh[i * RPI / 16] + k_off[i % KO]);
+        else
+          k[i].load(kc + __shfl(ko, i * RPI + krow) + (k_off[0] - krow * p.k_slot));
+      }
+    };
+    auto load_v = [&]() {
+#pragma unroll
+      for (int i = 0; i < NX; ++i) {
+        int64_t off = 0;
+        if constexpr (!P16) off = __shfl(vo, 16 * (i / 4) + 4 * g + i % 4);
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
-          v[i][n].keep(in);
-          fine = fine && v[i][n].finite();
+          if constexpr (P16) v[i][n].load(vh[i / 4] + v_off[i % 4][n]);
+          else v[i][n].load(vc + off + (v_off[0][n] - 4 * g * p.v_slot));
         }
       }
-      if (first_tok == last_tok || __all(fine)) {
-        add_values(ph, pl, nothing, all_rows);
-      } else {
-        for (int pos_t = first_pos; pos_t <= last_pos; ++pos_t) {
-          const auto seen = [&](int i) {
-            const int pos = pos0 + 16 * (i / 4) + 4 * g + i % 4;
-            return pos <= pos_t && (!p.window || pos > pos_t - p.window);
-          };
-          add_values(
-              ph, pl,
-              [&](int i, uint32_t w) {
-                if constexpr (sizeof(T) == 4) return seen(i) ? w : 0;
-                else return w & ((seen(2 * i) ? 0xffffu : 0) | (seen(2 * i + 1) ? 0xffff0000u : 0));
-              },
-              [&](int j) { return hi[j] == pos_t; });
-        }
-      }
-    }
-    if (next < end) load_v();
-    ok = ok_next;
-    tile = next;
-  }
+    };
 
-  // The block's waves join: a row's base is the largest, sums are scaled to it.
-  constexpr int kPitch = DP + 4;  // rows 4 banks apart
-  __shared__ float2 ml[kWaves][16];
-  __shared__ __align__(16) float part_acc[kWaves][16][kPitch];
-  const float v_scale = p.v_scale ? p.v_scale[head] : 1.f;
-  for (int j = 0; j < R; ++j) {
-    const int rows = min(16, p.M - r0 - 16 * j);
-    if (rows <= 0) break;
-    // (a select, so that the arrays stay in registers)
-    float my_base = base[0], my_sum = sum[0];
-#pragma unroll
-    for (int i = 1; i < R; ++i) {
-      my_base = j == i ? base[i] : my_base;
-      my_sum = j == i ? sum[i] : my_sum;
+    __syncthreads();  // Q
+    int tile = begin + wave;
+    uint64_t ok = 0;
+    if (tile < end) {
+      look_up(tile);
+      ok = place(tile);
+      load_k();
+      load_v();
+      look_up(tile + kWaves);
     }
-    my_sum = over_groups(my_sum, [](float a, float b) { return a + b; });
-    if (j) __syncthreads();
-    if (g == 0) ml[wave][l15] = make_float2(my_base, my_sum);
-    __syncthreads();
-    float top = ml[0][l15].x;
+    while (tile < end) {
+      const int pos0 = tile * TS;
+      const bool whole = pos0 >= low_last && pos0 + TS - 1 <= first_pos && ok == kAll;
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) top = fmaxf(top, ml[w][l15].x);
-    const float mine = weight(my_base, top);
-    if (l15 < rows) {
+      for (int i = 0; i < NL; ++i) {
+        if (p.D < DP) k[i].keep(k_in);
+        kt[k_place(i * RPI + krow, chunk)] = k[i];
+      }
+      const uint64_t ok_next = place(tile + kWaves);
+      load_k();
+      look_up(tile + 2 * kWaves);
+      f4_t sc[R][NH] = {};
 #pragma unroll
-      for (int n = 0; n < NB; ++n)
+      for (int s = 0; s < NK; ++s) {
+        OpT q[R];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int j = 0; j < R; ++j) q[j] = sq[j][s][lane];
 #pragma unroll
-          for (int e = 0; e < VB; e += 4) {
-            f4_t x;
+        for (int h = 0; h < NH; ++h) {
+          const KRow row = kt[k_place(16 * h + l15, 4 * s + g)];
+          u32x4 w;
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              float y = acc[0][n][e + u][i];
+          for (int i = 0; i < 4; ++i) w[i] = row.word(i);
 #pragma unroll
-              for (int m = 1; m < R; ++m) y = j == m ? acc[m][n][e + u][i] : y;
-              x[u] = y * mine;
-            }
-            *reinterpret_cast<f4_t*>(&part_acc[wave][l15][(n * 16 + 4 * g + i) * VB + e]) = x;
+          for (int j = 0; j < R; ++j) sc[j][h] = mma(__builtin_bit_cast(OpT, w), q[j], sc[j][h]);
+        }
+        if (s % 2) __builtin_amdgcn_sched_barrier(0);
+      }
+      // Positions that a row does not see; values that no row sees are no part
+      // of the sums, whatever they are.
+      if (!whole) {
+        const uint32_t there = static_cast<uint32_t>(ok) >> 4 * g;
+        const uint32_t there_hi = static_cast<uint32_t>(ok >> 32) >> 4 * g;
+        bool fine = true;
+#pragma unroll
+        for (int i = 0; i < NX; ++i) {
+          const int t = 16 * (i / 4) + i % 4, pos = pos0 + 4 * g + t;
+          const bool in = ((t < 32 ? there >> t : there_hi >> (t - 32)) & 1);
+#pragma unroll
+          for (int j = 0; j < R; ++j) {
+            const int back = pos_0 + tok[j] - pos;
+            const bool seen = in && back >= 0 && (!p.window || back < p.window);
+            sc[j][i / 4][i % 4] = seen ? sc[j][i / 4][i % 4] : -INFINITY;
           }
-    }
-    __syncthreads();
-    const int quads = p.D / 4;
-    for (int u = threadIdx.x; u < rows * quads; u += kBlock) {
-      const int row = u / quads, d = (u - row * quads) * 4, r = r0 + 16 * j + row;
-      float b = ml[0][row].x;
+          const bool any = in && pos <= last_pos && pos >= low_first;
 #pragma unroll
-      for (int w = 1; w < kWaves; ++w) b = fmaxf(b, ml[w][row].x);
-      float l = 0.f;
-      f4_t x = {};
+          for (int n = 0; n < NB; ++n) {
+            v[i][n].keep(any);
+            if (first_tok < last_tok) fine = fine && v[i][n].finite();
+          }
+        }
+        // A value that is not finite where some new tokens see it and others do
+        // not: 0 * inf would be NaN for all of them, so it is taken out, and
+        // the rows that see it get NaN themselves.  Rare, and so in LDS, in
+        // loops: unrolled in registers it took 70 more of them.
+        if (!__all(fine)) {
+          C* const vt = reinterpret_cast<C*>(kt);  // [TS][DP]
+          auto v_at = [&](int i, int n) {
+            return reinterpret_cast<VRow*>(vt + (16 * (i / 4) + 4 * g + i % 4) * DP +
+                                           (n * 16 + l15) * VB);
+          };
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        l += ml[w][row].y * weight(ml[w][row].x, b);
-        x += *reinterpret_cast<const f4_t*>(&part_acc[w][row][d]);
+          for (int i = 0; i < NX; ++i)
+#pragma unroll
+            for (int n = 0; n < NB; ++n) *v_at(i, n) = v[i][n];
+          wave_sync();
+#pragma unroll 1
+          for (int d = lane; d < DP; d += kWave) {
+            uint32_t rows[R] = {};  // those that see such a value
+#pragma unroll 1
+            for (int t = 0; t < TS; ++t) {
+              const bool bad = not_finite(vt[t * DP + d]);
+              if (bad) vt[t * DP + d] = C{};
+#pragma unroll
+              for (int j = 0; j < R; ++j) {
+                const int back = pos_0 + tok[j] - (pos0 + t);
+                const uint64_t see = __ballot(back >= 0 && (!p.window || back < p.window));
+                rows[j] |= bad ? static_cast<uint32_t>(see) & 0xffffu : 0u;
+              }
+            }
+#pragma unroll
+            for (int j = 0; j < R; ++j) poison[wave][j][d] = static_cast<uint16_t>(rows[j]);
+          }
+          wave_sync();
+#pragma unroll
+          for (int i = 0; i < NX; ++i)
+#pragma unroll
+            for (int n = 0; n < NB; ++n) v[i][n] = *v_at(i, n);
+#pragma unroll
+          for (int j = 0; j < R; ++j)
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int e = 0; e < VB; ++e) {
+                  const uint32_t bits = poison[wave][j][(n * 16 + 4 * g + i) * VB + e];
+                  acc[j][n][e][i] += __builtin_bit_cast(float, (0u - (bits >> l15 & 1)) & 0x7fc00000u);
+                }
+        }
       }
-      if (part.of > 1) {
-        const int64_t at = (static_cast<int64_t>(slot) * p.Hkv + head) * p.M + r;
-        *reinterpret_cast<f4_t*>(p.acc + at * p.D + d) = x;
-        if (d == 0) p.ml[at] = make_float2(b, l);
-        continue;
-      }
-      const int tok = r / p.G;
-      const int64_t hq = static_cast<int64_t>(head) * p.G + (r - tok * p.G);
-      const float inv = l == 0.f ? 0.f : v_scale / l;
-      float o[4];
+
+      u32x4 ph[R][NS], pl[R][NS];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = l == 0.f ? 0.f : x[i] * inv;
-      store_vec_f32<T, 4>(static_cast<T*>(p.out) + part.b * p.o_seq + tok * p.o_tok +
-                              hq * p.o_head + d, o);
-      if (p.lse && d == 0)
-        p.lse[(static_cast<int64_t>(part.b) * p.T + tok) * p.Hkv * p.G + hq] =
-            l == 0.f ? -INFINITY : (b + __log2f(l)) * 0.69314718056f;
+      for (int j = 0; j < R; ++j) {
+        float x[NX], top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < NX; ++i) {
+          x[i] = sc[j][i / 4][i % 4];
+          top = fmaxf(top, x[i]);
+        }
+        top = over_groups(top, [](float a, float c) { return fmaxf(a, c); });
+        const float now = fmaxf(base[j], top * scale2 - kShift);
+        const float from = now == -INFINITY ? 0.f : now;
+        const float keep = exp2_hw(base[j] - from);
+        base[j] = now;
+        float add = 0.f;
+#pragma unroll
+        for (int i = 0; i < NX; ++i) {
+          x[i] = exp2_hw(__builtin_fmaf(x[i], scale2, -from));
+          add += x[i];
+        }
+        sum[j] = sum[j] * keep + add;
+#pragma unroll
+        for (int i = 0; i < NX; i += KV)
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            uint32_t hi = 0, lo = 0;
+            if constexpr (sizeof(T) == 4) hi = __builtin_bit_cast(uint32_t, x[i + u]);
+            else split2(x[i + 2 * u], x[i + 2 * u + 1], hi, lo, T());
+            ph[j][i / KV][u] = hi;
+            pl[j][i / KV][u] = lo;
+          }
+        // (nothing to rescale in most tiles; the empty asm keeps the branch,
+        // without which old and scaled sums are both held)
+        if (__any(keep != 1.f)) {
+          asm volatile("");
+#pragma unroll
+          for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int e = 0; e < VB; ++e) acc[j][n][e] *= keep;
+        }
+      }
+      // acc += V^T P^T
+#pragma unroll
+      for (int m = 0; m < NS; ++m)
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+          for (int e = 0; e < VB; ++e) {
+            u32x4 w;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if constexpr (sizeof(T) == 4)
+                w[i] = v[m * KV + i][n].word(e);
+              else
+                w[i] = __builtin_amdgcn_perm(v[m * KV + 2 * i + 1][n].word(e / 2),
+                                             v[m * KV + 2 * i][n].word(e / 2),
+                                             e & 1 ? 0x07060302u : 0x05040100u);
+            }
+            const OpT a = __builtin_bit_cast(OpT, w);
+#pragma unroll
+            for (int j = 0; j < R; ++j) {
+              acc[j][n][e] = mma(a, __builtin_bit_cast(OpT, ph[j][m]), acc[j][n][e]);
+              if constexpr (sizeof(T) == 2)
+                acc[j][n][e] = mma(a, __builtin_bit_cast(OpT, pl[j][m]), acc[j][n][e]);
+            }
+            // (else all operands are turned before the first product, in
+            // twice the registers)
+            if (e % 2) __builtin_amdgcn_sched_barrier(0);
+          }
+      load_v();
+      ok = ok_next;
+      tile += kWaves;
     }
+
+    // The waves join: a row's base is the largest, sums are scaled to it.
+    for (int j = 0; j < R; ++j) {
+      const int rows = min(16, p.M - r0 - 16 * j);
+      if (rows <= 0) break;
+      // (a select, so that the arrays stay in registers)
+      float my_base = base[0], my_sum = sum[0];
+#pragma unroll
+      for (int i = 1; i < R; ++i) {
+        my_base = j == i ? base[i] : my_base;
+        my_sum = j == i ? sum[i] : my_sum;
+      }
+      my_sum = over_groups(my_sum, [](float a, float c) { return a + c; });
+      __syncthreads();
+      if (g == 0) ml[wave][l15] = make_float2(my_base, my_sum);
+      __syncthreads();
+      float top = ml[0][l15].x;
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) top = fmaxf(top, ml[w][l15].x);
+      const float mine = weight(my_base, top);
+      if (l15 < rows) {
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < VB; e += 4) {
+              f4_t x;
+#pragma unroll
+              for (int u = 0; u < 4; ++u) {
+                float y = acc[0][n][e + u][i];
+#pragma unroll
+                for (int m = 1; m < R; ++m) y = j == m ? acc[m][n][e + u][i] : y;
+                x[u] = y * mine;
+              }
+              *reinterpret_cast<f4_t*>(&sh.acc[wave][l15][(n * 16 + 4 * g + i) * VB + e]) = x;
+            }
+      }
+      __syncthreads();
+      const int quads = p.D / 4;
+      for (int u = threadIdx.x; u < rows * quads; u += kBlock) {
+        const int row = u / quads, d = (u - row * quads) * 4, r = r0 + 16 * j + row;
+        float m = ml[0][row].x;
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) m = fmaxf(m, ml[w][row].x);
+        float l = 0.f;
+        f4_t x = {};
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+          l += ml[w][row].y * weight(ml[w][row].x, m);
+          x += *reinterpret_cast<const f4_t*>(&sh.acc[w][row][d]);
+        }
+        if (all) {
+          write_row<T>(p, b, head, r, d, x, m, l);
+        } else {
+          const int64_t to = (static_cast<int64_t>(slot) * p.Hkv + head) * p.M + r;
+          *reinterpret_cast<f4_t*>(p.acc + to * p.D + d) = x;
+          if (d == 0) p.ml[to] = make_float2(m, l);
+        }
+      }
+    }
+
+    at += span.n;
+    if (at >= g1) break;
+    if (++b == bt.b0 + kWave) bt = batch_at<TS>(p, b);
+    __syncthreads();  // the join's reads are over
   }
 }
 
-// Joins the parts of sequences that have several: a block for a (sequence,
-// head) and every gridDim.y-th of its rows; D / 4 lanes (a power of two of
-// them) read a part's row, the block's teams take parts in turn.
+// Joins the pieces of sequences that lie in several shares: a block for a
+// (sequence, head) and some of its rows.  `team` lanes read a piece's row, 4
+// elements each; as many teams as there are pieces (a power of two of them)
+// share a row, so that few pieces leave the block to several rows.
 template <typename T>
 __global__ void __launch_bounds__(kBlock) join_kernel(Params p, int team) {
   __shared__ float2 ml[16];
-  __shared__ __align__(16) float sums[kBlock * 4];
+  __shared__ __align__(16) f4_t sums[kBlock];
   const int b = blockIdx.x / p.Hkv, head = blockIdx.x % p.Hkv;
   const int2 meta = p.meta[b];
-  if (meta.y <= 1) return;
+  const int pieces = meta.y;
+  if (pieces <= 1) return;
   const int teams = kBlock / team, own = threadIdx.x / team, d = threadIdx.x % team * 4;
-  const float v_scale = p.v_scale ? p.v_scale[head] : 1.f;
-  for (int r = blockIdx.y; r < p.M; r += gridDim.y) {
+  int split = 1;  // teams of a row
+  while (split < pieces && split < teams) split *= 2;
+  const int part = own % split, step = gridDim.y * (teams / split);
+  for (int r0 = blockIdx.y * (teams / split); r0 < p.M; r0 += step) {
+    const int r = r0 + own / split;
     float base = -INFINITY, sum = 0.f;
     f4_t acc = {};
-#pragma unroll 4
-    for (int i = own; i < meta.y; i += teams) {
-      const int64_t at = (static_cast<int64_t>(meta.x + i) * p.Hkv + head) * p.M + r;
-      const float2 x = p.ml[at];
-      f4_t y = {};
-      if (d < p.D) y = *reinterpret_cast<const f4_t*>(p.acc + at * p.D + d);
-      const float now = fmaxf(base, x.x), a = weight(base, now), c = weight(x.x, now);
-      sum = sum * a + x.y * c;
-      acc = acc * a + y * c;
-      base = now;
+    constexpr int kAhead = 4;  // pieces that a lane requests together
+    for (int i0 = part; i0 < pieces && r < p.M; i0 += kAhead * split) {
+      float2 x[kAhead];
+      f4_t y[kAhead];
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a) {
+        const int i = i0 + a * split;
+        x[a] = make_float2(-INFINITY, 0.f);
+        y[a] = f4_t{};
+        if (i < pieces) {
+          // The first piece, then the first ones of the shares that follow.
+          const int slot = i ? (meta.x & ~1) + 2 * i : meta.x;
+          const int64_t at = (static_cast<int64_t>(slot) * p.Hkv + head) * p.M + r;
+          x[a] = p.ml[at];
+          if (d < p.D) y[a] = *reinterpret_cast<const f4_t*>(p.acc + at * p.D + d);
+        }
+      }
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a) {
+        const float now = fmaxf(base, x[a].x), c = weight(base, now), e = weight(x[a].x, now);
+        sum = sum * c + x[a].y * e;
+        acc = acc * c + y[a] * e;
+        base = now;
+      }
     }
     if (threadIdx.x % team == 0) ml[own] = make_float2(base, sum);
     __syncthreads();
-    float top = ml[0].x;
-    for (int i = 1; i < teams; ++i) top = fmaxf(top, ml[i].x);
-    acc *= weight(base, top);
-    *reinterpret_cast<f4_t*>(&sums[threadIdx.x * 4]) = acc;
+    float top = -INFINITY;
+    for (int i = own - part; i < own - part + split; ++i) top = fmaxf(top, ml[i].x);
+    sums[threadIdx.x] = acc * weight(base, top);
     __syncthreads();
-    if (own == 0 && d < p.D) {
+    if (part == 0 && r < p.M && d < p.D) {
       float l = 0.f;
       f4_t x = {};
-      for (int i = 0; i < teams; ++i) {
-        l += ml[i].y * weight(ml[i].x, top);
-        x += *reinterpret_cast<const f4_t*>(&sums[(i * team + threadIdx.x) * 4]);
+      for (int i = 0; i < split; ++i) {
+        l += ml[own + i].y * weight(ml[own + i].x, top);
+        x += sums[threadIdx.x + i * team];
       }
-      const int tok = r / p.G;
-      const int64_t hq = static_cast<int64_t>(head) * p.G + (r - tok * p.G);
-      const float inv = l == 0.f ? 0.f : v_scale / l;
-      float o[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = l == 0.f ? 0.f : x[i] * inv;
-      store_vec_f32<T, 4>(static_cast<T*>(p.out) + b * p.o_seq + tok * p.o_tok + hq * p.o_head +
-                              d, o);
-      if (p.lse && d == 0)
-        p.lse[(static_cast<int64_t>(b) * p.T + tok) * p.Hkv * p.G + hq] =
-            l == 0.f ? -INFINITY : (top + __log2f(l)) * 0.69314718056f;
+      write_row<T>(p, b, head, r, d, x, top, l);
     }
     __syncthreads();
   }
 }
 
 template <typename T, typename C, int DP, int R>
-void launch_pages(const Params& p, hipStream_t s) {
-  const dim3 grid(static_cast<uint32_t>(p.slots) * p.groups * p.Hkv);
+void launch_pages(Params& p, hipStream_t s) {
+  // As many blocks as run at once.
+  const int64_t lines = static_cast<int64_t>(p.Hkv) * p.groups;
+  p.shares = static_cast<int>(std::min<int64_t>(
+      p.shares, std::max<int64_t>(1, int64_t{num_cus()} * waves_of<T, C, DP, R>() / lines)));
+  const dim3 grid(static_cast<uint32_t>(p.shares * lines));
   if (p.page_size % 16 == 0)
     hipLaunchKernelGGL((attention_kernel<T, C, DP, R, true>), grid, dim3(kBlock), 0, s, p);
   else
@@ -668,34 +832,32 @@ void launch_pages(const Params& p, hipStream_t s) {
 }
 
 template <typename T, typename C, int DP>
-void launch_rows(const Params& p, int tiles, hipStream_t s) {
-  if constexpr (DP <= 128) {
-    if (tiles == 2) return launch_pages<T, C, DP, 2>(p, s);
-  }
-  launch_pages<T, C, DP, 1>(p, s);
+void launch_rows(Params& p, int tiles, hipStream_t s) {
+  if (tiles == 1) launch_pages<T, C, DP, 1>(p, s);
+  else launch_pages<T, C, DP, 2>(p, s);
 }
 
 // `tiles`: row tiles of a wave, as the entry point counted p.groups by.
 template <typename T, typename C>
-int run(const Params& p, int tiles, hipStream_t s) {
+int run(Params& p, int tiles, hipStream_t s) {
   if (p.D <= 64) launch_rows<T, C, 64>(p, tiles, s);
   else if (p.D <= 128) launch_rows<T, C, 128>(p, tiles, s);
   else launch_rows<T, C, 256>(p, tiles, s);
   int st = launch_status();
-  if (st != XK_OK || p.alone) return st;
+  if (st != XK_OK || p.shares == 1) return st;
   const int team = p.D <= 64 ? 16 : (p.D <= 128 ? 32 : 64);
   const int64_t heads = static_cast<int64_t>(p.B) * p.Hkv;
   const dim3 grid(static_cast<uint32_t>(heads),
-                  static_cast<uint32_t>(std::min<int64_t>(p.M, cdiv(1024, heads))));
+                  static_cast<uint32_t>(std::min<int64_t>(p.M, cdiv(2048, heads))));
   hipLaunchKernelGGL((join_kernel<T>), grid, dim3(kBlock), 0, s, p, team);
   return launch_status();
 }
 
-int run_f32(const Params& p, int tiles, hipStream_t s);
-int run_bf16(const Params& p, int tiles, hipStream_t s);
-int run_f16(const Params& p, int tiles, hipStream_t s);
-int run_bf16_f8(const Params& p, int tiles, hipStream_t s);
-int run_f16_f8(const Params& p, int tiles, hipStream_t s);
+int run_f32(Params& p, int tiles, hipStream_t s);
+int run_bf16(Params& p, int tiles, hipStream_t s);
+int run_f16(Params& p, int tiles, hipStream_t s);
+int run_bf16_f8(Params& p, int tiles, hipStream_t s);
+int run_f16_f8(Params& p, int tiles, hipStream_t s);
 
 }  // namespace paged
 }  // namespace xk

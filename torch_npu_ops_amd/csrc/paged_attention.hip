@@ -11,27 +11,25 @@ constexpr int64_t kMostPitch = int64_t{1} << 27;      // bytes from one position
 
 struct Plan {
   int tiles;  // row tiles of a wave
-  int64_t groups, want, slots, bytes;
-  bool alone;
+  int64_t groups, shares, bytes;
 };
 
 // False where the sizes are beyond what a launch holds.
 bool plan_of(int64_t B, int64_t T, int64_t G, int64_t Hkv, int64_t D, int64_t positions,
-             xk_dtype dtype, Plan& x) {
-  const int64_t M = T * G, tile = dtype == XK_F32 ? 16 : 32;
-  x.tiles = M > 16 && D <= 128 ? 2 : 1;
+             Plan& x) {
+  const int64_t M = T * G;
+  x.tiles = M > 16 ? 2 : 1;
   x.groups = cdiv(M, 16 * x.tiles);
-  // Blocks in all: with one sequence the parts are equal, and one round of two
-  // blocks a compute unit is full; ragged batches get four rounds to even out.
-  const int64_t blocks = static_cast<int64_t>(num_cus()) * (B == 1 ? 2 : 8);
-  x.want = std::max<int64_t>(1, blocks / (Hkv * x.groups));
-  const int64_t most = std::max<int64_t>(1, cdiv(cdiv(positions, tile), kMinChunk));
-  x.alone = most == 1;
-  x.slots = std::min(x.want + B, B * most);
-  const int64_t rows = x.slots * Hkv * M;
-  if (x.slots * x.groups * Hkv >= INT32_MAX || rows >= (int64_t{1} << 40)) return false;
+  // The shares of a head and row group: two blocks a compute unit in all (the
+  // kernels that only fit once take half), none without a least share.
+  const int64_t lines = Hkv * x.groups;
+  const int64_t most = cdiv(B * std::max<int64_t>(1, cdiv(positions, 16)), kWaves);
+  x.shares = std::min(std::max<int64_t>(1, 2 * num_cus() / lines), most);
+  const int64_t rows = 2 * x.shares * Hkv * M;
+  if (x.shares * lines >= INT32_MAX || B * Hkv >= INT32_MAX || rows >= (int64_t{1} << 40))
+    return false;
   auto up = [](int64_t n) { return cdiv(n, 256) * 256; };
-  x.bytes = x.alone ? 0 : up(B * 8) + up(rows * 8) + up(rows * D * 4);
+  x.bytes = up(B * 8) + up(rows * 8) + up(rows * D * 4);
   return true;
 }
 
@@ -54,11 +52,10 @@ using namespace xk;
 
 extern "C" int64_t xk_paged_attention_workspace_bytes(int64_t B, int64_t T, int64_t Hq,
                                                       int64_t Hkv, int64_t head_dim,
-                                                      int64_t max_pages, int64_t page_size,
-                                                      xk_dtype dtype) {
+                                                      int64_t max_pages, int64_t page_size) {
   paged::Plan x;
   if (paged::check_sizes(B, T, Hq, Hkv, head_dim, max_pages, page_size) != XK_OK || B == 0 ||
-      !paged::plan_of(B, T, Hq / Hkv, Hkv, head_dim, max_pages * page_size, dtype, x))
+      !paged::plan_of(B, T, Hq / Hkv, Hkv, head_dim, max_pages * page_size, x))
     return 0;
   return x.bytes;
 }
@@ -100,10 +97,9 @@ extern "C" int xk_paged_attention(
     return XK_ERR_INVALID;
   const int64_t positions = num_pages ? max_pages * page_size : 0;
   Plan x;
-  if (!plan_of(B, T, Hq / Hkv, Hkv, head_dim, max_pages * page_size, dtype, x))
+  if (!plan_of(B, T, Hq / Hkv, Hkv, head_dim, max_pages * page_size, x))
     return XK_ERR_INVALID;
-  if (x.bytes && (!workspace || workspace_bytes < static_cast<size_t>(x.bytes) ||
-                  !aligned(workspace, 256)))
+  if (!workspace || workspace_bytes < static_cast<size_t>(x.bytes) || !aligned(workspace, 256))
     return XK_ERR_WORKSPACE;
   Params p{};
   p.q = q;
@@ -112,17 +108,19 @@ extern "C" int xk_paged_attention(
   p.q_head = stride_q_head;
   p.kc = static_cast<const char*>(k_cache);
   p.k_page = stride_kc_page * cb;
-  p.k_slot = stride_kc_slot * cb;
+  p.k_slot = static_cast<uint32_t>(stride_kc_slot * cb);
   p.k_head = stride_kc_head * cb;
   p.vc = static_cast<const char*>(v_cache);
   p.v_page = stride_vc_page * cb;
-  p.v_slot = stride_vc_slot * cb;
+  p.v_slot = static_cast<uint32_t>(stride_vc_slot * cb);
   p.v_head = stride_vc_head * cb;
   p.num_pages = static_cast<int>(num_pages);
   p.page_size = static_cast<int>(page_size);
-  p.page_shift = -1;
-  if ((page_size & (page_size - 1)) == 0)
-    for (p.page_shift = 0; (int64_t{1} << p.page_shift) < page_size;) ++p.page_shift;
+  // n / page_size for n < 2^28: n * magic is off by less than 2^28 * page_size
+  // from n * 2^shift / page_size, which is below the 2^shift of one step.
+  p.page_shift = 28;
+  while ((int64_t{1} << (p.page_shift - 28)) < page_size) ++p.page_shift;
+  p.page_magic = static_cast<uint32_t>(cdiv(int64_t{1} << p.page_shift, page_size));
   p.table = block_table;
   p.table_row = stride_table_row;
   p.max_pages = static_cast<int>(max_pages);
@@ -144,18 +142,14 @@ extern "C" int xk_paged_attention(
   p.D = static_cast<int>(head_dim);
   p.M = static_cast<int>(T * (Hq / Hkv));
   p.groups = static_cast<int>(x.groups);
-  p.want = static_cast<int>(x.want);
-  p.slots = static_cast<int>(x.slots);
-  p.alone = x.alone;
-  if (!x.alone) {
-    char* ws = static_cast<char*>(workspace);
-    const int64_t rows = x.slots * Hkv * p.M;
-    p.meta = reinterpret_cast<int2*>(ws);
-    ws += cdiv(B * 8, 256) * 256;
-    p.ml = reinterpret_cast<float2*>(ws);
-    ws += cdiv(rows * 8, 256) * 256;
-    p.acc = reinterpret_cast<float*>(ws);
-  }
+  p.shares = static_cast<int>(x.shares);
+  char* ws = static_cast<char*>(workspace);
+  const int64_t rows = 2 * x.shares * Hkv * p.M;
+  p.meta = reinterpret_cast<int2*>(ws);
+  ws += cdiv(B * 8, 256) * 256;
+  p.ml = reinterpret_cast<float2*>(ws);
+  ws += cdiv(rows * 8, 256) * 256;
+  p.acc = reinterpret_cast<float*>(ws);
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (dtype) {
     case XK_F32: return run_f32(p, x.tiles, s);

@@ -3,6 +3,6 @@
 
 namespace xk {
 namespace paged {
-int run_bf16(const Params& p, int tiles, hipStream_t s) { return run<bf16, bf16>(p, tiles, s); }
+int run_bf16(Params& p, int tiles, hipStream_t s) { return run<bf16, bf16>(p, tiles, s); }
 }  // namespace paged
 }  // namespace xk

@@ -3,6 +3,6 @@
 
 namespace xk {
 namespace paged {
-int run_f16(const Params& p, int tiles, hipStream_t s) { return run<f16, f16>(p, tiles, s); }
+int run_f16(Params& p, int tiles, hipStream_t s) { return run<f16, f16>(p, tiles, s); }
 }  // namespace paged
 }  // namespace xk

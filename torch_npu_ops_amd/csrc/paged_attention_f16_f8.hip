@@ -3,6 +3,6 @@
 
 namespace xk {
 namespace paged {
-int run_f16_f8(const Params& p, int tiles, hipStream_t s) { return run<f16, f8>(p, tiles, s); }
+int run_f16_f8(Params& p, int tiles, hipStream_t s) { return run<f16, f8>(p, tiles, s); }
 }  // namespace paged
 }  // namespace xk

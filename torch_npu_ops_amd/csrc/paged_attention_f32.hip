@@ -3,6 +3,6 @@
 
 namespace xk {
 namespace paged {
-int run_f32(const Params& p, int tiles, hipStream_t s) { return run<float, float>(p, tiles, s); }
+int run_f32(Params& p, int tiles, hipStream_t s) { return run<float, float>(p, tiles, s); }
 }  // namespace paged
 }  // namespace xk
