@@ -714,7 +714,8 @@ int xk_rotary_cache_append(
  *   has no part in that row.
  *   q, k_cache and v_cache 16-byte aligned (8 for an 8-bit cache), their
  *   strides whole vectors of that size, out's of 4 elements (else
- *   XK_ERR_UNSUPPORTED); a place's pitch below 2^27 bytes.
+ *   XK_ERR_UNSUPPORTED); pitches of places below 2^27 bytes, of pages below
+ *   2^35, neither negative.
  *   The split of the positions follows from all lengths of the batch: a
  *   sequence's last bits depend on the batch, but not on the run.
  *   workspace >= xk_paged_attention_workspace_bytes(...) bytes for the same

@@ -62,11 +62,12 @@ struct Params {
   const void* q;
   int64_t q_seq, q_tok, q_head;  // elements
   const char* kc;
-  int64_t k_page, k_head;  // bytes
-  uint32_t k_slot;
+  int64_t k_head;   // bytes
+  uint32_t k_page;  // 8 bytes
+  uint32_t k_slot;  // bytes
   const char* vc;
-  int64_t v_page, v_head;
-  uint32_t v_slot;
+  int64_t v_head;
+  uint32_t v_page, v_slot;
   int num_pages, page_size;
   uint32_t page_magic;  // n / page_size = n * magic >> shift for n < 2^28
   int page_shift;
@@ -160,15 +161,20 @@ __device__ __forceinline__ uint32_t widen(uint32_t w, bool high) {
         : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, false));
 }
 
+// Bytes in device memory; the type says so to the compiler where a pointer came
+// from integers.
+using GlobalBytes = const __attribute__((address_space(1))) char*;
+
 // N elements of the cache as loaded, and as words of T.
 template <typename T, typename C, int N>
 struct alignas(N * sizeof(C) < 16 ? N * sizeof(C) : 16) Row {
   static constexpr int kBytes = N * static_cast<int>(sizeof(C));
   static constexpr int kRaw = kBytes / 4, kWords = N * static_cast<int>(sizeof(T)) / 4;
   uint32_t raw[kRaw];
-  __device__ __forceinline__ void load(const char* at) {
+  __device__ __forceinline__ void load(GlobalBytes at) {
     using U = typename RawOf<kBytes>::type;
-    const U x = __builtin_nontemporal_load(reinterpret_cast<const U*>(at));
+    const U x = __builtin_nontemporal_load(
+        reinterpret_cast<const __attribute__((address_space(1))) U*>(at));
     if constexpr (kRaw == 1) {
       raw[0] = x;
     } else {
@@ -226,14 +232,20 @@ __device__ __forceinline__ float over_groups(float v, F f) {
   return f(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y));
 }
 
-// A wave-uniform pointer in scalar registers, to which loads add a lane's 32-bit
+// A wave-uniform address in scalar registers, to which loads add a lane's 32-bit
 // offset: left to itself the compiler adds offsets first and keeps 64 bits for
 // each lane and load.
-__device__ __forceinline__ const char* scalar(const char* x) {
-  const uint64_t u = reinterpret_cast<uint64_t>(x);
+__device__ __forceinline__ GlobalBytes scalar(uint64_t u) {
   const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(u));
   const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(u >> 32));
-  return reinterpret_cast<const char*>(static_cast<uint64_t>(hi) << 32 | lo);
+  return reinterpret_cast<GlobalBytes>(static_cast<uint64_t>(hi) << 32 | lo);
+}
+
+// The offset, not to be widened outside the loop: a load takes a scalar address
+// and 32 bits a lane only where it sees both.
+__device__ __forceinline__ uint32_t lane_offset(uint32_t x) {
+  asm volatile("" : "+v"(x));
+  return x;
 }
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -316,13 +328,14 @@ __global__ void __launch_bounds__(kBlock, (waves_of<T, C, DP, R>())) attention_k
   using KRow = Row<T, C, KV>;
   using VRow = Row<T, C, VB>;
 
-  constexpr int kPitch = DP + 4;  // rows of the join 4 banks apart
+  constexpr int DJ = DP < 128 ? DP : 128;  // elements that are joined together
+  constexpr int kPitch = DJ + 4;           // rows of the join 4 banks apart
   union Shared {
     KRow k[kWaves][TS * CH];
     float acc[kWaves][16][kPitch];
   };
   __shared__ __align__(16) Shared sh;
-  __shared__ __align__(16) OpT sq[R][NK][kWave];  // Q, as the operands take it
+  __shared__ __align__(16) OpT sq[R * NK][kWave];  // Q, as the operands take it
   __shared__ float2 ml[kWaves][16];
   __shared__ uint16_t poison[kWaves][R][DP];  // a bit for each row of a tile
 
@@ -361,8 +374,8 @@ __global__ void __launch_bounds__(kBlock, (waves_of<T, C, DP, R>())) attention_k
 #pragma unroll
     for (int n = 0; n < NB; ++n)
       v_off[i][n] = (4 * g + i) * p.v_slot + min((n * 16 + l15) * VB, p.D - VB) * CB;
-  const char* const kc = p.kc + head * p.k_head;
-  const char* const vc = p.vc + head * p.v_head;
+  const uint64_t kc = reinterpret_cast<uint64_t>(p.kc + head * p.k_head);
+  const uint64_t vc = reinterpret_cast<uint64_t>(p.vc + head * p.v_head);
   // Scores are scaled by something positive, that leaves a masked one -inf: a
   // sign goes to Q, and 1.2e-38 for 0 makes every finite score 0 too.
   float scale2 = p.scale2;
@@ -387,48 +400,156 @@ __global__ void __launch_bounds__(kBlock, (waves_of<T, C, DP, R>())) attention_k
     return static_cast<int>(static_cast<uint64_t>(pos) * p.page_magic >> p.page_shift);
   };
 
-  for (;;) {
-    Span span;
-    span.len = __builtin_amdgcn_readlane(bt.own.len, b - bt.b0);
-    span.t0 = __builtin_amdgcn_readlane(bt.own.t0, b - bt.b0);
-    span.n = __builtin_amdgcn_readlane(bt.own.n, b - bt.b0);
-    const int len = span.len;
-    // The block's piece of the sequence; the first of a share and the last
-    // have places of their own where they are not all of it.
-    const int64_t from_g = max<int64_t>(g0, at), to_g = min<int64_t>(g1, at + span.n);
-    const bool all = to_g - from_g == span.n;
-    const int slot = 2 * share + (from_g > g0);
-    if (from_g == at && head == 0 && group == 0 && threadIdx.x == 0) {
-      const int last = static_cast<int>(divide(at + span.n - 1, size));
-      p.meta[b] = make_int2(slot, last - share + 1);
+  // The piece of a sequence that lies in the share: its positions, and its
+  // tiles without those that no row of the group sees.
+  struct Piece {
+    int b, len, n;
+    int64_t at;
+    int begin, end;
+    const int32_t* table;
+  };
+  auto piece_of = [&](int seq, int64_t where) {
+    Piece x;
+    x.b = seq;
+    x.at = where;
+    x.len = __builtin_amdgcn_readlane(bt.own.len, seq - bt.b0);
+    x.n = __builtin_amdgcn_readlane(bt.own.n, seq - bt.b0);
+    const int t0 = __builtin_amdgcn_readlane(bt.own.t0, seq - bt.b0);
+    const int first_pos = x.len - p.T + first_tok, last_pos = x.len - p.T + last_tok;
+    x.begin = t0 + static_cast<int>(max<int64_t>(g0 - where, 0));
+    x.end = t0 + static_cast<int>(min<int64_t>(g1 - where, x.n));
+    if (p.window) x.begin = max(x.begin, max(0, first_pos - p.window + 1) / TS);
+    x.end = min(x.end, last_pos < 0 ? 0 : last_pos / TS + 1);
+    x.table = p.table + seq * p.table_row;
+    return x;
+  };
+  // The wave's share of Q's operands of a sequence, requested and stored.
+  constexpr int NQ = (R * NK + kWaves - 1) / kWaves;
+  u32x4 qx[NQ];
+  auto load_q = [&](int seq) {
+#pragma unroll
+    for (int c = 0; c < NQ; ++c) {
+      const int u = c * kWaves + wave, j = u / NK, s = u % NK;
+      const int r = r0 + 16 * j + l15, t = r / p.G, d = (4 * s + g) * KV;
+      qx[c] = u32x4{};
+      if (u < R * NK && r < p.M && d < p.D)
+        qx[c] = *reinterpret_cast<const u32x4*>(
+            static_cast<const T*>(p.q) + seq * p.q_seq + t * p.q_tok +
+            (static_cast<int64_t>(head) * p.G + (r - t * p.G)) * p.q_head + d);
     }
+  };
+  auto store_q = [&]() {
+#pragma unroll
+    for (int c = 0; c < NQ; ++c) {
+      const int u = c * kWaves + wave;
+      if (negate) qx[c] ^= sizeof(T) == 4 ? 0x80000000u : 0x80008000u;
+      if (u < R * NK) sq[u][lane] = __builtin_bit_cast(OpT, qx[c]);
+    }
+  };
 
+  Piece cur = piece_of(b, at);
+  load_q(b);
+  bool loaded = false;  // the registers hold the piece's first tile of the wave
+  KRow k[NL];
+  VRow v[NX][NB];
+  uint64_t ok = 0;  // which positions of the tile there are
+  // The table's entries of a tile (P16: one for each half; else the lane's
+  // position's).  Positions past the sequence's end stand for its last ones.
+  auto pos_of = [&](int len, int tile, int h) {
+    return min(tile * TS + (P16 ? 16 * h : lane % TS), P16 ? (len - 1) & ~15 : len - 1);
+  };
+  int entry[P16 ? NH : 1];
+  auto look_up = [&](const int32_t* table, int len, int tile) {
+#pragma unroll
+    for (int h = 0; h < (P16 ? NH : 1); ++h) entry[h] = table[page_of(pos_of(len, tile, h))];
+  };
+  // Where a tile's rows are, and which of them are in a page that there is
+  // (a bit each); the others are read from the first page.
+  GlobalBytes kh[NH], vh[NH];
+  uint64_t ko = 0, vo = 0;
+  auto place = [&](int len, int tile) -> uint64_t {
+    if constexpr (P16) {
+      uint64_t ok = 0;
+#pragma unroll
+      for (int h = 0; h < NH; ++h) {
+        const uint32_t e = __builtin_amdgcn_readfirstlane(entry[h]);
+        const bool in = e < static_cast<uint32_t>(p.num_pages);
+        const uint64_t page = in ? e : 0;
+        const int pos = pos_of(len, tile, h);
+        const uint64_t row = pos - page_of(pos) * p.page_size;
+        kh[h] = scalar(kc + (page * p.k_page << 3) + row * p.k_slot);
+        vh[h] = scalar(vc + (page * p.v_page << 3) + row * p.v_slot);
+        ok |= in ? uint64_t{0xffff} << (16 * h) : 0;
+      }
+      return ok;
+    } else {
+      const uint32_t e = entry[0];
+      const bool in = e < static_cast<uint32_t>(p.num_pages);
+      const uint64_t page = in ? e : 0;
+      const int pos = pos_of(len, tile, 0);
+      const uint64_t row = pos - page_of(pos) * p.page_size;
+      ko = kc + (page * p.k_page << 3) + row * p.k_slot;
+      vo = vc + (page * p.v_page << 3) + row * p.v_slot;
+      return __ballot(in) & kAll;
+    }
+  };
+  auto load_k = [&]() {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      if constexpr (P16)
+        k[i].load(kh[i * RPI / 16] + lane_offset(k_off[i % KO]));
+      else
+        k[i].load(reinterpret_cast<GlobalBytes>(__shfl(ko, i * RPI + krow)) +
+                  (k_off[0] - krow * p.k_slot));
+    }
+  };
+  auto load_v = [&]() {
+#pragma unroll
+    for (int i = 0; i < NX; ++i) {
+      uint64_t at_row = 0;
+      if constexpr (!P16) at_row = __shfl(vo, 16 * (i / 4) + 4 * g + i % 4);
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        if constexpr (P16)
+          v[i][n].load(vh[i / 4] + lane_offset(v_off[i % 4][n]));
+        else
+          v[i][n].load(reinterpret_cast<GlobalBytes>(at_row) +
+                       (v_off[0][n] - 4 * g * p.v_slot));
+      }
+    }
+  };
+  // Chunks beyond the head stay zero in LDS.
+  auto clear_k = [&]() {
+    if (!k_in) {
+#pragma unroll
+      for (int i = 0; i < NL; ++i) kt[k_place(i * RPI + krow, chunk)] = KRow{};
+    }
+  };
+
+  for (;;) {
+    const int len = cur.len, end = cur.end;
+    // The piece after this one: its first tile of the wave is requested in the
+    // last step of this one, its queries now.
+    const bool more = cur.at + cur.n < g1;
+    Piece next = cur;
+    if (more) {
+      if (cur.b + 1 == bt.b0 + kWave) bt = batch_at<TS>(p, cur.b + 1);
+      next = piece_of(cur.b + 1, cur.at + cur.n);
+    }
+    // The first piece of a share and the last have places of their own where
+    // they are not all of a sequence.
+    const bool all = cur.at >= g0 && cur.at + cur.n <= g1;
+    const int slot = 2 * share + (cur.at > g0);
+    if (cur.at >= g0 && head == 0 && group == 0 && threadIdx.x == 0) {
+      const int last = static_cast<int>(divide(cur.at + cur.n - 1, size));
+      p.meta[cur.b] = make_int2(slot, last - share + 1);
+    }
     // Rows: token r / G of the sequence's new ones, at position len - T + token.
     const int pos_0 = len - p.T;
     const int first_pos = pos_0 + first_tok, last_pos = pos_0 + last_tok;
     const int low_first = p.window ? max(0, first_pos - p.window + 1) : 0;
     const int low_last = p.window ? max(0, last_pos - p.window + 1) : 0;
-    for (int u = wave; u < R * NK; u += kWaves) {
-      const int j = u / NK, s = u % NK, r = r0 + 16 * j + l15, t = r / p.G;
-      const int d = (4 * s + g) * KV;
-      u32x4 x = {};
-      if (r < p.M && d < p.D)
-        x = *reinterpret_cast<const u32x4*>(
-            static_cast<const T*>(p.q) + b * p.q_seq + t * p.q_tok +
-            (static_cast<int64_t>(head) * p.G + (r - t * p.G)) * p.q_head + d);
-      if (negate) x ^= sizeof(T) == 4 ? 0x80000000u : 0x80008000u;
-      sq[j][s][lane] = __builtin_bit_cast(OpT, x);
-    }
 
-    // The piece's tiles, without those that no row of the group sees.
-    int begin = span.t0 + static_cast<int>(from_g - at);
-    int end = span.t0 + static_cast<int>(to_g - at);
-    begin = max(begin, low_first / TS);
-    end = min(end, last_pos < 0 ? 0 : last_pos / TS + 1);
-    const int32_t* const table = p.table + b * p.table_row;
-
-    KRow k[NL];
-    VRow v[NX][NB];
     f4_t acc[R][NB][VB] = {};
     float base[R], sum[R];
 #pragma unroll
@@ -436,97 +557,47 @@ __global__ void __launch_bounds__(kBlock, (waves_of<T, C, DP, R>())) attention_k
       base[j] = -INFINITY;
       sum[j] = 0.f;
     }
-
-    // The table's entries of a tile (P16: one for each half; else the lane's
-    // position's), -1 where there is no position.
-    int entry[P16 ? NH : 1];
-    auto look_up = [&](int tile) {
-#pragma unroll
-      for (int h = 0; h < (P16 ? NH : 1); ++h) {
-        const int pos = tile * TS + (P16 ? 16 * h : lane % TS);
-        const bool in = tile < end && pos < len;
-        const int e = table[in ? page_of(pos) : 0];
-        entry[h] = in ? e : -1;
-      }
-    };
-    // Where a tile's rows are, and which of its positions there are (a bit
-    // each).  Rows that are not there are read from the first page.
-    const char *kh[NH], *vh[NH];
-    int64_t ko = 0, vo = 0;
-    auto place = [&](int tile) -> uint64_t {
-      if constexpr (P16) {
-        uint64_t ok = 0;
-#pragma unroll
-        for (int h = 0; h < NH; ++h) {
-          const int pos = tile * TS + 16 * h;
-          const int e = __builtin_amdgcn_readfirstlane(entry[h]);
-          const bool in = static_cast<uint32_t>(e) < static_cast<uint32_t>(p.num_pages);
-          const uint32_t at_row = in ? pos - page_of(pos) * p.page_size : 0;
-          const int64_t page = in ? e : 0;
-          kh[h] = scalar(kc + (page * p.k_page + static_cast<int64_t>(at_row) * p.k_slot));
-          vh[h] = scalar(vc + (page * p.v_page + static_cast<int64_t>(at_row) * p.v_slot));
-          ok |= in ? uint64_t{0xffff} << (16 * h) : 0;
-        }
-        return ok;
-      } else {
-        const int pos = tile * TS + lane % TS;
-        const bool in = static_cast<uint32_t>(entry[0]) < static_cast<uint32_t>(p.num_pages);
-        const uint32_t at_row = in ? pos - page_of(pos) * p.page_size : 0;
-        const int64_t page = in ? entry[0] : 0;
-        ko = page * p.k_page + static_cast<int64_t>(at_row) * p.k_slot;
-        vo = page * p.v_page + static_cast<int64_t>(at_row) * p.v_slot;
-        return __ballot(in) & kAll;
-      }
-    };
-    auto load_k = [&]() {
-#pragma unroll
-      for (int i = 0; i < NL; ++i) {
-        if constexpr (P16)
-          k[i].load(kh[i * RPI / 16] + k_off[i % KO]);
-        else
-          k[i].load(kc + __shfl(ko, i * RPI + krow) + (k_off[0] - krow * p.k_slot));
-      }
-    };
-    auto load_v = [&]() {
-#pragma unroll
-      for (int i = 0; i < NX; ++i) {
-        int64_t off = 0;
-        if constexpr (!P16) off = __shfl(vo, 16 * (i / 4) + 4 * g + i % 4);
-#pragma unroll
-        for (int n = 0; n < NB; ++n) {
-          if constexpr (P16) v[i][n].load(vh[i / 4] + v_off[i % 4][n]);
-          else v[i][n].load(vc + off + (v_off[0][n] - 4 * g * p.v_slot));
-        }
-      }
-    };
-
-    __syncthreads();  // Q
-    int tile = begin + wave;
-    uint64_t ok = 0;
-    if (tile < end) {
-      look_up(tile);
-      ok = place(tile);
+    store_q();
+    clear_k();
+    int tile = cur.begin + wave;
+    const int ahead = next.begin + wave;
+    const bool go_on = more && ahead < next.end;
+    // A piece with one tile of the wave was entered without the table's entries
+    // of what comes after it.
+    const bool cross = go_on && tile < end && (!loaded || tile + kWaves < end);
+    if (tile < end && !loaded) {
+      look_up(cur.table, len, tile);
+      ok = place(len, tile);
       load_k();
+      // (the loop's order, by which it counts the loads to wait for)
+      const bool same = tile + kWaves < end || !cross;
+      look_up(same ? cur.table : next.table, same ? len : next.len,
+              same ? tile + kWaves : ahead);
       load_v();
-      look_up(tile + kWaves);
     }
+    if (more) load_q(next.b);
+    __syncthreads();  // Q
+    loaded = cross;
     while (tile < end) {
       const int pos0 = tile * TS;
       const bool whole = pos0 >= low_last && pos0 + TS - 1 <= first_pos && ok == kAll;
+      if (k_in) {
 #pragma unroll
-      for (int i = 0; i < NL; ++i) {
-        if (p.D < DP) k[i].keep(k_in);
-        kt[k_place(i * RPI + krow, chunk)] = k[i];
+        for (int i = 0; i < NL; ++i) kt[k_place(i * RPI + krow, chunk)] = k[i];
       }
-      const uint64_t ok_next = place(tile + kWaves);
+      // The wave's next two tiles, in this piece or the next one.
+      const bool in_1 = tile + kWaves < end || !cross, in_2 = tile + 2 * kWaves < end || !cross;
+      const int tile_1 = in_1 ? tile + kWaves : ahead;
+      const uint64_t ok_next = place(in_1 ? len : next.len, tile_1);
       load_k();
-      look_up(tile + 2 * kWaves);
+      look_up(in_2 ? cur.table : next.table, in_2 ? len : next.len,
+              in_2 ? tile + 2 * kWaves : (in_1 ? ahead : ahead + kWaves));
       f4_t sc[R][NH] = {};
 #pragma unroll
       for (int s = 0; s < NK; ++s) {
         OpT q[R];
 #pragma unroll
-        for (int j = 0; j < R; ++j) q[j] = sq[j][s][lane];
+        for (int j = 0; j < R; ++j) q[j] = sq[j * NK + s][lane];
 #pragma unroll
         for (int h = 0; h < NH; ++h) {
           const KRow row = kt[k_place(16 * h + l15, 4 * s + g)];
@@ -536,7 +607,7 @@ __global__ void __launch_bounds__(kBlock, (waves_of<T, C, DP, R>())) attention_k
 #pragma unroll
           for (int j = 0; j < R; ++j) sc[j][h] = mma(__builtin_bit_cast(OpT, w), q[j], sc[j][h]);
         }
-        if (s % 2) __builtin_amdgcn_sched_barrier(0);
+        if (s % 4 == 3) __builtin_amdgcn_sched_barrier(0);
       }
       // Positions that a row does not see; values that no row sees are no part
       // of the sums, whatever they are.
@@ -598,6 +669,7 @@ __global__ void __launch_bounds__(kBlock, (waves_of<T, C, DP, R>())) attention_k
           for (int i = 0; i < NX; ++i)
 #pragma unroll
             for (int n = 0; n < NB; ++n) v[i][n] = *v_at(i, n);
+          clear_k();
 #pragma unroll
           for (int j = 0; j < R; ++j)
 #pragma unroll
@@ -643,14 +715,15 @@ __global__ void __launch_bounds__(kBlock, (waves_of<T, C, DP, R>())) attention_k
             ph[j][i / KV][u] = hi;
             pl[j][i / KV][u] = lo;
           }
-        // (nothing to rescale in most tiles; the empty asm keeps the branch,
-        // without which old and scaled sums are both held)
+        // (nothing to rescale in most tiles; the empty asm keeps the products
+        // in the branch: before it, old and scaled sums would both be held)
         if (__any(keep != 1.f)) {
-          asm volatile("");
+          float by = keep;
+          asm volatile("" : "+v"(by));
 #pragma unroll
           for (int n = 0; n < NB; ++n)
 #pragma unroll
-            for (int e = 0; e < VB; ++e) acc[j][n][e] *= keep;
+            for (int e = 0; e < VB; ++e) acc[j][n][e] *= by;
         }
       }
       // acc += V^T P^T
@@ -686,7 +759,8 @@ __global__ void __launch_bounds__(kBlock, (waves_of<T, C, DP, R>())) attention_k
       tile += kWaves;
     }
 
-    // The waves join: a row's base is the largest, sums are scaled to it.
+    // The waves join: a row's base is the largest, sums are scaled to it.  Wide
+    // heads join in two halves.
     for (int j = 0; j < R; ++j) {
       const int rows = min(16, p.M - r0 - 16 * j);
       if (rows <= 0) break;
@@ -698,58 +772,56 @@ __global__ void __launch_bounds__(kBlock, (waves_of<T, C, DP, R>())) attention_k
         my_sum = j == i ? sum[i] : my_sum;
       }
       my_sum = over_groups(my_sum, [](float a, float c) { return a + c; });
-      __syncthreads();
-      if (g == 0) ml[wave][l15] = make_float2(my_base, my_sum);
-      __syncthreads();
-      float top = ml[0][l15].x;
 #pragma unroll
-      for (int w = 1; w < kWaves; ++w) top = fmaxf(top, ml[w][l15].x);
-      const float mine = weight(my_base, top);
-      if (l15 < rows) {
+      for (int half = 0; half < DP / DJ; ++half) {
+        __syncthreads();
+        if (half == 0 && g == 0) ml[wave][l15] = make_float2(my_base, my_sum);
+        if (l15 < rows) {
 #pragma unroll
-        for (int n = 0; n < NB; ++n)
+          for (int n = half * (NB * DJ / DP); n < (half + 1) * (NB * DJ / DP); ++n)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int e = 0; e < VB; e += 4) {
-              f4_t x;
+              for (int e = 0; e < VB; e += 4) {
+                f4_t x;
 #pragma unroll
-              for (int u = 0; u < 4; ++u) {
-                float y = acc[0][n][e + u][i];
+                for (int u = 0; u < 4; ++u) {
+                  float y = acc[0][n][e + u][i];
 #pragma unroll
-                for (int m = 1; m < R; ++m) y = j == m ? acc[m][n][e + u][i] : y;
-                x[u] = y * mine;
+                  for (int m = 1; m < R; ++m) y = j == m ? acc[m][n][e + u][i] : y;
+                  x[u] = y;
+                }
+                *reinterpret_cast<f4_t*>(
+                    &sh.acc[wave][l15][(n * 16 + 4 * g + i) * VB + e - half * DJ]) = x;
               }
-              *reinterpret_cast<f4_t*>(&sh.acc[wave][l15][(n * 16 + 4 * g + i) * VB + e]) = x;
-            }
-      }
-      __syncthreads();
-      const int quads = p.D / 4;
-      for (int u = threadIdx.x; u < rows * quads; u += kBlock) {
-        const int row = u / quads, d = (u - row * quads) * 4, r = r0 + 16 * j + row;
-        float m = ml[0][row].x;
-#pragma unroll
-        for (int w = 1; w < kWaves; ++w) m = fmaxf(m, ml[w][row].x);
-        float l = 0.f;
-        f4_t x = {};
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-          l += ml[w][row].y * weight(ml[w][row].x, m);
-          x += *reinterpret_cast<const f4_t*>(&sh.acc[w][row][d]);
         }
-        if (all) {
-          write_row<T>(p, b, head, r, d, x, m, l);
-        } else {
-          const int64_t to = (static_cast<int64_t>(slot) * p.Hkv + head) * p.M + r;
-          *reinterpret_cast<f4_t*>(p.acc + to * p.D + d) = x;
-          if (d == 0) p.ml[to] = make_float2(m, l);
+        __syncthreads();
+        const int quads = (min(p.D, (half + 1) * DJ) - half * DJ) / 4;
+        for (int u = threadIdx.x; u < rows * quads; u += kBlock) {
+          const int row = u / quads, d = (u - row * quads) * 4, r = r0 + 16 * j + row;
+          float m = ml[0][row].x;
+#pragma unroll
+          for (int w = 1; w < kWaves; ++w) m = fmaxf(m, ml[w][row].x);
+          float l = 0.f;
+          f4_t x = {};
+#pragma unroll
+          for (int w = 0; w < kWaves; ++w) {
+            const float by = weight(ml[w][row].x, m);
+            l += ml[w][row].y * by;
+            x += *reinterpret_cast<const f4_t*>(&sh.acc[w][row][d]) * by;
+          }
+          if (all) {
+            write_row<T>(p, cur.b, head, r, half * DJ + d, x, m, l);
+          } else {
+            const int64_t to = (static_cast<int64_t>(slot) * p.Hkv + head) * p.M + r;
+            *reinterpret_cast<f4_t*>(p.acc + to * p.D + half * DJ + d) = x;
+            if (half * DJ + d == 0) p.ml[to] = make_float2(m, l);
+          }
         }
       }
     }
-
-    at += span.n;
-    if (at >= g1) break;
-    if (++b == bt.b0 + kWave) bt = batch_at<TS>(p, b);
+    if (!more) break;
+    cur = next;
     __syncthreads();  // the join's reads are over
   }
 }

@@ -8,6 +8,7 @@ namespace {
 
 constexpr int64_t kMostPositions = int64_t{1} << 28;  // a sequence's, by its table row
 constexpr int64_t kMostPitch = int64_t{1} << 27;      // bytes from one position to the next
+constexpr int64_t kMostPage = int64_t{1} << 35;       // and from one page to the next
 
 struct Plan {
   int tiles;  // row tiles of a wave
@@ -92,8 +93,9 @@ extern "C" int xk_paged_attention(
       stride_vc_head % n || !aligned(out, 4 * eb) || stride_o_seq % 4 || stride_o_tok % 4 ||
       stride_o_head % 4)
     return XK_ERR_UNSUPPORTED;
-  if (stride_kc_slot < 0 || stride_vc_slot < 0 || stride_kc_slot * cb >= kMostPitch ||
-      stride_vc_slot * cb >= kMostPitch)
+  if (stride_kc_slot < 0 || stride_vc_slot < 0 || stride_kc_slot >= kMostPitch / cb ||
+      stride_vc_slot >= kMostPitch / cb || stride_kc_page < 0 || stride_vc_page < 0 ||
+      stride_kc_page >= kMostPage / cb || stride_vc_page >= kMostPage / cb)
     return XK_ERR_INVALID;
   const int64_t positions = num_pages ? max_pages * page_size : 0;
   Plan x;
@@ -107,11 +109,11 @@ extern "C" int xk_paged_attention(
   p.q_tok = stride_q_tok;
   p.q_head = stride_q_head;
   p.kc = static_cast<const char*>(k_cache);
-  p.k_page = stride_kc_page * cb;
+  p.k_page = static_cast<uint32_t>(stride_kc_page * cb / 8);
   p.k_slot = static_cast<uint32_t>(stride_kc_slot * cb);
   p.k_head = stride_kc_head * cb;
   p.vc = static_cast<const char*>(v_cache);
-  p.v_page = stride_vc_page * cb;
+  p.v_page = static_cast<uint32_t>(stride_vc_page * cb / 8);
   p.v_slot = static_cast<uint32_t>(stride_vc_slot * cb);
   p.v_head = stride_vc_head * cb;
   p.num_pages = static_cast<int>(num_pages);
