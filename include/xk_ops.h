@@ -724,7 +724,7 @@ int xk_rotary_cache_append(
  */
 int64_t xk_paged_attention_workspace_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hkv,
                                            int64_t head_dim, int64_t max_pages,
-                                           int64_t page_size);
+                                           int64_t page_size, xk_dtype dtype);
 int xk_paged_attention(
     const void* q, int64_t stride_q_seq, int64_t stride_q_tok, int64_t stride_q_head,
     const void* k_cache, int64_t stride_kc_page, int64_t stride_kc_slot, int64_t stride_kc_head,

@@ -122,7 +122,7 @@ SIGNATURES: dict[str, tuple[list, object]] = {
     "xk_rotary_cache_append": (
         [P, I64, I64, P, I64, I64, I64, P, I64, I64, P, I64, I64, I64, P, I64, I64, I64, P, I64,
          I64, I64, INT, I64, I64, P, INT, P, INT, P, I64, INT, F32, P, P, I64, I64, INT, P], INT),
-    "xk_paged_attention_workspace_bytes": ([I64, I64, I64, I64, I64, I64, I64], I64),
+    "xk_paged_attention_workspace_bytes": ([I64, I64, I64, I64, I64, I64, I64, INT], I64),
     "xk_paged_attention": (
         [P, I64, I64, I64, P, I64, I64, I64, P, I64, I64, I64, INT, I64, I64, P, I64, I64, P, F32,
          I64, P, P, P, I64, I64, I64, P, I64, I64, I64, I64, I64, INT, P, SZ, P], INT),

@@ -84,11 +84,26 @@ struct Params {
   int64_t o_seq, o_tok, o_head;
   float* lse;
   int B, T, G, Hkv, D, M, groups;  // M = T * G rows of a head in `groups` groups
+  uint32_t g_magic;                // r / G = r * g_magic >> g_shift for r < 2^28
+  int g_shift;
   int shares;                      // of a head and group, at the most
   int2* meta;                      // [B]: first piece, pieces
   float2* ml;                      // [2 * shares][Hkv][M]: base, sum
   float* acc;                      // [2 * shares][Hkv][M][D]
 };
+
+// The kernel's arguments, loaded again: values that are used once a sequence are
+// not kept in scalar registers through the loop, where they are short.
+using LateParams = const __attribute__((address_space(4))) Params*;
+__device__ __forceinline__ LateParams late_params() {
+  auto x = reinterpret_cast<uint64_t>(__builtin_amdgcn_kernarg_segment_ptr());
+  asm volatile("" : "+s"(x));
+  return reinterpret_cast<LateParams>(x);
+}
+template <typename P>
+__device__ __forceinline__ int token_of(P p, int r) {
+  return static_cast<int>(static_cast<uint64_t>(r) * p->g_magic >> p->g_shift);
+}
 
 // A sequence's tiles: from the first that a row sees to the last; an empty
 // sequence has one, so that its rows are written.
@@ -272,20 +287,20 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t&
 }
 
 // Writes 4 elements of a finished row, and its lse.
-template <typename T>
-__device__ __forceinline__ void write_row(const Params& p, int b, int head, int r, int d,
-                                          f4_t x, float base, float l) {
-  const int tok = r / p.G;
-  const int64_t hq = static_cast<int64_t>(head) * p.G + (r - tok * p.G);
+template <typename T, typename P>
+__device__ __forceinline__ void write_row(P p, int b, int head, int r, int d, f4_t x, float base,
+                                          float l) {
+  const int tok = token_of(p, r);
+  const int64_t hq = static_cast<int64_t>(head) * p->G + (r - tok * p->G);
   // A row that sees nothing has no weights: 0.
-  const float inv = l == 0.f ? 0.f : (p.v_scale ? p.v_scale[head] : 1.f) / l;
+  const float inv = l == 0.f ? 0.f : (p->v_scale ? p->v_scale[head] : 1.f) / l;
   float o[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) o[i] = l == 0.f ? 0.f : x[i] * inv;
-  store_vec_f32<T, 4>(static_cast<T*>(p.out) + b * p.o_seq + tok * p.o_tok + hq * p.o_head + d,
-                      o);
-  if (p.lse && d == 0)
-    p.lse[(static_cast<int64_t>(b) * p.T + tok) * p.Hkv * p.G + hq] =
+  store_vec_f32<T, 4>(
+      static_cast<T*>(p->out) + b * p->o_seq + tok * p->o_tok + hq * p->o_head + d, o);
+  if (p->lse && d == 0)
+    p->lse[(static_cast<int64_t>(b) * p->T + tok) * p->Hkv * p->G + hq] =
         l == 0.f ? -INFINITY : (base + __log2f(l)) * 0.69314718056f;
 }
 
@@ -322,7 +337,7 @@ __global__ void __launch_bounds__(kBlock, (waves_of<T, C, DP, R>())) attention_k
   constexpr int VB = KV < DP / 16 ? KV : DP / 16;  // V: elements of a load
   constexpr int NB = DP / (16 * VB);               // and loads of a row
   constexpr int NX = KV * NS;                      // scores of a lane and row tile
-  constexpr uint64_t kAll = TS == 64 ? ~uint64_t{0} : (uint64_t{1} << TS) - 1;
+  constexpr uint64_t kAll = ~uint64_t{0} >> (64 - TS);
   // log2 of what p is scaled by (see above).
   constexpr float kShift = std::is_same<T, f16>::value ? 14.f : 0.f;
   using KRow = Row<T, C, KV>;
@@ -383,12 +398,12 @@ __global__ void __launch_bounds__(kBlock, (waves_of<T, C, DP, R>())) attention_k
   const bool negate = scale2 < 0.f;
   scale2 = fmaxf(fabsf(scale2), 1.17549435e-38f);
   const int r0 = group * 16 * R;
-  const int first_tok = r0 / p.G, last_tok = min(p.M - 1, r0 + 16 * R - 1) / p.G;
+  const int first_tok = token_of(&p, r0), last_tok = token_of(&p, min(p.M - 1, r0 + 16 * R - 1));
   int tok[R];  // of the lane's rows; beyond them, one that sees nothing
 #pragma unroll
   for (int j = 0; j < R; ++j) {
     const int r = r0 + 16 * j + l15;
-    tok[j] = r < p.M ? r / p.G : -(1 << 30);
+    tok[j] = r < p.M ? token_of(&p, r) : -(1 << 30);
   }
   // K's chunks lie in the wave's part of LDS with a row's chunks permuted, so
   // that the 16 rows of one operand's read fall on different banks.
@@ -427,15 +442,16 @@ __global__ void __launch_bounds__(kBlock, (waves_of<T, C, DP, R>())) attention_k
   constexpr int NQ = (R * NK + kWaves - 1) / kWaves;
   u32x4 qx[NQ];
   auto load_q = [&](int seq) {
+    const LateParams late = late_params();
 #pragma unroll
     for (int c = 0; c < NQ; ++c) {
       const int u = c * kWaves + wave, j = u / NK, s = u % NK;
-      const int r = r0 + 16 * j + l15, t = r / p.G, d = (4 * s + g) * KV;
+      const int r = r0 + 16 * j + l15, t = token_of(late, r), d = (4 * s + g) * KV;
       qx[c] = u32x4{};
-      if (u < R * NK && r < p.M && d < p.D)
+      if (u < R * NK && r < late->M && d < late->D)
         qx[c] = *reinterpret_cast<const u32x4*>(
-            static_cast<const T*>(p.q) + seq * p.q_seq + t * p.q_tok +
-            (static_cast<int64_t>(head) * p.G + (r - t * p.G)) * p.q_head + d);
+            static_cast<const T*>(late->q) + seq * late->q_seq + t * late->q_tok +
+            (static_cast<int64_t>(head) * late->G + (r - t * late->G)) * late->q_head + d);
     }
   };
   auto store_q = [&]() {
@@ -493,6 +509,8 @@ __global__ void __launch_bounds__(kBlock, (waves_of<T, C, DP, R>())) attention_k
       return __ballot(in) & kAll;
     }
   };
+  // (of a tile that there is not, 16 bytes in place of each 1 KB)
+  uint32_t wanted = ~0u;
   auto load_k = [&]() {
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
@@ -542,7 +560,7 @@ __global__ void __launch_bounds__(kBlock, (waves_of<T, C, DP, R>())) attention_k
     const int slot = 2 * share + (cur.at > g0);
     if (cur.at >= g0 && head == 0 && group == 0 && threadIdx.x == 0) {
       const int last = static_cast<int>(divide(cur.at + cur.n - 1, size));
-      p.meta[cur.b] = make_int2(slot, last - share + 1);
+      late_params()->meta[cur.b] = make_int2(slot, last - share + 1);
     }
     // Rows: token r / G of the sequence's new ones, at position len - T + token.
     const int pos_0 = len - p.T;
@@ -557,17 +575,18 @@ __global__ void __launch_bounds__(kBlock, (waves_of<T, C, DP, R>())) attention_k
       base[j] = -INFINITY;
       sum[j] = 0.f;
     }
-    store_q();
-    clear_k();
     int tile = cur.begin + wave;
     const int ahead = next.begin + wave;
     const bool go_on = more && ahead < next.end;
     // A piece with one tile of the wave was entered without the table's entries
     // of what comes after it.
     const bool cross = go_on && tile < end && (!loaded || tile + kWaves < end);
+    if (tile < end && !loaded) look_up(cur.table, len, tile);
+    store_q();
+    clear_k();
     if (tile < end && !loaded) {
-      look_up(cur.table, len, tile);
       ok = place(len, tile);
+      wanted = ~0u;
       load_k();
       // (the loop's order, by which it counts the loads to wait for)
       const bool same = tile + kWaves < end || !cross;
@@ -588,6 +607,7 @@ __global__ void __launch_bounds__(kBlock, (waves_of<T, C, DP, R>())) attention_k
       // The wave's next two tiles, in this piece or the next one.
       const bool in_1 = tile + kWaves < end || !cross, in_2 = tile + 2 * kWaves < end || !cross;
       const int tile_1 = in_1 ? tile + kWaves : ahead;
+      wanted = tile_1 < (in_1 ? end : next.end) ? ~0u : 0u;
       const uint64_t ok_next = place(in_1 ? len : next.len, tile_1);
       load_k();
       look_up(in_2 ? cur.table : next.table, in_2 ? len : next.len,
@@ -796,9 +816,10 @@ __global__ void __launch_bounds__(kBlock, (waves_of<T, C, DP, R>())) attention_k
               }
         }
         __syncthreads();
-        const int quads = (min(p.D, (half + 1) * DJ) - half * DJ) / 4;
-        for (int u = threadIdx.x; u < rows * quads; u += kBlock) {
-          const int row = u / quads, d = (u - row * quads) * 4, r = r0 + 16 * j + row;
+        const LateParams late = late_params();
+        for (int u = threadIdx.x; u < rows * (DJ / 4); u += kBlock) {
+          const int row = u / (DJ / 4), d = u % (DJ / 4) * 4, r = r0 + 16 * j + row;
+          if (half * DJ + d >= late->D) continue;
           float m = ml[0][row].x;
 #pragma unroll
           for (int w = 1; w < kWaves; ++w) m = fmaxf(m, ml[w][row].x);
@@ -811,11 +832,11 @@ __global__ void __launch_bounds__(kBlock, (waves_of<T, C, DP, R>())) attention_k
             x += *reinterpret_cast<const f4_t*>(&sh.acc[w][row][d]) * by;
           }
           if (all) {
-            write_row<T>(p, cur.b, head, r, half * DJ + d, x, m, l);
+            write_row<T>(late, cur.b, head, r, half * DJ + d, x, m, l);
           } else {
-            const int64_t to = (static_cast<int64_t>(slot) * p.Hkv + head) * p.M + r;
-            *reinterpret_cast<f4_t*>(p.acc + to * p.D + half * DJ + d) = x;
-            if (half * DJ + d == 0) p.ml[to] = make_float2(m, l);
+            const int64_t to = (static_cast<int64_t>(slot) * late->Hkv + head) * late->M + r;
+            *reinterpret_cast<f4_t*>(late->acc + to * late->D + half * DJ + d) = x;
+            if (half * DJ + d == 0) late->ml[to] = make_float2(m, l);
           }
         }
       }
@@ -846,7 +867,7 @@ __global__ void __launch_bounds__(kBlock) join_kernel(Params p, int team) {
     const int r = r0 + own / split;
     float base = -INFINITY, sum = 0.f;
     f4_t acc = {};
-    constexpr int kAhead = 4;  // pieces that a lane requests together
+    constexpr int kAhead = 8;  // pieces that a lane requests together
     for (int i0 = part; i0 < pieces && r < p.M; i0 += kAhead * split) {
       float2 x[kAhead];
       f4_t y[kAhead];
@@ -884,7 +905,7 @@ __global__ void __launch_bounds__(kBlock) join_kernel(Params p, int team) {
         l += ml[own + i].y * weight(ml[own + i].x, top);
         x += sums[threadIdx.x + i * team];
       }
-      write_row<T>(p, b, head, r, d, x, top, l);
+      write_row<T>(&p, b, head, r, d, x, top, l);
     }
     __syncthreads();
   }

@@ -17,9 +17,11 @@ struct Plan {
 
 // False where the sizes are beyond what a launch holds.
 bool plan_of(int64_t B, int64_t T, int64_t G, int64_t Hkv, int64_t D, int64_t positions,
-             Plan& x) {
+             xk_dtype dtype, Plan& x) {
   const int64_t M = T * G;
-  x.tiles = M > 16 ? 2 : 1;
+  if (M >= kMostPositions) return false;
+  // (two row tiles of fp32 heads of 256 do not fit the registers)
+  x.tiles = M > 16 && (D <= 128 || dtype != XK_F32) ? 2 : 1;
   x.groups = cdiv(M, 16 * x.tiles);
   // The shares of a head and row group: two blocks a compute unit in all (the
   // kernels that only fit once take half), none without a least share.
@@ -32,6 +34,14 @@ bool plan_of(int64_t B, int64_t T, int64_t G, int64_t Hkv, int64_t D, int64_t po
   auto up = [](int64_t n) { return cdiv(n, 256) * 256; };
   x.bytes = up(B * 8) + up(rows * 8) + up(rows * D * 4);
   return true;
+}
+
+// n / by = n * magic >> shift for n < 2^28: by * magic is above 2^shift by e < by
+// <= 2^(shift - 28), so n * magic / 2^shift is above n / by by less than 1 / by.
+void magic_of(int64_t by, uint32_t& magic, int& shift) {
+  shift = 28;
+  while ((int64_t{1} << (shift - 28)) < by) ++shift;
+  magic = static_cast<uint32_t>(cdiv(int64_t{1} << shift, by));
 }
 
 int check_sizes(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_pages,
@@ -53,10 +63,11 @@ using namespace xk;
 
 extern "C" int64_t xk_paged_attention_workspace_bytes(int64_t B, int64_t T, int64_t Hq,
                                                       int64_t Hkv, int64_t head_dim,
-                                                      int64_t max_pages, int64_t page_size) {
+                                                      int64_t max_pages, int64_t page_size,
+                                                      xk_dtype dtype) {
   paged::Plan x;
   if (paged::check_sizes(B, T, Hq, Hkv, head_dim, max_pages, page_size) != XK_OK || B == 0 ||
-      !paged::plan_of(B, T, Hq / Hkv, Hkv, head_dim, max_pages * page_size, x))
+      !paged::plan_of(B, T, Hq / Hkv, Hkv, head_dim, max_pages * page_size, dtype, x))
     return 0;
   return x.bytes;
 }
@@ -99,7 +110,7 @@ extern "C" int xk_paged_attention(
     return XK_ERR_INVALID;
   const int64_t positions = num_pages ? max_pages * page_size : 0;
   Plan x;
-  if (!plan_of(B, T, Hq / Hkv, Hkv, head_dim, max_pages * page_size, x))
+  if (!plan_of(B, T, Hq / Hkv, Hkv, head_dim, max_pages * page_size, dtype, x))
     return XK_ERR_INVALID;
   if (!workspace || workspace_bytes < static_cast<size_t>(x.bytes) || !aligned(workspace, 256))
     return XK_ERR_WORKSPACE;
@@ -118,11 +129,7 @@ extern "C" int xk_paged_attention(
   p.v_head = stride_vc_head * cb;
   p.num_pages = static_cast<int>(num_pages);
   p.page_size = static_cast<int>(page_size);
-  // n / page_size for n < 2^28: n * magic is off by less than 2^28 * page_size
-  // from n * 2^shift / page_size, which is below the 2^shift of one step.
-  p.page_shift = 28;
-  while ((int64_t{1} << (p.page_shift - 28)) < page_size) ++p.page_shift;
-  p.page_magic = static_cast<uint32_t>(cdiv(int64_t{1} << p.page_shift, page_size));
+  magic_of(page_size, p.page_magic, p.page_shift);
   p.table = block_table;
   p.table_row = stride_table_row;
   p.max_pages = static_cast<int>(max_pages);
@@ -142,6 +149,7 @@ extern "C" int xk_paged_attention(
   p.G = static_cast<int>(Hq / Hkv);
   p.Hkv = static_cast<int>(Hkv);
   p.D = static_cast<int>(head_dim);
+  magic_of(Hq / Hkv, p.g_magic, p.g_shift);
   p.M = static_cast<int>(T * (Hq / Hkv));
   p.groups = static_cast<int>(x.groups);
   p.shares = static_cast<int>(x.shares);

@@ -1442,7 +1442,7 @@ std::tuple<torch::Tensor, std::optional<torch::Tensor>> npu_paged_attention(
                                                                       : block_table.contiguous();
   auto lens = seq_lens.contiguous();
   const int64_t bytes = xk_paged_attention_workspace_bytes(B, T, Hq, Hkv, D, table.size(1),
-                                                           k_cache.size(1));
+                                                           k_cache.size(1), xdt(q));
   if (bytes > 0) ws = workspace(bytes, q.device());
   check(xk_paged_attention(
             qr.data_ptr(), s[0], s[1], s[2], k_cache.data_ptr(), pitch_of(k_cache, 0),

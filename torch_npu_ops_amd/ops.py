@@ -1495,7 +1495,7 @@ def npu_paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
         lse = _f32(q, B, T, Hq) if output_lse else None
         if T > 0:
             size = lib().xk_paged_attention_workspace_bytes(B, T, Hq, Hkv, D, table.size(1),
-                                                            k_cache.size(1))
+                                                            k_cache.size(1), xk_dtype(q))
             ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
             st = lib().xk_paged_attention(
                 q4.data_ptr(), *(_stride(q4, d) for d in range(3)), k_cache.data_ptr(),
