@@ -714,8 +714,8 @@ int xk_rotary_cache_append(
  *   has no part in that row.
  *   q, k_cache and v_cache 16-byte aligned (8 for an 8-bit cache), their
  *   strides whole vectors of that size, out's of 4 elements (else
- *   XK_ERR_UNSUPPORTED); pitches of places below 2^27 bytes, of pages below
- *   2^35, neither negative.
+ *   XK_ERR_UNSUPPORTED); the pitch of places times page_size below 2^32 bytes
+ *   (and itself below 2^27), that of pages below 2^35, neither negative.
  *   The split of the positions follows from all lengths of the batch: a
  *   sequence's last bits depend on the batch, but not on the run.
  *   workspace >= xk_paged_attention_workspace_bytes(...) bytes for the same

@@ -280,8 +280,11 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t&
 }
 __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo, f16) {
   const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
-  const auto l = __builtin_amdgcn_cvt_pkrtz(a - static_cast<float>(h[0]),
-                                            b - static_cast<float>(h[1]));
+  float minus = -1.f;  // (a product takes fp16 operands as they are, a difference does not)
+  asm("" : "+v"(minus));
+  const auto l =
+      __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf(static_cast<float>(h[0]), minus, a),
+                                 __builtin_fmaf(static_cast<float>(h[1]), minus, b));
   hi = __builtin_bit_cast(uint32_t, h);
   lo = __builtin_bit_cast(uint32_t, l);
 }
@@ -306,8 +309,9 @@ __device__ __forceinline__ void write_row(P p, int b, int head, int r, int d, f4
 
 // ---------------------------------------------------------------------------
 // The kernel.  DP: the head's length, rounded up to 64, 128 or 256.  R: row
-// tiles of a wave.  P16: pages are whole runs of 16 positions, so that a half
-// tile lies in one page and its address is one scalar.
+// tiles of a wave.  RUN: positions (16 at least, a tile at most) that pages are
+// whole runs of, with one scalar address each; 0 for none, an address for each
+// lane and load.
 // ---------------------------------------------------------------------------
 // Tiles hold 8 KB of keys where rows are short: fewer rounds of statistics.
 template <typename T, typename C, int DP>
@@ -323,7 +327,7 @@ constexpr int waves_of() {
   return DP * R / 4 + 2 * kTile > 128 ? 1 : 2;
 }
 
-template <typename T, typename C, int DP, int R, bool P16>
+template <typename T, typename C, int DP, int R, int RUN>
 __global__ void __launch_bounds__(kBlock, (waves_of<T, C, DP, R>())) attention_kernel(Params p) {
   using OpT = typename Op<T>::type;
   constexpr int CB = sizeof(C);
@@ -376,19 +380,6 @@ __global__ void __launch_bounds__(kBlock, (waves_of<T, C, DP, R>())) attention_k
   at += __builtin_amdgcn_readlane(bt.incl - bt.own.n, b);
   b += bt.b0;
 
-  // What holds for every sequence: lane offsets from the start of a half tile;
-  // beyond the head the row's last vector again.
-  const int chunk = lane % CH, krow = lane / CH;
-  const bool k_in = chunk * KV < p.D;
-  uint32_t k_off[KO], v_off[4][NB];
-#pragma unroll
-  for (int i = 0; i < KO; ++i)
-    k_off[i] = (i * RPI + krow) * p.k_slot + min(chunk * KV, p.D - KV) * CB;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int n = 0; n < NB; ++n)
-      v_off[i][n] = (4 * g + i) * p.v_slot + min((n * 16 + l15) * VB, p.D - VB) * CB;
   const uint64_t kc = reinterpret_cast<uint64_t>(p.kc + head * p.k_head);
   const uint64_t vc = reinterpret_cast<uint64_t>(p.vc + head * p.v_head);
   // Scores are scaled by something positive, that leaves a masked one -inf: a
@@ -399,12 +390,6 @@ __global__ void __launch_bounds__(kBlock, (waves_of<T, C, DP, R>())) attention_k
   scale2 = fmaxf(fabsf(scale2), 1.17549435e-38f);
   const int r0 = group * 16 * R;
   const int first_tok = token_of(&p, r0), last_tok = token_of(&p, min(p.M - 1, r0 + 16 * R - 1));
-  int tok[R];  // of the lane's rows; beyond them, one that sees nothing
-#pragma unroll
-  for (int j = 0; j < R; ++j) {
-    const int r = r0 + 16 * j + l15;
-    tok[j] = r < p.M ? token_of(&p, r) : -(1 << 30);
-  }
   // K's chunks lie in the wave's part of LDS with a row's chunks permuted, so
   // that the 16 rows of one operand's read fall on different banks.
   KRow* const kt = sh.k[wave];
@@ -463,58 +448,82 @@ __global__ void __launch_bounds__(kBlock, (waves_of<T, C, DP, R>())) attention_k
     }
   };
 
+  // The table's entries of a tile (one, one for each half, or the lane's
+  // position's).  Positions past the sequence's end stand for its last ones.
+  constexpr int NE = RUN ? TS / RUN : 1;
+  auto pos_of = [&](int len, int tile, int h) {
+    return RUN ? min(tile * TS + RUN * h, (len - 1) & -RUN) : min(tile * TS + lane % TS, len - 1);
+  };
+  int entry[NE];
+  auto look_up = [&](const int32_t* table, int len, int tile) {
+#pragma unroll
+    for (int h = 0; h < NE; ++h) entry[h] = table[page_of(pos_of(len, tile, h))];
+  };
+  // What the first tile waits for is requested before all else is computed.
   Piece cur = piece_of(b, at);
+  if (cur.begin + wave < cur.end) look_up(cur.table, cur.len, cur.begin + wave);
   load_q(b);
+  bool first = true;
   bool loaded = false;  // the registers hold the piece's first tile of the wave
+  // What holds for every sequence: lane offsets from the start of a half tile;
+  // beyond the head the row's last vector again.
+  const int chunk = lane % CH, krow = lane / CH;
+  const bool k_in = chunk * KV < p.D;
+  uint32_t k_off[KO], v_off[4][NB];
+#pragma unroll
+  for (int i = 0; i < KO; ++i)
+    k_off[i] = (i * RPI + krow) * p.k_slot + min(chunk * KV, p.D - KV) * CB;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+      v_off[i][n] = (4 * g + i) * p.v_slot + min((n * 16 + l15) * VB, p.D - VB) * CB;
+  int tok[R];  // of the lane's rows; beyond them, one that sees nothing
+#pragma unroll
+  for (int j = 0; j < R; ++j) {
+    const int r = r0 + 16 * j + l15;
+    tok[j] = r < p.M ? token_of(&p, r) : -(1 << 30);
+  }
   KRow k[NL];
   VRow v[NX][NB];
   uint64_t ok = 0;  // which positions of the tile there are
-  // The table's entries of a tile (P16: one for each half; else the lane's
-  // position's).  Positions past the sequence's end stand for its last ones.
-  auto pos_of = [&](int len, int tile, int h) {
-    return min(tile * TS + (P16 ? 16 * h : lane % TS), P16 ? (len - 1) & ~15 : len - 1);
-  };
-  int entry[P16 ? NH : 1];
-  auto look_up = [&](const int32_t* table, int len, int tile) {
-#pragma unroll
-    for (int h = 0; h < (P16 ? NH : 1); ++h) entry[h] = table[page_of(pos_of(len, tile, h))];
-  };
   // Where a tile's rows are, and which of them are in a page that there is
   // (a bit each); the others are read from the first page.
   GlobalBytes kh[NH], vh[NH];
   uint64_t ko = 0, vo = 0;
   auto place = [&](int len, int tile) -> uint64_t {
-    if constexpr (P16) {
-      uint64_t ok = 0;
+    uint64_t ok = 0;
 #pragma unroll
-      for (int h = 0; h < NH; ++h) {
-        const uint32_t e = __builtin_amdgcn_readfirstlane(entry[h]);
-        const bool in = e < static_cast<uint32_t>(p.num_pages);
-        const uint64_t page = in ? e : 0;
-        const int pos = pos_of(len, tile, h);
-        const uint64_t row = pos - page_of(pos) * p.page_size;
-        kh[h] = scalar(kc + (page * p.k_page << 3) + row * p.k_slot);
-        vh[h] = scalar(vc + (page * p.v_page << 3) + row * p.v_slot);
-        ok |= in ? uint64_t{0xffff} << (16 * h) : 0;
-      }
-      return ok;
-    } else {
-      const uint32_t e = entry[0];
+    for (int h = 0; h < NE; ++h) {
+      const uint32_t e = RUN ? __builtin_amdgcn_readfirstlane(entry[h]) : entry[h];
       const bool in = e < static_cast<uint32_t>(p.num_pages);
       const uint64_t page = in ? e : 0;
-      const int pos = pos_of(len, tile, 0);
-      const uint64_t row = pos - page_of(pos) * p.page_size;
+      const int pos = pos_of(len, tile, h);
+      const uint32_t row = pos - page_of(pos) * p.page_size;
       ko = kc + (page * p.k_page << 3) + row * p.k_slot;
       vo = vc + (page * p.v_page << 3) + row * p.v_slot;
-      return __ballot(in) & kAll;
+      if constexpr (RUN == 0) {
+        ok = __ballot(in) & kAll;
+      } else {
+        constexpr int kPer = RUN / 16;  // half tiles of a run
+        kh[h * kPer] = scalar(ko);
+        vh[h * kPer] = scalar(vo);
+#pragma unroll
+        for (int u = 1; u < kPer; ++u) {
+          kh[h * kPer + u] = kh[h * kPer] + u * (16 * p.k_slot);
+          vh[h * kPer + u] = vh[h * kPer] + u * (16 * p.v_slot);
+        }
+        ok |= in ? (~uint64_t{0} >> (64 - RUN)) << (RUN * h) : 0;
+      }
     }
+    return ok;
   };
   // (of a tile that there is not, 16 bytes in place of each 1 KB)
   uint32_t wanted = ~0u;
   auto load_k = [&]() {
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
-      if constexpr (P16)
+      if constexpr (RUN > 0)
         k[i].load(kh[i * RPI / 16] + lane_offset(k_off[i % KO]));
       else
         k[i].load(reinterpret_cast<GlobalBytes>(__shfl(ko, i * RPI + krow)) +
@@ -525,10 +534,10 @@ __global__ void __launch_bounds__(kBlock, (waves_of<T, C, DP, R>())) attention_k
 #pragma unroll
     for (int i = 0; i < NX; ++i) {
       uint64_t at_row = 0;
-      if constexpr (!P16) at_row = __shfl(vo, 16 * (i / 4) + 4 * g + i % 4);
+      if constexpr (RUN == 0) at_row = __shfl(vo, 16 * (i / 4) + 4 * g + i % 4);
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
-        if constexpr (P16)
+        if constexpr (RUN > 0)
           v[i][n].load(vh[i / 4] + lane_offset(v_off[i % 4][n]));
         else
           v[i][n].load(reinterpret_cast<GlobalBytes>(at_row) +
@@ -581,7 +590,8 @@ __global__ void __launch_bounds__(kBlock, (waves_of<T, C, DP, R>())) attention_k
     // A piece with one tile of the wave was entered without the table's entries
     // of what comes after it.
     const bool cross = go_on && tile < end && (!loaded || tile + kWaves < end);
-    if (tile < end && !loaded) look_up(cur.table, len, tile);
+    if (tile < end && !loaded && !first) look_up(cur.table, len, tile);
+    first = false;
     store_q();
     clear_k();
     if (tile < end && !loaded) {
@@ -918,10 +928,15 @@ void launch_pages(Params& p, hipStream_t s) {
   p.shares = static_cast<int>(std::min<int64_t>(
       p.shares, std::max<int64_t>(1, int64_t{num_cus()} * waves_of<T, C, DP, R>() / lines)));
   const dim3 grid(static_cast<uint32_t>(p.shares * lines));
-  if (p.page_size % 16 == 0)
-    hipLaunchKernelGGL((attention_kernel<T, C, DP, R, true>), grid, dim3(kBlock), 0, s, p);
-  else
-    hipLaunchKernelGGL((attention_kernel<T, C, DP, R, false>), grid, dim3(kBlock), 0, s, p);
+  constexpr int kTile = subs_of<T, C, DP>() * 64 / static_cast<int>(sizeof(T));
+  auto launch = [&](auto run) {
+    if constexpr (run <= kTile)
+      hipLaunchKernelGGL((attention_kernel<T, C, DP, R, run>), grid, dim3(kBlock), 0, s, p);
+  };
+  if (kTile >= 64 && p.page_size % 64 == 0) launch(std::integral_constant<int, 64>());
+  else if (kTile >= 32 && p.page_size % 32 == 0) launch(std::integral_constant<int, 32>());
+  else if (p.page_size % 16 == 0) launch(std::integral_constant<int, 16>());
+  else launch(std::integral_constant<int, 0>());
 }
 
 template <typename T, typename C, int DP>

@@ -1,5 +1,7 @@
 // xk_paged_attention: checks, the plan's host part and the choice of instance
 // (the kernels are in paged_attention.h).
+#include <algorithm>
+
 #include "paged_attention.h"
 
 namespace xk {
@@ -106,7 +108,8 @@ extern "C" int xk_paged_attention(
     return XK_ERR_UNSUPPORTED;
   if (stride_kc_slot < 0 || stride_vc_slot < 0 || stride_kc_slot >= kMostPitch / cb ||
       stride_vc_slot >= kMostPitch / cb || stride_kc_page < 0 || stride_vc_page < 0 ||
-      stride_kc_page >= kMostPage / cb || stride_vc_page >= kMostPage / cb)
+      stride_kc_page >= kMostPage / cb || stride_vc_page >= kMostPage / cb ||
+      std::max(stride_kc_slot, stride_vc_slot) * cb * page_size > UINT32_MAX)
     return XK_ERR_INVALID;
   const int64_t positions = num_pages ? max_pages * page_size : 0;
   Plan x;
