@@ -569,7 +569,8 @@ __global__ void __launch_bounds__(kBlock, (waves_of<T, C, DP, R>())) attention_k
     const int slot = 2 * share + (cur.at > g0);
     if (cur.at >= g0 && head == 0 && group == 0 && threadIdx.x == 0) {
       const int last = static_cast<int>(divide(cur.at + cur.n - 1, size));
-      late_params()->meta[cur.b] = make_int2(slot, last - share + 1);
+      int2* meta = late_params()->meta;  // NULL where one share holds all
+      if (meta) meta[cur.b] = make_int2(slot, last - share + 1);
     }
     // Rows: token r / G of the sequence's new ones, at position len - T + token.
     const int pos_0 = len - p.T;

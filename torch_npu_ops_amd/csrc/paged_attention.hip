@@ -34,7 +34,8 @@ bool plan_of(int64_t B, int64_t T, int64_t G, int64_t Hkv, int64_t D, int64_t po
   if (x.shares * lines >= INT32_MAX || B * Hkv >= INT32_MAX || rows >= (int64_t{1} << 40))
     return false;
   auto up = [](int64_t n) { return cdiv(n, 256) * 256; };
-  x.bytes = up(B * 8) + up(rows * 8) + up(rows * D * 4);
+  // One share holds every sequence whole.
+  x.bytes = x.shares > 1 ? up(B * 8) + up(rows * 8) + up(rows * D * 4) : 0;
   return true;
 }
 
@@ -115,7 +116,8 @@ extern "C" int xk_paged_attention(
   Plan x;
   if (!plan_of(B, T, Hq / Hkv, Hkv, head_dim, max_pages * page_size, dtype, x))
     return XK_ERR_INVALID;
-  if (!workspace || workspace_bytes < static_cast<size_t>(x.bytes) || !aligned(workspace, 256))
+  if (x.bytes && (!workspace || workspace_bytes < static_cast<size_t>(x.bytes) ||
+                  !aligned(workspace, 256)))
     return XK_ERR_WORKSPACE;
   Params p{};
   p.q = q;
@@ -156,13 +158,15 @@ extern "C" int xk_paged_attention(
   p.M = static_cast<int>(T * (Hq / Hkv));
   p.groups = static_cast<int>(x.groups);
   p.shares = static_cast<int>(x.shares);
-  char* ws = static_cast<char*>(workspace);
-  const int64_t rows = 2 * x.shares * Hkv * p.M;
-  p.meta = reinterpret_cast<int2*>(ws);
-  ws += cdiv(B * 8, 256) * 256;
-  p.ml = reinterpret_cast<float2*>(ws);
-  ws += cdiv(rows * 8, 256) * 256;
-  p.acc = reinterpret_cast<float*>(ws);
+  if (x.bytes) {
+    char* ws = static_cast<char*>(workspace);
+    const int64_t rows = 2 * x.shares * Hkv * p.M;
+    p.meta = reinterpret_cast<int2*>(ws);
+    ws += cdiv(B * 8, 256) * 256;
+    p.ml = reinterpret_cast<float2*>(ws);
+    ws += cdiv(rows * 8, 256) * 256;
+    p.acc = reinterpret_cast<float*>(ws);
+  }
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (dtype) {
     case XK_F32: return run_f32(p, x.tiles, s);
