@@ -12,12 +12,14 @@
 // before it is rounded to fp32.
 //
 // What bounds it: HBM for many tokens, one wave's chain (position -> angle ->
-// LDS -> rotation -> store) for few.  So a wave takes one token, or a slice of
-// one where tokens are few, forms cos and sin of the token's pairs once (one
-// pair a lane at r = 128) into its LDS table, and then its lanes take units of
-// two vectors: the two vectors that a rotation by halves pairs, or two
-// neighbours.  A lane reads what it overwrites itself, so outputs may be the
-// inputs.  The first units' loads are requested before the angle is formed.
+// LDS -> rotation -> store) for few.  So a block's four waves take four tokens,
+// or parts of two, of one or of a part of one: they form cos and sin of its
+// tokens' pairs once, into LDS, and then lanes take units of two vectors, the two
+// that a rotation by halves pairs or any two.  A lane reads what it overwrites
+// itself, so outputs may be the inputs.  The first units' loads are requested
+// before the angle is formed.  What is read and written passes once, so both ask
+// for no room in the caches (75.2 us without, 66.5 with, for the 335 MB of 16384
+// tokens of 32 + 8 bf16 heads of 128: 5.2 TB/s, what a copy reaches over as much).
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -30,9 +32,15 @@ namespace {
 using f8 = unsigned char;  // e4m3, as stored
 constexpr float kF8Max = 448.f;
 constexpr int kBlock = 256;
+constexpr int kWaves = kBlock / kWave;
 constexpr int kMaxDim = 512;
 constexpr int kMaxHeads = 4096;
-constexpr int kAhead = 2;  // units that a lane requests together
+// Units that a lane requests together, and takes in all where tokens fill the
+// card.  16384 tokens of 32 + 8 bf16 heads of 128, us: 2 and 3 64.1, 2 and 5
+// 67.3, 2 and 2 75.0, 3 and 3 63.9, 5 and 5 66.2; 8192 in fp32 59.9, 61.6, 65.9,
+// 60.6, 63.3; heads of 256 with 64 turned in fp32 31.6, 30.3, 31.2, 30.5, 29.9.
+constexpr int kAhead = 2;
+constexpr int kUnits = 3;
 
 struct Rows {  // [tokens, heads, D]
   const void* src;
@@ -63,20 +71,31 @@ struct RotaryParams {
   int D, hq, hkv;
   int units;       // of a head
   uint32_t magic;  // ceil(2^32 / units); 0 for one unit
-  int slices;      // waves of a token
+  int of_wave;     // log2 of a block's waves that take one token
+  int slices;      // blocks that take the same tokens
 };
 
 // cos and sin of t f.  n quarter turns are taken off in 64 bits (the second
-// fma adds what pi/2's first 53 bits leave out), so that the rest, at most
-// pi/4, is right to 2^-25 before cosf and sinf see it.
+// fma adds what pi/2's first 53 bits leave out), so that the rest r, at most
+// pi/4, is right to 2^-25 when it is rounded.  There the Taylor series end at
+// r^9 and r^10: what follows is below r^11/11! < 2^-28 and r^12/12! < 2^-32.
 __device__ __forceinline__ void turn_of(double t, float f, float& c, float& s) {
   const double a = t * static_cast<double>(f);
   const double n = __builtin_rint(a * 0.63661977236758134308);
-  double r = __builtin_fma(n, -1.57079632679489655800, a);
-  r = __builtin_fma(n, -6.12323399573676603587e-17, r);
-  float sr, cr;
-  sincosf(static_cast<float>(r), &sr, &cr);
-  const int q = static_cast<int>(static_cast<int64_t>(n)) & 3;
+  const double d = __builtin_fma(n, -6.12323399573676603587e-17,
+                                 __builtin_fma(n, -1.57079632679489655800, a));
+  const float r = static_cast<float>(d), z = r * r;
+  float sr = __builtin_fmaf(z, 1.f / 362880, -1.f / 5040);
+  sr = __builtin_fmaf(z, sr, 1.f / 120);
+  sr = __builtin_fmaf(z, sr, -1.f / 6);
+  sr = __builtin_fmaf(z * r, sr, r);
+  float cr = __builtin_fmaf(z, -1.f / 3628800, 1.f / 40320);
+  cr = __builtin_fmaf(z, cr, -1.f / 720);
+  cr = __builtin_fmaf(z, cr, 1.f / 24);
+  cr = __builtin_fmaf(z, cr, -0.5f);
+  cr = __builtin_fmaf(z, cr, 1.f);
+  // n modulo 4, exact for every n.
+  const int q = static_cast<int>(__builtin_fma(__builtin_floor(n * 0.25), -4.0, n));
   const float x = q & 1 ? sr : cr, y = q & 1 ? cr : sr;
   c = (q == 1 || q == 2) ? -x : x;
   s = q >= 2 ? -y : y;
@@ -114,6 +133,14 @@ __device__ __forceinline__ Vec<f8, V> to_f8(const float (&x)[V], float scale) {
   return o;
 }
 
+template <typename T, int V>
+__device__ __forceinline__ void put(T* d, const float (&x)[V]) {
+  Vec<T, V> o;
+#pragma unroll
+  for (int i = 0; i < V; ++i) o.v[i] = from_f32<T>(x[i]);
+  st_stream(reinterpret_cast<Vec<T, V>*>(d), o);
+}
+
 // T: the tokens' type.  C: the cache's (f8 or T), void without a cache.
 // V: elements of a vector; NEXT: pairs are neighbours.
 template <typename T, typename C, int V, bool NEXT>
@@ -123,15 +150,18 @@ __global__ void __launch_bounds__(kBlock) rotary_kernel(RotaryParams p) {
   extern __shared__ __align__(16) float2 tab_all[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lane = threadIdx.x % kWave;
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * (kBlock / kWave) + wave;
-  const int64_t tok = id / p.slices;
-  if (tok >= p.T) return;  // whole wave
-  const int slice = static_cast<int>(id - tok * p.slices);
-  float2* tab = tab_all + wave * p.half;
+  // The block's tokens, the wave's one and its part of that.
+  const uint32_t group = p.slices == 1 ? blockIdx.x : blockIdx.x / p.slices;
+  const int in_block = wave >> p.of_wave, part = wave & ((1 << p.of_wave) - 1);
+  const int slice = ((blockIdx.x - group * p.slices) << p.of_wave) + part;
+  int64_t tok = static_cast<int64_t>(group) * (kWaves >> p.of_wave) + in_block;
+  const bool none = tok >= p.T;  // the last block's
+  if (none) tok = p.T - 1;
+  float2* tab = tab_all + in_block * p.half;
 
   const int heads = p.hq + p.hkv * (kCache ? 2 : 1);
-  const int total = heads * p.units;
-  const int step = p.slices * kWave;
+  const int total = none ? 0 : heads * p.units;
+  const int step = (p.slices << p.of_wave) * kWave;
   // Half pairs: units below `pairs` hold two vectors half a turn apart.
   const int pairs = NEXT ? 0 : p.half / V;
 
@@ -149,12 +179,20 @@ __global__ void __launch_bounds__(kBlock) rotary_kernel(RotaryParams p) {
   auto request = [&](int u, Unit& w) {
     w.head = p.magic ? static_cast<int>(__umulhi(static_cast<uint32_t>(u), p.magic)) : u;
     const int i = u - w.head * p.units;
+    // (The two vectors of a unit without such pairs are far from each other too,
+    // so that neighbouring lanes take neighbouring vectors; a pair of neighbours
+    // is one unit where a vector is one element.)
     const bool apart = i < pairs;
-    w.at = apart ? i * V : (NEXT ? 2 * i * V : p.half * 2 + 2 * (i - pairs) * V);
-    w.bt = w.at + (apart ? p.half : V);
+    if constexpr (NEXT && V == 1) {
+      w.at = 2 * i;
+      w.bt = w.at + 1;
+    } else {
+      w.at = (apart || NEXT ? 0 : p.half) + i * V;
+      w.bt = w.at + (apart ? p.half : (p.units - pairs) * V);
+    }
     const T* s = src_of(w.head);
-    w.a = *reinterpret_cast<const VT*>(s + w.at);
-    w.b = *reinterpret_cast<const VT*>(s + (w.bt < p.D ? w.bt : w.at));
+    w.a = ld_stream(reinterpret_cast<const VT*>(s + w.at));
+    w.b = ld_stream(reinterpret_cast<const VT*>(s + (w.bt < p.D ? w.bt : w.at)));
   };
 
   int u0 = slice * kWave + lane;
@@ -183,15 +221,12 @@ __global__ void __launch_bounds__(kBlock) rotary_kernel(RotaryParams p) {
   }
   if (p.pos) {
     const double t = static_cast<double>(load_int(p.pos, p.pos_i64, tok));
-    for (int i = lane; i < p.half; i += kWave) {
+    for (int i = part * kWave + lane; i < p.half; i += kWave << p.of_wave) {
       float c, s;
       turn_of(t, p.freq[i], c, s);
       tab[i] = make_float2(c * p.len, s * p.len * p.sign);
     }
-    // The wave reads what its own lanes wrote.
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    __syncthreads();
   }
 
   auto finish = [&](Unit& w) {
@@ -236,8 +271,8 @@ __global__ void __launch_bounds__(kBlock) rotary_kernel(RotaryParams p) {
       const bool is_q = w.head < p.hq;
       T* d = is_q ? static_cast<T*>(p.q.dst) + tok * p.q.dt + w.head * p.q.dh
                   : static_cast<T*>(p.k.dst) + tok * p.k.dt + (w.head - p.hq) * p.k.dh;
-      store_vec_f32<T, V>(d + w.at, a);
-      if (two) store_vec_f32<T, V>(d + w.bt, b);
+      put<T, V>(d + w.at, a);
+      if (two) put<T, V>(d + w.bt, b);
       return;
     }
     if constexpr (kCache) {
@@ -251,8 +286,8 @@ __global__ void __launch_bounds__(kBlock) rotary_kernel(RotaryParams p) {
         *reinterpret_cast<Vec<f8, V>*>(d + w.at) = to_f8<V>(a, scale);
         if (two) *reinterpret_cast<Vec<f8, V>*>(d + w.bt) = to_f8<V>(b, scale);
       } else {
-        store_vec_f32<C, V>(d + w.at, a);
-        if (two) store_vec_f32<C, V>(d + w.bt, b);
+        put<C, V>(d + w.at, a);
+        if (two) put<C, V>(d + w.bt, b);
       }
     }
   };
@@ -279,13 +314,16 @@ int launch_v(RotaryParams& p, bool next, hipStream_t s) {
   const int64_t total = heads * p.units;
   // (u * units < 2^32 keeps the multiplication by `magic` exact: u is below
   // 2 * kMaxHeads * units, units at most kMaxDim.)
-  // Waves of a token: one where tokens alone fill the card (16 waves a
-  // compute unit), else as many as there are units to take.
+  // Waves of a token: as many as leave a lane kUnits units, more where tokens
+  // alone do not give a compute unit 16 waves, but none without a unit.
+  const int64_t full = cdiv(total, kWave);
   const int64_t room = std::max<int64_t>(1, 16 * num_cus() / p.T);
-  p.slices = static_cast<int>(std::min(room, cdiv(total, kWave)));
-  const int64_t blocks = cdiv(p.T * p.slices, kBlock / kWave);
+  const int64_t want = std::max(std::min(room, full), cdiv(full, kUnits));
+  p.of_wave = want >= 4 ? 2 : want >= 2 ? 1 : 0;
+  p.slices = static_cast<int>(cdiv(want, 1 << p.of_wave));
+  const int64_t blocks = cdiv(p.T, kWaves >> p.of_wave) * p.slices;
   if (blocks > INT32_MAX) return XK_ERR_INVALID;
-  const size_t lds = sizeof(float2) * (p.pos ? p.half : 0) * (kBlock / kWave);
+  const size_t lds = sizeof(float2) * (p.pos ? p.half : 0) * (kWaves >> p.of_wave);
   const dim3 grid(static_cast<uint32_t>(blocks));
   if (next)
     hipLaunchKernelGGL((rotary_kernel<T, C, V, true>), grid, dim3(kBlock), lds, s, p);
