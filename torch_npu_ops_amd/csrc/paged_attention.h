@@ -874,47 +874,62 @@ __global__ void __launch_bounds__(kBlock) join_kernel(Params p, int team) {
   int split = 1;  // teams of a row
   while (split < pieces && split < teams) split *= 2;
   const int part = own % split, step = gridDim.y * (teams / split);
+  // The first piece, then the first ones of the shares that follow.
+  const int64_t apart = 2 * static_cast<int64_t>(p.Hkv) * p.M;
+  const int64_t first = (static_cast<int64_t>(meta.x) * p.Hkv + head) * p.M;
+  const int64_t even = (static_cast<int64_t>(meta.x & ~1) * p.Hkv + head) * p.M;
   for (int r0 = blockIdx.y * (teams / split); r0 < p.M; r0 += step) {
     const int r = r0 + own / split;
     float base = -INFINITY, sum = 0.f;
     f4_t acc = {};
-    constexpr int kAhead = 8;  // pieces that a lane requests together
-    for (int i0 = part; i0 < pieces && r < p.M; i0 += kAhead * split) {
-      float2 x[kAhead];
-      f4_t y[kAhead];
+    // `ahead` pieces that a lane requests together: one where it has no more
+    // (with eight for all, the statistics of those that are not there took most
+    // of the time).
+    auto take = [&](auto ahead) {
+      constexpr int kAhead = ahead;
+      for (int i0 = part; i0 < pieces && r < p.M; i0 += kAhead * split) {
+        float2 x[kAhead];
+        f4_t y[kAhead];
 #pragma unroll
-      for (int a = 0; a < kAhead; ++a) {
-        const int i = i0 + a * split;
-        x[a] = make_float2(-INFINITY, 0.f);
-        y[a] = f4_t{};
-        if (i < pieces) {
-          // The first piece, then the first ones of the shares that follow.
-          const int slot = i ? (meta.x & ~1) + 2 * i : meta.x;
-          const int64_t at = (static_cast<int64_t>(slot) * p.Hkv + head) * p.M + r;
-          x[a] = p.ml[at];
-          if (d < p.D) y[a] = *reinterpret_cast<const f4_t*>(p.acc + at * p.D + d);
+        for (int a = 0; a < kAhead; ++a) {
+          const int i = i0 + a * split;
+          x[a] = make_float2(-INFINITY, 0.f);
+          y[a] = f4_t{};
+          if (i < pieces) {
+            const int64_t at = (i ? even + i * apart : first) + r;
+            x[a] = p.ml[at];
+            if (d < p.D) y[a] = *reinterpret_cast<const f4_t*>(p.acc + at * p.D + d);
+          }
+        }
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+          if constexpr (kAhead == 1) {  // (the lane's only one)
+            base = x[a].x;
+            sum = x[a].y;
+            acc = y[a];
+          } else {
+            const float now = fmaxf(base, x[a].x), c = weight(base, now), e = weight(x[a].x, now);
+            sum = sum * c + x[a].y * e;
+            acc = acc * c + y[a] * e;
+            base = now;
+          }
         }
       }
-#pragma unroll
-      for (int a = 0; a < kAhead; ++a) {
-        const float now = fmaxf(base, x[a].x), c = weight(base, now), e = weight(x[a].x, now);
-        sum = sum * c + x[a].y * e;
-        acc = acc * c + y[a] * e;
-        base = now;
-      }
-    }
+    };
+    if (split >= pieces) take(std::integral_constant<int, 1>());
+    else take(std::integral_constant<int, 8>());
     if (threadIdx.x % team == 0) ml[own] = make_float2(base, sum);
-    __syncthreads();
-    float top = -INFINITY;
-    for (int i = own - part; i < own - part + split; ++i) top = fmaxf(top, ml[i].x);
-    sums[threadIdx.x] = acc * weight(base, top);
+    sums[threadIdx.x] = acc;
     __syncthreads();
     if (part == 0 && r < p.M && d < p.D) {
-      float l = 0.f;
+      float top = base, l = 0.f;
+      for (int i = 1; i < split; ++i) top = fmaxf(top, ml[own + i].x);
       f4_t x = {};
       for (int i = 0; i < split; ++i) {
-        l += ml[own + i].y * weight(ml[own + i].x, top);
-        x += sums[threadIdx.x + i * team];
+        const float2 one = ml[own + i];
+        const float by = weight(one.x, top);
+        l += one.y * by;
+        x += sums[threadIdx.x + i * team] * by;
       }
       write_row<T>(&p, b, head, r, d, x, top, l);
     }
