@@ -228,6 +228,58 @@ def test_lengths_beyond_the_table_and_empty_pools(dev):
             assert o.shape == (B, T, 4, 64) and lse.shape == (B, T, 4)
 
 
+@pytest.mark.parametrize("dtype,cache", TYPES)
+@pytest.mark.parametrize("page", [48, 64, 96, 256])
+@pytest.mark.parametrize("D", [64, 128])
+def test_runs_of_pages(dev, dtype, cache, page, D):
+    """Pages that hold whole tiles, halves or quarters of them: a table entry
+    serves 64, 32 or 16 positions."""
+    lens = [0, 1, page, page + 1, 3 * page - 1, 1100, 63]
+    kc, vc, table = _pool(60 + page, lens, page, 2, D, cache)
+    for T in (1, 6):
+        print(f"runs page={page} D={D} T={T}", flush=True)
+        _check(dev, _api("cpp"), _query(61, len(lens), T, 8, D, dtype), kc, vc, table, lens, None,
+               0 if T == 1 else 200, *_scales(62, 2, cache))
+
+
+@pytest.mark.parametrize("dtype,cache", TYPES)
+def test_many_new_tokens(dev, dtype, cache):
+    """Row groups of a head, each with positions of its own."""
+    lens = [70, 71, 300, 12]
+    kc, vc, table = _pool(63, lens, 16, 2, 64, cache)
+    for window in (0, 50):
+        _check(dev, _api("cpp"), _query(64, 4, 70, 8, 64, dtype), kc, vc, table, lens, None, window,
+               *_scales(65, 2, cache))
+
+
+@pytest.mark.parametrize("dtype,cache", TYPES)
+def test_many_short_sequences(dev, dtype, cache):
+    """Shares that hold many sequences whole, of a tile or none each."""
+    g = torch.Generator().manual_seed(66)
+    lens = torch.randint(0, 40, (700,), generator=g).tolist()
+    kc, vc, table = _pool(67, lens, 16, 8, 64, cache)
+    _check(dev, _api("cpp"), _query(68, 700, 1, 16, 64, dtype), kc, vc, table, lens, None, 0,
+           *_scales(69, 8, cache))
+
+
+@pytest.mark.parametrize("D", [64, 256])
+def test_many_pieces(dev, D):
+    """More pieces of a sequence than the lanes that join them take at once."""
+    lens = [30001]
+    kc, vc, table = _pool(70, lens, 16, 1, D, BF16)
+    for T in (1, 3):
+        _check(dev, _api("cpp"), _query(71, 1, T, 4, D, BF16), kc, vc, table, lens)
+
+
+@pytest.mark.parametrize("dtype,cache", TYPES)
+def test_one_share_needs_no_workspace(dev, dtype, cache):
+    lens = [20, 7]
+    kc, vc, table = _pool(72, lens, 16, 2, 64, cache)
+    for api in ("cpp", "py"):
+        _check(dev, _api(api), _query(73, 2, 1, 8, 64, dtype), kc, vc, table, lens, None, 0,
+               *_scales(74, 2, cache))
+
+
 # --------------------------------------------------------------------------
 # layouts
 # --------------------------------------------------------------------------
@@ -401,3 +453,32 @@ def test_two_streams_at_once(dev):
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(alone[i], o) for o in got[i])
+
+
+def test_two_graphs_and_eager_calls(dev):
+    """Two captured calls replayed at once on two streams, eager ones between."""
+    api = _api("cpp")
+    calls, graphs, outs = [], [], []
+    for i, lens in enumerate(([5000, 20], [100, 3000])):
+        kc, vc, table = _pool(80 + i, lens, 16, 2, 128, BF16)
+        q = _query(82 + i, 2, 1, 16, 128, BF16)
+        calls.append([t.to(dev) for t in (q, kc, vc, table, torch.tensor(lens, dtype=torch.int32))])
+    alone = [api.npu_paged_attention(*c)[0] for c in calls]
+    torch.cuda.synchronize()
+    for c in calls:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(api.npu_paged_attention(*c)[0])
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in calls]
+    for i in range(5):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        eager = [api.npu_paged_attention(*c)[0] for c in calls]
+        torch.cuda.synchronize()
+        for a, o, e in zip(alone, outs, eager):
+            assert torch.equal(a, o) and torch.equal(a, e), i

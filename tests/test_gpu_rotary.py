@@ -268,3 +268,21 @@ def test_many_tokens(dev):
     kc = torch.zeros(pages, page, hkv, D, dtype=F16)
     _check_append(dev, _api("cpp"), q, k, v, kc, kc.clone(), _slots(2, T, pages * page),
                   torch.arange(T) + 30000, _freq(D))
+
+
+def test_more_blocks_than_a_dimension_holds(dev):
+    """2^26 tokens and some: more blocks of four than 2^32 threads are."""
+    T, D = (1 << 26) + 5, 2
+    f = torch.ones(1)
+    x = torch.zeros(T, 1, D, dtype=BF16, device=dev)
+    x[:, 0, 0] = 1.0
+    pos = torch.zeros(T, dtype=torch.int32, device=dev)
+    at = torch.tensor([0, 3, (1 << 25) + 1, (1 << 26) - 1, 1 << 26, T - 1])
+    turns = torch.arange(1, 7)
+    pos[at.to(dev)] = turns.to(dev, torch.int32)
+    y, none = _api("cpp").npu_rotary_embedding(x, None, pos, f.to(dev))
+    assert none is None
+    want, err = rotary.turn(x[at.to(dev)].cpu(), turns, f)
+    assert_within(y[at.to(dev)], want, err, "chosen tokens")
+    y[at.to(dev)] = x[at.to(dev)]
+    assert torch.equal(y, x)  # the others' angle is 0

@@ -88,6 +88,21 @@ def test_attention_refuses(change, status):
     assert _attend(**change) == status
 
 
+@pytest.mark.parametrize("change", [
+    # pages of 2^32 bytes, from place to place and from page to page of 2^35
+    dict(page=1 << 20, width=1, kcs=1 << 12), dict(page=1 << 20, width=1, vcs=1 << 12),
+    dict(kcp=1 << 34), dict(vcp=1 << 34), dict(vcp=-2048),
+    # more positions than a sequence has, in one page and without a table
+    dict(page=(1 << 28) + 1, width=1), dict(page=1 << 62, width=0),
+    # a scale that is not finite as a power of two
+    dict(scale=3e38), dict(scale=-3e38),
+    dict(B=(1 << 24) + 1), dict(T=(1 << 20) + 1), dict(Hq=1 << 17), dict(B=1 << 23),
+    # blocks
+    dict(T=1 << 20, Hq=1 << 16, Hkv=1 << 16, row=1 << 14, width=1 << 14)], ids=str)
+def test_attention_refuses_what_a_launch_does_not_hold(change):
+    assert _attend(ws=PTR, size=1 << 60, **change) == INVALID
+
+
 def test_attention_refuses_small_workspaces():
     lib = _lib.lib()
     need = lib.xk_paged_attention_workspace_bytes(2, 1, 8, 2, 64, 1000, 16, _lib.XK_BF16)

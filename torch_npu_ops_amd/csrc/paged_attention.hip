@@ -11,6 +11,9 @@ namespace {
 constexpr int64_t kMostPositions = int64_t{1} << 28;  // a sequence's, by its table row
 constexpr int64_t kMostPitch = int64_t{1} << 27;      // bytes from one position to the next
 constexpr int64_t kMostPage = int64_t{1} << 35;       // and from one page to the next
+constexpr int64_t kMostBlocks = int64_t{1} << 24;     // a launch holds 2^32 threads in a dimension
+
+constexpr float kLog2e = 1.44269504088896f;
 
 struct Plan {
   int tiles;  // row tiles of a wave
@@ -31,7 +34,7 @@ bool plan_of(int64_t B, int64_t T, int64_t G, int64_t Hkv, int64_t D, int64_t po
   const int64_t most = cdiv(B * std::max<int64_t>(1, cdiv(positions, 16)), kWaves);
   x.shares = std::min(std::max<int64_t>(1, 2 * num_cus() / lines), most);
   const int64_t rows = 2 * x.shares * Hkv * M;
-  if (x.shares * lines >= INT32_MAX || B * Hkv >= INT32_MAX || rows >= (int64_t{1} << 40))
+  if (x.shares * lines >= kMostBlocks || B * Hkv >= kMostBlocks || rows >= (int64_t{1} << 40))
     return false;
   auto up = [](int64_t n) { return cdiv(n, 256) * 256; };
   // One share holds every sequence whole.
@@ -50,7 +53,7 @@ void magic_of(int64_t by, uint32_t& magic, int& shift) {
 int check_sizes(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_pages,
                 int64_t page_size) {
   if (B < 0 || T <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || D <= 0 || D > 256 || D % 8 ||
-      max_pages < 0 || page_size <= 0)
+      max_pages < 0 || page_size <= 0 || page_size > kMostPositions)
     return XK_ERR_INVALID;
   if (B > (1 << 24) || T > (1 << 20) || Hq > (1 << 16) ||
       (max_pages > 0 && page_size > kMostPositions / max_pages))
@@ -88,7 +91,8 @@ extern "C" int xk_paged_attention(
   using namespace paged;
   const int st = check_sizes(B, T, Hq, Hkv, head_dim, max_pages, page_size);
   if (st != XK_OK) return st;
-  if (num_pages < 0 || num_pages > INT32_MAX || window < 0 || !std::isfinite(scale))
+  if (num_pages < 0 || num_pages > INT32_MAX || window < 0 ||
+      !std::isfinite(scale * kLog2e))
     return XK_ERR_INVALID;
   const bool eight = cache_dtype == XK_F8E4M3;
   if (!is_float_dtype(dtype) || (eight ? dtype == XK_F32 : cache_dtype != dtype))
@@ -140,7 +144,7 @@ extern "C" int xk_paged_attention(
   p.max_pages = static_cast<int>(max_pages);
   p.lens = seq_lens;
   p.most_len = static_cast<int>(positions);
-  p.scale2 = scale * 1.44269504088896f;
+  p.scale2 = scale * kLog2e;
   p.window = static_cast<int>(std::min<int64_t>(window, kMostPositions + (1 << 20)));
   p.k_scale = k_scale;
   p.v_scale = v_scale;

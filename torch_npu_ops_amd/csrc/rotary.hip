@@ -151,9 +151,10 @@ __global__ void __launch_bounds__(kBlock) rotary_kernel(RotaryParams p) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lane = threadIdx.x % kWave;
   // The block's tokens, the wave's one and its part of that.
-  const uint32_t group = p.slices == 1 ? blockIdx.x : blockIdx.x / p.slices;
+  const uint32_t id = blockIdx.y * gridDim.x + blockIdx.x;
+  const uint32_t group = p.slices == 1 ? id : id / p.slices;
   const int in_block = wave >> p.of_wave, part = wave & ((1 << p.of_wave) - 1);
-  const int slice = ((blockIdx.x - group * p.slices) << p.of_wave) + part;
+  const int slice = ((id - group * p.slices) << p.of_wave) + part;
   int64_t tok = static_cast<int64_t>(group) * (kWaves >> p.of_wave) + in_block;
   const bool none = tok >= p.T;  // the last block's
   if (none) tok = p.T - 1;
@@ -322,9 +323,11 @@ int launch_v(RotaryParams& p, bool next, hipStream_t s) {
   p.of_wave = want >= 4 ? 2 : want >= 2 ? 1 : 0;
   p.slices = static_cast<int>(cdiv(want, 1 << p.of_wave));
   const int64_t blocks = cdiv(p.T, kWaves >> p.of_wave) * p.slices;
-  if (blocks > INT32_MAX) return XK_ERR_INVALID;
+  if (blocks > INT32_MAX) return XK_ERR_UNSUPPORTED;
   const size_t lds = sizeof(float2) * (p.pos ? p.half : 0) * (kWaves >> p.of_wave);
-  const dim3 grid(static_cast<uint32_t>(blocks));
+  // (2^32 threads at the most in a dimension; blocks past the last token have none.)
+  const int64_t wide = std::min<int64_t>(blocks, 1 << 23);
+  const dim3 grid(static_cast<uint32_t>(wide), static_cast<uint32_t>(cdiv(blocks, wide)));
   if (next)
     hipLaunchKernelGGL((rotary_kernel<T, C, V, true>), grid, dim3(kBlock), lds, s, p);
   else
