@@ -135,10 +135,13 @@ __device__ __forceinline__ Batch batch_at(const Params& p, int b0) {
 __device__ __forceinline__ int64_t divide(int64_t a, uint32_t b) {
   return a <= UINT32_MAX ? static_cast<uint32_t>(a) / b : a / b;
 }
-// Tiles of a share: whole rounds of the block's waves.
+// Tiles of a share: one for each of the block's waves at the least (fewer, in
+// more pieces, took 10.4 us instead of 9.9 for one sequence of 900), else as
+// equal as they come (in whole rounds of the waves 7 fp32 sequences of 1777
+// took 24.9 us instead of 23.4, 48 of four new tokens 42.1 instead of 39.8).
 __device__ __forceinline__ uint32_t share_size(int64_t total, int shares) {
   const int64_t n = divide(total + shares - 1, shares);
-  return static_cast<uint32_t>((n + kWaves - 1) / kWaves * kWaves);
+  return static_cast<uint32_t>(max<int64_t>(n, kWaves));
 }
 
 // ---------------------------------------------------------------------------
@@ -645,18 +648,23 @@ __global__ void __launch_bounds__(kBlock, (waves_of<T, C, DP, R>())) attention_k
       if (!whole) {
         const uint32_t there = static_cast<uint32_t>(ok) >> 4 * g;
         const uint32_t there_hi = static_cast<uint32_t>(ok >> 32) >> 4 * g;
+        // (how far a position lies back, and past the first one seen, as
+        // unsigned numbers: one comparison each)
+        const uint32_t span = p.window ? p.window : INT32_MAX;
+        const uint32_t most = last_pos - low_first;
+        const int past = pos0 + 4 * g - low_first;
         bool fine = true;
 #pragma unroll
         for (int i = 0; i < NX; ++i) {
-          const int t = 16 * (i / 4) + i % 4, pos = pos0 + 4 * g + t;
+          const int t = 16 * (i / 4) + i % 4;
           const bool in = ((t < 32 ? there >> t : there_hi >> (t - 32)) & 1);
 #pragma unroll
           for (int j = 0; j < R; ++j) {
-            const int back = pos_0 + tok[j] - pos;
-            const bool seen = in && back >= 0 && (!p.window || back < p.window);
+            const uint32_t back = pos_0 + tok[j] - (pos0 + 4 * g) - t;
+            const bool seen = in && back < span;
             sc[j][i / 4][i % 4] = seen ? sc[j][i / 4][i % 4] : -INFINITY;
           }
-          const bool any = in && pos <= last_pos && pos >= low_first;
+          const bool any = in && static_cast<uint32_t>(past + t) <= most;
 #pragma unroll
           for (int n = 0; n < NB; ++n) {
             v[i][n].keep(any);
