@@ -201,6 +201,60 @@ def test_drafts_do_not_see_later_drafts(dev, dtype, bad):
                     assert o[:, 2:].cpu()[..., rest].isfinite().all()
 
 
+@pytest.mark.parametrize("dtype,cache", TYPES)
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_later_drafts_with_many_rows(dev, dtype, cache, D):
+    """The same with rows for more than one tile, in every head length, and
+    with places that nobody sees filled likewise."""
+    lens, T, bad = [50, 64, 7, 200], 4, math.nan
+    ks, vs = _scales(90, 2, cache)
+    on = lambda t: None if t is None else t.to(dev)  # noqa: E731
+    for which in (0, 1):
+        for window in (0, 30):
+            kc, vc, table = _pool(91, lens, 16, 2, D, cache, fill=bad)
+            clean = _pool(91, lens, 16, 2, D, cache, fill=0.0)
+            for b, n in enumerate(lens):
+                place = (kc, vc)[which][table[b, (n - 2) // 16], (n - 2) % 16]
+                x = place.float()
+                x[:, 5] = bad
+                place.copy_(x.to(cache))
+            q = _query(92, 4, T, 20, D, dtype)
+            want = opa.attention(q, *clean, lens, None, window, ks, vs)
+            o, _ = _api("cpp").npu_paged_attention(
+                on(q), on(kc), on(vc), on(table), torch.tensor(lens, dtype=torch.int32).to(dev), None,
+                window, on(ks), on(vs))
+            assert_within(o[:, :2], want["o"][:, :2], want["o_err"][:, :2], f"before {which} {window}")
+            after = o[:, 2:].cpu()
+            assert (after[..., 5] if which else after).isnan().all()
+            if which:
+                rest = [i for i in range(D) if i != 5]
+                assert_within(after[..., rest], want["o"][:, 2:][..., rest],
+                              want["o_err"][:, 2:][..., rest], f"after {window}")
+
+
+@pytest.mark.parametrize("dtype,cache", TYPES)
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_either_side_of_the_choice_of_row_tiles(dev, dtype, cache, D):
+    """Batches with little and with much to read, whose rows of tokens and
+    heads fill one tile and a half."""
+    for lens in ([300, 0, 40], [5000, 3000, 34000, 1]):
+        kc, vc, table = _pool(93, lens, 64, 1, D, cache)
+        for window in (0, 2000):
+            _check(dev, _api("cpp"), _query(94, len(lens), 3, 8, D, dtype), kc, vc, table, lens, None,
+                   window, *_scales(95, 1, cache))
+
+
+def test_windows_beyond_every_length(dev):
+    lens = [700, 3]
+    kc, vc, table = _pool(96, lens, 16, 2, 64, BF16)
+    q = _query(97, 2, 5, 8, 64, BF16)
+    for api in ("cpp", "py"):
+        args = [t.to(dev) for t in (q, kc, vc, table, torch.tensor(lens, dtype=torch.int32))]
+        want = _api(api).npu_paged_attention(*args)[0]
+        for window in (700, 1 << 28, (1 << 31) - 1, 1 << 31, (1 << 63) - 1):
+            assert torch.equal(_api(api).npu_paged_attention(*args, None, window)[0], want)
+
+
 def test_pages_that_are_not_there(dev):
     """Entries outside the cache count as masked, in the middle too."""
     lens = [100, 40, 64]

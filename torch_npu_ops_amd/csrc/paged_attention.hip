@@ -18,7 +18,15 @@ constexpr float kLog2e = 1.44269504088896f;
 struct Plan {
   int tiles;  // row tiles of a wave
   int64_t groups, shares, bytes;
+  int64_t most;  // shares that there can be
 };
+
+// The shares of a head and row group: two blocks a compute unit in all (the
+// kernels that only fit once take half), none without a least share.
+void cut(Plan& x, int64_t M, int64_t Hkv) {
+  x.groups = cdiv(M, 16 * x.tiles);
+  x.shares = std::min(std::max<int64_t>(1, 2 * num_cus() / (Hkv * x.groups)), x.most);
+}
 
 // False where the sizes are beyond what a launch holds.
 bool plan_of(int64_t B, int64_t T, int64_t G, int64_t Hkv, int64_t D, int64_t positions,
@@ -27,12 +35,9 @@ bool plan_of(int64_t B, int64_t T, int64_t G, int64_t Hkv, int64_t D, int64_t po
   if (M >= kMostPositions) return false;
   // (two row tiles of fp32 heads of 256 do not fit the registers)
   x.tiles = M > 16 && (D <= 128 || dtype != XK_F32) ? 2 : 1;
-  x.groups = cdiv(M, 16 * x.tiles);
-  // The shares of a head and row group: two blocks a compute unit in all (the
-  // kernels that only fit once take half), none without a least share.
+  x.most = cdiv(B * std::max<int64_t>(1, cdiv(positions, 16)), kWaves);
+  cut(x, M, Hkv);
   const int64_t lines = Hkv * x.groups;
-  const int64_t most = cdiv(B * std::max<int64_t>(1, cdiv(positions, 16)), kWaves);
-  x.shares = std::min(std::max<int64_t>(1, 2 * num_cus() / lines), most);
   const int64_t rows = 2 * x.shares * Hkv * M;
   if (x.shares * lines >= kMostBlocks || B * Hkv >= kMostBlocks || rows >= (int64_t{1} << 40))
     return false;
@@ -120,6 +125,19 @@ extern "C" int xk_paged_attention(
   Plan x;
   if (!plan_of(B, T, Hq / Hkv, Hkv, head_dim, max_pages * page_size, dtype, x))
     return XK_ERR_INVALID;
+  // Two blocks with a row tile each read all twice, but are sooner through a few
+  // tiles: where a block's part of the keys is at most 40 KB.  1, 4 and 16
+  // sequences of up to 2000, 4 tokens, 32 / 4 heads, us with one tile and two:
+  // 64 bf16 11.8, 13.6; 15.9, 18.9; 26.9, 27.3 (32 KB); 128 bf16 11.4, 13.5; 18.6,
+  // 20.6 (16); 37.6, 33.7 (64); 128 e4m3 14.0, 17.7; 19.6, 28.0; 32.5, 41.6 (32);
+  // 256 bf16 16.4, 21.6; 29.1, 37.5 (32); 61.9, 59.1 (128).
+  const int64_t M = T * (Hq / Hkv);
+  const int64_t seen = window && window < positions - T ? window + T : positions;
+  if (x.tiles == 2 && M <= 32 &&
+      B * seen * Hkv * head_dim * cb <= (int64_t{80} << 10) * num_cus()) {
+    x.tiles = 1;
+    cut(x, M, Hkv);  // (fewer shares: the workspace suffices)
+  }
   if (x.bytes && (!workspace || workspace_bytes < static_cast<size_t>(x.bytes) ||
                   !aligned(workspace, 256)))
     return XK_ERR_WORKSPACE;

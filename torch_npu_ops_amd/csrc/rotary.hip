@@ -314,7 +314,7 @@ int launch_v(RotaryParams& p, bool next, hipStream_t s) {
   const int64_t heads = p.hq + static_cast<int64_t>(p.hkv) * (std::is_void<C>::value ? 1 : 2);
   const int64_t total = heads * p.units;
   // (u * units < 2^32 keeps the multiplication by `magic` exact: u is below
-  // 2 * kMaxHeads * units, units at most kMaxDim.)
+  // 3 * kMaxHeads * units, units at most kMaxDim / 2.)
   // Waves of a token: as many as leave a lane kUnits units, more where tokens
   // alone do not give a compute unit 16 waves, but none without a unit.
   const int64_t full = cdiv(total, kWave);
