@@ -126,15 +126,16 @@ extern "C" int xk_paged_attention(
   if (!plan_of(B, T, Hq / Hkv, Hkv, head_dim, max_pages * page_size, dtype, x))
     return XK_ERR_INVALID;
   // Two blocks with a row tile each read all twice, but are sooner through a few
-  // tiles: where a block's part of the keys is at most 40 KB.  1, 4 and 16
-  // sequences of up to 2000, 4 tokens, 32 / 4 heads, us with one tile and two:
-  // 64 bf16 11.8, 13.6; 15.9, 18.9; 26.9, 27.3 (32 KB); 128 bf16 11.4, 13.5; 18.6,
-  // 20.6 (16); 37.6, 33.7 (64); 128 e4m3 14.0, 17.7; 19.6, 28.0; 32.5, 41.6 (32);
-  // 256 bf16 16.4, 21.6; 29.1, 37.5 (32); 61.9, 59.1 (128).
+  // tiles: where a block's part of the keys is at most 56 KB by the table's width.
+  // 1, 4 and 16 sequences of 1900 on average, 2600 at the most, 4 tokens, 32 / 4
+  // heads, us with one tile and two (and that part in KB): 64 bf16 11.7, 13.5;
+  // 16.0, 18.9; 26.9, 27.3 (43); 128 bf16 11.5, 13.6; 18.6, 20.6 (21); 37.6, 33.7
+  // (85); 128 e4m3 13.9, 17.7; 19.6, 28.3; 32.5, 41.6 (43); 256 bf16 16.4, 21.6;
+  // 29.1, 37.5 (43); 61.9, 59.1 (170).
   const int64_t M = T * (Hq / Hkv);
   const int64_t seen = window && window < positions - T ? window + T : positions;
   if (x.tiles == 2 && M <= 32 &&
-      B * seen * Hkv * head_dim * cb <= (int64_t{80} << 10) * num_cus()) {
+      B * seen * Hkv * head_dim * cb <= (int64_t{112} << 10) * num_cus()) {
     x.tiles = 1;
     cut(x, M, Hkv);  // (fewer shares: the workspace suffices)
   }
