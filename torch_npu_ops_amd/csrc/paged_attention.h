@@ -11,7 +11,7 @@
 // small part of what the matrix cores do at that rate, so the rows of a
 // 16-row MFMA tile that are not used cost nothing.
 //
-// Work: the positions of all sequences, in tiles of 16 to 64, are one line
+// Work: the positions of all sequences, in tiles of 16 (fp32) or 32, are one line
 // that the blocks of a head cut in equal shares, on the device, from the
 // lengths that are there (seq_lens never reaches the host); as many blocks as
 // the card runs at once.  A block goes through the sequences that its share
@@ -316,35 +316,39 @@ __device__ __forceinline__ void write_row(P p, int b, int head, int r, int d, f4
 // whole runs of, with one scalar address each; 0 for none, an address for each
 // lane and load.
 // ---------------------------------------------------------------------------
-// Tiles hold 8 KB of keys where rows are short: fewer rounds of statistics.
-template <typename T, typename C, int DP>
-constexpr int subs_of() {  // products with V of a tile
-  return DP * static_cast<int>(sizeof(C)) * (64 / static_cast<int>(sizeof(T))) <= 4096 ? 2 : 1;
-}
-// Waves of a SIMD: two where the sums and a tile's keys and values take at most
-// half of 256 registers (a third of that is needed beside them).
+// Whether the sums and a tile's keys and values take at most half of 256 registers
+// (a third of that is needed beside them).  Where they do, the kernel is held to
+// 256: with 512 the sums go to the accumulator registers and are moved to be
+// rescaled (48 sequences of 4 tokens, f16 heads of 64: 31.7 us instead of 30.1).
 template <typename T, typename C, int DP, int R>
-constexpr int waves_of() {
-  constexpr int kTile = DP * static_cast<int>(sizeof(C)) * subs_of<T, C, DP>() * 64 /
-                        static_cast<int>(sizeof(T)) / 256;
-  return DP * R / 4 + 2 * kTile > 128 ? 1 : 2;
+constexpr bool fits_twice() {
+  constexpr int kTile = DP * static_cast<int>(sizeof(C)) * 64 / static_cast<int>(sizeof(T)) / 256;
+  return DP * R / 4 + 2 * kTile <= 128;
+}
+// Blocks of a compute unit: two where much is computed for each byte, else one,
+// which has fewer pieces to begin, to finish and to join.  us with one and two:
+// 48 sequences of 4 tokens, 8 rows a head and token, up to 6000 positions, e4m3
+// heads of 128 87.4, 77.8, of 64 61.4, 63.5; bf16 114.0, 121.8 and 61.1, 65.2; one
+// token, 64 sequences, bf16 heads of 128 176.4, 179.3; 128 with e4m3 heads of 256
+// 72.7, 71.3; one sequence of 8192, bf16 15.0, 17.7.
+template <typename T, typename C, int DP, int R>
+constexpr int blocks_of() {
+  return sizeof(C) == 1 && DP * R >= 256 && fits_twice<T, C, DP, R>() ? 2 : 1;
 }
 
 template <typename T, typename C, int DP, int R, int RUN>
-__global__ void __launch_bounds__(kBlock, (waves_of<T, C, DP, R>())) attention_kernel(Params p) {
+__global__ void __launch_bounds__(kBlock, (fits_twice<T, C, DP, R>() ? 2 : 1)) attention_kernel(Params p) {
   using OpT = typename Op<T>::type;
   constexpr int CB = sizeof(C);
   constexpr int KV = 16 / sizeof(T);  // values of an operand in a lane
-  constexpr int SUB = 4 * KV;         // positions of one product with V
-  constexpr int NS = subs_of<T, C, DP>(), TS = SUB * NS, NH = TS / 16;
-  constexpr int NK = DP / SUB;  // products over a head
+  constexpr int TS = 4 * KV, NH = TS / 16;  // positions of a tile: of a product with V
+  constexpr int NK = DP / TS;               // products over a head
   constexpr int CH = DP / KV;   // K: chunks of a row, a lane each
   constexpr int RPI = kWave / CH, NL = TS / RPI;   // rows of a load, loads of a tile
   constexpr int KO = RPI < 16 ? 16 / RPI : 1;      // loads of a half tile
   constexpr int VB = KV < DP / 16 ? KV : DP / 16;  // V: elements of a load
   constexpr int NB = DP / (16 * VB);               // and loads of a row
-  constexpr int NX = KV * NS;                      // scores of a lane and row tile
-  constexpr uint64_t kAll = ~uint64_t{0} >> (64 - TS);
+  constexpr uint32_t kAll = ~0u >> (32 - TS);
   // log2 of what p is scaled by (see above).
   constexpr float kShift = std::is_same<T, f16>::value ? 14.f : 0.f;
   using KRow = Row<T, C, KV>;
@@ -488,14 +492,14 @@ __global__ void __launch_bounds__(kBlock, (waves_of<T, C, DP, R>())) attention_k
     tok[j] = r < p.M ? token_of(&p, r) : -(1 << 30);
   }
   KRow k[NL];
-  VRow v[NX][NB];
-  uint64_t ok = 0;  // which positions of the tile there are
+  VRow v[KV][NB];
+  uint32_t ok = 0;  // which positions of the tile there are
   // Where a tile's rows are, and which of them are in a page that there is
   // (a bit each); the others are read from the first page.
   GlobalBytes kh[NH], vh[NH];
   uint64_t ko = 0, vo = 0;
-  auto place = [&](int len, int tile) -> uint64_t {
-    uint64_t ok = 0;
+  auto place = [&](int len, int tile) -> uint32_t {
+    uint32_t ok = 0;
 #pragma unroll
     for (int h = 0; h < NE; ++h) {
       const uint32_t e = RUN ? __builtin_amdgcn_readfirstlane(entry[h]) : entry[h];
@@ -506,7 +510,7 @@ __global__ void __launch_bounds__(kBlock, (waves_of<T, C, DP, R>())) attention_k
       ko = kc + (page * p.k_page << 3) + row * p.k_slot;
       vo = vc + (page * p.v_page << 3) + row * p.v_slot;
       if constexpr (RUN == 0) {
-        ok = __ballot(in) & kAll;
+        ok = static_cast<uint32_t>(__ballot(in)) & kAll;
       } else {
         constexpr int kPer = RUN / 16;  // half tiles of a run
         kh[h * kPer] = scalar(ko);
@@ -516,7 +520,7 @@ __global__ void __launch_bounds__(kBlock, (waves_of<T, C, DP, R>())) attention_k
           kh[h * kPer + u] = kh[h * kPer] + u * (16 * p.k_slot);
           vh[h * kPer + u] = vh[h * kPer] + u * (16 * p.v_slot);
         }
-        ok |= in ? (~uint64_t{0} >> (64 - RUN)) << (RUN * h) : 0;
+        ok |= in ? (~0u >> (32 - RUN)) << (RUN * h) : 0;
       }
     }
     return ok;
@@ -535,7 +539,7 @@ __global__ void __launch_bounds__(kBlock, (waves_of<T, C, DP, R>())) attention_k
   };
   auto load_v = [&]() {
 #pragma unroll
-    for (int i = 0; i < NX; ++i) {
+    for (int i = 0; i < KV; ++i) {
       uint64_t at_row = 0;
       if constexpr (RUN == 0) at_row = __shfl(vo, 16 * (i / 4) + 4 * g + i % 4);
 #pragma unroll
@@ -622,7 +626,7 @@ __global__ void __launch_bounds__(kBlock, (waves_of<T, C, DP, R>())) attention_k
       const bool in_1 = tile + kWaves < end || !cross, in_2 = tile + 2 * kWaves < end || !cross;
       const int tile_1 = in_1 ? tile + kWaves : ahead;
       wanted = tile_1 < (in_1 ? end : next.end) ? ~0u : 0u;
-      const uint64_t ok_next = place(in_1 ? len : next.len, tile_1);
+      const uint32_t ok_next = place(in_1 ? len : next.len, tile_1);
       load_k();
       look_up(in_2 ? cur.table : next.table, in_2 ? len : next.len,
               in_2 ? tile + 2 * kWaves : (in_1 ? ahead : ahead + kWaves));
@@ -646,8 +650,7 @@ __global__ void __launch_bounds__(kBlock, (waves_of<T, C, DP, R>())) attention_k
       // Positions that a row does not see; values that no row sees are no part
       // of the sums, whatever they are.
       if (!whole) {
-        const uint32_t there = static_cast<uint32_t>(ok) >> 4 * g;
-        const uint32_t there_hi = static_cast<uint32_t>(ok >> 32) >> 4 * g;
+        const uint32_t there = ok >> 4 * g;
         // (how far a position lies back, and past the first one seen, as
         // unsigned numbers: one comparison each)
         const uint32_t span = p.window ? p.window : INT32_MAX;
@@ -655,9 +658,9 @@ __global__ void __launch_bounds__(kBlock, (waves_of<T, C, DP, R>())) attention_k
         const int past = pos0 + 4 * g - low_first;
         bool fine = true;
 #pragma unroll
-        for (int i = 0; i < NX; ++i) {
+        for (int i = 0; i < KV; ++i) {
           const int t = 16 * (i / 4) + i % 4;
-          const bool in = ((t < 32 ? there >> t : there_hi >> (t - 32)) & 1);
+          const bool in = there >> t & 1;
 #pragma unroll
           for (int j = 0; j < R; ++j) {
             const uint32_t back = pos_0 + tok[j] - (pos0 + 4 * g) - t;
@@ -682,7 +685,7 @@ __global__ void __launch_bounds__(kBlock, (waves_of<T, C, DP, R>())) attention_k
                                            (n * 16 + l15) * VB);
           };
 #pragma unroll
-          for (int i = 0; i < NX; ++i)
+          for (int i = 0; i < KV; ++i)
 #pragma unroll
             for (int n = 0; n < NB; ++n) *v_at(i, n) = v[i][n];
           wave_sync();
@@ -705,7 +708,7 @@ __global__ void __launch_bounds__(kBlock, (waves_of<T, C, DP, R>())) attention_k
           }
           wave_sync();
 #pragma unroll
-          for (int i = 0; i < NX; ++i)
+          for (int i = 0; i < KV; ++i)
 #pragma unroll
             for (int n = 0; n < NB; ++n) v[i][n] = *v_at(i, n);
           clear_k();
@@ -723,12 +726,12 @@ __global__ void __launch_bounds__(kBlock, (waves_of<T, C, DP, R>())) attention_k
         }
       }
 
-      u32x4 ph[R][NS], pl[R][NS];
+      u32x4 ph[R], pl[R];
 #pragma unroll
       for (int j = 0; j < R; ++j) {
-        float x[NX], top = -INFINITY;
+        float x[KV], top = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < NX; ++i) {
+        for (int i = 0; i < KV; ++i) {
           x[i] = sc[j][i / 4][i % 4];
           top = fmaxf(top, x[i]);
         }
@@ -739,21 +742,19 @@ __global__ void __launch_bounds__(kBlock, (waves_of<T, C, DP, R>())) attention_k
         base[j] = now;
         float add = 0.f;
 #pragma unroll
-        for (int i = 0; i < NX; ++i) {
+        for (int i = 0; i < KV; ++i) {
           x[i] = exp2_hw(__builtin_fmaf(x[i], scale2, -from));
           add += x[i];
         }
         sum[j] = sum[j] * keep + add;
 #pragma unroll
-        for (int i = 0; i < NX; i += KV)
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            uint32_t hi = 0, lo = 0;
-            if constexpr (sizeof(T) == 4) hi = __builtin_bit_cast(uint32_t, x[i + u]);
-            else split2(x[i + 2 * u], x[i + 2 * u + 1], hi, lo, T());
-            ph[j][i / KV][u] = hi;
-            pl[j][i / KV][u] = lo;
-          }
+        for (int u = 0; u < 4; ++u) {
+          uint32_t hi = 0, lo = 0;
+          if constexpr (sizeof(T) == 4) hi = __builtin_bit_cast(uint32_t, x[u]);
+          else split2(x[2 * u], x[2 * u + 1], hi, lo, T());
+          ph[j][u] = hi;
+          pl[j][u] = lo;
+        }
         // (nothing to rescale in most tiles; the empty asm keeps the products
         // in the branch: before it, old and scaled sums would both be held)
         if (__any(keep != 1.f)) {
@@ -767,32 +768,29 @@ __global__ void __launch_bounds__(kBlock, (waves_of<T, C, DP, R>())) attention_k
       }
       // acc += V^T P^T
 #pragma unroll
-      for (int m = 0; m < NS; ++m)
+      for (int n = 0; n < NB; ++n)
 #pragma unroll
-        for (int n = 0; n < NB; ++n)
+        for (int e = 0; e < VB; ++e) {
+          u32x4 w;
 #pragma unroll
-          for (int e = 0; e < VB; ++e) {
-            u32x4 w;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              if constexpr (sizeof(T) == 4)
-                w[i] = v[m * KV + i][n].word(e);
-              else
-                w[i] = __builtin_amdgcn_perm(v[m * KV + 2 * i + 1][n].word(e / 2),
-                                             v[m * KV + 2 * i][n].word(e / 2),
-                                             e & 1 ? 0x07060302u : 0x05040100u);
-            }
-            const OpT a = __builtin_bit_cast(OpT, w);
-#pragma unroll
-            for (int j = 0; j < R; ++j) {
-              acc[j][n][e] = mma(a, __builtin_bit_cast(OpT, ph[j][m]), acc[j][n][e]);
-              if constexpr (sizeof(T) == 2)
-                acc[j][n][e] = mma(a, __builtin_bit_cast(OpT, pl[j][m]), acc[j][n][e]);
-            }
-            // (else all operands are turned before the first product, in
-            // twice the registers)
-            if (e % 2) __builtin_amdgcn_sched_barrier(0);
+          for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 4)
+              w[i] = v[i][n].word(e);
+            else
+              w[i] = __builtin_amdgcn_perm(v[2 * i + 1][n].word(e / 2), v[2 * i][n].word(e / 2),
+                                           e & 1 ? 0x07060302u : 0x05040100u);
           }
+          const OpT a = __builtin_bit_cast(OpT, w);
+#pragma unroll
+          for (int j = 0; j < R; ++j) {
+            acc[j][n][e] = mma(a, __builtin_bit_cast(OpT, ph[j]), acc[j][n][e]);
+            if constexpr (sizeof(T) == 2)
+              acc[j][n][e] = mma(a, __builtin_bit_cast(OpT, pl[j]), acc[j][n][e]);
+          }
+          // (else all operands are turned before the first product, in
+          // twice the registers)
+          if (e % 2) __builtin_amdgcn_sched_barrier(0);
+        }
       load_v();
       ok = ok_next;
       tile += kWaves;
@@ -950,23 +948,26 @@ void launch_pages(Params& p, hipStream_t s) {
   // As many blocks as run at once.
   const int64_t lines = static_cast<int64_t>(p.Hkv) * p.groups;
   p.shares = static_cast<int>(std::min<int64_t>(
-      p.shares, std::max<int64_t>(1, int64_t{num_cus()} * waves_of<T, C, DP, R>() / lines)));
+      p.shares, std::max<int64_t>(1, int64_t{num_cus()} * blocks_of<T, C, DP, R>() / lines)));
   const dim3 grid(static_cast<uint32_t>(p.shares * lines));
-  constexpr int kTile = subs_of<T, C, DP>() * 64 / static_cast<int>(sizeof(T));
+  constexpr int kTile = 64 / static_cast<int>(sizeof(T));
   auto launch = [&](auto run) {
     if constexpr (run <= kTile)
       hipLaunchKernelGGL((attention_kernel<T, C, DP, R, run>), grid, dim3(kBlock), 0, s, p);
   };
-  if (kTile >= 64 && p.page_size % 64 == 0) launch(std::integral_constant<int, 64>());
-  else if (kTile >= 32 && p.page_size % 32 == 0) launch(std::integral_constant<int, 32>());
+  if (kTile >= 32 && p.page_size % 32 == 0) launch(std::integral_constant<int, 32>());
   else if (p.page_size % 16 == 0) launch(std::integral_constant<int, 16>());
   else launch(std::integral_constant<int, 0>());
 }
 
 template <typename T, typename C, int DP>
 void launch_rows(Params& p, int tiles, hipStream_t s) {
-  if (tiles == 1) launch_pages<T, C, DP, 1>(p, s);
-  else launch_pages<T, C, DP, 2>(p, s);
+  if constexpr (sizeof(T) == 4 && DP == 256) {  // (two tiles do not fit the registers)
+    launch_pages<T, C, DP, 1>(p, s);
+  } else {
+    if (tiles == 1) launch_pages<T, C, DP, 1>(p, s);
+    else launch_pages<T, C, DP, 2>(p, s);
+  }
 }
 
 // `tiles`: row tiles of a wave, as the entry point counted p.groups by.

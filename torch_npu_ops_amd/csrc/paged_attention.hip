@@ -21,8 +21,8 @@ struct Plan {
   int64_t most;  // shares that there can be
 };
 
-// The shares of a head and row group: two blocks a compute unit in all (the
-// kernels that only fit once take half), none without a least share.
+// The shares of a head and row group: at most two blocks a compute unit in all
+// (most kernels take one), none without a least share.
 void cut(Plan& x, int64_t M, int64_t Hkv) {
   x.groups = cdiv(M, 16 * x.tiles);
   x.shares = std::min(std::max<int64_t>(1, 2 * num_cus() / (Hkv * x.groups)), x.most);
@@ -126,16 +126,14 @@ extern "C" int xk_paged_attention(
   if (!plan_of(B, T, Hq / Hkv, Hkv, head_dim, max_pages * page_size, dtype, x))
     return XK_ERR_INVALID;
   // Two blocks with a row tile each read all twice, but are sooner through a few
-  // tiles: where a block's part of the keys is at most 56 KB by the table's width.
-  // 1, 4 and 16 sequences of 1900 on average, 2600 at the most, 4 tokens, 32 / 4
-  // heads, us with one tile and two (and that part in KB): 64 bf16 11.7, 13.5;
-  // 16.0, 18.9; 26.9, 27.3 (43); 128 bf16 11.5, 13.6; 18.6, 20.6 (21); 37.6, 33.7
-  // (85); 128 e4m3 13.9, 17.7; 19.6, 28.3; 32.5, 41.6 (43); 256 bf16 16.4, 21.6;
-  // 29.1, 37.5 (43); 61.9, 59.1 (170).
+  // tiles: where a block has at most 384 positions by the table's width.  4 and 16
+  // sequences of 1900 on average, 2600 at the most (170 and 680 a block), 4 tokens,
+  // 32 / 4 heads, us with one tile and two: 64 bf16 13.8, 16.1; 21.4, 20.3; e4m3
+  // 14.3, 15.9; 21.5, 19.7; 128 bf16 18.1, 20.5; 34.2, 29.9; e4m3 16.4, 20.6; 26.8,
+  // 29.5; 256 bf16 29.0, 37.8; 61.4, 59.5; e4m3 23.8, 31.5; 43.4, 46.7.
   const int64_t M = T * (Hq / Hkv);
   const int64_t seen = window && window < positions - T ? window + T : positions;
-  if (x.tiles == 2 && M <= 32 &&
-      B * seen * Hkv * head_dim * cb <= (int64_t{112} << 10) * num_cus()) {
+  if (x.tiles == 2 && M <= 32 && B * seen * Hkv <= int64_t{384} * num_cus()) {
     x.tiles = 1;
     cut(x, M, Hkv);  // (fewer shares: the workspace suffices)
   }
