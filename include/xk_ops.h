@@ -709,7 +709,7 @@ int xk_rotary_cache_append(
  *     position are not read; positions of a page outside [0, num_pages) count
  *     as masked.  Sequences may share pages.  max_pages * page_size at most 2^28.
  *   seq_lens : int32 [B], clamped to [0, max_pages * page_size].
- *   At most 2^24 sequences, 2^20 tokens, 2^16 heads, and 2^24 blocks (16 rows of
+ *   At most 2^24 sequences, 2^20 tokens, 2^16 heads, and 2^24 - 128 blocks (16 rows of
  *   T * Hq / Hkv, 32 where there are more, of a head each).  out overlaps no input.
  *   A row that sees nothing (a length below T, an empty sequence) is 0, its lse
  *   -inf.  What the cache holds at positions that a row does not see (NaN, inf)

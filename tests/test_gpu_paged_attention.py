@@ -244,6 +244,17 @@ def test_either_side_of_the_choice_of_row_tiles(dev, dtype, cache, D):
                    window, *_scales(95, 1, cache))
 
 
+@pytest.mark.parametrize("dtype,cache", TYPES)
+@pytest.mark.parametrize("D,hkv", [(8, 8), (8, 12), (16, 6), (32, 7), (64, 2), (64, 10)])
+def test_heads_that_share_cache_lines(dev, dtype, cache, D, hkv):
+    """Rows of 8 to 256 bytes, numbers of heads with and without common factors."""
+    lens = [1500, 0, 33, 700]
+    kc, vc, table = _pool(98, lens, 16, hkv, D, cache)
+    for T in (1, 9):
+        _check(dev, _api("cpp"), _query(99, 4, T, 2 * hkv, D, dtype), kc, vc, table, lens, None, 0,
+               *_scales(100, hkv, cache))
+
+
 def test_windows_beyond_every_length(dev):
     lens = [700, 3]
     kc, vc, table = _pool(96, lens, 16, 2, 64, BF16)

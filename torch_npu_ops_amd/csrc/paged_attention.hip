@@ -11,7 +11,8 @@ namespace {
 constexpr int64_t kMostPositions = int64_t{1} << 28;  // a sequence's, by its table row
 constexpr int64_t kMostPitch = int64_t{1} << 27;      // bytes from one position to the next
 constexpr int64_t kMostPage = int64_t{1} << 35;       // and from one page to the next
-constexpr int64_t kMostBlocks = int64_t{1} << 24;     // a launch holds 2^32 threads in a dimension
+constexpr int64_t kMostBlocks = int64_t{1} << 24;     // a launch holds 2^32 threads in a dimension,
+                                                      // of which 128 blocks may be idle
 
 constexpr float kLog2e = 1.44269504088896f;
 
@@ -39,7 +40,7 @@ bool plan_of(int64_t B, int64_t T, int64_t G, int64_t Hkv, int64_t D, int64_t po
   cut(x, M, Hkv);
   const int64_t lines = Hkv * x.groups;
   const int64_t rows = 2 * x.shares * Hkv * M;
-  if (x.shares * lines >= kMostBlocks || B * Hkv >= kMostBlocks || rows >= (int64_t{1} << 40))
+  if (x.shares * lines > kMostBlocks - 128 || B * Hkv >= kMostBlocks || rows >= (int64_t{1} << 40))
     return false;
   auto up = [](int64_t n) { return cdiv(n, 256) * 256; };
   // One share holds every sequence whole.
