@@ -316,12 +316,6 @@ __device__ __forceinline__ void write_row(P p, int b, int head, int r, int d, f4
         l == 0.f ? -INFINITY : (base + __log2f(l)) * 0.69314718056f;
 }
 
-// ---------------------------------------------------------------------------
-// The kernel.  DP: the head's length, rounded up to 64, 128 or 256.  R: row
-// tiles of a wave.  RUN: positions (16 at least, a tile at most) that pages are
-// whole runs of, with one scalar address each; 0 for none, an address for each
-// lane and load.
-// ---------------------------------------------------------------------------
 // Whether the sums and a tile's keys and values take at most half of 256 registers
 // (a third of that is needed beside them).  Where they do, the kernel is held to
 // 256: with 512 the sums go to the accumulator registers and are moved to be
@@ -342,6 +336,12 @@ constexpr int blocks_of() {
   return sizeof(C) == 1 && DP * R >= 256 && fits_twice<T, C, DP, R>() ? 2 : 1;
 }
 
+// ---------------------------------------------------------------------------
+// The kernel.  DP: the head's length, rounded up to 64, 128 or 256.  R: row
+// tiles of a wave.  RUN: positions (16 at least, a tile at most) that pages are
+// whole runs of, with one scalar address each; 0 for none, an address for each
+// lane and load.
+// ---------------------------------------------------------------------------
 template <typename T, typename C, int DP, int R, int RUN>
 __global__ void __launch_bounds__(kBlock, (fits_twice<T, C, DP, R>() ? 2 : 1)) attention_kernel(Params p) {
   using OpT = typename Op<T>::type;
@@ -956,7 +956,6 @@ __global__ void __launch_bounds__(kBlock) join_kernel(Params p, int team) {
 
 template <typename T, typename C, int DP, int R>
 void launch_pages(Params& p, hipStream_t s) {
-  // As many blocks as run at once.
   const int64_t lines = static_cast<int64_t>(p.Hkv) * p.groups;
   p.shares = static_cast<int>(std::min<int64_t>(
       p.shares, std::max<int64_t>(1, int64_t{num_cus()} * blocks_of<T, C, DP, R>() / lines)));
@@ -965,7 +964,7 @@ void launch_pages(Params& p, hipStream_t s) {
   // lines; for heads that share 512 bytes it is the other way: 185 and 176 with 8
   // bf16 heads of 128).
   p.near = 0;
-  while (p.near < 4 && p.k_head << (p.near + 1) <= 128 && p.Hkv % (2 << p.near) == 0) ++p.near;
+  while (p.near < 4 && p.k_head * (2 << p.near) <= 128 && p.Hkv % (2 << p.near) == 0) ++p.near;
   const dim3 grid(static_cast<uint32_t>(cdiv(p.shares * lines >> p.near, 8) << (3 + p.near)));
   constexpr int kTile = 64 / static_cast<int>(sizeof(T));
   auto launch = [&](auto run) {
