@@ -235,11 +235,14 @@ __device__ __forceinline__ bool not_finite(C x) {
   else return !__builtin_isfinite(to_f32(x));
 }
 
-// The wave's lanes see what its others wrote to LDS before.
+// Orders the wave's accesses to LDS: its lanes see what its others wrote
+// before, and overwrite nothing that these have yet to read.  A wave's accesses
+// run in the order of the program, so this takes no instruction; without it the
+// compiler may exchange a lane's store and its load of what another lane stored.
 __device__ __forceinline__ void wave_sync() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
   __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
 }
 
 // The larger of the values of lanes that differ in bits 4 and 5, and the sum.
@@ -633,6 +636,7 @@ __global__ void __launch_bounds__(kBlock, (fits_twice<T, C, DP, R>() ? 2 : 1)) a
 #pragma unroll
         for (int i = 0; i < NL; ++i) kt[k_place(i * RPI + krow, chunk)] = k[i];
       }
+      wave_sync();
       // The wave's next two tiles, in this piece or the next one.
       const bool in_1 = tile + kWaves < end || !cross, in_2 = tile + 2 * kWaves < end || !cross;
       const int tile_1 = in_1 ? tile + kWaves : ahead;
@@ -658,6 +662,7 @@ __global__ void __launch_bounds__(kBlock, (fits_twice<T, C, DP, R>() ? 2 : 1)) a
         }
         if (s % 4 == 3) __builtin_amdgcn_sched_barrier(0);
       }
+      wave_sync();  // V's rows or the next tile's keys may take their place
       // Positions that a row does not see; values that no row sees are no part
       // of the sums, whatever they are.
       if (!whole) {
@@ -722,6 +727,7 @@ __global__ void __launch_bounds__(kBlock, (fits_twice<T, C, DP, R>() ? 2 : 1)) a
           for (int i = 0; i < KV; ++i)
 #pragma unroll
             for (int n = 0; n < NB; ++n) v[i][n] = *v_at(i, n);
+          wave_sync();
           clear_k();
 #pragma unroll
           for (int j = 0; j < R; ++j)
