@@ -697,7 +697,9 @@ int xk_rotary_cache_append(
  *     o = softmax(scale * q k^T) v
  * over the positions up to the token's own, seq_len - T + t for token t, and
  * with window > 0 only the last `window` of them.  Scores, softmax and sums in
- * fp32; one rounding, at the end.  Hq / Hkv query heads share a key-value head.
+ * fp32 (in the product with v the weights of fp16 tokens have 22 bits and are
+ * right to 2^-39 of the largest); one rounding to `dtype`, at the end.  Hq / Hkv
+ * query heads share a key-value head.
  *   q, out : [B, T, Hq, head_dim] with strides in `dtype`; head_dim a multiple
  *     of 8, at most 256.  lse : fp32 [B, T, Hq] dense or NULL: the natural
  *     logarithm of the sum of exp(scores), for joining with other parts.

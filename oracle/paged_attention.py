@@ -5,8 +5,8 @@ Beside every result stands a bound of what the kernel's arithmetic may add.
 u = 2^-24.  A score is a product of D terms added in fp32 and two more
 roundings: ds = (D + 8) u scale sum |q k|, and its part of the exponent a
 rounding of what it is taken from (u of the largest |score|, twice).  A weight
-is off by that, by its exponential (4 u) and, for 16-bit types, by the rest of
-its two-part split (2^-16 for bf16, 2^-20 for fp16).  The sums of n weights
+is off by that, by its exponential (4 u) and, for fp16, by the rest of its two
+parts (2^-21; three of bf16 hold it whole).  The sums of n weights
 pass at most 32 additions in a product, n / 16 in a lane and 64 between lanes,
 waves and parts.  The result is off by what the weights are, twice (the sum
 that it is divided by has the same bound), and a few roundings.
@@ -21,7 +21,7 @@ import math
 import torch
 
 U = 2.0 ** -24
-SPLIT = {torch.bfloat16: 2.0 ** -16, torch.float16: 2.0 ** -20, torch.float32: 0.0}
+SPLIT = {torch.bfloat16: 0.0, torch.float16: 2.0 ** -21, torch.float32: 0.0}
 
 
 def gather(cache, row, length):

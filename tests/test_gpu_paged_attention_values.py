@@ -1,0 +1,67 @@
+"""GPU checks of what the attention over a paged cache gives where its
+arithmetic shows.  Bounds are derived from the formulas (u = 2^-24)."""
+import pytest
+import torch
+
+from oracle import paged_attention as opa
+from rounding_tol import assert_within
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+FP8 = torch.float8_e4m3fn
+TYPES = [(BF16, BF16), (F16, F16), (F32, F32), (BF16, FP8), (F16, FP8)]
+U = 2.0 ** -24
+
+
+def _api(name):
+    from torch_npu_ops_amd import _xk_torch, ops
+    return {"cpp": _xk_torch, "py": ops}[name]
+
+
+def _parts(x, dtype):
+    """x (float64) as three values of dtype, each cut off what the ones before leave."""
+    out = []
+    for _ in range(3):
+        step = torch.exp2(torch.frexp(x)[1].double() - (7 if dtype == BF16 else 10))
+        out.append((torch.trunc(x / step) * step).to(dtype))
+        x = x - out[-1].double()
+    return out
+
+
+def cancelling(dtype, cache, seed=0):
+    """Two positions with scores 0 and s, values -a and b: in the element whose
+    a / b is exp(s), up to 2^-13 of it, o = (b exp(s) - a) / (1 + exp(s)) shows
+    the weight's last bits.  Rows of 64 heads, each with an element of its own;
+    a < b from 8 to 15, so that a / b has all bits and 8 bits hold a and b."""
+    pairs = [(a, b) for a in range(8, 16) for b in range(a + 1, 16)]
+    g = torch.Generator().manual_seed(seed)
+    B, hq, D = 16, 64, 64
+    pair = torch.tensor([pairs[d % len(pairs)] for d in range(D)], dtype=torch.float64)
+    own = torch.arange(hq)
+    near = 1 + (torch.rand(B, hq, generator=g, dtype=torch.float64) - 0.5) * 2.0 ** -12
+    s = torch.log(pair[own, 0] / pair[own, 1] * near)
+    q = torch.zeros(B, 1, hq, D, dtype=dtype)
+    for i, x in enumerate(_parts(s, dtype)):
+        q[:, 0, :, i] = x
+    kc, vc = torch.zeros(B, 16, 1, D), torch.zeros(B, 16, 1, D)
+    kc[:, 1, 0, :3] = 1
+    vc[:, 0, 0], vc[:, 1, 0] = -pair[:, 0].float(), pair[:, 1].float()
+    table = torch.arange(B, dtype=torch.int32)[:, None]
+    return q, kc.to(cache), vc.to(cache), table, [2] * B
+
+
+@pytest.mark.parametrize("dtype,cache", TYPES)
+def test_weights_keep_their_digits(dev, dtype, cache):
+    """|score| <= 1 in powers of two, off by 2 u from its sum of three, u from
+    the scale's rounding, u from the product with it: 4 u, 3 u of the weight;
+    its exponential 2 u; its parts in fp16 2^-21, in bf16 nothing; products and
+    sums 6 u, the division 2 u."""
+    rel = (2.0 ** -21 if dtype == F16 else 0.0) + 13 * U
+    q, kc, vc, table, lens = cancelling(dtype, cache)
+    want = opa.attention(q, kc, vc, table, lens, 1.0)["o"]
+    size = opa.attention(q, kc, vc.float().abs().to(cache), table, lens, 1.0)["o"]
+    n = torch.tensor(lens, dtype=torch.int32)
+    for api in ("cpp", "py"):
+        o, _ = _api(api).npu_paged_attention(*(t.to(dev) for t in (q, kc, vc, table, n)), 1.0)
+        assert_within(o, want, size * rel, "o")

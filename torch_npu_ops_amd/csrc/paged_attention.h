@@ -35,9 +35,9 @@
 //   - The next tile's loads are requested as soon as this one's registers are
 //     free, and the loop has no condition on them: with one the compiler waits
 //     for the loads at the loop's end, to move their registers.
-// p is split in two 16-bit parts (hi + lo, 16 bits of mantissa and more) for
-// the product with V; fp16's is scaled by 2^14 so that small weights keep
-// their digits.  Scores, statistics and sums are fp32.
+// For the product with V p is cut in bf16 parts, three that hold all its 24 bits,
+// or in two of fp16, 22 bits, scaled by 2^14 so that small weights keep their
+// digits.  Scores, statistics and sums are fp32.
 //
 // Measured (us a call, both launches; TB/s of the keys and values): one sequence
 // of 524288, 8 bf16 heads of 128: 325 (6.6; a plain read of such rows 6.6 to 6.7);
@@ -282,23 +282,35 @@ __device__ __forceinline__ float weight(float a, float b) {
   return exp2_hw(a - (b == -INFINITY ? 0.f : b));
 }
 
-// Two values in 16 bits and what that leaves, also in 16 bits.  fp16's are cut,
-// not rounded: the second part holds the rest either way (22 bits of both).
-__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo, bf16) {
-  gdn::bf2_t h, l;
-  gdn::split2(a, b, h, l);
-  hi = __builtin_bit_cast(uint32_t, h);
-  lo = __builtin_bit_cast(uint32_t, l);
+// Two weights as parts of 16 bits, each cut off what the parts before it leave
+// (exact, and not negative): three of bf16 hold all 24 bits of fp32 (in two of
+// them, 16 bits, 3 to 5 of 4096 outputs of a sequence of 900 were not the nearest
+// bf16 values, 0 or 1 in fp32), two of fp16 22 bits, the last one rounded.
+template <typename T> struct Parts {
+  static constexpr int kCount = std::is_same<T, bf16>::value ? 3 : 2;
+};
+template <> struct Parts<float> {
+  static constexpr int kCount = 1;
+};
+__device__ __forceinline__ void split2(float a, float b, uint32_t (&part)[3], bf16) {
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    const uint32_t x = __builtin_bit_cast(uint32_t, a), y = __builtin_bit_cast(uint32_t, b);
+    part[i] = __builtin_amdgcn_perm(y, x, 0x07060302u);
+    a -= __builtin_bit_cast(float, x & 0xffff0000u);
+    b -= __builtin_bit_cast(float, y & 0xffff0000u);
+  }
 }
-__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo, f16) {
+__device__ __forceinline__ void split2(float a, float b, uint32_t (&part)[2], f16) {
   const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
   float minus = -1.f;  // (a product takes fp16 operands as they are, a difference does not)
   asm("" : "+v"(minus));
-  const auto l =
-      __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf(static_cast<float>(h[0]), minus, a),
-                                 __builtin_fmaf(static_cast<float>(h[1]), minus, b));
-  hi = __builtin_bit_cast(uint32_t, h);
-  lo = __builtin_bit_cast(uint32_t, l);
+  typedef float f2_t __attribute__((ext_vector_type(2)));
+  typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
+  const f2_t rest{__builtin_fmaf(static_cast<float>(h[0]), minus, a),
+                  __builtin_fmaf(static_cast<float>(h[1]), minus, b)};
+  part[0] = __builtin_bit_cast(uint32_t, h);
+  part[1] = __builtin_bit_cast(uint32_t, __builtin_convertvector(rest, h2_t));
 }
 
 // Writes 4 elements of a finished row, and its lse.
@@ -743,7 +755,8 @@ __global__ void __launch_bounds__(kBlock, (fits_twice<T, C, DP, R>() ? 2 : 1)) a
         }
       }
 
-      u32x4 ph[R], pl[R];
+      constexpr int kParts = Parts<T>::kCount;
+      u32x4 pw[R][kParts];
 #pragma unroll
       for (int j = 0; j < R; ++j) {
         float x[KV], top = -INFINITY;
@@ -766,11 +779,11 @@ __global__ void __launch_bounds__(kBlock, (fits_twice<T, C, DP, R>() ? 2 : 1)) a
         sum[j] = sum[j] * keep + add;
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          uint32_t hi = 0, lo = 0;
-          if constexpr (sizeof(T) == 4) hi = __builtin_bit_cast(uint32_t, x[u]);
-          else split2(x[2 * u], x[2 * u + 1], hi, lo, T());
-          ph[j][u] = hi;
-          pl[j][u] = lo;
+          uint32_t part[kParts];
+          if constexpr (sizeof(T) == 4) part[0] = __builtin_bit_cast(uint32_t, x[u]);
+          else split2(x[2 * u], x[2 * u + 1], part, T());
+#pragma unroll
+          for (int i = 0; i < kParts; ++i) pw[j][i][u] = part[i];
         }
         // (nothing to rescale in most tiles; the empty asm keeps the products
         // in the branch: before it, old and scaled sums would both be held)
@@ -799,11 +812,10 @@ __global__ void __launch_bounds__(kBlock, (fits_twice<T, C, DP, R>() ? 2 : 1)) a
           }
           const OpT a = __builtin_bit_cast(OpT, w);
 #pragma unroll
-          for (int j = 0; j < R; ++j) {
-            acc[j][n][e] = mma(a, __builtin_bit_cast(OpT, ph[j]), acc[j][n][e]);
-            if constexpr (sizeof(T) == 2)
-              acc[j][n][e] = mma(a, __builtin_bit_cast(OpT, pl[j]), acc[j][n][e]);
-          }
+          for (int j = 0; j < R; ++j)
+#pragma unroll
+            for (int i = 0; i < kParts; ++i)
+              acc[j][n][e] = mma(a, __builtin_bit_cast(OpT, pw[j][i]), acc[j][n][e]);
           // (else all operands are turned before the first product, in
           // twice the registers)
           if (e % 2) __builtin_amdgcn_sched_barrier(0);
