@@ -698,7 +698,7 @@ int xk_rotary_cache_append(
  * over the positions up to the token's own, seq_len - T + t for token t, and
  * with window > 0 only the last `window` of them.  Scores, softmax and sums in
  * fp32 (in the product with v the weights of fp16 tokens have 22 bits and are
- * right to 2^-39 of the largest); one rounding to `dtype`, at the end.  Hq / Hkv
+ * right to 2^-38 of the largest); one rounding to `dtype`, at the end.  Hq / Hkv
  * query heads share a key-value head.
  *   q, out : [B, T, Hq, head_dim] with strides in `dtype`; head_dim a multiple
  *     of 8, at most 256.  lse : fp32 [B, T, Hq] dense or NULL: the natural
@@ -714,8 +714,12 @@ int xk_rotary_cache_append(
  *   At most 2^24 sequences, 2^20 tokens, 2^16 heads, and 2^24 - 128 blocks (16 rows of
  *   T * Hq / Hkv, 32 where there are more, of a head each).  out overlaps no input.
  *   A row that sees nothing (a length below T, an empty sequence) is 0, its lse
- *   -inf.  What the cache holds at positions that a row does not see (NaN, inf)
- *   has no part in that row.
+ *   -inf, and so is one whose scores are all -inf.  What the cache holds at
+ *   positions that a row does not see (NaN, inf) has no part in that row.  An
+ *   infinite value that it sees makes its element that infinity (NaN where both
+ *   signs meet; where its weight is below 2^-38 of the row's largest, NaN or that
+ *   infinity), a NaN makes its element NaN.  A score that is NaN or +inf makes
+ *   the row and its lse NaN.
  *   q, k_cache and v_cache 16-byte aligned (8 for an 8-bit cache), their
  *   strides whole vectors of that size, out's of 4 elements (else
  *   XK_ERR_UNSUPPORTED); the pitch of places times page_size below 2^32 bytes

@@ -65,3 +65,61 @@ def test_weights_keep_their_digits(dev, dtype, cache):
     for api in ("cpp", "py"):
         o, _ = _api(api).npu_paged_attention(*(t.to(dev) for t in (q, kc, vc, table, n)), 1.0)
         assert_within(o, want, size * rel, "o")
+
+
+def _pool(seed, lens, page, hkv, D, dtype):
+    g = torch.Generator().manual_seed(seed)
+    count = [-(-n // page) for n in lens]
+    order = torch.randperm(sum(count), generator=g).to(torch.int32)
+    table = torch.zeros(len(lens), max(count), dtype=torch.int32)
+    at = 0
+    for b, c in enumerate(count):
+        table[b, :c] = order[at:at + c]
+        at += c
+    kc, vc = (torch.randn(at, page, hkv, D, generator=g).to(dtype) for _ in range(2))
+    return kc, vc, table
+
+
+# Element -> signs at positions from the sequence's end: in the last tile, which
+# no draft or some see, in tiles that all see, in the first, outside a window.
+INFINITIES = {3: {1: 1}, 5: {2: -1}, 7: {1: 1, 3: -1}, 11: {40: 1}, 13: {70: -1, 90: -1},
+              17: {2: 1, 80: 1}, 19: {41: 1, 75: -1}, 23: {300: 1}, 31: {299: -1}}
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("D,G,page", [(64, 4, 16), (64, 12, 10), (128, 2, 32), (128, 8, 32),
+                                      (256, 1, 16), (256, 10, 24)])
+@pytest.mark.parametrize("T,window", [(1, 0), (1, 75), (4, 0), (4, 76)])
+def test_infinite_values_that_a_row_sees(dev, dtype, D, G, page, T, window):
+    """They make its element infinite, NaN where both signs meet; weights whose
+    last bits are zeros (equal scores) and any others; no other row or element."""
+    lens, hkv = [300, 131, 93], 2
+    for std in (0.0, 1.0):
+        kc, vc, table = _pool(D + T, lens, page, hkv, D, dtype)
+        g = torch.Generator().manual_seed(7)
+        q = (torch.randn(3, T, hkv * G, D, generator=g) * std).to(dtype)
+        want = opa.attention(q, kc, vc, table, lens, None, window)
+        plus, minus = (torch.zeros(3, T, D, dtype=torch.bool) for _ in range(2))
+        for b, n in enumerate(lens):
+            for e, places in INFINITIES.items():
+                for back, sign in places.items():
+                    j = n - back
+                    if j < 0:
+                        continue
+                    vc[table[b, j // page], j % page, :, e] = sign * float("inf")
+                    for t in range(T):
+                        at = n - T + t
+                        if j <= at and not (window and j <= at - window):
+                            (plus if sign > 0 else minus)[b, t, e] = True
+        n = torch.tensor(lens, dtype=torch.int32)
+        for api in ("cpp", "py"):
+            o, lse = _api(api).npu_paged_attention(*(x.to(dev) for x in (q, kc, vc, table, n)), None,
+                                                   window, output_lse=True)
+            o = o.cpu()
+            wide = lambda m: m[:, :, None].expand(o.shape)  # noqa: E731
+            assert torch.equal(o.isnan(), wide(plus & minus))
+            assert torch.equal(o == float("inf"), wide(plus & ~minus))
+            assert torch.equal(o == -float("inf"), wide(minus & ~plus))
+            fine = o.isfinite()
+            assert_within(o[fine], want["o"][fine], want["o_err"][fine], "the others")
+            assert_within(lse, want["lse"], want["lse_err"], "lse")

@@ -229,10 +229,15 @@ struct alignas(N * sizeof(C) < 16 ? N * sizeof(C) : 16) Row {
     return bad == 0;
   }
 };
+// 1 for infinity, 2 for minus infinity, 3 for NaN, else 0.
 template <typename C>
-__device__ __forceinline__ bool not_finite(C x) {
-  if constexpr (std::is_same<C, f8>::value) return (x.v & 0x7f) == 0x7f;
-  else return !__builtin_isfinite(to_f32(x));
+__device__ __forceinline__ uint32_t not_finite(C x) {
+  if constexpr (std::is_same<C, f8>::value) {
+    return (x.v & 0x7f) == 0x7f ? 3 : 0;
+  } else {
+    const float y = to_f32(x);
+    return y != y ? 3 : (y == INFINITY ? 1 : (y == -INFINITY ? 2 : 0));
+  }
 }
 
 // Orders the wave's accesses to LDS: its lanes see what its others wrote
@@ -282,10 +287,13 @@ __device__ __forceinline__ float weight(float a, float b) {
   return exp2_hw(a - (b == -INFINITY ? 0.f : b));
 }
 
-// Two weights as parts of 16 bits, each cut off what the parts before it leave
-// (exact, and not negative): three of bf16 hold all 24 bits of fp32 (in two of
-// them, 16 bits, 3 to 5 of 4096 outputs of a sequence of 900 were not the nearest
-// bf16 values, 0 or 1 in fp32), two of fp16 22 bits, the last one rounded.
+// Two weights as parts of 16 bits, each cut off what the parts before it leave:
+// three of bf16 hold all 24 bits of fp32 (in two of them, 16 bits, 3 to 5 of 4096
+// outputs of a sequence of 900 were not the nearest bf16 values, 0 or 1 in fp32),
+// two of fp16 22 bits, the last one rounded.  No part of a weight is negative, and
+// none 0 (fp16's from 2^-38 on, bf16's from 2^-78), so that an infinite value
+// times all of them is infinite: bf16 takes 2^-24 of a part less off than that
+// part, fp16's second part is the smallest there is at the least.
 template <typename T> struct Parts {
   static constexpr int kCount = std::is_same<T, bf16>::value ? 3 : 2;
 };
@@ -297,8 +305,9 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t (&part)[3], bf
   for (int i = 0; i < 3; ++i) {
     const uint32_t x = __builtin_bit_cast(uint32_t, a), y = __builtin_bit_cast(uint32_t, b);
     part[i] = __builtin_amdgcn_perm(y, x, 0x07060302u);
-    a -= __builtin_bit_cast(float, x & 0xffff0000u);
-    b -= __builtin_bit_cast(float, y & 0xffff0000u);
+    constexpr float kLess = -0x1.fffffep-1f;  // 2^-24 - 1
+    a = __builtin_fmaf(__builtin_bit_cast(float, x & 0xffff0000u), kLess, a);
+    b = __builtin_fmaf(__builtin_bit_cast(float, y & 0xffff0000u), kLess, b);
   }
 }
 __device__ __forceinline__ void split2(float a, float b, uint32_t (&part)[2], f16) {
@@ -307,10 +316,14 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t (&part)[2], f1
   asm("" : "+v"(minus));
   typedef float f2_t __attribute__((ext_vector_type(2)));
   typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
+  typedef uint16_t u2_t __attribute__((ext_vector_type(2)));
   const f2_t rest{__builtin_fmaf(static_cast<float>(h[0]), minus, a),
                   __builtin_fmaf(static_cast<float>(h[1]), minus, b)};
-  part[0] = __builtin_bit_cast(uint32_t, h);
-  part[1] = __builtin_bit_cast(uint32_t, __builtin_convertvector(rest, h2_t));
+  const u2_t hi = __builtin_bit_cast(u2_t, h);
+  const u2_t lo = __builtin_bit_cast(u2_t, __builtin_convertvector(rest, h2_t));
+  part[0] = __builtin_bit_cast(uint32_t, hi);
+  part[1] = __builtin_bit_cast(
+      uint32_t, __builtin_elementwise_max(lo, __builtin_elementwise_min(hi, u2_t{1, 1})));
 }
 
 // Writes 4 elements of a finished row, and its lse.
@@ -384,7 +397,8 @@ __global__ void __launch_bounds__(kBlock, (fits_twice<T, C, DP, R>() ? 2 : 1)) a
   __shared__ __align__(16) Shared sh;
   __shared__ __align__(16) OpT sq[R * NK][kWave];  // Q, as the operands take it
   __shared__ float2 ml[kWaves][16];
-  __shared__ uint16_t poison[kWaves][R][DP];  // a bit for each row of a tile
+  // Rows of a tile that see infinity (the lower 16 bits), minus infinity, or NaN (both).
+  __shared__ uint32_t poison[kWaves][R][DP];
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lane = threadIdx.x % kWave, l15 = lane % 16, g = lane / 16;
@@ -704,7 +718,7 @@ __global__ void __launch_bounds__(kBlock, (fits_twice<T, C, DP, R>() ? 2 : 1)) a
         }
         // A value that is not finite where some new tokens see it and others do
         // not: 0 * inf would be NaN for all of them, so it is taken out, and
-        // the rows that see it get NaN themselves.  Rare, and so in LDS, in
+        // added to the sums of the rows that see it.  Rare, and so in LDS, in
         // loops: unrolled in registers it took 70 more of them.
         if (!__all(fine)) {
           C* const vt = reinterpret_cast<C*>(kt);  // [TS][DP]
@@ -722,17 +736,18 @@ __global__ void __launch_bounds__(kBlock, (fits_twice<T, C, DP, R>() ? 2 : 1)) a
             uint32_t rows[R] = {};  // those that see such a value
 #pragma unroll 1
             for (int t = 0; t < TS; ++t) {
-              const bool bad = not_finite(vt[t * DP + d]);
+              const uint32_t bad = not_finite(vt[t * DP + d]);
               if (bad) vt[t * DP + d] = C{};
 #pragma unroll
               for (int j = 0; j < R; ++j) {
                 const int back = pos_0 + tok[j] - (pos0 + t);
                 const uint64_t see = __ballot(back >= 0 && (!p.window || back < p.window));
-                rows[j] |= bad ? static_cast<uint32_t>(see) & 0xffffu : 0u;
+                const uint32_t of = static_cast<uint32_t>(see) & 0xffffu;
+                rows[j] |= (bad & 1 ? of : 0u) | (bad & 2 ? of << 16 : 0u);
               }
             }
 #pragma unroll
-            for (int j = 0; j < R; ++j) poison[wave][j][d] = static_cast<uint16_t>(rows[j]);
+            for (int j = 0; j < R; ++j) poison[wave][j][d] = rows[j];
           }
           wave_sync();
 #pragma unroll
@@ -749,8 +764,9 @@ __global__ void __launch_bounds__(kBlock, (fits_twice<T, C, DP, R>() ? 2 : 1)) a
               for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int e = 0; e < VB; ++e) {
-                  const uint32_t bits = poison[wave][j][(n * 16 + 4 * g + i) * VB + e];
-                  acc[j][n][e][i] += __builtin_bit_cast(float, (0u - (bits >> l15 & 1)) & 0x7fc00000u);
+                  const uint32_t bits = poison[wave][j][(n * 16 + 4 * g + i) * VB + e] >> l15;
+                  acc[j][n][e][i] += bits & 1 ? INFINITY : 0.f;
+                  acc[j][n][e][i] -= bits >> 16 & 1 ? INFINITY : 0.f;
                 }
         }
       }
@@ -768,7 +784,7 @@ __global__ void __launch_bounds__(kBlock, (fits_twice<T, C, DP, R>() ? 2 : 1)) a
         top = over_groups(top, [](float a, float c) { return fmaxf(a, c); });
         const float now = fmaxf(base[j], top * scale2 - kShift);
         const float from = now == -INFINITY ? 0.f : now;
-        const float keep = exp2_hw(base[j] - from);
+        const float before = base[j], keep = exp2_hw(before - from);
         base[j] = now;
         float add = 0.f;
 #pragma unroll
@@ -788,7 +804,8 @@ __global__ void __launch_bounds__(kBlock, (fits_twice<T, C, DP, R>() ? 2 : 1)) a
         // (nothing to rescale in most tiles; the empty asm keeps the products
         // in the branch: before it, old and scaled sums would both be held)
         if (__any(keep != 1.f)) {
-          float by = keep;
+          // (0 before the first score, when a sum may be infinite already)
+          float by = before == -INFINITY ? 1.f : keep;
           asm volatile("" : "+v"(by));
 #pragma unroll
           for (int n = 0; n < NB; ++n)
