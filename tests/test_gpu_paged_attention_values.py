@@ -123,3 +123,27 @@ def test_infinite_values_that_a_row_sees(dev, dtype, D, G, page, T, window):
             fine = o.isfinite()
             assert_within(o[fine], want["o"][fine], want["o_err"][fine], "the others")
             assert_within(lse, want["lse"], want["lse_err"], "lse")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("T,G", [(1, 4), (3, 8)])
+def test_a_scale_that_is_nan(dev, dtype, T, G):
+    """Every row of its head that sees something is NaN; the other heads, and
+    rows that see nothing, are as ever."""
+    lens, page, hkv, D = [300, 2, 33], 16, 3, 64
+    kc, vc, table = _pool(1, lens, page, hkv, D, FP8)
+    q = torch.randn(3, T, hkv * G, D, generator=torch.Generator().manual_seed(2)).to(dtype)
+    ks, vs = torch.tensor([0.5, float("nan"), 2.0]), torch.tensor([1.0, 0.5, 2.0])
+    want = opa.attention(q, kc, vc, table, lens, None, 0, ks.nan_to_num(1.0), vs)
+    n = torch.tensor(lens, dtype=torch.int32)
+    for api in ("cpp", "py"):
+        o, lse = _api(api).npu_paged_attention(
+            *(x.to(dev) for x in (q, kc, vc, table, n)), None, 0, ks.to(dev), vs.to(dev), True)
+        o, lse = o.cpu(), lse.cpu()
+        there = want["lse"].isfinite()
+        bad = there.clone()
+        bad[:, :, :G], bad[:, :, 2 * G:] = False, False
+        assert bad.any() and (T == 1 or not there.all())
+        assert o[bad].isnan().all() and lse[bad].isnan().all()
+        assert_within(o[~bad], want["o"][~bad], want["o_err"][~bad], "o")
+        assert_within(lse[~bad], want["lse"][~bad], want["lse_err"][~bad], "lse")

@@ -430,11 +430,11 @@ __global__ void __launch_bounds__(kBlock, (fits_twice<T, C, DP, R>() ? 2 : 1)) a
   const uint64_t kc = reinterpret_cast<uint64_t>(p.kc + head * p.k_head);
   const uint64_t vc = reinterpret_cast<uint64_t>(p.vc + head * p.v_head);
   // Scores are scaled by something positive, that leaves a masked one -inf: a
-  // sign goes to Q, and 1.2e-38 for 0 makes every finite score 0 too.
+  // sign and NaN go to Q, and 1.2e-38 for 0 makes every finite score 0 too.
   float scale2 = p.scale2;
   if (p.k_scale) scale2 *= p.k_scale[head];
-  const bool negate = scale2 < 0.f;
-  scale2 = fmaxf(fabsf(scale2), 1.17549435e-38f);
+  const bool negate = scale2 < 0.f, nan = scale2 != scale2;
+  scale2 = nan ? 1.f : fmaxf(fabsf(scale2), 1.17549435e-38f);
   const int r0 = group * 16 * R;
   const int first_tok = token_of(&p, r0), last_tok = token_of(&p, min(p.M - 1, r0 + 16 * R - 1));
   // K's chunks lie in the wave's part of LDS with a row's chunks permuted, so
@@ -491,6 +491,7 @@ __global__ void __launch_bounds__(kBlock, (fits_twice<T, C, DP, R>() ? 2 : 1)) a
     for (int c = 0; c < NQ; ++c) {
       const int u = c * kWaves + wave;
       if (negate) qx[c] ^= sizeof(T) == 4 ? 0x80000000u : 0x80008000u;
+      if (nan) qx[c] = u32x4{} + 0x7fff7fffu;
       if (u < R * NK) sq[u][lane] = __builtin_bit_cast(OpT, qx[c]);
     }
   };
