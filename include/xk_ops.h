@@ -705,7 +705,7 @@ int xk_rotary_cache_append(
  *     logarithm of the sum of exp(scores), for joining with other parts.
  *   k_cache, v_cache : as in xk_rotary_cache_append; the new tokens' keys and
  *     values are in it already.  A value stands for itself times k_scale[head]
- *     or v_scale[head].
+ *     or v_scale[head] (a NaN there makes the head's rows NaN).
  *   block_table : int32 [B, max_pages] (row pitch in elements): position j of
  *     a sequence is in page block_table[j / page_size].  Entries past the last
  *     position are not read; positions of a page outside [0, num_pages) count

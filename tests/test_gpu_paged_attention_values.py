@@ -147,3 +147,41 @@ def test_a_scale_that_is_nan(dev, dtype, T, G):
         assert o[bad].isnan().all() and lse[bad].isnan().all()
         assert_within(o[~bad], want["o"][~bad], want["o_err"][~bad], "o")
         assert_within(lse[~bad], want["lse"][~bad], want["lse_err"][~bad], "lse")
+
+
+@pytest.mark.parametrize("dtype,cache", TYPES)
+@pytest.mark.parametrize("T,G", [(1, 4), (3, 8)])
+def test_a_scale_of_zero(dev, dtype, cache, T, G):
+    """The mean of the values seen, however large the scores would be; NaN
+    where a query or a key that a row sees is not finite (0 * inf)."""
+    lens, page, hkv, D = [300, 2, 33], 16, 2, 64
+    kc, vc, table = _pool(3, lens, page, hkv, D, cache)
+    q = torch.randn(3, T, hkv * G, D, generator=torch.Generator().manual_seed(4)).to(dtype)
+    if cache != FP8:  # products beyond fp32 in bf16 and fp32
+        kc, q = kc * (1e4 if dtype == F16 else 9e18), q * (1e4 if dtype == F16 else 9e18)
+    ks = torch.tensor([0.0, -0.0]) if cache == FP8 else None
+    scale = 1.0 if cache == FP8 else 0.0
+    want = opa.attention(q, torch.zeros_like(kc), vc, table, lens, 0.0)
+    n = torch.tensor(lens, dtype=torch.int32)
+    on = lambda x: None if x is None else x.to(dev)  # noqa: E731
+    for api in ("cpp", "py"):
+        args = [kc, vc, table, n, scale, 0, ks, None, True]
+        call = lambda q, *a: _api(api).npu_paged_attention(  # noqa: E731
+            q.to(dev), *(on(x) if torch.is_tensor(x) else x for x in a))
+        o, lse = call(q, *args)
+        assert_within(o, want["o"], want["o_err"], "o")
+        assert_within(lse, want["lse"], want["lse_err"], "lse")
+        bad = q.clone()
+        bad[0, 0, 1, 5], bad[1, T - 1, 2, 7] = float("inf"), float("nan")
+        o, lse = (x.cpu() for x in call(bad, *args))
+        hit = torch.zeros(o.shape[:3], dtype=torch.bool)
+        hit[0, 0, 1] = hit[1, T - 1, 2] = True
+        assert o[hit].isnan().all() and lse[hit].isnan().all()
+        assert_within(o[~hit], want["o"][~hit], want["o_err"][~hit], "the other rows")
+        keys = kc.clone()
+        keys[table[2, (33 - 2) // page], (33 - 2) % page, 1, 9] = float("nan" if cache == FP8 else "-inf")
+        o, lse = (x.cpu() for x in call(q, keys, *args[1:]))
+        hit = torch.zeros(o.shape[:3], dtype=torch.bool)
+        hit[2, max(0, T - 2):, G:] = True
+        assert o[hit].isnan().all() and lse[hit].isnan().all()
+        assert_within(o[~hit], want["o"][~hit], want["o_err"][~hit], "rows that do not see the key")
