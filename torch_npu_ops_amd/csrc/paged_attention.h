@@ -579,16 +579,17 @@ __global__ void __launch_bounds__(kBlock, (fits_twice<T, C, DP, R>() ? 2 : 1)) a
     }
     return ok;
   };
-  // (of a tile that there is not, 16 bytes in place of each 1 KB)
-  uint32_t wanted = ~0u;
+  // Of a tile that there is not, all lanes of a load take one vector, in a row
+  // that there is (where each position has an address, the row's first one).
+  uint32_t wanted = ~0u;  // or 0, for the lanes' offsets
   auto load_k = [&]() {
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
       if constexpr (RUN > 0)
-        k[i].load(kh[i * RPI / 16] + lane_offset(k_off[i % KO]));
+        k[i].load(kh[i * RPI / 16] + lane_offset(k_off[i % KO] & wanted));
       else
         k[i].load(reinterpret_cast<GlobalBytes>(__shfl(ko, i * RPI + krow)) +
-                  (k_off[0] - krow * p.k_slot));
+                  ((k_off[0] - krow * p.k_slot) & wanted));
     }
   };
   auto load_v = [&]() {
@@ -599,10 +600,10 @@ __global__ void __launch_bounds__(kBlock, (fits_twice<T, C, DP, R>() ? 2 : 1)) a
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
         if constexpr (RUN > 0)
-          v[i][n].load(vh[i / 4] + lane_offset(v_off[i % 4][n]));
+          v[i][n].load(vh[i / 4] + lane_offset(v_off[i % 4][n] & wanted));
         else
           v[i][n].load(reinterpret_cast<GlobalBytes>(at_row) +
-                       (v_off[0][n] - 4 * g * p.v_slot));
+                       ((v_off[0][n] - 4 * g * p.v_slot) & wanted));
       }
     }
   };
