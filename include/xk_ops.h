@@ -649,9 +649,11 @@ int xk_gated_residual_rms_norm_bwd(
  * with f = inv_freq, fp32 [rotary_dim / 2].  Pairs are elements (i, i +
  * rotary_dim / 2), or (2i, 2i + 1) with interleaved != 0, of the first
  * rotary_dim; the others are copied.  A longer context than trained is the
- * caller's inv_freq and scale.  The angle is formed in 64 bits: positions up
- * to 2^29 lose nothing.  One rounding, at the end.  inverse != 0 turns by -t f
- * (and multiplies by scale as well): the backward pass, for gradients.
+ * caller's inv_freq and scale.  The angle is formed and brought below a quarter
+ * turn in 64 bits (positions up to 2^29 lose nothing); its cosine and sine are
+ * formed in fp32, right to 2^-23.5, as are the products; one rounding to `dtype`,
+ * at the end.  inverse != 0 turns by -t f (and multiplies by scale as well): the
+ * backward pass, for gradients.
  *   q, k : [num_tokens, heads, head_dim] in `dtype` with token and head
  *     strides (any, zero for broadcast inputs); outputs may be their inputs
  *     (the same start and strides) and must not overlap otherwise.  Hq or Hk

@@ -5,10 +5,16 @@ float64 (no reference implementation in this form; test infrastructure).
 
 on pairs (i, i + r/2) or (2i, 2i + 1) of the first r elements of a head.
 
-Beside every result stands a bound of what the kernel's arithmetic may add:
-the angle's rest (at most pi/4) is rounded to fp32 (2^-25), its cosine and
-sine are off by 2 steps at most (2^-22 for values up to 1), one rounding by L,
-one of each product and one of the sum: 8 * 2^-23 of L (|u| + |v|).
+Beside every result stands a bound of what the kernel's arithmetic may add,
+for positions up to 2^29.  With h = 2^-25, half a step of fp32 below 1, the
+angle's rest r (at most pi/4) is off by h when it is rounded, its square z by
+2 h z.  Cosine: 1 + z p with |p| <= 1/2, p off by 0.63 h (its last step, 1/24's
+rounding): 0.39 h, z 0.62 h, the sum's rounding h, the rest 0.71 h, in all
+2.8 h.  Sine: r + z r p with |p| <= 1/6, p off by 0.52 h: 0.26 h, z r twice
+rounded 0.33 h, the end of the series 0.06 h, the sum h, the rest 0.88 h, in all
+2.8 h.  Then each is rounded by the product with L (2 h of it), the products
+with u and v (2 h of them); the last rounding is the output's.  In all 2.8 h +
+4 h of L (|u| + |v|).
 
 Pins (tests/test_oracle_rotary.py): complex multiplication, the rows of the
 framework's other rotations, and float64 autograd.
@@ -17,7 +23,8 @@ from __future__ import annotations
 
 import torch
 
-ERR = 2.0 ** -20
+TURN = 2.8 * 2.0 ** -25  # of a cosine or sine
+ERR = TURN + 4 * 2.0 ** -25
 
 
 def turn(x, positions, inv_freq, interleaved=False, scale=1.0, inverse=False):

@@ -79,6 +79,8 @@ struct RotaryParams {
 // fma adds what pi/2's first 53 bits leave out), so that the rest r, at most
 // pi/4, is right to 2^-25 when it is rounded.  There the Taylor series end at
 // r^9 and r^10: what follows is below r^11/11! < 2^-28 and r^12/12! < 2^-32.
+// With their roundings both are off by at most 2.8 * 2^-25 (measured: 2.35; the
+// nearest fp32 values: 1).
 __device__ __forceinline__ void turn_of(double t, float f, float& c, float& s) {
   const double a = t * static_cast<double>(f);
   const double n = __builtin_rint(a * 0.63661977236758134308);
