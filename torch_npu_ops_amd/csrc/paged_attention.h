@@ -40,9 +40,9 @@
 // digits.  Scores, statistics and sums are fp32.
 //
 // Measured (us a call, both launches; TB/s of the keys and values): one sequence
-// of 524288, 8 bf16 heads of 128: 325 (6.6; a plain read of such rows 6.6 to 6.7);
-// 131072: 92 (5.8); 64 of up to 4096 in pages of 16: 176 (6.1); the same with all
-// of 4096 in e4m3: 103 (5.2); one of 900: 9.7.
+// of 524288, 8 bf16 heads of 128: 329 (6.5; a plain read of such rows 6.6 to 6.7);
+// 131072: 91 (5.9); 64 of up to 4096 in pages of 16: 177 (6.1); the same with all
+// of 4096 in e4m3: 94 (5.7); one of 900: 10.2.
 #pragma once
 
 #include <cmath>

@@ -131,7 +131,11 @@ extern "C" int xk_paged_attention(
   // sequences of 1900 on average, 2600 at the most (170 and 680 a block), 4 tokens,
   // 32 / 4 heads, us with one tile and two: 64 bf16 13.8, 16.1; 21.4, 20.3; e4m3
   // 14.3, 15.9; 21.5, 19.7; 128 bf16 18.1, 20.5; 34.2, 29.9; e4m3 16.4, 20.6; 26.8,
-  // 29.5; 256 bf16 29.0, 37.8; 61.4, 59.5; e4m3 23.8, 31.5; 43.4, 46.7.
+  // 29.5; 256 bf16 29.0, 37.8; 61.4, 59.5; e4m3 23.8, 31.5; 43.4, 46.7.  The width
+  // is all that the host knows of the lengths: a table much wider than they are
+  // gets two.  More than 32 rows get two as well, which is right where there is much
+  // to read (32 sequences of 2500, 64 rows, bf16 heads of 256: 105.9, 91.7) and not
+  // where there is little (8, 48 rows: 64 15.6, 18.7; 128 21.2, 24.8; 256 36.6, 48.6).
   const int64_t M = T * (Hq / Hkv);
   const int64_t seen = window && window < positions - T ? window + T : positions;
   if (x.tiles == 2 && M <= 32 && B * seen * Hkv <= int64_t{384} * num_cus()) {
