@@ -680,7 +680,8 @@ int xk_rotary_embedding(
  *     NULL = 1; positive) to the nearest e4m3 value, at most 448.
  *   slots : int32/int64 [num_tokens]: page * page_size + place of a token.  A
  *     slot outside the cache (-1 for padding) stores nothing; q is turned all
- *     the same.  Two tokens of a call must not have the same slot.
+ *     the same.  Two tokens of a call must not have the same slot, and no two
+ *     rows of the caches the same place.
  */
 int xk_rotary_cache_append(
     const void* q, int64_t stride_q_tok, int64_t stride_q_head, void* q_out,

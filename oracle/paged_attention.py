@@ -5,8 +5,8 @@ Beside every result stands a bound of what the kernel's arithmetic may add.
 u = 2^-24.  A score is a product of D terms added in fp32 and two more
 roundings: ds = (D + 8) u scale sum |q k|, and its part of the exponent a
 rounding of what it is taken from (u of the largest |score|, twice).  A weight
-is off by that, by its exponential (4 u) and, for fp16, by the rest of its two
-parts (2^-21; three of bf16 hold it whole).  The sums of n weights
+is off by that, by its exponential (4 u) and by its parts (two of fp16 2^-21,
+three of bf16 u, among the roundings at the end).  The sums of n weights
 pass at most 32 additions in a product, n / 16 in a lane and 64 between lanes,
 waves and parts.  The result is off by what the weights are, twice (the sum
 that it is divided by has the same bound), and a few roundings.

@@ -55,9 +55,9 @@ def cancelling(dtype, cache, seed=0):
 def test_weights_keep_their_digits(dev, dtype, cache):
     """|score| <= 1 in powers of two, off by 2 u from its sum of three, u from
     the scale's rounding, u from the product with it: 4 u, 3 u of the weight;
-    its exponential 2 u; its parts in fp16 2^-21, in bf16 nothing; products and
-    sums 6 u, the division 2 u."""
-    rel = (2.0 ** -21 if dtype == F16 else 0.0) + 13 * U
+    its exponential 2 u; its parts in fp16 2^-21, in bf16 u; products and sums
+    6 u, the division 2 u."""
+    rel = (2.0 ** -21 if dtype == F16 else U if dtype == BF16 else 0.0) + 13 * U
     q, kc, vc, table, lens = cancelling(dtype, cache)
     want = opa.attention(q, kc, vc, table, lens, 1.0)["o"]
     size = opa.attention(q, kc, vc.float().abs().to(cache), table, lens, 1.0)["o"]
@@ -128,8 +128,8 @@ def test_infinite_values_that_a_row_sees(dev, dtype, D, G, page, T, window):
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("T,G", [(1, 4), (3, 8)])
 def test_a_scale_that_is_nan(dev, dtype, T, G):
-    """Every row of its head that sees something is NaN; the other heads, and
-    rows that see nothing, are as ever."""
+    """Every row of its head that sees something is NaN, with a scale of values
+    but the lse; the other heads, and rows that see nothing, are as ever."""
     lens, page, hkv, D = [300, 2, 33], 16, 3, 64
     kc, vc, table = _pool(1, lens, page, hkv, D, FP8)
     q = torch.randn(3, T, hkv * G, D, generator=torch.Generator().manual_seed(2)).to(dtype)
@@ -147,6 +147,12 @@ def test_a_scale_that_is_nan(dev, dtype, T, G):
         assert o[bad].isnan().all() and lse[bad].isnan().all()
         assert_within(o[~bad], want["o"][~bad], want["o_err"][~bad], "o")
         assert_within(lse[~bad], want["lse"][~bad], want["lse_err"][~bad], "lse")
+        o, lse = (x.cpu() for x in _api(api).npu_paged_attention(
+            *(x.to(dev) for x in (q, kc, vc, table, n)), None, 0, ks.nan_to_num(1.0).to(dev),
+            (vs * (ks / ks)).to(dev), True))
+        assert o[bad].isnan().all()
+        assert_within(o[~bad], want["o"][~bad], want["o_err"][~bad], "o")
+        assert_within(lse, want["lse"], want["lse_err"], "lse")
 
 
 @pytest.mark.parametrize("dtype,cache", TYPES)
@@ -185,3 +191,49 @@ def test_a_scale_of_zero(dev, dtype, cache, T, G):
         hit[2, max(0, T - 2):, G:] = True
         assert o[hit].isnan().all() and lse[hit].isnan().all()
         assert_within(o[~hit], want["o"][~hit], want["o_err"][~hit], "rows that do not see the key")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("T,G", [(1, 4), (3, 8)])
+def test_scores_that_are_not_finite(dev, dtype, T, G):
+    """NaN and inf make a row NaN; a score of -inf has no weight, and a row of
+    such alone is 0 with an lse of -inf.  Rows before them are as ever."""
+    lens, page, hkv, D = [300, 90, 40], 16, 2, 64
+    kc, vc, table = _pool(5, lens, page, hkv, D, dtype)
+    q = torch.randn(3, T, hkv * G, D, generator=torch.Generator().manual_seed(6)).to(dtype)
+    q[..., 3] = q[..., 3].abs() + 0.5
+    n = torch.tensor(lens, dtype=torch.int32)
+
+    def call(api, keys):
+        o, lse = _api(api).npu_paged_attention(*(x.to(dev) for x in (q, keys, vc, table, n)),
+                                               output_lse=True)
+        return o.cpu(), lse.cpu()
+
+    def put(keys, b, j, head, x):
+        keys[table[b, j // page], j % page, head, 3] = x
+    inf = float("inf")
+    for api in ("cpp", "py"):
+        for bad in (float("nan"), inf):
+            for j in (lens[0] - 1, 7):  # one that the last token sees, one that all do
+                keys = kc.clone()
+                put(keys, 0, j, 1, bad)
+                want = opa.attention(q, kc, vc, table, lens)
+                o, lse = call(api, keys)
+                hit = torch.zeros(lse.shape, dtype=torch.bool)
+                hit[0, T - 1 if j > 7 else 0:, G:] = True
+                assert o[hit].isnan().all() and lse[hit].isnan().all()
+                assert_within(o[~hit], want["o"][~hit], want["o_err"][~hit], "o")
+                assert_within(lse[~hit], want["lse"][~hit], want["lse_err"][~hit], "lse")
+        # without weight: as if the page were not there
+        keys, without = kc.clone(), table.clone()
+        for j in range(32, 48):
+            put(keys, 1, j, slice(None), -inf)
+        without[1, 2] = -1
+        for j in range(lens[2]):
+            put(keys, 2, j, slice(None), -inf)
+        without[2] = -1
+        want = opa.attention(q, kc, vc, without, lens)
+        o, lse = call(api, keys)
+        assert (o[2] == 0).all() and (lse[2] == -inf).all()
+        assert_within(o, want["o"], want["o_err"], "o")
+        assert_within(lse, want["lse"], want["lse_err"], "lse")

@@ -299,8 +299,8 @@ __device__ __forceinline__ float weight(float a, float b) {
 // outputs of a sequence of 900 were not the nearest bf16 values, 0 or 1 in fp32),
 // two of fp16 22 bits, the last one rounded.  No part of a weight is negative, and
 // none 0 (fp16's from 2^-38 on, bf16's from 2^-78), so that an infinite value
-// times all of them is infinite: bf16 takes 2^-24 of a part less off than that
-// part, fp16's second part is the smallest there is at the least.
+// times all of them is infinite: of a part 2^-24 is left to the next one in bf16
+// (which is off by as much), fp16's second part is the smallest there is at least.
 template <typename T> struct Parts {
   static constexpr int kCount = std::is_same<T, bf16>::value ? 3 : 2;
 };
