@@ -109,7 +109,7 @@ extern "C" int xk_paged_attention(
       (num_pages && (!k_cache || !v_cache)))
     return XK_ERR_INVALID;
   // Vectors of 16 bytes (8 of an 8-bit cache) have to be aligned.
-  const int eb = elem_bytes(dtype), cb = elem_bytes(cache_dtype), n = 16 / eb;
+  const int eb = elem_bytes(dtype), cb = eight ? 1 : eb, n = 16 / eb;
   const int cv = n * cb;
   if (!aligned(q, 16) || stride_q_seq % n || stride_q_tok % n || stride_q_head % n ||
       !aligned(k_cache, cv) || !aligned(v_cache, cv) || stride_kc_page % n ||

@@ -194,8 +194,6 @@ inline int elem_bytes(xk_dtype dt) {
       return 2;
     case XK_I64:
       return 8;
-    case XK_F8E4M3:
-      return 1;
     default:
       return 4;
   }
